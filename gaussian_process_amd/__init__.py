@@ -4,7 +4,8 @@ from .regression import GaussianProcessRegression
 from .expectation_propagation import GaussianProcessExpectationPropagation
 from .distillation import GaussianProcessDistillation
 from .kernels import RBF, ARD, KernelValue
+from .orthogonal import orthogonalize
 
 __all__ = ["GaussianProcessRegression", "GaussianProcessExpectationPropagation",
            "GaussianProcessDistillation", "RBF", "ARD",
-           "KernelValue"]
+           "KernelValue", "orthogonalize"]

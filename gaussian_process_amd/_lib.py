@@ -12,6 +12,14 @@ GPX_KIND = {"rbf": 0, "ard": 1}
 GPX_FULL, GPX_LOWER = 0, 1
 GPX_NB = 128
 
+GPX_TYPE = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
+
+
+class Strided(C.Structure):
+    """gpx_strided: element strides of a stack of matrices."""
+    _fields_ = [("bs", C.c_longlong), ("rs", C.c_longlong), ("cs", C.c_longlong)]
+
+
 _dp = C.c_void_p      # device pointer
 _hp = C.POINTER(C.c_double)  # host double*
 _i, _d, _sz = C.c_int, C.c_double, C.c_size_t
@@ -61,6 +69,9 @@ SIGNATURES = {
     "gpx_ep_scale": (_i, [C.c_void_p, _i, _dp, _i, _dp, _dp, _i, _dp, _i]),
     "gpx_ep_sweep": (_i, [C.c_void_p, _i, _dp, _i, _dp, _dp, _dp, C.POINTER(C.c_int), _i, _dp]),
     "gpx_ep_sweep_work_elems": (C.c_size_t, [_i]),
+    "gpx_orthogonalize": (_i, [C.c_void_p, _i, _i, _i, _i, _dp, C.POINTER(Strided), _i, _hp, _d, _d, _d, _dp,
+                               C.POINTER(Strided), _dp, C.POINTER(Strided), _dp, _sz]),
+    "gpx_orthogonalize_work_bytes": (_sz, [_i, _i, _i, _i]),
     "gpx_ep_recompute": (_i, [C.c_void_p, _i, _dp, _i, _dp, _dp, _dp, _dp, _dp, _i, _dp, _dp, _dp]),
 }
 

@@ -8,10 +8,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libgpx.so")
-SOURCES = ["gemm_f64.hip", "leaf.hip", "gram.hip", "blas2.hip", "trsv.hip", "ep.hip", "gpx_api.hip"]
+SOURCES = ["gemm_f64.hip", "leaf.hip", "gram.hip", "blas2.hip", "trsv.hip", "ep.hip", "orthogonalize.hip",
+           "gpx_api.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
-         "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-Wall", "-Wno-unused-function"]
+         "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-Wall", "-Wno-unused-function",
+         # no packed fp32 arithmetic: some forms of it have given wrong results on this hardware
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target, deps):

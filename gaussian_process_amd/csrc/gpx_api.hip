@@ -253,24 +253,6 @@ int fetch_info(gpx_handle* h, int* info) {
   return 0;
 }
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) { enter(dev); }
-  // an entry point working for handle h: its device current, its split-K workspace the thread's
-  explicit DeviceGuard(const gpx_handle* h) {
-    enter(h->device);
-    gpx_gemm_set_workspace(h->gemm_ws, h->gemm_ws ? GPX_GEMM_WS_ELEMS : 0);
-  }
-  void enter(int dev) {
-    (void)hipGetDevice(&prev);
-    if (prev != dev) (void)hipSetDevice(dev);
-    else prev = -1;
-  }
-  ~DeviceGuard() {
-    if (prev >= 0) (void)hipSetDevice(prev);
-  }
-};
-
 // scratch slots inside h->red (doubles): the tail is for scalars
 constexpr size_t RED_SCALARS = 64;
 inline double* red_scalars(gpx_handle* h) { return h->red + (GPX_RED_ELEMS - RED_SCALARS); }

@@ -105,6 +105,25 @@ struct GemmDesc {
 void gpx_gemm_set_workspace(double* ws, size_t elems);
 constexpr size_t GPX_GEMM_WS_ELEMS = (size_t)256 * 128 * 128;   // 256 workgroups x one 128 x 128 tile: 32 MiB
 
+// The device of an entry point made current for its duration.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) { enter(dev); }
+  // an entry point working for handle h: its device current, its split-K workspace the thread's
+  explicit DeviceGuard(const gpx_handle* h) {
+    enter(h->device);
+    gpx_gemm_set_workspace(h->gemm_ws, h->gemm_ws ? GPX_GEMM_WS_ELEMS : 0);
+  }
+  void enter(int dev) {
+    (void)hipGetDevice(&prev);
+    if (prev != dev) (void)hipSetDevice(dev);
+    else prev = -1;
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
 int gpx_gemm_launch(hipStream_t s, const GemmDesc& g);
 
 // leaf kernels (leaf.hip: 128x128 diagonal block Cholesky + inverse on the matrix cores)

@@ -2,6 +2,7 @@
 
 PyTorch is used only for allocation, H2D/D2H copies and stream identity; all arithmetic is in
 libgpx.so."""
+import contextlib
 import ctypes as C
 import threading
 
@@ -49,6 +50,20 @@ class Runtime:
             cur.wait_event(ev)
         self._stream = cur
         _lib.check(self.lib.gpx_set_stream(self.h, C.c_void_p(cur.cuda_stream)), "gpx_set_stream")
+
+    @contextlib.contextmanager
+    def current_stream(self):
+        """The handle on torch's current stream for calls that use none of its scratch: such calls need not wait
+        for what other streams do with the handle, so no event is recorded (the calls may be captured into a graph)
+        and the binding of bind_stream() is put back."""
+        with self.lock, self.torch.cuda.device(self.index):
+            cur = self.torch.cuda.current_stream(self.dev)
+            _lib.check(self.lib.gpx_set_stream(self.h, C.c_void_p(cur.cuda_stream)), "gpx_set_stream")
+            try:
+                yield self
+            finally:
+                old = self._stream.cuda_stream if self._stream is not None else 0
+                _lib.check(self.lib.gpx_set_stream(self.h, C.c_void_p(old)), "gpx_set_stream")
 
     # ---- buffers -------------------------------------------------------------------
     def matrix(self, rows, cols):
@@ -110,3 +125,13 @@ def on_device(fn):
 
 def ptr(t):
     return C.c_void_p(t.data_ptr())
+
+
+def tensor_runtime(*tensors):
+    """The runtime of the one MI355X that all the given tensors (None allowed) live on."""
+    devices = {t.device for t in tensors if t is not None}
+    if any(d.type != "cuda" for d in devices):
+        raise _lib.GpxError("the tensors must be on an MI355X (no CPU fallback)")
+    if len(devices) != 1:
+        raise ValueError("the tensors are on different devices: %s" % ", ".join(sorted(map(str, devices))))
+    return runtime(devices.pop().index)

@@ -274,6 +274,35 @@ int gpx_ep_sweep(gpx_handle* h, int n, double* Sigma, int ld, const double* y, d
 /* Number of doubles gpx_ep_sweep needs in `work` for n sites (2 n x 256 delayed columns + 6 n state). */
 size_t gpx_ep_sweep_work_elems(int n);
 
+/* ---- learned maps: element types --------------------------------------------------------- */
+#define GPX_F64 0
+#define GPX_F32 1
+#define GPX_F16 2
+#define GPX_BF16 3
+
+/* ---- orthogonalisation of an update by Newton-Schulz products ---------------------------- */
+/* out = alpha * O + beta * base, where O comes from the n x m matrix G (or each of `batch` of them) by
+ *   X = G / (|G|_F + eps);  `steps` times:  A = X X^T,  B = b A + c A A,  X = a X + B X;   O = X
+ * (of the transpose when n > m; the result is the same).  With (a, b, c) = (3.4445, -4.7750, 2.0315) and 5 steps
+ * every singular value of O lies within about 0.7 .. 1.2: the update of an optimiser that orthogonalises the
+ * momentum of matrix-shaped parameters.  It has no counterpart in the reference.
+ * Matrix z, element (i, j) of G is G[z * bs + i * rs + j * cs] (strides in ELEMENTS, not negative: a
+ * transposed view is rs = 1); likewise out and base (base may be NULL when beta == 0).  dtype: GPX_F64, GPX_F32,
+ * GPX_F16, GPX_BF16, one type for G, base and out.  out may overlap G in any way (G is read before out is written) and
+ * may be base with the same strides, but must not overlap base otherwise; no two elements of out may share memory.
+ * Arithmetic: GPX_F64 in fp64.  The other types on the fp16 matrix cores with fp32 accumulation and intermediates
+ * scaled by powers of two: GPX_BF16 with one fp16 value per element (its 11 bits lie under the 8 of the result),
+ * GPX_F32 and GPX_F16 with two (22 bits).  The norm is summed in fp64.
+ * coef_host: (a, b, c), host memory.  GPX_EINVAL if the polynomial lets a singular value grow beyond 1000
+ * (the iteration diverges).  1 <= steps <= 64; n, m <= 65536; batch <= 65535.
+ * work: gpx_orthogonalize_work_bytes(dtype, batch, n, m) device bytes, 16-byte aligned, not shared by calls that may
+ * overlap in time.  No other scratch is used and nothing is allocated: the call may be captured into a graph. */
+typedef struct gpx_strided { long long bs, rs, cs; } gpx_strided;
+int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const void* G, const gpx_strided* g_st,
+                      int steps, const double* coef_host, double eps, double alpha, double beta, const void* base,
+                      const gpx_strided* base_st, void* out, const gpx_strided* out_st, void* work, size_t work_bytes);
+size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m);
+
 #ifdef __cplusplus
 }
 #endif
