@@ -4,8 +4,10 @@ from .regression import GaussianProcessRegression
 from .expectation_propagation import GaussianProcessExpectationPropagation
 from .distillation import GaussianProcessDistillation
 from .kernels import RBF, ARD, KernelValue
+from .delta import gated_delta_rule, gated_delta_rule_backward, gated_delta_rule_step
 from .orthogonal import orthogonalize
 
 __all__ = ["GaussianProcessRegression", "GaussianProcessExpectationPropagation",
            "GaussianProcessDistillation", "RBF", "ARD",
-           "KernelValue", "orthogonalize"]
+           "KernelValue", "gated_delta_rule", "gated_delta_rule_backward", "gated_delta_rule_step",
+           "orthogonalize"]

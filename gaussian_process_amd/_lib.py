@@ -20,6 +20,13 @@ class Strided(C.Structure):
     _fields_ = [("bs", C.c_longlong), ("rs", C.c_longlong), ("cs", C.c_longlong)]
 
 
+class Delta(C.Structure):
+    """gpx_delta: sizes and inputs of a gated delta rule."""
+    _fields_ = ([(n, C.c_int) for n in ("dtype", "batch", "tokens", "sequences", "key_heads", "value_heads", "dk", "dv")]
+                + [("scale", C.c_double)] + [(n, C.c_void_p) for n in ("offsets", "q", "k", "v", "g", "beta")]
+                + [(n, Strided) for n in ("q_st", "k_st", "v_st", "g_st", "beta_st")])
+
+
 _dp = C.c_void_p      # device pointer
 _hp = C.POINTER(C.c_double)  # host double*
 _i, _d, _sz = C.c_int, C.c_double, C.c_size_t
@@ -72,6 +79,11 @@ SIGNATURES = {
     "gpx_orthogonalize": (_i, [C.c_void_p, _i, _i, _i, _i, _dp, C.POINTER(Strided), _i, _hp, _d, _d, _d, _dp,
                                C.POINTER(Strided), _dp, C.POINTER(Strided), _dp, _sz]),
     "gpx_orthogonalize_work_bytes": (_sz, [_i, _i, _i, _i]),
+    "gpx_delta_work_bytes": (_sz, [C.POINTER(Delta), _i]),
+    "gpx_delta_forward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, _dp, _dp, _i, _dp, _sz]),
+    "gpx_delta_backward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, C.POINTER(Strided), _dp, _dp, _dp, _dp, _dp, _dp, _dp,
+                                _dp, _sz, _dp, _sz]),
+    "gpx_delta_step": (_i, [C.c_void_p, C.POINTER(Delta), _i, _dp, _dp, _dp, _dp]),
     "gpx_ep_recompute": (_i, [C.c_void_p, _i, _dp, _i, _dp, _dp, _dp, _dp, _dp, _i, _dp, _dp, _dp]),
 }
 

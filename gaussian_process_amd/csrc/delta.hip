@@ -1,0 +1,1023 @@
+// The gated delta rule, gpx_delta_* in include/gpx.h:
+//   Sbar_t = exp(g_t) S_{t-1};  e_t = v_t - Sbar_t^T k_t;  S_t = Sbar_t + beta_t k_t e_t^T;  o_t = scale S_t^T q_t
+//
+// Chunks of C = 64 tokens.  With G the running sum of g in the chunk, D_ij = exp(G_i - G_j) (i >= j),
+// N = strictly lower part of K K^T o D, P = lower part of Q K^T o D, S the state before the chunk:
+//   X = V - diag(exp G) K S;   E = T X with T = (I + N diag(beta))^-1;   U = diag(beta) E
+//   O = scale (diag(exp G) Q S + P U);   S' = exp(G_C) S + K^T diag(exp(G_C - G)) U
+// (in terms of the errors E instead of beta E, so that beta = 0 divides nothing).  Backward, given dO and dS':
+//   dU = scale P^T dO + diag(exp(G_C - G)) K dS';   dX = T^T diag(beta) dU;   dV = dX;   dA = -dX E^T
+//   dS = exp(G_C) dS' + scale Q^T diag(exp G) dO - K^T diag(exp G) dX
+//   dP = scale dO U^T;   dQ = scale diag(exp G) dO S^T + (dP o D) K;   dbeta_j = E_j . dU_j + sum_i dA_ij N_ij
+//   dK = dKr + dKc:  dKr = (dA diag(beta) o D) K - diag(exp G) dX S^T        (the key that reads: row of N, of K S)
+//                    dKc = (dA diag(beta) o D)^T K + (dP o D)^T Q + diag(exp(G_C - G)) U dS'^T   (the key that writes)
+//   dG = q . dQ + k . dKr - k . dKc, and at the last token + sum_j (k . [state part of dKc])_j + exp(G_C) <dS', S>
+// because G_i enters only as exp(G_i) with what token i reads and exp(-G_j) with what token j writes; dg is the sum
+// of dG from its token to the end of the chunk.
+//
+// G is summed in 64 bits, since differences of it are taken, and g is read as max(g, -200): exp(-200) is 0 in fp32,
+// and a g of -infinity then gives no infinity minus infinity.
+//
+// Kernels: prep (parallel over chunks: T, P, G), scan (over the chunks of a sequence, parallel over heads and slices of
+// dv, which are independent), its reverse, and grads (parallel over chunks).  Short inputs and single tokens go through
+// the recurrence itself.
+#include <algorithm>
+#include <cmath>
+
+#include "gpx_internal.h"
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int C = 64;          // tokens per chunk
+constexpr int DVT = 32;        // columns of a slice of dv
+constexpr int PV = 40;         // LDS pitch of [..][DVT] tiles: rows 40 banks apart, 4 rows at a time nearly conflict-free
+constexpr int PC = 68;         // LDS pitch of [..][64] tiles
+constexpr float G_MIN = -200.f;
+
+// Where the chunks of a problem are.  Slot numbers need no table: sequence s starts at slot offsets[s] / C + s, which
+// leaves room for every sequence's last, partly filled chunk.
+struct Plan {
+  int sequences, tokens, batch;
+  const int* off;        // sanitised offsets (device) or nullptr: sequence s is batch row s
+  int chunks_per_row;    // plain batches
+  __device__ __forceinline__ int begin(int s) const { return off ? off[s] : 0; }
+  __device__ __forceinline__ int end(int s) const { return off ? off[s + 1] : tokens; }
+  __device__ __forceinline__ int slot0(int s) const { return off ? off[s] / C + s : s * chunks_per_row; }
+  // the sequence and first token of a slot; len = tokens of the chunk (0: no chunk in this slot)
+  __device__ __forceinline__ void locate(int slot, int& s, int& t0, int& len) const {
+    if (off == nullptr) {
+      s = slot / chunks_per_row;
+      t0 = (slot % chunks_per_row) * C;
+    } else {
+      int lo = 0, hi = sequences - 1;   // the last s with slot0(s) <= slot
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (slot0(mid) <= slot) lo = mid; else hi = mid - 1;
+      }
+      s = lo;
+      t0 = begin(s) + (slot - slot0(s)) * C;
+    }
+    len = min(C, end(s) - t0);
+    if (len < 0 || slot < slot0(s)) len = 0;   // behind the sequence's last chunk, or before the first sequence
+  }
+  __device__ __forceinline__ long row(int s) const { return off ? 0 : s; }   // batch row
+};
+
+// offsets made non-decreasing and inside [0, tokens]: every later kernel's accesses follow from these
+__global__ void delta_plan_kernel(const int* in, int n, int tokens, int* out) {
+  const int lane = threadIdx.x;
+  int carry = 0;
+  for (int base = 0; base < n; base += 64) {
+    const int i = base + lane;
+    int v = i < n ? min(max(in[i], 0), tokens) : 0;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(v, o);
+      if (lane >= o) v = max(v, u);
+    }
+    v = max(v, carry);
+    carry = __shfl(v, 63);
+    if (i < n) out[i] = v;
+  }
+}
+
+struct Args {
+  gpx_delta d;
+  Plan p;
+  int group;                    // value heads per key head
+  int dvp;                      // dv rounded up to DVT
+  float scale;
+  // per (slot, value head): T and P (C x C), G (C doubles), E and dX (C x dvp), S and dS (dk x dvp)
+  float *T, *P, *E, *dX, *S, *dS, *part;
+  double* G;
+  const float *state, *d_state_out;
+  float *state_out, *d_state, *d_g, *d_beta;
+  void *o, *d_q, *d_k, *d_v;
+  const void* d_o;
+  gpx_strided do_st;
+  int save;
+};
+
+template <typename T> __device__ __forceinline__ float ld(const void* p, long i) { return (float)reinterpret_cast<const T*>(p)[i]; }
+template <typename T> __device__ __forceinline__ void st(void* p, long i, float v) { reinterpret_cast<T*>(p)[i] = (T)v; }
+
+// acc (16 x 16, rows (lane >> 4) * 4 + e, column lane & 15) += A B over k < K (a multiple of 4).  A is 16 x K, stored
+// [row][k] or with TA [k][row]; B is K x 16, stored [k][col] or with TB [col][k].
+template <bool TA, bool TB>
+__device__ __forceinline__ f4 mm(const float* A, int pa, const float* B, int pb, int K, f4 acc) {
+  const int r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  const float* a = TA ? A + g * pa + r : A + r * pa + g;
+  const float* b = TB ? B + r * pb + g : B + g * pb + r;
+  const int sa = TA ? 4 * pa : 4, sb = TB ? 4 : 4 * pb;
+#pragma unroll 4
+  for (int k = 0; k < K; k += 4, a += sa, b += sb) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(*a, *b, acc, 0, 0, 0);
+  return acc;
+}
+
+// tokens t0 .. t0 + len of one head, rows of w elements, into an LDS tile of C rows x W (pitch p); zeros elsewhere
+template <typename T, int W>
+__device__ __forceinline__ void load_rows(float* dst, int p, const void* src, const gpx_strided& s, long row, int t0, int len, int head,
+                                          int c0, int w, int nt) {
+  const long base = row * s.bs + t0 * s.rs + head * s.cs + c0;
+  for (int i = threadIdx.x; i < C * W; i += nt) {
+    const int r = i / W, c = i % W;
+    dst[r * p + c] = r < len && c < w ? ld<T>(src, base + r * s.rs + c) : 0.f;
+  }
+}
+
+// ---- prep: one chunk of one value head -----------------------------------------------------------------------------
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_prep_kernel(const Args a) {
+  constexpr int PK = DK + 4;
+  extern __shared__ __align__(16) char smem[];
+  float* K = reinterpret_cast<float*>(smem);
+  float* Q = K + C * PK;
+  float* A = Q + C * PK;
+  double* G = reinterpret_cast<double*>(A + C * PC);
+  float* beta = reinterpret_cast<float*>(G + C);
+  const int hv = blockIdx.x % a.d.value_heads, slot = blockIdx.x / a.d.value_heads;
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (len == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, hk = hv / a.group;
+  const long row = a.p.row(s);
+  load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 256);
+  load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 256);
+  const long at = (long)slot * a.d.value_heads + hv;
+  if (wave == 0) {
+    float g = 0.f, b = 0.f;
+    if (lane < len) {
+      g = a.d.g[row * a.d.g_st.bs + (t0 + lane) * a.d.g_st.rs + hv * a.d.g_st.cs];
+      b = a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs];
+    }
+    double x = g < G_MIN ? G_MIN : g;
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    G[lane] = x;
+    beta[lane] = b;
+    a.G[at * C + lane] = x;
+  }
+  __syncthreads();
+  // K K^T and Q K^T: wave w the rows 16 w ..
+  for (int j = 0; j < 4; ++j) {
+    f4 n = {0, 0, 0, 0}, p = {0, 0, 0, 0};
+    if (j <= wave) {
+      n = mm<false, true>(K + wave * 16 * PK, PK, K + j * 16 * PK, PK, DK, n);
+      p = mm<false, true>(Q + wave * 16 * PK, PK, K + j * 16 * PK, PK, DK, p);
+    }
+    const int c = j * 16 + (lane & 15);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = wave * 16 + (lane >> 4) * 4 + e;
+      const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
+      A[r * PC + c] = r > c ? n[e] * D * beta[c] : 0.f;
+      a.P[at * C * C + r * C + c] = r >= c ? p[e] * D : 0.f;
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {   // T = (I + A)^-1, lane c its column c
+    float x[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      float v = i == lane ? 1.f : 0.f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) v = fmaf(-A[i * PC + l], x[l], v);
+      x[i] = v;
+      a.T[at * C * C + i * C + lane] = v;
+    }
+  }
+}
+
+// ---- scan: one slice of dv of one value head of one sequence ----------------------------------------------------------
+// Slices of a head read the same keys: blocks with equal id % 8 share an XCD and its L2.
+__device__ __forceinline__ bool scan_coords(unsigned id, int slices, int heads, int& slice, int& head) {
+  const unsigned per = 8u * slices;
+  head = (int)(id / per * 8 + id % 8);
+  slice = (int)(id % per / 8);
+  return head < heads;
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_scan_kernel(const Args a) {
+  constexpr int PK = DK + 4, RT = DK / 64;   // row tiles of S per wave
+  extern __shared__ __align__(16) char smem[];
+  float* K = reinterpret_cast<float*>(smem);
+  float* Q = K + C * PK;
+  float* Tm = Q + C * PK;
+  float* Pm = Tm + C * PC;
+  float* S = Pm + C * PC;        // DK x DVT
+  float* X = S + DK * PV;        // C x DVT, then exp(G_C - G) U
+  float* U = X + C * PV;
+  float* eg = U + C * PV;        // exp(G), exp(G_C - G), beta
+  float* tail = eg + C;
+  float* beta = tail + C;
+  int slice, head;
+  if (!scan_coords(blockIdx.x, a.dvp / DVT, a.p.sequences * a.d.value_heads, slice, head)) return;
+  const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
+  const int c0 = slice * DVT, w = min(DVT, a.d.dv - c0);
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15;
+  const long row = a.p.row(s);
+  const int begin = a.p.begin(s), end = a.p.end(s);
+  f4 acc[RT][2];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
+        acc[i][j][e] = a.state != nullptr && r < a.d.dk && c < w ? a.state[((long)head * a.d.dk + r) * a.d.dv + c0 + c] : 0.f;
+      }
+  for (int t0 = begin, slot = a.p.slot0(s); t0 < end; t0 += C, ++slot) {
+    const int len = min(C, end - t0);
+    const long at = (long)slot * a.d.value_heads + hv;
+    load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 256);
+    load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 256);
+    load_rows<T, DVT>(X, PV, a.d.v, a.d.v_st, row, t0, len, hv, c0, w, 256);
+    for (int i = t; i < C * C; i += 256) {
+      Tm[(i >> 6) * PC + (i & 63)] = a.T[at * C * C + i];
+      Pm[(i >> 6) * PC + (i & 63)] = a.P[at * C * C + i];
+    }
+    const double last = a.G[at * C + C - 1];
+    if (wave == 0) {
+      const double g = a.G[at * C + lane];
+      eg[lane] = expf((float)g);
+      tail[lane] = expf((float)(last - g));
+      beta[lane] = lane < len ? a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
+          S[r * PV + c] = acc[i][j][e];
+          if (a.save && r < a.d.dk) a.S[(at * a.d.dk + r) * a.dvp + c0 + c] = acc[i][j][e];
+        }
+    __syncthreads();
+    f4 o[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f4 zero = {0, 0, 0, 0};
+      const f4 ks = mm<false, false>(K + wave * 16 * PK, PK, S + j * 16, PV, DK, zero);
+      o[j] = mm<false, false>(Q + wave * 16 * PK, PK, S + j * 16, PV, DK, zero);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = wave * 16 + r4 + e;
+        X[r * PV + j * 16 + col] -= eg[r] * ks[e];
+        o[j][e] *= eg[r];
+      }
+    }
+    __syncthreads();
+    f4 ev[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f4 zero = {0, 0, 0, 0};
+      ev[j] = mm<false, false>(Tm + wave * 16 * PC, PC, X + j * 16, PV, 16 * wave + 16, zero);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = wave * 16 + r4 + e, c = j * 16 + col;
+        const float u = beta[r] * ev[j][e];
+        U[r * PV + c] = u;
+        X[r * PV + c] = tail[r] * u;
+        if (a.save) a.E[(at * C + r) * a.dvp + c0 + c] = ev[j][e];
+      }
+    __syncthreads();
+    const float keep = expf((float)last);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      o[j] = mm<false, false>(Pm + wave * 16 * PC, PC, U + j * 16, PV, 16 * wave + 16, o[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = wave * 16 + r4 + e, c = j * 16 + col;
+        if (r < len && c < w)
+          st<T>(a.o, ((row * a.d.tokens + t0 + r) * a.d.value_heads + hv) * (long)a.d.dv + c0 + c, a.scale * o[j][e]);
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        acc[i][j] *= keep;
+        acc[i][j] = mm<true, false>(K + (wave * RT + i) * 16, PK, X + j * 16, PV, C, acc[i][j]);
+      }
+    }
+    __syncthreads();
+  }
+  if (a.state_out != nullptr) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
+          if (r < a.d.dk && c < w) a.state_out[((long)head * a.d.dk + r) * a.d.dv + c0 + c] = acc[i][j][e];
+        }
+  }
+}
+
+// ---- reverse scan: dS from the last chunk to the first ---------------------------------------------------------------
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_back_kernel(const Args a) {
+  constexpr int PK = DK + 4, RT = DK / 64;
+  extern __shared__ __align__(16) char smem[];
+  float* K = reinterpret_cast<float*>(smem);
+  float* Q = K + C * PK;
+  float* Tm = Q + C * PK;
+  float* Pm = Tm + C * PC;
+  float* S = Pm + C * PC;        // dS', DK x DVT
+  float* Y = S + DK * PV;        // dO, then scale exp(G) dO
+  float* Z = Y + C * PV;         // beta dU, then exp(G) dX
+  float* eg = Z + C * PV;
+  float* tail = eg + C;
+  float* beta = tail + C;
+  int slice, head;
+  if (!scan_coords(blockIdx.x, a.dvp / DVT, a.p.sequences * a.d.value_heads, slice, head)) return;
+  const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
+  const int c0 = slice * DVT, w = min(DVT, a.d.dv - c0);
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15;
+  const long row = a.p.row(s);
+  const int begin = a.p.begin(s), end = a.p.end(s), chunks = (end - begin + C - 1) / C;
+  f4 acc[RT][2];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
+        acc[i][j][e] =
+            a.d_state_out != nullptr && r < a.d.dk && c < w ? a.d_state_out[((long)head * a.d.dk + r) * a.d.dv + c0 + c] : 0.f;
+      }
+  for (int n = chunks - 1; n >= 0; --n) {
+    const int t0 = begin + n * C, slot = a.p.slot0(s) + n, len = min(C, end - t0);
+    const long at = (long)slot * a.d.value_heads + hv;
+    load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 256);
+    load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 256);
+    load_rows<T, DVT>(Y, PV, a.d_o, a.do_st, row, t0, len, hv, c0, w, 256);
+    for (int i = t; i < C * C; i += 256) {
+      Tm[(i >> 6) * PC + (i & 63)] = a.T[at * C * C + i];
+      Pm[(i >> 6) * PC + (i & 63)] = a.P[at * C * C + i];
+    }
+    const double last = a.G[at * C + C - 1];
+    if (wave == 0) {
+      const double g = a.G[at * C + lane];
+      eg[lane] = expf((float)g);
+      tail[lane] = expf((float)(last - g));
+      beta[lane] = lane < len ? a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
+          S[r * PV + c] = acc[i][j][e];
+          if (r < a.d.dk) a.dS[(at * a.d.dk + r) * a.dvp + c0 + c] = acc[i][j][e];
+        }
+    __syncthreads();
+    float dots[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f4 zero = {0, 0, 0, 0};
+      const f4 kd = mm<false, false>(K + wave * 16 * PK, PK, S + j * 16, PV, DK, zero);
+      // P^T dO: rows of P from this row block on
+      const f4 po = mm<true, false>(Pm + wave * 16 * PC + wave * 16, PC, Y + wave * 16 * PV + j * 16, PV, C - 16 * wave, zero);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = wave * 16 + r4 + e, c = j * 16 + col;
+        const float du = a.scale * po[e] + tail[r] * kd[e];
+        Z[r * PV + c] = beta[r] * du;
+        dots[e] = fmaf(a.E[(at * C + r) * a.dvp + c0 + c], du, dots[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {   // E . dU of this slice, per row
+      for (int m = 1; m < 16; m <<= 1) dots[e] += __shfl_xor(dots[e], m);
+      if (col == 0) a.part[(at * (a.dvp / DVT) + slice) * C + wave * 16 + r4 + e] = dots[e];
+    }
+    __syncthreads();
+    f4 dx[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f4 zero = {0, 0, 0, 0};
+      dx[j] = mm<true, false>(Tm + wave * 16 * PC + wave * 16, PC, Z + wave * 16 * PV + j * 16, PV, C - 16 * wave, zero);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = wave * 16 + r4 + e, c = j * 16 + col;
+        a.dX[(at * C + r) * a.dvp + c0 + c] = dx[j][e];
+        Z[r * PV + c] = -eg[r] * dx[j][e];
+        Y[r * PV + c] *= a.scale * eg[r];
+      }
+    __syncthreads();
+    const float keep = expf((float)last);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[i][j] *= keep;
+        acc[i][j] = mm<true, false>(Q + (wave * RT + i) * 16, PK, Y + j * 16, PV, C, acc[i][j]);
+        acc[i][j] = mm<true, false>(K + (wave * RT + i) * 16, PK, Z + j * 16, PV, C, acc[i][j]);
+      }
+    __syncthreads();
+  }
+  if (a.d_state != nullptr) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
+          if (r < a.d.dk && c < w) a.d_state[((long)head * a.d.dk + r) * a.d.dv + c0 + c] = acc[i][j][e];
+        }
+  }
+}
+
+// ---- grads: one chunk of one key head, its value heads one after the other ------------------------------------------
+// 8 waves.  Products with C rows and DK columns: wave w the 16 rows of block w & 3 and the columns of half w >> 2.
+template <typename T, int DK>
+__global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
+  constexpr int PK = DK + 4, CT = DK / 32;   // column tiles of 16 per wave
+  extern __shared__ __align__(16) char smem[];
+  float* K = reinterpret_cast<float*>(smem);
+  float* Q = K + C * PK;
+  float* S = Q + C * PK;         // slices of S and dS', later M1 and M2 (C x C)
+  float* dS = S + DK * PV;
+  float* E = dS + DK * PV;       // slices of E, dX, dO, U
+  float* dX = E + C * PV;
+  float* Y = dX + C * PV;
+  float* U = Y + C * PV;
+  double* G = reinterpret_cast<double*>(U + C * PV);
+  float* beta = reinterpret_cast<float*>(G + C);
+  float* dG = beta + C;          // 2 x C: the two column halves
+  float* colb = dG + 2 * C;      // dbeta's sums over the rows, one per wave row block (4 x C)
+  float* red = colb + 4 * C;     // 8 + 1
+  float* M1 = S;
+  float* M2 = M1 + C * PC;
+  static_assert(2 * C * PC <= 2 * DK * PV + 4 * C * PV, "M1 and M2 lie over the slices");
+  const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (len == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15;
+  const int rb = wave & 3, ch = wave >> 2;   // row block, column half
+  const long row = a.p.row(s);
+  load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 512);
+  load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 512);
+  f4 dq[CT], dk[CT];   // over the value heads
+#pragma unroll
+  for (int j = 0; j < CT; ++j) dq[j] = dk[j] = f4{0, 0, 0, 0};
+  for (int m = 0; m < a.group; ++m) {
+    const int hv = hk * a.group + m;
+    const long at = (long)slot * a.d.value_heads + hv;
+    if (wave == 0) {
+      G[lane] = a.G[at * C + lane];
+      beta[lane] = lane < len ? a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs] : 0.f;
+    }
+    f4 q1[CT], kr[CT], kc[CT], dp[2], da[2];
+#pragma unroll
+    for (int j = 0; j < CT; ++j) q1[j] = kr[j] = kc[j] = f4{0, 0, 0, 0};
+    dp[0] = dp[1] = da[0] = da[1] = f4{0, 0, 0, 0};
+    float ss = 0.f;
+    for (int c0 = 0; c0 < a.dvp; c0 += DVT) {
+      const int w = min(DVT, a.d.dv - c0);
+      __syncthreads();
+      for (int i = t; i < DK * DVT; i += 512) {
+        const int r = i / DVT, c = i % DVT;
+        const long p = (at * a.d.dk + r) * a.dvp + c0 + c;
+        const float x = r < a.d.dk ? a.S[p] : 0.f, y = r < a.d.dk ? a.dS[p] : 0.f;
+        S[r * PV + c] = x;
+        dS[r * PV + c] = y;
+        ss = fmaf(x, y, ss);
+      }
+      for (int i = t; i < C * DVT; i += 512) {
+        const int r = i / DVT, c = i % DVT;
+        const long p = (at * C + r) * a.dvp + c0 + c;
+        const float e = a.E[p], x = a.dX[p];
+        E[r * PV + c] = e;
+        U[r * PV + c] = beta[r] * e;
+        dX[r * PV + c] = x;
+        if (r < len && c < w) st<T>(a.d_v, ((row * a.d.tokens + t0 + r) * a.d.value_heads + hv) * (long)a.d.dv + c0 + c, x);
+      }
+      load_rows<T, DVT>(Y, PV, a.d_o, a.do_st, row, t0, len, hv, c0, w, 512);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int cb = ch * 2 + j;
+        if (cb <= rb) {
+          dp[j] = mm<false, true>(Y + rb * 16 * PV, PV, U + cb * 16 * PV, PV, DVT, dp[j]);
+          da[j] = mm<false, true>(dX + rb * 16 * PV, PV, E + cb * 16 * PV, PV, DVT, da[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const int cb = (ch * CT + j) * 16;
+        q1[j] = mm<false, true>(Y + rb * 16 * PV, PV, S + cb * PV, PV, DVT, q1[j]);
+        kr[j] = mm<false, true>(dX + rb * 16 * PV, PV, S + cb * PV, PV, DVT, kr[j]);
+        kc[j] = mm<false, true>(U + rb * 16 * PV, PV, dS + cb * PV, PV, DVT, kc[j]);
+      }
+    }
+    __syncthreads();   // the slices are done with: M1 and M2 take their place
+    const double last = G[C - 1];
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_down(ss, o);
+    if (lane == 0) red[wave] = ss;
+    float cj[4] = {0, 0, 0, 0};   // k . state part of dKc
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 16 + r4 + e, c = (ch * CT + j) * 16 + col;
+        const float eg = expf((float)G[r]);
+        q1[j][e] *= a.scale * eg;
+        kr[j][e] *= -eg;
+        kc[j][e] *= expf((float)(last - G[r]));
+        cj[e] = fmaf(K[r * PK + c], kc[j][e], cj[e]);
+      }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int cb = ch * 2 + j;
+      f4 kk = {0, 0, 0, 0};
+      if (cb <= rb) kk = mm<false, true>(K + rb * 16 * PK, PK, K + cb * 16 * PK, PK, DK, kk);
+      const int c = cb * 16 + col;
+      float db = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 16 + r4 + e;
+        const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
+        M1[r * PC + c] = r >= c ? a.scale * dp[j][e] * D : 0.f;
+        M2[r * PC + c] = r > c ? -da[j][e] * beta[c] * D : 0.f;
+        db -= r > c ? da[j][e] * kk[e] * D : 0.f;
+      }
+      db += __shfl_xor(db, 16);
+      db += __shfl_xor(db, 32);
+      if (lane < 16) colb[rb * C + c] = db;
+    }
+    __syncthreads();
+    float dg[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const int cb = (ch * CT + j) * 16;
+      q1[j] = mm<false, false>(M1 + rb * 16 * PC, PC, K + cb, PK, 16 * rb + 16, q1[j]);
+      kr[j] = mm<false, false>(M2 + rb * 16 * PC, PC, K + cb, PK, 16 * rb + 16, kr[j]);
+      kc[j] = mm<true, false>(M2 + rb * 16 * PC + rb * 16, PC, K + rb * 16 * PK + cb, PK, C - 16 * rb, kc[j]);
+      kc[j] = mm<true, false>(M1 + rb * 16 * PC + rb * 16, PC, Q + rb * 16 * PK + cb, PK, C - 16 * rb, kc[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 16 + r4 + e, c = cb + col;
+        dg[e] = fmaf(Q[r * PK + c], q1[j][e], fmaf(K[r * PK + c], kr[j][e] - kc[j][e], dg[e]));
+      }
+      dq[j] += q1[j];
+      dk[j] += kr[j] + kc[j];
+    }
+    float csum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      csum += cj[e];
+      for (int o = 1; o < 16; o <<= 1) dg[e] += __shfl_xor(dg[e], o);
+      if (col == 0) dG[ch * C + rb * 16 + r4 + e] = dg[e];
+    }
+    for (int o = 32; o > 0; o >>= 1) csum += __shfl_down(csum, o);
+    __syncthreads();
+    if (lane == 0) red[wave] = fmaf(expf((float)last), red[wave], csum);
+    __syncthreads();
+    if (wave == 0) {
+      float end = 0.f;
+      for (int i = 0; i < 8; ++i) end += red[i];
+      float v = dG[lane] + dG[C + lane] + (lane == C - 1 ? end : 0.f);
+      for (int o = 1; o < 64; o <<= 1) {
+        const float u = __shfl_down(v, o);
+        if (lane + o < 64) v += u;
+      }
+      if (lane < len) {
+        const long p = (row * a.d.tokens + t0 + lane) * a.d.value_heads + hv;
+        a.d_g[p] = v;
+        float b = (colb[lane] + colb[C + lane]) + (colb[2 * C + lane] + colb[3 * C + lane]);
+        const float* part = a.part + at * (a.dvp / DVT) * C + lane;
+        for (int i = 0; i < a.dvp / DVT; ++i) b += part[i * C];
+        a.d_beta[p] = b;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < CT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = rb * 16 + r4 + e, c = (ch * CT + j) * 16 + col;
+      if (r < len && c < a.d.dk) {
+        const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + c;
+        st<T>(a.d_q, p, dq[j][e]);
+        st<T>(a.d_k, p, dk[j][e]);
+      }
+    }
+}
+
+// ---- the recurrence itself ---------------------------------------------------------------------------------------------
+// 64 columns of a state per workgroup: thread = 4 columns x RPT rows, in registers for all of its tokens.  One
+// reduction per token, since o = scale (q^T Sbar + (q . k) beta e).
+struct StepArgs {
+  Args a;
+  const int* slot;   // step: the state of each row
+  int slots;
+  int step;
+};
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_recurrent_kernel(const StepArgs x) {
+  constexpr int RPT = DK / 16;
+  const Args& a = x.a;
+  __shared__ float sm[2][4][2][64];   // parity, wave, k S / q S, column
+  __shared__ float qk[2][2][DK];      // parity, k / q
+  const int slices = (a.d.dv + 63) / 64, heads = a.d.value_heads;
+  const int slice = blockIdx.x % slices, hv = blockIdx.x / slices % heads, s = blockIdx.x / slices / heads;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, hk = hv / a.group;
+  const int cc = (lane & 15) * 4, c0 = slice * 64 + cc, r0 = (wave * 4 + (lane >> 4)) * RPT;
+  const bool vec = (a.d.dv & 3) == 0;   // rows of states are 16-byte aligned
+  int own = s, tok, end;
+  long row = 0;
+  if (x.step) {
+    if (x.slot != nullptr) {
+      own = x.slot[s];
+      if (own < 0 || own >= x.slots) return;
+      bool first = true;   // an earlier row of this slot takes this one too
+      for (int b = 0; b < s; b += 64) first = first && !__any(b + lane < s && x.slot[b + lane] == own);
+      if (!first) return;
+    }
+    tok = s;
+    end = a.d.batch;
+  } else {
+    row = a.p.row(s);
+    tok = a.p.begin(s);
+    end = a.p.end(s);
+  }
+  const long base = ((long)own * heads + hv) * a.d.dk * (long)a.d.dv;
+  float S[RPT][4];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = r0 + i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) S[i][j] = 0.f;
+    if (a.state != nullptr && r < a.d.dk) {
+      const float* p = a.state + base + (long)r * a.d.dv + c0;
+      if (vec && c0 < a.d.dv) {
+        const f4 v = *reinterpret_cast<const f4*>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[i][j] = v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c0 + j < a.d.dv) S[i][j] = p[j];
+      }
+    }
+  }
+  for (int par = 0; tok < end; par ^= 1) {
+    // element offsets of this token: rows are the batch when stepping
+    const long br = x.step ? tok : row, tr = x.step ? 0 : tok;
+    for (int i = t; i < 2 * DK; i += 256) {
+      const int c = i % DK;
+      float v = 0.f;
+      if (c < a.d.dk)
+        v = i < DK ? ld<T>(a.d.k, br * a.d.k_st.bs + tr * a.d.k_st.rs + hk * a.d.k_st.cs + c)
+                   : ld<T>(a.d.q, br * a.d.q_st.bs + tr * a.d.q_st.rs + hk * a.d.q_st.cs + c);
+      qk[par][i / DK][c] = v;
+    }
+    const float decay = expf(a.d.g[br * a.d.g_st.bs + tr * a.d.g_st.rs + hv * a.d.g_st.cs]);
+    const float beta = a.d.beta[br * a.d.beta_st.bs + tr * a.d.beta_st.rs + hv * a.d.beta_st.cs];
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = c0 + j < a.d.dv ? ld<T>(a.d.v, br * a.d.v_st.bs + tr * a.d.v_st.rs + hv * a.d.v_st.cs + c0 + j) : 0.f;
+    __syncthreads();
+    float ks[4] = {0, 0, 0, 0}, qs[4] = {0, 0, 0, 0}, dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const float kv = qk[par][0][r0 + i], qv = qk[par][1][r0 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        S[i][j] *= decay;
+        ks[j] = fmaf(kv, S[i][j], ks[j]);
+        qs[j] = fmaf(qv, S[i][j], qs[j]);
+      }
+    }
+    for (int i = lane; i < DK; i += 64) dot = fmaf(qk[par][0][i], qk[par][1][i], dot);
+    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ks[j] += __shfl_xor(ks[j], 16);
+      qs[j] += __shfl_xor(qs[j], 16);
+      ks[j] += __shfl_xor(ks[j], 32);
+      qs[j] += __shfl_xor(qs[j], 32);
+      if (lane < 16) {
+        sm[par][wave][0][cc + j] = ks[j];
+        sm[par][wave][1][cc + j] = qs[j];
+      }
+    }
+    __syncthreads();
+    float u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float k4 = (sm[par][0][0][cc + j] + sm[par][1][0][cc + j]) + (sm[par][2][0][cc + j] + sm[par][3][0][cc + j]);
+      u[j] = beta * (v[j] - k4);
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const float kv = qk[par][0][r0 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[i][j] = fmaf(kv, u[j], S[i][j]);
+    }
+    if (t < 16) {
+      const long p = (x.step ? ((long)tok * heads + hv) : ((row * a.d.tokens + tok) * heads + hv)) * (long)a.d.dv + c0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float q4 = (sm[par][0][1][cc + j] + sm[par][1][1][cc + j]) + (sm[par][2][1][cc + j] + sm[par][3][1][cc + j]);
+        if (c0 + j < a.d.dv) st<T>(a.o, p + j, a.scale * fmaf(dot, u[j], q4));
+      }
+    }
+    if (!x.step) {
+      ++tok;
+    } else if (x.slot == nullptr) {
+      break;
+    } else {   // the next row of the same slot
+      int next = end;
+      for (int b = tok + 1; b < end && next == end; b += 64) {
+        const unsigned long long hit = __ballot(b + lane < end && x.slot[min(b + lane, end - 1)] == own);
+        if (hit) next = b + __ffsll(hit) - 1;
+      }
+      tok = next;
+    }
+  }
+  if (a.state_out == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = r0 + i;
+    if (r >= a.d.dk) continue;
+    float* p = a.state_out + base + (long)r * a.d.dv + c0;
+    if (vec && c0 < a.d.dv) {
+      *reinterpret_cast<f4*>(p) = f4{S[i][0], S[i][1], S[i][2], S[i][3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c0 + j < a.d.dv) p[j] = S[i][j];
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+constexpr int RECURRENT_MAX = 16;   // longest input (tokens per row, or packed tokens) that takes the recurrence
+
+int sequences_of(const gpx_delta* d) { return d->sequences > 0 ? d->sequences : d->batch; }
+long slots_of(const gpx_delta* d) {
+  return d->sequences > 0 ? d->tokens / C + (long)d->sequences : (long)d->batch * ((d->tokens + C - 1) / C);
+}
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Parts of a workspace, in this order (use 0: forward, 1: forward that saves, 2: scratch of backward); nullptr base:
+// sizes only.
+size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
+  const size_t heads = (size_t)slots_of(d) * d->value_heads, dvp = (size_t)(d->dv + DVT - 1) / DVT * DVT;
+  size_t at = 0;
+  auto part = [&](size_t bytes) {
+    char* p = base == nullptr ? nullptr : base + at;
+    at += up256(bytes);
+    return p;
+  };
+  Args dummy;
+  Args& x = a != nullptr ? *a : dummy;
+  if (use < 2) {
+    char* p = part(d->sequences > 0 ? (size_t)(d->sequences + 1) * 4 : 0);
+    if (off != nullptr) *off = reinterpret_cast<int*>(p);
+    x.G = reinterpret_cast<double*>(part(heads * C * 8));
+    x.T = reinterpret_cast<float*>(part(heads * C * C * 4));
+    x.P = reinterpret_cast<float*>(part(heads * C * C * 4));
+  }
+  if (use == 1) {
+    x.E = reinterpret_cast<float*>(part(heads * C * dvp * 4));
+    x.S = reinterpret_cast<float*>(part(heads * d->dk * dvp * 4));
+  }
+  if (use == 2) {
+    x.dX = reinterpret_cast<float*>(part(heads * C * dvp * 4));
+    x.dS = reinterpret_cast<float*>(part(heads * d->dk * dvp * 4));
+    x.part = reinterpret_cast<float*>(part(heads * (dvp / DVT) * C * 4));
+  }
+  return at;
+}
+
+bool recurrent(const gpx_delta* d, int save) { return !save && d->tokens <= RECURRENT_MAX; }
+
+int check_delta(const gpx_delta* d, const char* what) {
+  GPX_REQUIRE(d != nullptr, "%s: null description", what);
+  GPX_REQUIRE(d->dtype == GPX_F32 || d->dtype == GPX_F16 || d->dtype == GPX_BF16, "%s: unknown element type %d", what, d->dtype);
+  GPX_REQUIRE(d->batch >= 0 && d->tokens >= 0 && d->sequences >= 0, "%s: negative size", what);
+  GPX_REQUIRE(d->key_heads >= 1 && d->value_heads >= 1 && d->value_heads % d->key_heads == 0,
+              "%s: %d value heads are not a multiple of %d key heads", what, d->value_heads, d->key_heads);
+  GPX_REQUIRE(d->dk >= 1 && d->dk <= 128, "%s: dk = %d is outside [1, 128]", what, d->dk);
+  GPX_REQUIRE(d->dv >= 1 && d->dv <= 1024, "%s: dv = %d is outside [1, 1024]", what, d->dv);
+  GPX_REQUIRE(d->tokens <= (1 << 30) && d->batch <= (1 << 24) && d->sequences <= (1 << 24), "%s: size out of range", what);
+  GPX_REQUIRE(d->sequences == 0 || (d->batch == 1 && d->offsets != nullptr), "%s: packed sequences need batch == 1 and offsets", what);
+  GPX_REQUIRE(std::isfinite(d->scale), "%s: scale is not finite", what);
+  // blocks of a launch: 32 bits, with room
+  const double heads = (double)std::max<long>(slots_of(d), sequences_of(d)) * d->value_heads;
+  GPX_REQUIRE(heads * 40 < 2.0e9, "%s: too many heads and chunks for one call", what);
+  for (const gpx_strided* s : {&d->q_st, &d->k_st, &d->v_st, &d->g_st, &d->beta_st})
+    GPX_REQUIRE(s->bs >= 0 && s->rs >= 0 && s->cs >= 0, "%s: negative stride", what);
+  if (d->batch > 0 && d->tokens > 0)
+    GPX_REQUIRE(d->q && d->k && d->v && d->g && d->beta, "%s: null input", what);
+  return 0;
+}
+
+Args make_args(const gpx_delta* d) {
+  Args a = {};
+  a.d = *d;
+  a.group = d->value_heads / d->key_heads;
+  a.dvp = (d->dv + DVT - 1) / DVT * DVT;
+  a.scale = (float)d->scale;
+  a.p.sequences = sequences_of(d);
+  a.p.tokens = d->tokens;
+  a.p.batch = d->batch;
+  a.p.chunks_per_row = (d->tokens + C - 1) / C;
+  a.p.off = nullptr;
+  return a;
+}
+
+template <typename F>
+int allow_lds(F* kernel, size_t bytes) {
+  GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return 0;
+}
+
+#define DELTA_TRY(expr)       \
+  do {                        \
+    int rc_ = (expr);         \
+    if (rc_ != 0) return rc_; \
+  } while (0)
+
+unsigned scan_grid(const Args& a) {
+  const unsigned heads = (unsigned)a.p.sequences * a.d.value_heads, slices = a.dvp / DVT;
+  return (heads + 7) / 8 * 8 * slices;
+}
+
+template <typename T, int DK>
+int run_forward(hipStream_t s, const Args& a, int rec) {
+  if (rec) {
+    StepArgs x = {a, nullptr, 0, 0};
+    const unsigned grid = (unsigned)a.p.sequences * a.d.value_heads * ((a.d.dv + 63) / 64);
+    hipLaunchKernelGGL((delta_recurrent_kernel<T, DK>), dim3(grid), dim3(256), 0, s, x);
+    GPX_HIP(hipGetLastError());
+    return 0;
+  }
+  constexpr size_t prep = (2 * C * (DK + 4) + C * PC) * 4 + C * 8 + C * 4;
+  constexpr size_t scan = (2 * C * (DK + 4) + 2 * C * PC + DK * PV + 2 * C * PV + 3 * C) * 4;
+  static_assert(scan <= 160 * 1024, "LDS");
+  DELTA_TRY(allow_lds(&delta_prep_kernel<T, DK>, prep));
+  DELTA_TRY(allow_lds(&delta_scan_kernel<T, DK>, scan));
+  const unsigned n = (unsigned)(slots_of(&a.d) * a.d.value_heads);
+  if (n > 0) {
+    hipLaunchKernelGGL((delta_prep_kernel<T, DK>), dim3(n), dim3(256), prep, s, a);
+    GPX_HIP(hipGetLastError());
+  }
+  hipLaunchKernelGGL((delta_scan_kernel<T, DK>), dim3(scan_grid(a)), dim3(256), scan, s, a);
+  GPX_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T, int DK>
+int run_backward(hipStream_t s, const Args& a) {
+  constexpr size_t back = (2 * C * (DK + 4) + 2 * C * PC + DK * PV + 2 * C * PV + 3 * C) * 4;
+  constexpr size_t grads = (2 * C * (DK + 4) + 2 * DK * PV + 4 * C * PV) * 4 + C * 8 + (C + 2 * C + 4 * C + 16) * 4;
+  static_assert(grads <= 160 * 1024, "LDS");
+  DELTA_TRY(allow_lds(&delta_back_kernel<T, DK>, back));
+  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK>, grads));
+  hipLaunchKernelGGL((delta_back_kernel<T, DK>), dim3(scan_grid(a)), dim3(256), back, s, a);
+  GPX_HIP(hipGetLastError());
+  const unsigned n = (unsigned)(slots_of(&a.d) * a.d.key_heads);
+  if (n > 0) {
+    hipLaunchKernelGGL((delta_grads_kernel<T, DK>), dim3(n), dim3(512), grads, s, a);
+    GPX_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+#define DELTA_DISPATCH(fn, ...)                                                                             \
+  (a.d.dk <= 64 ? (a.d.dtype == GPX_F32   ? fn<float, 64>(__VA_ARGS__)                                       \
+                   : a.d.dtype == GPX_F16 ? fn<_Float16, 64>(__VA_ARGS__)                                    \
+                                          : fn<__bf16, 64>(__VA_ARGS__))                                     \
+                : (a.d.dtype == GPX_F32   ? fn<float, 128>(__VA_ARGS__)                                      \
+                   : a.d.dtype == GPX_F16 ? fn<_Float16, 128>(__VA_ARGS__)                                   \
+                                          : fn<__bf16, 128>(__VA_ARGS__)))
+
+template <typename T, int DK>
+int run_step(hipStream_t s, const Args& a, int slots, const int* slot) {
+  StepArgs x = {a, slot, slots, 1};
+  const unsigned grid = (unsigned)a.d.batch * a.d.value_heads * ((a.d.dv + 63) / 64);
+  hipLaunchKernelGGL((delta_recurrent_kernel<T, DK>), dim3(grid), dim3(256), 0, s, x);
+  GPX_HIP(hipGetLastError());
+  return 0;
+}
+
+int plan(hipStream_t s, const gpx_delta* d, Args& a, int* off) {
+  if (d->sequences == 0) return 0;
+  hipLaunchKernelGGL(delta_plan_kernel, dim3(1), dim3(64), 0, s, d->offsets, d->sequences + 1, d->tokens, off);
+  GPX_HIP(hipGetLastError());
+  a.p.off = off;
+  return 0;
+}
+
+int check_work(const gpx_delta* d, int use, const void* work, size_t work_bytes, const char* what) {
+  const size_t need = lay_out(d, use, nullptr, nullptr, nullptr);
+  GPX_REQUIRE(need == 0 || (work != nullptr && (reinterpret_cast<uintptr_t>(work) & 255) == 0), "%s: work null or misaligned", what);
+  GPX_REQUIRE(work_bytes >= need, "%s: work holds %zu of %zu bytes", what, work_bytes, need);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gpx_delta_work_bytes(const gpx_delta* d, int use) {
+  if (use < 0 || use > 2 || check_delta(d, "delta_work_bytes") != 0) return 0;
+  return lay_out(d, use, nullptr, nullptr, nullptr);
+}
+
+int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, void* o, float* state_out, int save,
+                      void* work, size_t work_bytes) {
+  GPX_REQUIRE(h != nullptr, "null handle");
+  DELTA_TRY(check_delta(d, "delta_forward"));
+  if (sequences_of(d) == 0) return 0;
+  GPX_REQUIRE(o != nullptr || d->tokens == 0, "delta_forward: null output");
+  GPX_REQUIRE(state == nullptr || gpx_aligned16(state), "delta_forward: state must be 16-byte aligned");
+  GPX_REQUIRE(state_out == nullptr || gpx_aligned16(state_out), "delta_forward: state_out must be 16-byte aligned");
+  save = save != 0;
+  DELTA_TRY(check_work(d, save, work, work_bytes, "delta_forward"));
+  DeviceGuard dg(h->device);
+  Args a = make_args(d);
+  int* off = nullptr;
+  lay_out(d, save, static_cast<char*>(work), &a, &off);
+  DELTA_TRY(plan(h->stream, d, a, off));
+  a.state = state;
+  a.o = o;
+  a.state_out = state_out;
+  a.save = save;
+  const int rec = recurrent(d, save);
+  return DELTA_DISPATCH(run_forward, h->stream, a, rec);
+}
+
+int gpx_delta_backward(gpx_handle* h, const gpx_delta* d, const void* d_o, const gpx_strided* d_o_st, const float* d_state_out,
+                       void* d_q, void* d_k, void* d_v, float* d_g, float* d_beta, float* d_state, const void* saved, size_t saved_bytes,
+                       void* scratch, size_t scratch_bytes) {
+  GPX_REQUIRE(h != nullptr, "null handle");
+  DELTA_TRY(check_delta(d, "delta_backward"));
+  if (sequences_of(d) == 0) return 0;
+  if (d->tokens > 0) {
+    GPX_REQUIRE(d_o != nullptr && d_o_st != nullptr, "delta_backward: null gradient of o");
+    GPX_REQUIRE(d_o_st->bs >= 0 && d_o_st->rs >= 0 && d_o_st->cs >= 0, "delta_backward: negative stride");
+    GPX_REQUIRE(d_q && d_k && d_v && d_g && d_beta, "delta_backward: null output");
+  }
+  DELTA_TRY(check_work(d, 1, saved, saved_bytes, "delta_backward"));
+  DELTA_TRY(check_work(d, 2, scratch, scratch_bytes, "delta_backward"));
+  DeviceGuard dg(h->device);
+  Args a = make_args(d);
+  int* off = nullptr;
+  lay_out(d, 1, static_cast<char*>(const_cast<void*>(saved)), &a, &off);
+  lay_out(d, 2, static_cast<char*>(scratch), &a, nullptr);
+  if (d->sequences > 0) a.p.off = off;   // the forward call's plan
+  a.d_o = d_o;
+  if (d_o_st != nullptr) a.do_st = *d_o_st;
+  a.d_state_out = d_state_out;
+  a.d_q = d_q;
+  a.d_k = d_k;
+  a.d_v = d_v;
+  a.d_g = d_g;
+  a.d_beta = d_beta;
+  a.d_state = d_state;
+  return DELTA_DISPATCH(run_backward, h->stream, a);
+}
+
+int gpx_delta_step(gpx_handle* h, const gpx_delta* d, int slots, const int* slot, const float* state, float* state_out, void* o) {
+  GPX_REQUIRE(h != nullptr, "null handle");
+  DELTA_TRY(check_delta(d, "delta_step"));
+  GPX_REQUIRE(d->tokens == 1 && d->sequences == 0, "delta_step: one token per row");
+  GPX_REQUIRE(slots >= 0 && (slot != nullptr || slots == d->batch), "delta_step: %d states for %d rows", slots, d->batch);
+  if (d->batch == 0) return 0;
+  GPX_REQUIRE(o != nullptr && state_out != nullptr && state != nullptr, "delta_step: null state or output");
+  GPX_REQUIRE(gpx_aligned16(state) && gpx_aligned16(state_out), "delta_step: states must be 16-byte aligned");
+  DeviceGuard dg(h->device);
+  Args a = make_args(d);
+  a.state = state;
+  a.state_out = state_out;
+  a.o = o;
+  return DELTA_DISPATCH(run_step, h->stream, a, slots, slot);
+}
+
+}  // extern "C"

@@ -1,0 +1,216 @@
+"""The gated delta rule on the MI355X (``gpx_delta_*``): regression over a stream.
+
+No counterpart in the reference.  It stands beside the exact GP as its streaming relative: the GP solves
+for all targets at once in O(n^3), this keeps one dk x dv map from keys to values and corrects it by the
+error of every token, in order, while it forgets -- for each sequence and head
+
+    Sbar = exp(g) S;   e = v - Sbar^T k;   S <- Sbar + beta k e^T;   o = scale S^T q
+
+Shapes: q, k (B, T, Hk, dk); v, o (B, T, Hv, dv), Hv a multiple of Hk (value head i reads key head
+i // (Hv // Hk)); g (the LOG of the decay, -inf forgets everything) and beta (B, T, Hv) in float32; states
+(sequences, Hv, dk, dv) in float32.  q, k, v, o: float32, float16 or bfloat16, one type, sums in float32.
+1 <= dk <= 128, 1 <= dv <= 1024, any T.  Any strides; q, k, v with a last dimension that is not dense are copied first.
+
+Gradients are functions of their own, as everywhere in this package: nothing is recorded behind the
+caller's back, so a forward and a backward call may be captured into a graph together."""
+import ctypes as C
+
+from . import _lib
+from .device import ptr, tensor_runtime
+from .orthogonal import check_tensor, type_id
+
+_TYPES = ("float32", "float16", "bfloat16")
+
+
+def _dense(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _st(t):
+    """{batch, token, head} strides; a dimension of one has none."""
+    return _lib.Strided(*(t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)))
+
+
+def _opt(t):
+    return ptr(t) if t is not None else None
+
+
+def _check(q, k, v, g, beta, dims):
+    import torch
+    for name, t, n in (("q", q, dims), ("k", k, dims), ("v", v, dims), ("g", g, dims - 1), ("beta", beta, dims - 1)):
+        check_tensor(t, name)
+        if t.dim() != n:
+            raise ValueError("%s must have %d dimensions" % (name, n))
+    dtype = type_id(q, _TYPES)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must have one type")
+    for name, t in (("g", g), ("beta", beta)):
+        if t.dtype != torch.float32:
+            raise TypeError("%s must be float32" % name)
+    if q.shape != k.shape:
+        raise ValueError("q and k must have the same shape")
+    if v.shape[:-2] != q.shape[:-2] or g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+        raise ValueError("q, k, v, g and beta do not agree in batch, tokens or value heads")
+    Hk, dk = q.shape[-2:]
+    Hv, dv = v.shape[-2:]
+    if Hk < 1 or Hv < 1 or Hv % Hk:
+        raise ValueError("the value heads (%d) must be a multiple of the key heads (%d)" % (Hv, Hk))
+    if not 1 <= dk <= 128 or not 1 <= dv <= 1024:
+        raise ValueError("dk = %d must be in [1, 128], dv = %d in [1, 1024]" % (dk, dv))
+    return dtype
+
+
+def _check_state(t, shape, name, like):
+    import torch
+    if t is None:
+        return None
+    check_tensor(t, name)
+    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must be float32 of shape %s" % (name, tuple(shape)))
+    return t
+
+
+def _aligned(t):
+    """t, or a packed copy where the library's 16-byte accesses to states would not fit."""
+    import torch
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _desc(dtype, q, k, v, g, beta, scale, offsets, sequences):
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2:]
+    return _lib.Delta(dtype, B, T, sequences, Hk, Hv, dk, dv, float(scale), offsets.data_ptr() if offsets is not None else None,
+                      q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _st(q), _st(k), _st(v), _st(g),
+                      _st(beta))
+
+
+def _version(t):
+    return None if t.is_inference() else t._version   # inference tensors do not count their writes
+
+
+class Saved:
+    """What a forward call keeps for its backward call."""
+
+    def __init__(self, desc, inputs, state, work):
+        self.desc, self.inputs, self.has_state, self.work = desc, inputs, state is not None, work
+        self.versions = [_version(t) for t in inputs]
+
+
+def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scale=None, save_for_backward=False):
+    """(o, final_state), and with ``save_for_backward`` also what ``gated_delta_rule_backward`` needs.
+
+    cu_seqlens: None, each batch row is a sequence; or B = 1 and an int32 tensor on the device of n + 1 ends of packed
+    sequences (sequence s is tokens cu_seqlens[s] to cu_seqlens[s + 1]; empty ones pass their state through).  Values
+    outside [0, T] are clamped and a decreasing one is read as the one before it; outputs of tokens that belong
+    to no sequence are zeros.  initial_state: (sequences, Hv, dk, dv) float32, None for zeros.  scale: dk ** -0.5 by default.
+
+    Long inputs run in chunks of 64 tokens on the matrix cores, up to 16 tokens go through the recurrence.  Asynchronous
+    on the current stream; may be captured into a graph after one call outside."""
+    import torch
+    dtype = _check(q, k, v, g, beta, 4)
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2:]
+    sequences = 0
+    if cu_seqlens is not None:
+        check_tensor(cu_seqlens, "cu_seqlens")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise ValueError("cu_seqlens must be a one-dimensional int32 tensor of at least two values")
+        if B != 1:
+            raise ValueError("packed sequences need a batch of one")
+        sequences = cu_seqlens.numel() - 1
+    shape = (sequences or B, Hv, dk, dv)
+    _check_state(initial_state, shape, "initial_state", q)
+    rt = tensor_runtime(q, k, v, g, beta, initial_state, cu_seqlens)
+    with rt.current_stream():
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        if cu_seqlens is not None:
+            cu_seqlens = cu_seqlens.contiguous()
+        state = _aligned(initial_state)
+        d = _desc(dtype, q, k, v, g, beta, dk ** -0.5 if scale is None else scale, cu_seqlens, sequences)
+        o = (torch.zeros if sequences else torch.empty)((B, T, Hv, dv), dtype=q.dtype, device=q.device)
+        final = torch.empty(shape, dtype=torch.float32, device=q.device)
+        save = int(bool(save_for_backward))
+        size = int(rt.lib.gpx_delta_work_bytes(C.byref(d), save))
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
+        _lib.check(rt.lib.gpx_delta_forward(rt.h, C.byref(d), _opt(state), ptr(o), ptr(final), save, ptr(work), size),
+                   "gpx_delta_forward")
+    if not save_for_backward:
+        return o, final
+    inputs = [t for t in (q, k, v, g, beta, cu_seqlens) if t is not None]
+    return o, final, Saved(d, inputs, initial_state, work)
+
+
+def gated_delta_rule_backward(saved, d_o, d_final_state=None):
+    """(d_q, d_k, d_v, d_g, d_beta, d_initial_state) of sum(d_o * o) + sum(d_final_state * final_state).
+
+    ``saved`` comes from the forward call; it is only read, so the call may be repeated with other d_o.  d_q, d_k, d_v have the type of
+    q, k, v, the others float32; d_initial_state is None if the forward call had no initial_state.  Tokens that belong
+    to no sequence get zeros."""
+    import torch
+    if not isinstance(saved, Saved):
+        raise TypeError("saved must come from gated_delta_rule(..., save_for_backward=True)")
+    if [_version(t) for t in saved.inputs] != saved.versions:
+        raise RuntimeError("an input of the forward call has been modified in place since")
+    q, k, v, g, beta = saved.inputs[:5]
+    d = saved.desc
+    check_tensor(d_o, "d_o")
+    if d_o.shape != v.shape or d_o.dtype != v.dtype:
+        raise ValueError("d_o must have the shape and the type of o")
+    shape = (d.sequences or d.batch, d.value_heads, d.dk, d.dv)
+    _check_state(d_final_state, shape, "d_final_state", q)
+    rt = tensor_runtime(q, d_o, d_final_state)
+    with rt.current_stream():
+        d_o, d_final = _dense(d_o), _aligned(d_final_state)
+        new = torch.zeros if d.sequences else torch.empty
+        grads = [new(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]
+        d_state = torch.empty(shape, dtype=torch.float32, device=q.device) if saved.has_state else None
+        size = int(rt.lib.gpx_delta_work_bytes(C.byref(d), 2))
+        scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
+        st = _st(d_o)
+        _lib.check(rt.lib.gpx_delta_backward(rt.h, C.byref(d), ptr(d_o), C.byref(st), _opt(d_final), *map(ptr, grads), _opt(d_state),
+                                             ptr(saved.work), saved.work.numel(), ptr(scratch), size), "gpx_delta_backward")
+    return (*grads, d_state)
+
+
+def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, scale=None):
+    """One token for each of B rows: q, k (B, Hk, dk); v (B, Hv, dv); g, beta (B, Hv).  Returns (o, state_out).
+
+    state: (n, Hv, dk, dv) float32, packed, n = B unless ``slots`` names the state of each row (int32 tensor on the device).
+    It is updated in place unless ``state_out`` (its shape, no other view of its memory) is given.  A row whose slot
+    is outside [0, n) is padding: its o is zero and no state is written for it; states that no row names are not touched.  Rows with
+    the same slot are taken in their order, as successive tokens of one sequence."""
+    import torch
+    dtype = _check(q, k, v, g, beta, 3)
+    B, Hk, dk = q.shape
+    Hv, dv = v.shape[1:]
+    check_tensor(state, "state")
+    n = state.shape[0] if state.dim() else 0
+    _check_state(state, (n, Hv, dk, dv), "state", q)
+    if slots is None:
+        if n != B:
+            raise ValueError("%d states for %d rows: name them with slots" % (n, B))
+    else:
+        check_tensor(slots, "slots")
+        if slots.dtype != torch.int32 or tuple(slots.shape) != (B,):
+            raise ValueError("slots must be an int32 tensor with one value per row")
+    if state_out is None:
+        state_out = state
+    _check_state(state_out, state.shape, "state_out", q)
+    for name, t in (("state", state), ("state_out", state_out)):
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError("%s must be packed and 16-byte aligned" % name)
+    if state_out.data_ptr() != state.data_ptr() and state.numel():
+        gap = abs(state_out.data_ptr() - state.data_ptr())
+        if gap < state.numel() * 4:
+            raise ValueError("state_out overlaps state")
+    rt = tensor_runtime(q, k, v, g, beta, state, slots, state_out)
+    with rt.current_stream():
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        if slots is not None:
+            slots = slots.contiguous()
+        o = (torch.empty if slots is None else torch.zeros)((B, Hv, dv), dtype=q.dtype, device=q.device)
+        d = _desc(dtype, *(t.unsqueeze(1) for t in (q, k, v, g, beta)), dk ** -0.5 if scale is None else scale, None, 0)
+        _lib.check(rt.lib.gpx_delta_step(rt.h, C.byref(d), n, _opt(slots), ptr(state), ptr(state_out), ptr(o)), "gpx_delta_step")
+    return o, state_out

@@ -303,6 +303,52 @@ int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const v
                       const gpx_strided* base_st, void* out, const gpx_strided* out_st, void* work, size_t work_bytes);
 size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m);
 
+/* ---- the gated delta rule: regression over a stream ---------------------------------------- */
+/* A state S (dk x dv) per sequence and value head maps keys to values; every token fades it and makes one gradient
+ * step of |v - S^T k|^2 / 2 with rate beta:
+ *   Sbar = exp(g) S;   e = v - Sbar^T k;   S <- Sbar + beta k e^T;   o = scale S^T q
+ * -- the rank-one updates in strict order of gpx_ep_sweep, with a matrix that forgets.  No counterpart in the reference.
+ *   q, k: batch x tokens x key_heads x dk;   v, o: batch x tokens x value_heads x dv   (dtype: GPX_F32, GPX_F16, GPX_BF16)
+ *   g (log decay), beta: batch x tokens x value_heads in fp32;   states: sequences x value_heads x dk x dv in fp32
+ * value_heads is a multiple of key_heads; value head i reads key head i / (value_heads / key_heads).  Element
+ * (b, t, h, c) of an input lies at b * bs + t * rs + h * cs + c (strides in elements, not negative).  Outputs and
+ * states are packed in the order written above.
+ * sequences == 0: every batch row is a sequence.  sequences > 0: batch == 1 and the tokens are packed sequences,
+ * offsets[s] .. offsets[s + 1] (sequences + 1 values in DEVICE memory, not decreasing; values outside [0, tokens] are
+ * clamped, a decreasing value is read as the one before it).  Tokens behind the last sequence or before the first are
+ * not read and their outputs not written.  Sequences may be empty: their state passes through.
+ * g may be -infinity (the state is forgotten).  beta == 0 and g == 0 leave the state as it is.  1 <= dk <= 128,
+ * 1 <= dv <= 1024.  States, decays and all sums are fp32 or wider. */
+typedef struct gpx_delta {
+  int dtype, batch, tokens, sequences, key_heads, value_heads, dk, dv;
+  double scale;
+  const int* offsets;
+  const void *q, *k, *v;
+  const float *g, *beta;
+  gpx_strided q_st, k_st, v_st, g_st, beta_st; /* {batch, token, head} */
+} gpx_delta;
+/* Device bytes of gpx_delta_forward's workspace (use 0), of the same when gpx_delta_backward will read it (use 1), and of
+ * gpx_delta_backward's own scratch (use 2). */
+size_t gpx_delta_work_bytes(const gpx_delta* d, int use);
+/* o and the states after the last tokens.  state (before the first tokens) NULL: zeros; state_out may be NULL or state.
+ * save == 0: work is scratch of gpx_delta_work_bytes(d, 0) bytes.  save != 0: of gpx_delta_work_bytes(d, 1) bytes, and
+ * keeps what gpx_delta_backward reads.  256-byte aligned, not shared by calls that may overlap in time. */
+int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, void* o, float* state_out, int save,
+                      void* work, size_t work_bytes);
+/* Gradients of sum(d_o o) + sum(d_state_out state_out) with respect to q, k, v (their type), g, beta and state (fp32;
+ * d_state may be NULL), all packed.  d_o: strides like v's; d_state_out NULL: zeros.  d and its inputs are those of the
+ * forward call with save != 0, saved what that call left in its work (only read); scratch as above.  The gradient of a
+ * shared key head is summed over its value heads in a fixed order; no atomics are used. */
+int gpx_delta_backward(gpx_handle* h, const gpx_delta* d, const void* d_o, const gpx_strided* d_o_st,
+                       const float* d_state_out, void* d_q, void* d_k, void* d_v, float* d_g, float* d_beta, float* d_state,
+                       const void* saved, size_t saved_bytes, void* scratch, size_t scratch_bytes);
+/* One token for each of d->batch rows (d->tokens == 1, d->sequences == 0): o is batch x value_heads x dv.  state and
+ * state_out (may be state) hold `slots` states; row b uses state slot[b] (device memory; NULL: b, and slots ==
+ * batch).  A row whose slot is outside [0, slots) is padding: neither o nor a state is written for it.  Rows of the
+ * same slot are taken in the order of the rows, as tokens of one sequence.  States of slots that no row names are
+ * not touched in state_out.  No workspace. */
+int gpx_delta_step(gpx_handle* h, const gpx_delta* d, int slots, const int* slot, const float* state, float* state_out, void* o);
+
 #ifdef __cplusplus
 }
 #endif
