@@ -5,15 +5,18 @@
 // coefficients (1.21 for the usual ones), so |X_ij| <= r, |A_ij| <= r^2 and |B_ij| <= max |b t + c t^2|: the
 // intermediates are stored in fp16, each scaled by the power of two that puts its bound just under fp16's largest
 // value, which leaves values down to 2^-28 of the bound as normal numbers.  fp16's 11 bits run at bf16's matrix
-// rate and lie 8 times nearer: five steps on random matrices end 0.0014 (relative, 2-norm) off in fp16 and 0.011 off
-// in bf16, against 0.0017 for rounding the exact result to bf16 once.  Results of more than 8 bits (fp32, fp16) use two fp16
-// planes per value, v = hi + lo with 22 bits, and three products (hi hi + hi lo + lo hi): 2.6e-7 off, like an fp32
-// product, at a third of the fp16 rate -- five times the rate of the fp32 matrix instructions.
+// rate and lie 8 times nearer.  X itself is kept as two fp16 planes, v = hi + lo with 22 bits, because the term a X hands
+// its rounding on from step to step (a = 3.4 at small singular values); the products read hi alone.  On 512 x 512 with a
+// few strong directions, relative, 2-norm: 0.0006 off, against 0.0027 with one plane of X and 0.0017 for rounding the
+// exact result to bf16.  Results of more than 8 bits (fp32, fp16) use two planes everywhere and three products (hi hi + hi lo
+// + lo hi): 1.5e-6 off at worst here, as an fp32 product, at a third of the fp16 rate -- five times that of the fp32
+// matrix instructions.
 //
 // Layout.  Every product has both operands k-contiguous: A needs rows of X; A is symmetric, so A A does too; and
 // B X needs rows of X^T, so the step's epilogue writes X in both orientations.  Buffers are padded to multiples of 64
-// with zeros, which the iteration preserves; an element's planes lie in one row: [row][plane][ld].
+// with zeros, which the iteration preserves; the planes of a row follow each other: [row][plane][ld].
 // The symmetric products compute tiles on and below the diagonal and write them twice.
+#include <algorithm>
 #include <cmath>
 
 #include "gpx_internal.h"
@@ -25,7 +28,7 @@ typedef float f16acc __attribute__((ext_vector_type(16)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int PAD = 64;
-constexpr int PARTS = 256;   // partial sums of the norm per matrix
+constexpr int PARTS = 1024;   // partial sums of the norm per matrix
 
 __host__ __device__ inline int pad64(int x) { return (x + PAD - 1) / PAD * PAD; }
 
@@ -33,17 +36,57 @@ template <typename T> __device__ __forceinline__ double to_f64(T v) { return (do
 template <> __device__ __forceinline__ double to_f64<double>(double v) { return v; }
 
 // ---- |G|_F^2: fixed partials per matrix --------------------------------------------------------------------------
-// Threads run along the unit stride of G (fast index), blocks over the other one.
+// 16 bytes of G at p (16-byte aligned: vec) or its elements one by one, `count` of them valid
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T x[N];
+  __device__ __forceinline__ void load(const T* p, long fs, int count, bool vec) {
+    if (vec && count >= N) {
+      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = e < count ? p[e * fs] : T(0);
+    }
+  }
+};
+
+// whether 16-byte accesses fit: dense along the fast index, every line and matrix on a 16-byte boundary
+template <typename T>
+__device__ __forceinline__ bool vector_ok(const T* g, long bs, long ss, long fs) {
+  constexpr int N = 16 / sizeof(T);
+  return fs == 1 && ss % N == 0 && bs % N == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+}
+
+// Threads run along the unit stride of G (fast index), blocks over the other one; four 16-byte loads under way per thread.
 template <typename T>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const T* G, long bs, long ss, long fs, int slow, int fast, double* part) {
+  constexpr int N = Vec<T>::N, U = 4;
   __shared__ double sm[4];
   const T* g = G + (long)blockIdx.y * bs;
+  const bool vec = vector_ok(G, bs, ss, fs);
   double v = 0.0;
-  for (int i = blockIdx.x; i < slow; i += gridDim.x)
-    for (int j = threadIdx.x; j < fast; j += 256) {
-      const double x = to_f64(g[i * ss + j * fs]);
-      v = fma(x, x, v);
+  const int per = (fast + 256 * N - 1) / (256 * N);   // a thread's pieces of one line
+  const int lines = (slow - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const long total = (long)lines * per;
+  int line = blockIdx.x, piece = 0;
+  for (long k = 0; k < total; k += U) {
+    Vec<T> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = (piece * 256 + threadIdx.x) * N;
+      const int count = line < slow ? fast - j : 0;
+      x[u].load(g + line * ss + j * fs, fs, count, vec);
+      if (++piece == per) {
+        piece = 0;
+        line += gridDim.x;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v = fma(to_f64(x[u].x[e]), to_f64(x[u].x[e]), v);
+  }
   for (int o = 32; o > 0; o >>= 1) v += __shfl_down(v, o);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -52,7 +95,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const T* G, long bs, long 
 
 // 1 / (sqrt(sum of the partials) + eps); every thread gets it
 __device__ __forceinline__ double inv_norm(const double* part, int nparts, double eps, double* sm /* 4 */) {
-  double v = (int)threadIdx.x < nparts ? part[threadIdx.x] : 0.0;
+  double v = 0.0;
+  for (int i = threadIdx.x; i < nparts; i += 256) v += part[i];
   for (int o = 32; o > 0; o >>= 1) v += __shfl_down(v, o);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -64,7 +108,7 @@ __device__ __forceinline__ double inv_norm(const double* part, int nparts, doubl
 template <typename T, int NPL>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const T* G, long bs, long rs, long cs, int n, int m, const double* part,
                                                       int nparts, double eps, double scale, _Float16* X, _Float16* XT,
-                                                      long plane) {
+                                                      long xs, long ts) {
   __shared__ float tile[64][65];
   __shared__ double sm[4];
   const int z = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, t = threadIdx.x;
@@ -72,36 +116,47 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const T* G, long bs, long 
   const double f = inv_norm(part + (long)z * PARTS, nparts, eps, sm) * scale;
   const T* g = G + z * bs;
   const bool along_rows = rs == 1 && cs != 1;
-  for (int q = 0; q < 16; ++q) {
-    const int a = q * 4 + (t >> 6), b = t & 63;
-    const int i = along_rows ? b : a, j = along_rows ? a : b;
-    float v = 0.f;
-    if (i0 + i < n && j0 + j < m) v = (float)(to_f64(g[(i0 + i) * rs + (j0 + j) * cs]) * f);
-    tile[i][j] = v;
+  {
+    constexpr int N = Vec<T>::N, LANES = 64 / N, LINES = 256 / LANES;   // threads of a line, lines at a time
+    const long ss = along_rows ? cs : rs, fs = along_rows ? rs : cs;
+    const bool vec = vector_ok(G, bs, ss, fs);
+    const int slow0 = along_rows ? j0 : i0, fast0 = along_rows ? i0 : j0, slow = along_rows ? m : n, fast = along_rows ? n : m;
+    const int b = (t % LANES) * N;
+    Vec<T> x[64 / LINES];
+#pragma unroll
+    for (int q = 0; q < 64 / LINES; ++q) {
+      const int a = q * LINES + t / LANES;
+      x[q].load(g + (slow0 + a) * ss + (fast0 + b) * fs, fs, slow0 + a < slow ? fast - fast0 - b : 0, vec);
+    }
+#pragma unroll
+    for (int q = 0; q < 64 / LINES; ++q) {
+      const int a = q * LINES + t / LANES;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = (float)(to_f64(x[q].x[e]) * f);
+        if (along_rows) tile[b + e][a] = v; else tile[a][b + e] = v;
+      }
+    }
   }
   __syncthreads();
   const int r = t >> 2, c0 = (t & 3) * 16;
-  X += z * plane;
-  XT += z * plane;
+  X += z * xs;
+  XT += z * ts;
   for (int half = 0; half < 2; ++half) {
     h8 xh, xl, th, tl;
     for (int e = 0; e < 8; ++e) {
       const int c = c0 + half * 8 + e;
       const float x = tile[r][c], y = tile[c][r];
       xh[e] = (_Float16)x;
+      xl[e] = (_Float16)(x - (float)xh[e]);
       th[e] = (_Float16)y;
-      if (NPL == 2) {
-        xl[e] = (_Float16)(x - (float)xh[e]);
-        tl[e] = (_Float16)(y - (float)th[e]);
-      }
+      if (NPL == 2) tl[e] = (_Float16)(y - (float)th[e]);
     }
-    const long px = (long)(i0 + r) * NPL * mp + j0 + c0 + half * 8, pt = (long)(j0 + r) * NPL * np + i0 + c0 + half * 8;
+    const long px = (long)(i0 + r) * 2 * mp + j0 + c0 + half * 8, pt = (long)(j0 + r) * NPL * np + i0 + c0 + half * 8;
     *reinterpret_cast<h8*>(X + px) = xh;
+    *reinterpret_cast<h8*>(X + px + mp) = xl;
     *reinterpret_cast<h8*>(XT + pt) = th;
-    if (NPL == 2) {
-      *reinterpret_cast<h8*>(X + px + mp) = xl;
-      *reinterpret_cast<h8*>(XT + pt + np) = tl;
-    }
+    if (NPL == 2) *reinterpret_cast<h8*>(XT + pt + np) = tl;
   }
 }
 
@@ -111,7 +166,9 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const T* G, long bs, long 
 struct NsGemm {
   const _Float16 *A, *B, *E;   // A: M rows, B: N rows, both K long; E like D
   _Float16 *D, *DT;
-  long sa, sb, sd;             // strides of the stack
+  long lda, ldb;               // elements from row to row of A and B, all planes
+  int dpl;                     // planes of D and E; DT has the products' planes
+  long sa, sb, sd, st;         // strides of the stack: A, B, D and E, DT
   int M, N, K;                 // padded to 64
   int lower;                   // M == N, tiles on and below the diagonal, DT == D
   float ca, cc;
@@ -128,60 +185,85 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, u
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst_wave, 16, voff, soff, 0, 0);
 }
 
-template <typename T>
-__device__ __forceinline__ void put(void* out, const void* base, long o, long b, float alpha, float beta, float v) {
-  float r = alpha * v;
-  if (base != nullptr) r += beta * (float)reinterpret_cast<const T*>(base)[b];
-  reinterpret_cast<T*>(out)[o] = (T)r;
+// alpha * v + beta * base to the caller's matrix, lanes along its unit stride, 16 elements of base under way at once
+template <typename T, int EM, int EN, int P>
+__device__ __forceinline__ void write_out(const NsGemm& g, const float* st, long z, int row0, int col0, int lane) {
+  const bool along_rows = g.ors == 1 && g.ocs != 1;
+  const int fast = along_rows ? EM : EN, per = 64 / fast;   // lanes of a line, lines at a time
+  const int lines = (along_rows ? EN : EM) / per, f = lane % fast, l0 = lane / fast;
+  T* out = reinterpret_cast<T*>(g.out) + z * g.obs;
+  const T* base = g.base == nullptr ? nullptr : reinterpret_cast<const T*>(g.base) + z * g.bbs;
+  for (int q0 = 0; q0 < lines; q0 += 16) {
+    float old[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int l = (q0 + u) * per + l0, i = row0 + (along_rows ? f : l), j = col0 + (along_rows ? l : f);
+      old[u] = base != nullptr && i < g.n && j < g.m ? (float)base[i * g.brs + j * g.bcs] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int l = (q0 + u) * per + l0, r = along_rows ? f : l, c = along_rows ? l : f, i = row0 + r, j = col0 + c;
+      if (i < g.n && j < g.m) {
+        float v = g.alpha * st[r * P + c];
+        if (base != nullptr) v = fmaf(g.beta, old[u], v);
+        out[i * g.ors + j * g.ocs] = (T)v;
+      }
+    }
+  }
 }
 
 // Tile BM x BN, WAVES_M x WAVES_N waves of (BM / WAVES_M) x (BN / WAVES_N) each in 32 x 32 x 16 matrix instructions.
 // A k-tile is 64 / NPL long: an LDS row is 128 bytes either way, 8 chunks of 16 bytes (NPL = 2: four of hi, four of
-// lo), chunk c of row r in slot c ^ (r & 7), so that the 16-byte fragment reads meet no bank twice.
-template <int BM, int BN, int WAVES_M, int WAVES_N, int NPL>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const NsGemm g, int tiles_n) {
+// lo), chunk c of row r in slot c ^ (r >> 1 & 7): 16 rows cover the 64 banks once in a 16-byte fragment read.
+template <int BM, int BN, int WAVES_M, int WAVES_N, int NPL, int STAGES>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const NsGemm g, int tiles_m, int tiles_n) {
   constexpr int NW = WAVES_M * WAVES_N, NT = 64 * NW;
   constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 32, TN = WN / 32;
   constexpr int BK = 64 / NPL, KS = BK / 16;
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
   extern __shared__ __align__(16) char smem[];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  // Workgroups with equal id % 8 share an XCD and its L2: each XCD takes a run of consecutive tiles, four tile rows high
   int ti, tj;
-  if (g.lower) {
-    const unsigned id = blockIdx.x;
-    unsigned r = (unsigned)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
-    while ((r + 1) * (r + 2) / 2 <= id) ++r;
-    while (r * (r + 1) / 2 > id) --r;
-    ti = r;
-    tj = id - r * (r + 1) / 2;
-  } else {
-    ti = blockIdx.x / tiles_n;
-    tj = blockIdx.x % tiles_n;
+  {
+    const unsigned per = gridDim.x >> 3, rest = gridDim.x & 7, x = blockIdx.x & 7;
+    const unsigned id = x * per + min(x, rest) + (blockIdx.x >> 3);
+    if (g.lower) {
+      unsigned r = (unsigned)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+      while ((r + 1) * (r + 2) / 2 <= id) ++r;
+      while (r * (r + 1) / 2 > id) --r;
+      ti = r;
+      tj = id - r * (r + 1) / 2;
+    } else {
+      const unsigned band = id / (4 * tiles_n), in = id % (4 * tiles_n), high = min(4u, (unsigned)tiles_m - band * 4);
+      ti = band * 4 + in % high;
+      tj = in / high;
+    }
   }
   const int i0 = ti * BM, j0 = tj * BN;
   const long z = blockIdx.y;
-  const long lda = (long)NPL * g.K * 2;   // bytes per row of A and of B
+  const long lda = g.lda * 2, ldb = g.ldb * 2;   // bytes
   const __amdgpu_buffer_rsrc_t ra =
       __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)(g.A + z * g.sa) + i0 * lda), 0, 0x7fffffff, 0x00020000);
   const __amdgpu_buffer_rsrc_t rb =
-      __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)(g.B + z * g.sb) + j0 * lda), 0, 0x7fffffff, 0x00020000);
+      __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)(g.B + z * g.sb) + j0 * ldb), 0, 0x7fffffff, 0x00020000);
   // per-lane sources of the DMA: piece p of NT lanes covers rows p * (NT / 8) ..; rows behind the matrix repeat its last
   constexpr int PA = BM * 8 / NT, PB = BN * 8 / NT;
   unsigned va[PA], vb[PB];
 #pragma unroll
   for (int p = 0; p < PA; ++p) {
-    const int s = p * NT + t, r = s >> 3, c = (s & 7) ^ (r & 7);
+    const int s = p * NT + t, r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
     const int rr = min(r, g.M - 1 - i0);
     va[p] = (unsigned)(rr * lda + (NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16));
   }
 #pragma unroll
   for (int p = 0; p < PB; ++p) {
-    const int s = p * NT + t, r = s >> 3, c = (s & 7) ^ (r & 7);
+    const int s = p * NT + t, r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
     const int rr = min(r, g.N - 1 - j0);
-    vb[p] = (unsigned)(rr * lda + (NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16));
+    vb[p] = (unsigned)(rr * ldb + (NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16));
   }
-  auto load = [&](int kt, int buf) {
-    char* sA = smem + buf * STAGE + wave * 1024;
+  auto load = [&](int kt, char* stage) {
+    char* sA = stage + wave * 1024;
     char* sB = sA + ABYTES;
     const unsigned so = (unsigned)kt * (BK * 2);
 #pragma unroll
@@ -199,148 +281,192 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const N
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
   const int r32 = lane & 31, kh = lane >> 5;
   const int nk = g.K / BK;
-  load(0, 0);
-  for (int kt = 0; kt < nk; ++kt) {
+  const int offA = (wm * WM + r32) * 128, offB = ABYTES + (wn * WN + r32) * 128;
+  h8 fa[2][TM][NPL], fb[2][TN][NPL];
+  auto fetch = [&](const char* stage, int s, int set) {
+    const int o0 = (((s * 2 + kh) ^ ((r32 >> 1) & 7)) * 16);
+#pragma unroll
+    for (int pl = 0; pl < NPL; ++pl) {
+      const int o = o0 ^ (pl * 64);
+#pragma unroll
+      for (int a = 0; a < TM; ++a) fa[set][a][pl] = *reinterpret_cast<const h8*>(stage + offA + a * 32 * 128 + o);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) fb[set][b][pl] = *reinterpret_cast<const h8*>(stage + offB + b * 32 * 128 + o);
+    }
+  };
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b) {
+        if (NPL == 2) {
+          acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][a][0], fb[set][b][NPL - 1], acc[a][b], 0, 0, 0);
+          acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][a][NPL - 1], fb[set][b][0], acc[a][b], 0, 0, 0);
+        }
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][a][0], fb[set][b][0], acc[a][b], 0, 0, 0);
+      }
+  };
+  // STAGES k-tiles are in flight.  The one barrier of a k-tile comes before its last matrix instructions, when every wave holds
+  // its last fragments: the stage is refilled and the next tile's first fragments are read under those.
+  constexpr int L = PA + PB;
+#pragma unroll
+  for (int p = 0; p < STAGES; ++p)
+    if (p < nk) load(p, smem + p * STAGE);
+  if (nk >= STAGES)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * L) : "memory");
+  else
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();   // tile kt has landed, and every wave is done with the buffer that tile kt + 1 goes to
-    if (kt + 1 < nk) load(kt + 1, (kt + 1) & 1);
-    const char* sA = smem + (kt & 1) * STAGE + (wm * WM + r32) * 128;
-    const char* sB = smem + (kt & 1) * STAGE + ABYTES + (wn * WN + r32) * 128;
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  fetch(smem, 0, 0);
+  int cur = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    const int nxt = cur + 1 == STAGES ? 0 : cur + 1;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int o0 = (((s * 2 + kh) ^ (r32 & 7)) * 16);
-      h8 fa[TM][NPL], fb[TN][NPL];
-#pragma unroll
-      for (int pl = 0; pl < NPL; ++pl) {
-        const int o = o0 ^ (pl * 64);
-#pragma unroll
-        for (int a = 0; a < TM; ++a) fa[a][pl] = *reinterpret_cast<const h8*>(sA + a * 32 * 128 + o);
-#pragma unroll
-        for (int b = 0; b < TN; ++b) fb[b][pl] = *reinterpret_cast<const h8*>(sB + b * 32 * 128 + o);
+      if (s + 1 < KS) {
+        fetch(smem + cur * STAGE, s + 1, (s + 1) & 1);
+      } else if (kt + 1 < nk) {
+        if (kt + STAGES <= nk)   // tiles kt + 1 .. kt + STAGES - 1 are under way: wait for the first of them
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * L) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (kt + STAGES < nk) load(kt + STAGES, smem + cur * STAGE);
+        fetch(smem + nxt * STAGE, 0, (s + 1) & 1);
       }
-#pragma unroll
-      for (int a = 0; a < TM; ++a)
-#pragma unroll
-        for (int b = 0; b < TN; ++b) {
-          if (NPL == 2) {
-            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[a][0], fb[b][NPL - 1], acc[a][b], 0, 0, 0);
-            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[a][NPL - 1], fb[b][0], acc[a][b], 0, 0, 0);
-          }
-          acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[a][0], fb[b][0], acc[a][b], 0, 0, 0);
-        }
+      multiply(s & 1);
     }
+    cur = nxt;
   }
+  static_assert(KS % 2 == 0, "the fragment sets alternate");
+  static_assert((STAGES - 1) * L < 64, "vmcnt has six bits");
   __syncthreads();   // the stages become the waves' own staging of 64 x 64 blocks
-  constexpr int P = 68;
-  float* st = reinterpret_cast<float*>(smem) + wave * (64 * P);
-  const long ldd = (long)NPL * g.N, ldt = (long)NPL * g.M;
+  constexpr int EM = WM % 64 ? 32 : 64, EN = WN % 64 ? 32 : 64, P = EN + 4;
+  constexpr int RL = EN / 8, RR = 64 / RL, RQ = EM / RR;   // row pass: lanes per row, rows at a time, times
+  constexpr int CL = EM / 8, CR = 64 / CL, CQ = EN / CR;   // column pass
+  float* st = reinterpret_cast<float*>(smem) + wave * (EM * P);
+  const long ldd = (long)g.dpl * g.N, ldt = (long)NPL * g.M;
+  const bool two = g.dpl == 2;
   const _Float16* E = g.E == nullptr ? nullptr : g.E + z * g.sd;
   _Float16* D = g.D == nullptr ? nullptr : g.D + z * g.sd;
-  _Float16* DT = g.DT == nullptr ? nullptr : g.DT + z * g.sd;
+  _Float16* DT = g.DT == nullptr ? nullptr : g.DT + z * g.st;
 #pragma unroll
-  for (int bi = 0; bi < WM / 64; ++bi)
+  for (int bi = 0; bi < WM / EM; ++bi)
 #pragma unroll
-    for (int bj = 0; bj < WN / 64; ++bj) {
-      const int row0 = i0 + wm * WM + bi * 64, col0 = j0 + wn * WN + bj * 64;
-      if (row0 >= g.M || col0 >= g.N) continue;   // uniform in the wave
+    for (int bj = 0; bj < WN / EN; ++bj) {
+      const int row0 = i0 + wm * WM + bi * EM, col0 = j0 + wn * WN + bj * EN;
+      if (row0 >= g.M || col0 >= g.N) continue;   // uniform in the wave; sizes are multiples of 64
+      // every load of E is under way before the first is used
+      h8 eh[RQ], el[RQ];
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int q = 0; q < RQ; ++q) {
+        eh[q] = el[q] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (E != nullptr) {
+          const _Float16* src = E + (row0 + q * RR + lane / RL) * ldd + col0 + (lane % RL) * 8;
+          eh[q] = *reinterpret_cast<const h8*>(src);
+          if (two) el[q] = *reinterpret_cast<const h8*>(src + g.N);
+        }
+      }
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+      for (int a = 0; a < EM / 32; ++a)
+#pragma unroll
+        for (int b = 0; b < EN / 32; ++b)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            st[(a * 32 + (e >> 2) * 8 + kh * 4 + (e & 3)) * P + b * 32 + r32] = acc[bi * 2 + a][bj * 2 + b][e];
+            st[(a * 32 + (e >> 2) * 8 + kh * 4 + (e & 3)) * P + b * 32 + r32] = acc[bi * (EM / 32) + a][bj * (EN / 32) + b][e];
       __builtin_amdgcn_wave_barrier();
-      // rows: 8 lanes x 8 columns, 8 rows at a time
-      for (int q = 0; q < 8; ++q) {
-        const int r = q * 8 + (lane >> 3), c = (lane & 7) * 8;
+#pragma unroll
+      for (int q = 0; q < RQ; ++q) {
+        const int r = q * RR + lane / RL, c = (lane % RL) * 8;
         float* p = st + r * P + c;
         float v[8];
+        h8 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = g.cc * p[e];
-        if (E != nullptr) {
-          const _Float16* src = E + (row0 + r) * ldd + col0 + c;
-          const h8 eh = *reinterpret_cast<const h8*>(src);
-          if (NPL == 2) {
-            const h8 el = *reinterpret_cast<const h8*>(src + g.N);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += g.ca * ((float)eh[e] + (float)el[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += g.ca * (float)eh[e];
-          }
+        for (int e = 0; e < 8; ++e) {
+          v[e] = fmaf(g.ca, (float)eh[q][e] + (float)el[q][e], g.cc * p[e]);
+          hi[e] = (_Float16)v[e];
+          lo[e] = (_Float16)(v[e] - (float)hi[e]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = v[e];
         if (D != nullptr) {
-          h8 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            hi[e] = (_Float16)v[e];
-            if (NPL == 2) lo[e] = (_Float16)(v[e] - (float)hi[e]);
-          }
           _Float16* dst = D + (row0 + r) * ldd + col0 + c;
           *reinterpret_cast<h8*>(dst) = hi;
-          if (NPL == 2) *reinterpret_cast<h8*>(dst + g.N) = lo;
+          if (two) *reinterpret_cast<h8*>(dst + g.N) = lo;
         }
       }
       __builtin_amdgcn_wave_barrier();
       if (DT != nullptr && !(g.lower && ti == tj)) {
-        for (int q = 0; q < 8; ++q) {   // columns: 8 lanes x 8 rows, 8 columns at a time
-          const int c = q * 8 + (lane >> 3), r = (lane & 7) * 8;
+#pragma unroll
+        for (int q = 0; q < CQ; ++q) {
+          const int c = q * CR + lane / CL, r = (lane % CL) * 8;
           h8 hi, lo;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float v = st[(r + e) * P + c];
             hi[e] = (_Float16)v;
-            if (NPL == 2) lo[e] = (_Float16)(v - (float)hi[e]);
+            lo[e] = (_Float16)(v - (float)hi[e]);
           }
           _Float16* dst = DT + (col0 + c) * ldt + row0 + r;
           *reinterpret_cast<h8*>(dst) = hi;
           if (NPL == 2) *reinterpret_cast<h8*>(dst + g.M) = lo;
         }
       }
-      if (g.out_type >= 0) {
-        // the caller's matrix, lanes along its unit stride
-        const bool along_rows = g.ors == 1 && g.ocs != 1;
-        for (int q = 0; q < 64; ++q) {
-          const int r = along_rows ? lane : q, c = along_rows ? q : lane;
-          const int i = row0 + r, j = col0 + c;
-          if (i < g.n && j < g.m) {
-            const long o = z * g.obs + i * g.ors + j * g.ocs, b = z * g.bbs + i * g.brs + j * g.bcs;
-            const float v = st[r * P + c];
-            if (g.out_type == GPX_F32) put<float>(g.out, g.base, o, b, g.alpha, g.beta, v);
-            else if (g.out_type == GPX_F16) put<_Float16>(g.out, g.base, o, b, g.alpha, g.beta, v);
-            else put<__bf16>(g.out, g.base, o, b, g.alpha, g.beta, v);
-          }
-        }
-      }
+      if (g.out_type == GPX_F32) write_out<float, EM, EN, P>(g, st, z, row0, col0, lane);
+      else if (g.out_type == GPX_F16) write_out<_Float16, EM, EN, P>(g, st, z, row0, col0, lane);
+      else if (g.out_type == GPX_BF16) write_out<__bf16, EM, EN, P>(g, st, z, row0, col0, lane);
       __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int BM, int BN, int WAVES_M, int WAVES_N, int NPL>
+template <int BM, int BN, int WAVES_M, int WAVES_N, int NPL, int STAGES>
 int launch_cfg(hipStream_t s, const NsGemm& g, int batch) {
   constexpr int NW = WAVES_M * WAVES_N;
-  constexpr size_t lds = std::max<size_t>(2 * (BM + BN) * 128, (size_t)NW * 64 * 68 * 4);
+  constexpr size_t lds = std::max<size_t>(STAGES * (BM + BN) * 128, (size_t)NW * (BM / WAVES_M % 64 ? 32 : 64) * ((BN / WAVES_N % 64 ? 32 : 64) + 4) * 4);
+  static_assert(BM * 8 % (64 * NW) == 0 && BN * 8 % (64 * NW) == 0 && BM / WAVES_M % 32 == 0 && BN / WAVES_N % 32 == 0, "tile");
+  static_assert(lds <= 160 * 1024, "LDS");
+  GPX_REQUIRE(!g.lower || BM == BN, "ns_gemm: half products need square tiles");
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
   const unsigned tiles = g.lower ? (unsigned)tm * (tm + 1) / 2 : (unsigned)tm * tn;
   static thread_local bool set[GPX_MAX_DEVICES] = {};
   int dev = 0;
   GPX_HIP(hipGetDevice(&dev));
   if (dev < GPX_MAX_DEVICES && !set[dev]) {
-    GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<BM, BN, WAVES_M, WAVES_N, NPL>),
+    GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<BM, BN, WAVES_M, WAVES_N, NPL, STAGES>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     set[dev] = true;
   }
-  hipLaunchKernelGGL((ns_gemm_kernel<BM, BN, WAVES_M, WAVES_N, NPL>), dim3(tiles, batch), dim3(64 * NW), lds, s, g, tn);
+  hipLaunchKernelGGL((ns_gemm_kernel<BM, BN, WAVES_M, WAVES_N, NPL, STAGES>), dim3(tiles, batch), dim3(64 * NW), lds, s, g, tm, tn);
   GPX_HIP(hipGetLastError());
   return 0;
 }
 
+// Tile by estimated time: rounds of the chip times what one round of a tile takes (measured at K = 4096, one plane, us;
+// two planes keep the ratios): 64 x 64 with 4 waves, two on a CU, 34; 128 x 128 with 8 waves 42; 192 x 192 with 6 waves
+// 84; 256 x 256 with 8 waves 110.  Larger tiles read LDS less per product, smaller ones fill the chip: A A at n = 4096
+// takes 162 / 117 / 84 / 97 us with them, B X 233 / 173 / 169 / 140, at n = 1024 8.8 / 14 / 26 / 35 and 10 / 14 / 27 / 36.
 template <int NPL>
 int ns_gemm(hipStream_t s, const NsGemm& g, int batch) {
-  return launch_cfg<128, 128, 2, 2, NPL>(s, g, batch);
+  const int tile[4] = {64, 128, 192, 256}, slots[4] = {512, 256, 256, 256};
+  const double unit[4] = {34, 42, 84, 110};
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 4; ++i) {
+    const double tm = (g.M + tile[i] - 1) / tile[i], tn = (g.N + tile[i] - 1) / tile[i];
+    const double cost = std::ceil((g.lower ? tm * (tm + 1) / 2 : tm * tn) * batch / slots[i]) * unit[i];
+    if (i == 0 || cost < least) {
+      best = i;
+      least = cost;
+    }
+  }
+  switch (best) {
+    case 0: return launch_cfg<64, 64, 2, 2, NPL, 4>(s, g, batch);
+    case 1: return launch_cfg<128, 128, 2, 4, NPL, 4>(s, g, batch);
+    case 2: return launch_cfg<192, 192, 2, 3, NPL, 3>(s, g, batch);
+    default: return launch_cfg<256, 256, 2, 4, NPL, 2>(s, g, batch);
+  }
 }
 
 // ---- fp64: the framework's own products ----------------------------------------------------------------------------
@@ -453,15 +579,15 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
              const double* k, double eps, double alpha, double beta, const void* base, const long* bst, void* out, const long* ost,
              char* work) {
   const int np = pad64(n), mp = pad64(m);
-  const long xs = (long)np * mp * NPL, as = (long)np * np * NPL;
+  const long xs = (long)np * mp * 2, ts = (long)np * mp * NPL, as = (long)np * np * NPL;
   double* part = reinterpret_cast<double*>(work);
   _Float16* X[2];
   _Float16* XT[2];
   _Float16* p = reinterpret_cast<_Float16*>(work + (size_t)batch * PARTS * 8);
   X[0] = p; p += batch * xs;
   X[1] = p; p += batch * xs;
-  XT[0] = p; p += batch * xs;
-  XT[1] = p; p += batch * xs;
+  XT[0] = p; p += batch * ts;
+  XT[1] = p; p += batch * ts;
   _Float16* A = p; p += batch * as;
   _Float16* B = p;
   int nparts = 0;
@@ -469,7 +595,7 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
   double r = 1.0;
   int sx = scale_exp(r);
   hipLaunchKernelGGL((ns_pack_kernel<T, NPL>), dim3(mp / 64, np / 64, batch), dim3(256), 0, s, (const T*)G, bs, rs, cs, n, m, part,
-                     nparts, eps, std::ldexp(1.0, sx), X[0], XT[0], xs);
+                     nparts, eps, std::ldexp(1.0, sx), X[0], XT[0], xs, ts);
   GPX_HIP(hipGetLastError());
   for (int it = 0; it < steps; ++it) {
     const int cur = it & 1;
@@ -479,18 +605,20 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
     NsGemm g = {};
     g.out_type = -1;
     // A = X X^T
-    g.A = g.B = X[cur]; g.sa = g.sb = xs; g.D = g.DT = A; g.sd = as;
+    g.A = g.B = X[cur]; g.lda = g.ldb = 2L * mp; g.sa = g.sb = xs;
+    g.D = g.DT = A; g.dpl = NPL; g.sd = g.st = as;
     g.M = g.N = np; g.K = mp; g.lower = 1;
     g.ca = 0.f; g.cc = (float)std::ldexp(1.0, sa - 2 * sx);
     NS_TRY(ns_gemm<NPL>(s, g, batch));
     // B = b A + c A A
-    g.A = g.B = g.E = A; g.sa = g.sb = as; g.D = g.DT = B; g.K = np;
+    g.A = g.B = g.E = A; g.lda = g.ldb = (long)NPL * np; g.sa = g.sb = as;
+    g.D = g.DT = B; g.K = np;
     g.ca = (float)(k[1] * std::ldexp(1.0, sb - sa));
     g.cc = (float)(k[2] * std::ldexp(1.0, sb - 2 * sa));
     NS_TRY(ns_gemm<NPL>(s, g, batch));
     // X <- a X + B X
     const bool last = it + 1 == steps;
-    g.A = B; g.sa = as; g.B = XT[cur]; g.sb = xs; g.E = X[cur]; g.sd = xs;
+    g.A = B; g.B = XT[cur]; g.sb = ts; g.E = X[cur]; g.dpl = 2; g.sd = xs; g.st = ts;
     g.D = last ? nullptr : X[cur ^ 1];
     g.DT = last ? nullptr : XT[cur ^ 1];
     g.M = np; g.N = mp; g.K = np; g.lower = 0;
@@ -551,7 +679,8 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m) {
   if (dtype == GPX_F64)   // the matrices of a stack take their turns in one set of buffers
     return parts + 8 * (2 * (size_t)small * pad32(large) + 2 * (size_t)small * pad32(small));
   const size_t np = pad64(small), mp = pad64(large);
-  return parts + (size_t)batch * 2 * planes_of(dtype) * (4 * np * mp + 2 * np * np);
+  const size_t pl = planes_of(dtype);   // X twice with two planes, X^T twice, A and B
+  return parts + (size_t)batch * 2 * ((4 + 2 * pl) * np * mp + 2 * pl * np * np);
 }
 
 int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const void* G, const gpx_strided* g_st, int steps,

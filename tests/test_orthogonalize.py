@@ -58,13 +58,13 @@ def test_work_bytes():
     from gaussian_process_amd import _lib
     lib = _lib.load()
     for dtype, planes in ((1, 2), (2, 2), (3, 1)):
-        assert lib.gpx_orthogonalize_work_bytes(dtype, 3, 65, 130) == 3 * (2048 + 2 * planes * (4 * 128 * 192 + 2 * 128 * 128))
+        assert lib.gpx_orthogonalize_work_bytes(dtype, 3, 65, 130) == 3 * (8192 + 2 * ((4 + 2 * planes) * 128 * 192 + 2 * planes * 128 * 128))
         assert lib.gpx_orthogonalize_work_bytes(dtype, 1, 130, 65) == lib.gpx_orthogonalize_work_bytes(dtype, 1, 65, 130)
-    assert lib.gpx_orthogonalize_work_bytes(0, 1, 5, 40) == 2048 + 8 * (2 * 5 * 64 + 2 * 5 * 32)
+    assert lib.gpx_orthogonalize_work_bytes(0, 1, 5, 40) == 8192 + 8 * (2 * 5 * 64 + 2 * 5 * 32)
     assert lib.gpx_orthogonalize_work_bytes(9, 1, 5, 40) == 0
     assert lib.gpx_orthogonalize_work_bytes(1, 1, 0, 40) == 0
     # 64-bit sizes
-    assert lib.gpx_orthogonalize_work_bytes(1, 1, 65536, 65536) == 2048 + 4 * 6 * 65536 ** 2
+    assert lib.gpx_orthogonalize_work_bytes(1, 1, 65536, 65536) == 8192 + 2 * 12 * 65536 ** 2
 
 
 # ---- GPU ----------------------------------------------------------------------------------------------------------
