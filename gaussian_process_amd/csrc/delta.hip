@@ -91,6 +91,8 @@ struct Args {
   // per (slot, value head): T and P (C x C), G (C doubles), E and dX (C x dvp), S and dS (dk x dvp)
   float *T, *P, *E, *dX, *S, *dS, *part;
   double* G;
+  __bf16 *Kf, *Qf, *KTf, *Tf, *Pf;   // fragments: K, Q, K^T per (slot, key head), T and P per (slot, value head)
+  float* fac;                        // per (slot, value head): exp(G), beta, exp(G_C - G) beta, exp(G_C); C each
   const float *state, *d_state_out;
   float *state_out, *d_state, *d_g, *d_beta;
   void *o, *d_q, *d_k, *d_v;
@@ -624,6 +626,533 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     }
 }
 
+// ---- planes -------------------------------------------------------------------------------------------------------------
+// Products run on the bf16 matrix cores with values split exactly into bf16 planes, x = x0 + x1 + x2 (8 bits each): a bf16 input
+// is one plane, an fp16 one two, anything in fp32 three.  A product of planes i and j is kept for i + j <= 2, which
+// leaves 2^-24, fp32's own rounding; the matrix cores sum in fp32.  Three planes against one cost 3/16 of the fp32
+// matrix instruction's time, three against three 6/16.
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Planes { static constexpr int N = 3; };
+template <> struct Planes<_Float16> { static constexpr int N = 2; };
+template <> struct Planes<__bf16> { static constexpr int N = 1; };
+
+// the high 16 bits of two floats as two bf16 (truncation; the remainders carry the rest)
+__device__ __forceinline__ unsigned high_pair(float a, float b) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+}
+__device__ __forceinline__ float truncated(float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u);
+}
+// NV floats -> NPL planes of NV bf16.  Each plane truncates to 8 bits, except the last, which is rounded where it is not exact
+// (NPL < 3).  An infinity's remainder is NaN, so infinite values give NaN.
+template <int NV, int NPL, typename V>
+__device__ __forceinline__ void split(const float* x, V* planes) {
+  float r[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) r[i] = x[i];
+#pragma unroll
+  for (int p = 0; p < NPL; ++p) {
+    unsigned w[NV / 2];
+    if (p == 2 || p + 1 < NPL) {
+#pragma unroll
+      for (int i = 0; i < NV; i += 2) w[i / 2] = high_pair(r[i], r[i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; i += 2) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        b2 v;
+        v[0] = (__bf16)r[i];
+        v[1] = (__bf16)r[i + 1];
+        w[i / 2] = __builtin_bit_cast(unsigned, v);
+      }
+    }
+    __builtin_memcpy(&planes[p], w, sizeof(w));
+    if (p + 1 < NPL) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) r[i] -= truncated(r[i]);
+    }
+  }
+}
+
+// acc += sum of A_i B_j over planes with i + j < LIM
+template <int NA, int NB, int LIM>
+__device__ __forceinline__ f4 planes_mma(const b8* a, const b8* b, f4 acc) {
+#pragma unroll
+  for (int n = LIM - 1; n >= 0; --n)   // small terms first
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int j = n - i;
+      if (j >= 0 && j < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc, 0, 0, 0);
+    }
+  return acc;
+}
+
+// a barrier that waits for this wave's LDS accesses, not for its global ones
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Fragments.  A matrix instruction's operand is 16 rows x 32 terms, lane l holding row l & 15 and 8 terms of group
+// g = l >> 4.  Operands that the scan reads are stored fragment by fragment, [plane][row block][term block][lane][8], so that a
+// wave loads one with 16 bytes per lane, in a row.  Natural order: terms 32 ks + 8 g + e.  State order: S lives in the
+// accumulators of the wave that updates it, lane l holding column l & 15 and rows 4 g + e of each of its DK / 64 tiles, and
+// serves from there as the other operand; the terms of wave w are therefore dk = 16 (w DK / 64) + 4 g + e, e < 4, and the
+// same of its second tile (none if DK = 64: zeros).
+__device__ __forceinline__ long frag(int block, int blocks, int ks, int lane) { return (((long)block * blocks + ks) * 64 + lane) * 8; }
+
+constexpr int KF = 4 * 4 * 64 * 8;   // elements of a plane of K or Q in state order, also of a C x C matrix twice over
+constexpr int TF = 4 * 2 * 64 * 8;   // of a C x C matrix
+
+// C rows of one head as planes in LDS, pitch DK + 8
+template <typename T, int DK>
+__device__ __forceinline__ void load_planes(__bf16* dst, const void* src, const gpx_strided& s, long row, int t0, int len, int head, int dk,
+                                            int t) {
+  constexpr int P = DK + 8, N = Planes<T>::N;
+  const T* base = reinterpret_cast<const T*>(src) + row * s.bs + t0 * s.rs + head * s.cs;
+  const bool vec = ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(s.rs * sizeof(T))) & 15) == 0;
+  for (int i = t; i < C * DK / 8; i += 256) {
+    const int r = i / (DK / 8), c = i % (DK / 8) * 8;
+    float x[8];
+    if (r < len && vec && c + 8 <= dk) {
+      T v[8];
+      constexpr int W = sizeof(T) * 8 / 16;
+      const uint4* q = reinterpret_cast<const uint4*>(base + r * s.rs + c);
+      uint4 u[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) u[k] = q[k];
+      __builtin_memcpy(v, u, sizeof(v));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = r < len && c + e < dk ? (float)base[r * s.rs + c + e] : 0.f;
+    }
+    b8 p[N];
+    split<8, N>(x, p);
+#pragma unroll
+    for (int k = 0; k < N; ++k) *reinterpret_cast<b8*>(dst + (k * C + r) * P + c) = p[k];
+  }
+}
+
+// T = (I + A)^-1 for the strictly lower A (LDS, pitch PC), 4 waves.  The 16 x 16 diagonal blocks by substitution, one column
+// per lane; then block T_ij = -T_ii sum_l A_il T_lj for i - j = 1, 2, 3, on the fp32 matrix cores.  tmp: 4 x 16 x 20 floats.
+__device__ __forceinline__ void unit_lower_inverse(const float* A, float* Ti, float* tmp, int wave, int lane) {
+  const int r4 = (lane >> 4) * 4, col = lane & 15;
+  for (int j = wave + 1; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) Ti[(wave * 16 + r4 + e) * PC + j * 16 + col] = 0.f;
+  if (lane < 16) {
+    const float* a = A + wave * 16 * PC + wave * 16;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == lane ? 1.f : 0.f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) v = fmaf(-a[i * PC + l], x[l], v);
+      x[i] = v;
+      Ti[(wave * 16 + i) * PC + wave * 16 + lane] = v;
+    }
+  }
+  __syncthreads();
+  float* mine = tmp + wave * 16 * 20;
+  for (int d = 1; d < 4; ++d) {
+    const int i = wave, j = wave - d;   // waves without a block only meet the barriers
+    if (j >= 0) {
+      f4 acc = {0, 0, 0, 0};
+      for (int l = j; l < i; ++l)
+        acc = mm<false, false>(A + i * 16 * PC + l * 16, PC, Ti + l * 16 * PC + j * 16, PC, 16, acc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(r4 + e) * 20 + col] = acc[e];
+    }
+    __syncthreads();
+    if (j >= 0) {
+      f4 acc = {0, 0, 0, 0};
+      acc = mm<false, false>(Ti + i * 16 * PC + i * 16, PC, mine, 20, 16, acc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) Ti[(i * 16 + r4 + e) * PC + j * 16 + col] = -acc[e];
+    }
+    __syncthreads();
+  }
+}
+
+// rows of a C x C matrix in LDS (pitch PC) as fragments in natural order
+template <int NPL>
+__device__ __forceinline__ void store_square(const float* M, __bf16* dst, int t) {
+  for (int i = t; i < TF / 8; i += 256) {
+    const int lane = i & 63, ks = i >> 6 & 1, rb = i >> 7;
+    const float* p = M + (rb * 16 + (lane & 15)) * PC + ks * 32 + (lane >> 4) * 8;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[e];
+    b8 v[NPL];
+    split<8, NPL>(x, v);
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) *reinterpret_cast<b8*>(dst + k * TF + i * 8) = v[k];
+  }
+}
+
+// Planes of what only the output sees: two (16 bits) under a 16-bit result
+template <typename T> struct OutPlanes { static constexpr int N = sizeof(T) == 2 ? 2 : 3; };
+
+// ---- prep: one chunk of one key head and its value heads -----------------------------------------------------------------
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
+  constexpr int N = Planes<T>::N, P = DK + 8, RT = DK / 64, KSN = DK / 32;
+  extern __shared__ __align__(16) char smem[];
+  __bf16* K = reinterpret_cast<__bf16*>(smem);
+  __bf16* Q = K + N * C * P;
+  float* A = reinterpret_cast<float*>(Q + N * C * P);
+  float* M = A + C * PC;
+  float* tmp = M + C * PC;
+  double* G = reinterpret_cast<double*>(tmp + 4 * 16 * 20);
+  float* beta = reinterpret_cast<float*>(G + C);
+  const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (len == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
+  const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
+  load_planes<T, DK>(K, a.d.k, a.d.k_st, row, t0, len, hk, a.d.dk, t);
+  load_planes<T, DK>(Q, a.d.q, a.d.q_st, row, t0, len, hk, a.d.dk, t);
+  __syncthreads();
+  // K and Q in state order, K^T in natural order
+  for (int i = t; i < KF / 8; i += 256) {
+    const int l = i & 63, w = i >> 6 & 3, rb = i >> 8;
+    const int r = rb * 16 + (l & 15), c = w * RT * 16 + (l >> 4) * 4;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const __bf16* x = K + (k * C + r) * P + c;
+      const __bf16* y = Q + (k * C + r) * P + c;
+      b4 z = {0, 0, 0, 0};
+      const b4 x0 = *reinterpret_cast<const b4*>(x), y0 = *reinterpret_cast<const b4*>(y);
+      const b4 x1 = RT == 2 ? *reinterpret_cast<const b4*>(x + 16 * (RT - 1)) : z;
+      const b4 y1 = RT == 2 ? *reinterpret_cast<const b4*>(y + 16 * (RT - 1)) : z;
+      *reinterpret_cast<b8*>(a.Kf + (atk * N + k) * KF + i * 8) = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+      *reinterpret_cast<b8*>(a.Qf + (atk * N + k) * KF + i * 8) = __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  for (int i = t; i < DK * C / 8; i += 256) {
+    const int l = i & 63, ks = i >> 6 & 1, rb = i >> 7;
+    const int c = rb * 16 + (l & 15), r = ks * 32 + (l >> 4) * 8;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      b8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = K[(k * C + r + e) * P + c];
+      *reinterpret_cast<b8*>(a.KTf + (atk * N + k) * (DK * C) + i * 8) = v;
+    }
+  }
+  // K K^T and Q K^T: wave w the rows 16 w ..
+  f4 nn[4], pp[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    nn[j] = pp[j] = f4{0, 0, 0, 0};
+    if (j > wave) continue;
+#pragma unroll
+    for (int ks = 0; ks < KSN; ++ks) {
+      b8 x[N], y[N], z[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        x[k] = *reinterpret_cast<const b8*>(K + (k * C + wave * 16 + col) * P + ks * 32 + g8);
+        y[k] = *reinterpret_cast<const b8*>(Q + (k * C + wave * 16 + col) * P + ks * 32 + g8);
+        z[k] = *reinterpret_cast<const b8*>(K + (k * C + j * 16 + col) * P + ks * 32 + g8);
+      }
+      nn[j] = planes_mma<N, N, 3>(x, z, nn[j]);
+      pp[j] = planes_mma<N, N, 3>(y, z, pp[j]);
+    }
+  }
+  for (int m = 0; m < a.group; ++m) {
+    const int hv = hk * a.group + m;
+    const long at = (long)slot * a.d.value_heads + hv;
+    if (wave == 0) {
+      float g = 0.f, b = 0.f;
+      if (lane < len) {
+        g = a.d.g[row * a.d.g_st.bs + (t0 + lane) * a.d.g_st.rs + hv * a.d.g_st.cs];
+        b = a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs];
+      }
+      double x = g < G_MIN ? G_MIN : g;
+      for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+      }
+      const double last = __shfl(x, 63);
+      G[lane] = x;
+      beta[lane] = b;
+      a.G[at * C + lane] = x;
+      float* f = a.fac + at * 4 * C + lane;   // exp(G), beta, exp(G_C - G) beta, exp(G_C)
+      f[0] = expf((float)x);
+      f[C] = b;
+      f[2 * C] = expf((float)(last - x)) * b;
+      f[3 * C] = expf((float)last);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = j * 16 + col;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = wave * 16 + r4 + e;
+        const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
+        A[r * PC + c] = r > c ? nn[j][e] * D * beta[c] : 0.f;
+        M[r * PC + c] = r >= c ? pp[j][e] * D : 0.f;
+      }
+    }
+    __syncthreads();
+    store_square<OutPlanes<T>::N>(M, a.Pf + at * OutPlanes<T>::N * TF, t);
+    __syncthreads();
+    unit_lower_inverse(A, M, tmp, wave, lane);
+    store_square<3>(M, a.Tf + at * 3 * TF, t);
+    __syncthreads();
+  }
+}
+
+// ---- the scan: NT tiles of 16 columns of dv of one value head of one sequence ------------------------------------------------
+// Bound by the chain from chunk to chunk: K S (each wave with its own rows of S from its accumulators, partial sums through
+// LDS), X, E = T X, K^T U.  Fragments are loaded for the next chunk as soon as this chunk has used them.
+template <typename T, int DK, int NT>
+__global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
+  constexpr int N = Planes<T>::N, RT = DK / 64, PT = C + 8;
+  __shared__ f4 part[4][4][NT][64];              // K S: wave, row block
+  __shared__ __align__(16) __bf16 X[3][NT * 16][PT], U[3][NT * 16][PT];
+  const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / (NT * 16);
+  int slice, head;
+  if (!scan_coords(blockIdx.x, slices, heads, slice, head)) return;
+  const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
+  const int c0 = slice * NT * 16;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15,
+            g8 = (lane >> 4) * 8;
+  const long row = a.p.row(s);
+  const int begin = a.p.begin(s), end = a.p.end(s), chunks = (end - begin + C - 1) / C;
+  const int slot0 = a.p.slot0(s);
+  f4 S[RT][NT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
+        S[i][j][e] = a.state != nullptr && r < a.d.dk && c < a.d.dv ? a.state[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
+      }
+  b8 kf[4][N], tf[2][3], kt[RT][2][N];
+  T v[NT][4];   // converted where they are used: a conversion here would wait for the load
+  f4 eg, tb;
+  float keep = 1.f;
+  const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + hv * a.d.v_st.cs + c0;
+  auto load_k = [&](int n) {
+    const __bf16* p = a.Kf + ((long)(slot0 + n) * a.d.key_heads + hk) * N * KF + lane * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) kf[i][k] = *reinterpret_cast<const b8*>(p + k * KF + (i * 4 + wave) * 512);
+  };
+  // Every load is issued whatever the chunk holds (behind the end it repeats the last token's, which is then not used): loads
+  // behind branches would make the compiler wait for all of them at once.
+  int vcol[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) vcol[j] = min(j * 16 + col, a.d.dv - 1 - c0);   // may be negative: the slice's columns are padding
+  auto load_v = [&](int n) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = V[(long)min(begin + n * C + wave * 16 + r4 + e, end - 1) * a.d.v_st.rs + vcol[j]];
+    eg = *reinterpret_cast<const f4*>(a.fac + ((long)(slot0 + n) * a.d.value_heads + hv) * 4 * C + wave * 16 + r4);
+  };
+  auto load_t = [&](int n) {
+    const long at = (long)(slot0 + n) * a.d.value_heads + hv;
+    const __bf16* p = a.Tf + at * 3 * TF + lane * 8;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      tf[0][k] = *reinterpret_cast<const b8*>(p + k * TF + wave * 2 * 512);
+      tf[1][k] = *reinterpret_cast<const b8*>(p + k * TF + (wave * 2 + 1) * 512);
+    }
+    tb = *reinterpret_cast<const f4*>(a.fac + at * 4 * C + 2 * C + wave * 16 + r4);
+  };
+  auto load_kt = [&](int n) {
+    const __bf16* p = a.KTf + ((long)(slot0 + n) * a.d.key_heads + hk) * N * (DK * C) + lane * 8;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          kt[i][ks][k] = *reinterpret_cast<const b8*>(p + k * (DK * C) + ((wave * RT + i) * 2 + ks) * 512);
+    keep = a.fac[((long)(slot0 + n) * a.d.value_heads + hv) * 4 * C + 3 * C];
+  };
+  if (chunks > 0) {
+    load_k(0);
+    load_v(0);
+    load_t(0);
+    load_kt(0);
+  }
+  for (int n = 0; n < chunks; ++n) {
+    const long at = (long)(slot0 + n) * a.d.value_heads + hv;
+    const int next = min(n + 1, chunks - 1), live = end - begin - n * C - wave * 16 - r4;   // rows e < live hold tokens
+    // S as planes and to memory
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = S[0][j][e];
+        x[4 + e] = RT == 2 ? S[RT - 1][j][e] : 0.f;
+      }
+      b8 sb[3];
+      split<8, 3>(x, sb);
+      f4* dst = reinterpret_cast<f4*>(a.S + ((at * (a.dvp / 16) + c0 / 16 + j) * 4 + wave) * 512 + lane * 8);
+      dst[0] = S[0][j];
+      if (RT == 2) dst[1] = S[RT - 1][j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[wave][i][j][lane] = planes_mma<N, 3, 3>(kf[i], sb, f4{0, 0, 0, 0});
+    }
+    load_k(next);
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const f4 p = (part[0][wave][j][lane] + part[1][wave][j][lane]) + (part[2][wave][j][lane] + part[3][wave][j][lane]);
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = e < live && c0 + j * 16 + col < a.d.dv ? fmaf(-eg[e], p[e], (float)v[j][e]) : 0.f;
+      b4 xp[3];
+      split<4, 3>(x, xp);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&X[k][j * 16 + col][wave * 16 + r4]) = xp[k];
+    }
+    load_v(next);
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      f4 ev = {0, 0, 0, 0};
+      b8 xb[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][g8]);
+      ev = planes_mma<3, 3, 3>(tf[0], xb, ev);
+      if (wave >= 2) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][32 + g8]);
+        ev = planes_mma<3, 3, 3>(tf[1], xb, ev);
+      }
+      *reinterpret_cast<f4*>(a.E + (at * a.dvp + c0 + j * 16 + col) * C + wave * 16 + r4) = ev;
+      float u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = tb[e] * ev[e];
+      b4 up[3];
+      split<4, 3>(u, up);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&U[k][j * 16 + col][wave * 16 + r4]) = up[k];
+    }
+    load_t(next);
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) S[i][j] *= keep;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        b8 ub[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) ub[k] = *reinterpret_cast<const b8*>(&U[k][j * 16 + col][ks * 32 + g8]);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) S[i][j] = planes_mma<N, 3, 3>(kt[i][ks], ub, S[i][j]);
+      }
+    }
+    load_kt(next);
+  }
+  if (a.state_out != nullptr) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
+          if (r < a.d.dk && c < a.d.dv) a.state_out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][j][e];
+        }
+  }
+}
+
+// ---- outputs: one chunk, 64 columns of dv, a wave for each 16 ----------------------------------------------------------------
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_out_kernel(const Args a) {
+  constexpr int N = Planes<T>::N, NO = OutPlanes<T>::N, RT = DK / 64;
+  constexpr int LIM = NO;   // planes i + j kept
+  __shared__ __align__(16) T st[C][64 + 8];
+  const int groups = (a.dvp + 63) / 64;
+  const int cg = blockIdx.x % groups;
+  const long at = blockIdx.x / groups;   // slot * value_heads + hv
+  const int hv = (int)(at % a.d.value_heads), slot = (int)(at / a.d.value_heads), hk = hv / a.group;
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (len == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
+  const int ct = cg * 4 + wave;   // column tile
+  if (ct * 16 < a.dvp) {
+    const float* fac = a.fac + at * 4 * C;
+    b8 sb[4][NO], ub[2][NO];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float* p = a.S + ((at * (a.dvp / 16) + ct) * 4 + w) * 512 + lane * 8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = RT == 2 || e < 4 ? p[e] : 0.f;
+      split<8, NO>(x, sb[w]);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const float* p = a.E + (at * a.dvp + ct * 16 + col) * C + ks * 32 + g8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = p[e] * fac[C + ks * 32 + g8 + e];
+      split<8, NO>(x, ub[ks]);
+    }
+    const __bf16* qf = a.Qf + ((long)slot * a.d.key_heads + hk) * N * KF + lane * 8;
+    const __bf16* pf = a.Pf + at * NO * TF + lane * 8;
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      f4 o = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        b8 q[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) q[k] = *reinterpret_cast<const b8*>(qf + k * KF + (rb * 4 + w) * 512);
+        o = planes_mma<N, NO, N == 2 ? 3 : LIM>(q, sb[w], o);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= fac[rb * 16 + r4 + e];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks * 2 > rb) continue;
+        b8 p[NO];
+#pragma unroll
+        for (int k = 0; k < NO; ++k) p[k] = *reinterpret_cast<const b8*>(pf + k * TF + (rb * 2 + ks) * 512);
+        o = planes_mma<NO, NO, LIM>(p, ub[ks], o);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[rb * 16 + r4 + e][wave * 16 + col] = (T)(a.scale * o[e]);
+    }
+  }
+  __syncthreads();
+  const int c0 = cg * 64, w = min(64, a.d.dv - c0);
+  T* out = reinterpret_cast<T*>(a.o) + ((a.p.row(s) * a.d.tokens + t0) * a.d.value_heads + hv) * (long)a.d.dv + c0;
+  const long rs = (long)a.d.value_heads * a.d.dv;
+  constexpr int V = 16 / sizeof(T);
+  if (w == 64 && (a.d.dv * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0) {
+    for (int i = t; i < C * 64 / V; i += 256) {
+      const int r = i / (64 / V), c = i % (64 / V) * V;
+      if (r < len) *reinterpret_cast<uint4*>(out + r * rs + c) = *reinterpret_cast<const uint4*>(&st[r][c]);
+    }
+  } else {
+    for (int i = t; i < C * 64; i += 256) {
+      const int r = i >> 6, c = i & 63;
+      if (r < len && c < w) out[r * rs + c] = st[r][c];
+    }
+  }
+}
+
 // ---- the recurrence itself ---------------------------------------------------------------------------------------------
 // 64 columns of a state per workgroup: thread = 4 columns x RPT rows, in registers for all of its tokens.  One
 // reduction per token, since o = scale (q^T Sbar + (q . k) beta e).
@@ -785,6 +1314,8 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Parts of a workspace, in this order (use 0: forward, 1: forward that saves, 2: scratch of backward); nullptr base:
 // sizes only.
+bool recurrent(const gpx_delta* d, int save) { return !save && d->tokens <= RECURRENT_MAX; }
+
 size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
   const size_t heads = (size_t)slots_of(d) * d->value_heads, dvp = (size_t)(d->dv + DVT - 1) / DVT * DVT;
   size_t at = 0;
@@ -798,11 +1329,24 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
   if (use < 2) {
     char* p = part(d->sequences > 0 ? (size_t)(d->sequences + 1) * 4 : 0);
     if (off != nullptr) *off = reinterpret_cast<int*>(p);
+  }
+  if (use == 0 && !recurrent(d, 0)) {
+    const size_t kheads = (size_t)slots_of(d) * d->key_heads, dkp = d->dk <= 64 ? 64 : 128;
+    const size_t n = d->dtype == GPX_F32 ? 3 : d->dtype == GPX_F16 ? 2 : 1, no = d->dtype == GPX_F32 ? 3 : 2;
+    x.G = reinterpret_cast<double*>(part(heads * C * 8));
+    x.fac = reinterpret_cast<float*>(part(heads * 4 * C * 4));
+    x.Kf = reinterpret_cast<__bf16*>(part(kheads * n * KF * 2));
+    x.Qf = reinterpret_cast<__bf16*>(part(kheads * n * KF * 2));
+    x.KTf = reinterpret_cast<__bf16*>(part(kheads * n * dkp * C * 2));
+    x.Tf = reinterpret_cast<__bf16*>(part(heads * 3 * TF * 2));
+    x.Pf = reinterpret_cast<__bf16*>(part(heads * no * TF * 2));
+    x.E = reinterpret_cast<float*>(part(heads * C * dvp * 4));
+    x.S = reinterpret_cast<float*>(part(heads * 128 * dvp * 4));
+  }
+  if (use == 1) {
     x.G = reinterpret_cast<double*>(part(heads * C * 8));
     x.T = reinterpret_cast<float*>(part(heads * C * C * 4));
     x.P = reinterpret_cast<float*>(part(heads * C * C * 4));
-  }
-  if (use == 1) {
     x.E = reinterpret_cast<float*>(part(heads * C * dvp * 4));
     x.S = reinterpret_cast<float*>(part(heads * d->dk * dvp * 4));
   }
@@ -813,8 +1357,6 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
   }
   return at;
 }
-
-bool recurrent(const gpx_delta* d, int save) { return !save && d->tokens <= RECURRENT_MAX; }
 
 int check_delta(const gpx_delta* d, const char* what) {
   GPX_REQUIRE(d != nullptr, "%s: null description", what);
@@ -869,6 +1411,27 @@ unsigned scan_grid(const Args& a) {
 }
 
 template <typename T, int DK>
+int run_chunks(hipStream_t s, const Args& a) {
+  constexpr int N = Planes<T>::N;
+  constexpr size_t lds = 2 * N * C * (DK + 8) * 2 + (2 * C * PC + 4 * 16 * 20) * 4 + C * 8 + C * 4;
+  static_assert(lds <= 160 * 1024, "LDS");
+  DELTA_TRY(allow_lds(&delta_chunk_kernel<T, DK>, lds));
+  const long slots = slots_of(&a.d);
+  if (slots > 0) {
+    hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(256), lds, s, a);
+    GPX_HIP(hipGetLastError());
+  }
+  const unsigned heads = (unsigned)a.p.sequences * a.d.value_heads;
+  hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1>), dim3((heads + 7) / 8 * 8 * (a.dvp / 16)), dim3(256), 0, s, a);
+  GPX_HIP(hipGetLastError());
+  if (slots > 0) {
+    hipLaunchKernelGGL((delta_out_kernel<T, DK>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
+    GPX_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+template <typename T, int DK>
 int run_forward(hipStream_t s, const Args& a, int rec) {
   if (rec) {
     StepArgs x = {a, nullptr, 0, 0};
@@ -877,6 +1440,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
     GPX_HIP(hipGetLastError());
     return 0;
   }
+  if (!a.save) return run_chunks<T, DK>(s, a);
   constexpr size_t prep = (2 * C * (DK + 4) + C * PC) * 4 + C * 8 + C * 4;
   constexpr size_t scan = (2 * C * (DK + 4) + 2 * C * PC + DK * PV + 2 * C * PV + 3 * C) * 4;
   static_assert(scan <= 160 * 1024, "LDS");
