@@ -80,7 +80,7 @@ SIGNATURES = {
                                C.POINTER(Strided), _dp, C.POINTER(Strided), _dp, _sz]),
     "gpx_orthogonalize_work_bytes": (_sz, [_i, _i, _i, _i]),
     "gpx_delta_work_bytes": (_sz, [C.POINTER(Delta), _i]),
-    "gpx_delta_forward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, _dp, _dp, _i, _dp, _sz]),
+    "gpx_delta_forward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, _dp, _dp, _dp, _sz, _dp, _sz]),
     "gpx_delta_backward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, C.POINTER(Strided), _dp, _dp, _dp, _dp, _dp, _dp, _dp,
                                 _dp, _sz, _dp, _sz]),
     "gpx_delta_step": (_i, [C.c_void_p, C.POINTER(Delta), _i, _dp, _dp, _dp, _dp]),

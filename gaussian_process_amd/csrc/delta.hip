@@ -23,6 +23,7 @@
 // the recurrence itself.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gpx_internal.h"
 
@@ -32,7 +33,6 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int C = 64;          // tokens per chunk
 constexpr int DVT = 32;        // columns of a slice of dv
-constexpr int PV = 40;         // LDS pitch of [..][DVT] tiles: rows 40 banks apart, 4 rows at a time nearly conflict-free
 constexpr int PC = 68;         // LDS pitch of [..][64] tiles
 constexpr float G_MIN = -200.f;
 
@@ -88,11 +88,17 @@ struct Args {
   int group;                    // value heads per key head
   int dvp;                      // dv rounded up to DVT
   float scale;
-  // per (slot, value head): T and P (C x C), G (C doubles), E and dX (C x dvp), S and dS (dk x dvp)
-  float *T, *P, *E, *dX, *S, *dS, *part;
-  double* G;
-  __bf16 *Kf, *Qf, *KTf, *Tf, *Pf;   // fragments: K, Q, K^T per (slot, key head), T and P per (slot, value head)
-  float* fac;                        // per (slot, value head): exp(G), beta, exp(G_C - G) beta, exp(G_C); C each
+  // Parts of the workspaces; "per key head", "per head": of a slot and a key or value head.  Fragments are explained below.
+  double* G;                    // per head: C
+  float* fac;                   // per head: exp(G), beta, exp(G_C - G) beta, exp(G_C), exp(G_C - G), exp(G) beta; C each
+  __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
+  __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
+  void* V;                      // per head: V^T, dvp x C, of the inputs' type
+  float *E, *Erow;              // per head: E^T, dvp x C; E, C x dvp
+  float *S, *Srow;              // per head: S in state order, dvp / 16 x 4 x 64 x 8; S, DK x dvp
+  float* Y;                     // per head: (scale P^T dO)^T, dvp x C
+  __bf16* Of;                   // per head: scale exp(G) dO as fragments, dvp / 16 x 2 x 64 x 8 by three planes
+  float *Z, *dS;                // per head: Z (dX = beta Z), C x dvp; dS', DK x dvp
   const float *state, *d_state_out;
   float *state_out, *d_state, *d_g, *d_beta;
   void *o, *d_q, *d_k, *d_v;
@@ -112,518 +118,16 @@ __device__ __forceinline__ f4 mm(const float* A, int pa, const float* B, int pb,
   const float* a = TA ? A + g * pa + r : A + r * pa + g;
   const float* b = TB ? B + r * pb + g : B + g * pb + r;
   const int sa = TA ? 4 * pa : 4, sb = TB ? 4 : 4 * pb;
-#pragma unroll 4
   for (int k = 0; k < K; k += 4, a += sa, b += sb) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(*a, *b, acc, 0, 0, 0);
   return acc;
 }
 
-// tokens t0 .. t0 + len of one head, rows of w elements, into an LDS tile of C rows x W (pitch p); zeros elsewhere
-template <typename T, int W>
-__device__ __forceinline__ void load_rows(float* dst, int p, const void* src, const gpx_strided& s, long row, int t0, int len, int head,
-                                          int c0, int w, int nt) {
-  const long base = row * s.bs + t0 * s.rs + head * s.cs + c0;
-  for (int i = threadIdx.x; i < C * W; i += nt) {
-    const int r = i / W, c = i % W;
-    dst[r * p + c] = r < len && c < w ? ld<T>(src, base + r * s.rs + c) : 0.f;
-  }
-}
-
-// ---- prep: one chunk of one value head -----------------------------------------------------------------------------
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_prep_kernel(const Args a) {
-  constexpr int PK = DK + 4;
-  extern __shared__ __align__(16) char smem[];
-  float* K = reinterpret_cast<float*>(smem);
-  float* Q = K + C * PK;
-  float* A = Q + C * PK;
-  double* G = reinterpret_cast<double*>(A + C * PC);
-  float* beta = reinterpret_cast<float*>(G + C);
-  const int hv = blockIdx.x % a.d.value_heads, slot = blockIdx.x / a.d.value_heads;
-  int s, t0, len;
-  a.p.locate(slot, s, t0, len);
-  if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, hk = hv / a.group;
-  const long row = a.p.row(s);
-  load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 256);
-  load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 256);
-  const long at = (long)slot * a.d.value_heads + hv;
-  if (wave == 0) {
-    float g = 0.f, b = 0.f;
-    if (lane < len) {
-      g = a.d.g[row * a.d.g_st.bs + (t0 + lane) * a.d.g_st.rs + hv * a.d.g_st.cs];
-      b = a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs];
-    }
-    double x = g < G_MIN ? G_MIN : g;
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
-    G[lane] = x;
-    beta[lane] = b;
-    a.G[at * C + lane] = x;
-  }
-  __syncthreads();
-  // K K^T and Q K^T: wave w the rows 16 w ..
-  for (int j = 0; j < 4; ++j) {
-    f4 n = {0, 0, 0, 0}, p = {0, 0, 0, 0};
-    if (j <= wave) {
-      n = mm<false, true>(K + wave * 16 * PK, PK, K + j * 16 * PK, PK, DK, n);
-      p = mm<false, true>(Q + wave * 16 * PK, PK, K + j * 16 * PK, PK, DK, p);
-    }
-    const int c = j * 16 + (lane & 15);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = wave * 16 + (lane >> 4) * 4 + e;
-      const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
-      A[r * PC + c] = r > c ? n[e] * D * beta[c] : 0.f;
-      a.P[at * C * C + r * C + c] = r >= c ? p[e] * D : 0.f;
-    }
-  }
-  __syncthreads();
-  if (wave == 0) {   // T = (I + A)^-1, lane c its column c
-    float x[C];
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      float v = i == lane ? 1.f : 0.f;
-#pragma unroll
-      for (int l = 0; l < i; ++l) v = fmaf(-A[i * PC + l], x[l], v);
-      x[i] = v;
-      a.T[at * C * C + i * C + lane] = v;
-    }
-  }
-}
-
-// ---- scan: one slice of dv of one value head of one sequence ----------------------------------------------------------
 // Slices of a head read the same keys: blocks with equal id % 8 share an XCD and its L2.
 __device__ __forceinline__ bool scan_coords(unsigned id, int slices, int heads, int& slice, int& head) {
   const unsigned per = 8u * slices;
   head = (int)(id / per * 8 + id % 8);
   slice = (int)(id % per / 8);
   return head < heads;
-}
-
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_scan_kernel(const Args a) {
-  constexpr int PK = DK + 4, RT = DK / 64;   // row tiles of S per wave
-  extern __shared__ __align__(16) char smem[];
-  float* K = reinterpret_cast<float*>(smem);
-  float* Q = K + C * PK;
-  float* Tm = Q + C * PK;
-  float* Pm = Tm + C * PC;
-  float* S = Pm + C * PC;        // DK x DVT
-  float* X = S + DK * PV;        // C x DVT, then exp(G_C - G) U
-  float* U = X + C * PV;
-  float* eg = U + C * PV;        // exp(G), exp(G_C - G), beta
-  float* tail = eg + C;
-  float* beta = tail + C;
-  int slice, head;
-  if (!scan_coords(blockIdx.x, a.dvp / DVT, a.p.sequences * a.d.value_heads, slice, head)) return;
-  const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
-  const int c0 = slice * DVT, w = min(DVT, a.d.dv - c0);
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15;
-  const long row = a.p.row(s);
-  const int begin = a.p.begin(s), end = a.p.end(s);
-  f4 acc[RT][2];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
-        acc[i][j][e] = a.state != nullptr && r < a.d.dk && c < w ? a.state[((long)head * a.d.dk + r) * a.d.dv + c0 + c] : 0.f;
-      }
-  for (int t0 = begin, slot = a.p.slot0(s); t0 < end; t0 += C, ++slot) {
-    const int len = min(C, end - t0);
-    const long at = (long)slot * a.d.value_heads + hv;
-    load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 256);
-    load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 256);
-    load_rows<T, DVT>(X, PV, a.d.v, a.d.v_st, row, t0, len, hv, c0, w, 256);
-    for (int i = t; i < C * C; i += 256) {
-      Tm[(i >> 6) * PC + (i & 63)] = a.T[at * C * C + i];
-      Pm[(i >> 6) * PC + (i & 63)] = a.P[at * C * C + i];
-    }
-    const double last = a.G[at * C + C - 1];
-    if (wave == 0) {
-      const double g = a.G[at * C + lane];
-      eg[lane] = expf((float)g);
-      tail[lane] = expf((float)(last - g));
-      beta[lane] = lane < len ? a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
-          S[r * PV + c] = acc[i][j][e];
-          if (a.save && r < a.d.dk) a.S[(at * a.d.dk + r) * a.dvp + c0 + c] = acc[i][j][e];
-        }
-    __syncthreads();
-    f4 o[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f4 zero = {0, 0, 0, 0};
-      const f4 ks = mm<false, false>(K + wave * 16 * PK, PK, S + j * 16, PV, DK, zero);
-      o[j] = mm<false, false>(Q + wave * 16 * PK, PK, S + j * 16, PV, DK, zero);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = wave * 16 + r4 + e;
-        X[r * PV + j * 16 + col] -= eg[r] * ks[e];
-        o[j][e] *= eg[r];
-      }
-    }
-    __syncthreads();
-    f4 ev[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f4 zero = {0, 0, 0, 0};
-      ev[j] = mm<false, false>(Tm + wave * 16 * PC, PC, X + j * 16, PV, 16 * wave + 16, zero);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = wave * 16 + r4 + e, c = j * 16 + col;
-        const float u = beta[r] * ev[j][e];
-        U[r * PV + c] = u;
-        X[r * PV + c] = tail[r] * u;
-        if (a.save) a.E[(at * C + r) * a.dvp + c0 + c] = ev[j][e];
-      }
-    __syncthreads();
-    const float keep = expf((float)last);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      o[j] = mm<false, false>(Pm + wave * 16 * PC, PC, U + j * 16, PV, 16 * wave + 16, o[j]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = wave * 16 + r4 + e, c = j * 16 + col;
-        if (r < len && c < w)
-          st<T>(a.o, ((row * a.d.tokens + t0 + r) * a.d.value_heads + hv) * (long)a.d.dv + c0 + c, a.scale * o[j][e]);
-      }
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        acc[i][j] *= keep;
-        acc[i][j] = mm<true, false>(K + (wave * RT + i) * 16, PK, X + j * 16, PV, C, acc[i][j]);
-      }
-    }
-    __syncthreads();
-  }
-  if (a.state_out != nullptr) {
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
-          if (r < a.d.dk && c < w) a.state_out[((long)head * a.d.dk + r) * a.d.dv + c0 + c] = acc[i][j][e];
-        }
-  }
-}
-
-// ---- reverse scan: dS from the last chunk to the first ---------------------------------------------------------------
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_back_kernel(const Args a) {
-  constexpr int PK = DK + 4, RT = DK / 64;
-  extern __shared__ __align__(16) char smem[];
-  float* K = reinterpret_cast<float*>(smem);
-  float* Q = K + C * PK;
-  float* Tm = Q + C * PK;
-  float* Pm = Tm + C * PC;
-  float* S = Pm + C * PC;        // dS', DK x DVT
-  float* Y = S + DK * PV;        // dO, then scale exp(G) dO
-  float* Z = Y + C * PV;         // beta dU, then exp(G) dX
-  float* eg = Z + C * PV;
-  float* tail = eg + C;
-  float* beta = tail + C;
-  int slice, head;
-  if (!scan_coords(blockIdx.x, a.dvp / DVT, a.p.sequences * a.d.value_heads, slice, head)) return;
-  const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
-  const int c0 = slice * DVT, w = min(DVT, a.d.dv - c0);
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15;
-  const long row = a.p.row(s);
-  const int begin = a.p.begin(s), end = a.p.end(s), chunks = (end - begin + C - 1) / C;
-  f4 acc[RT][2];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
-        acc[i][j][e] =
-            a.d_state_out != nullptr && r < a.d.dk && c < w ? a.d_state_out[((long)head * a.d.dk + r) * a.d.dv + c0 + c] : 0.f;
-      }
-  for (int n = chunks - 1; n >= 0; --n) {
-    const int t0 = begin + n * C, slot = a.p.slot0(s) + n, len = min(C, end - t0);
-    const long at = (long)slot * a.d.value_heads + hv;
-    load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 256);
-    load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 256);
-    load_rows<T, DVT>(Y, PV, a.d_o, a.do_st, row, t0, len, hv, c0, w, 256);
-    for (int i = t; i < C * C; i += 256) {
-      Tm[(i >> 6) * PC + (i & 63)] = a.T[at * C * C + i];
-      Pm[(i >> 6) * PC + (i & 63)] = a.P[at * C * C + i];
-    }
-    const double last = a.G[at * C + C - 1];
-    if (wave == 0) {
-      const double g = a.G[at * C + lane];
-      eg[lane] = expf((float)g);
-      tail[lane] = expf((float)(last - g));
-      beta[lane] = lane < len ? a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
-          S[r * PV + c] = acc[i][j][e];
-          if (r < a.d.dk) a.dS[(at * a.d.dk + r) * a.dvp + c0 + c] = acc[i][j][e];
-        }
-    __syncthreads();
-    float dots[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f4 zero = {0, 0, 0, 0};
-      const f4 kd = mm<false, false>(K + wave * 16 * PK, PK, S + j * 16, PV, DK, zero);
-      // P^T dO: rows of P from this row block on
-      const f4 po = mm<true, false>(Pm + wave * 16 * PC + wave * 16, PC, Y + wave * 16 * PV + j * 16, PV, C - 16 * wave, zero);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = wave * 16 + r4 + e, c = j * 16 + col;
-        const float du = a.scale * po[e] + tail[r] * kd[e];
-        Z[r * PV + c] = beta[r] * du;
-        dots[e] = fmaf(a.E[(at * C + r) * a.dvp + c0 + c], du, dots[e]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {   // E . dU of this slice, per row
-      for (int m = 1; m < 16; m <<= 1) dots[e] += __shfl_xor(dots[e], m);
-      if (col == 0) a.part[(at * (a.dvp / DVT) + slice) * C + wave * 16 + r4 + e] = dots[e];
-    }
-    __syncthreads();
-    f4 dx[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f4 zero = {0, 0, 0, 0};
-      dx[j] = mm<true, false>(Tm + wave * 16 * PC + wave * 16, PC, Z + wave * 16 * PV + j * 16, PV, C - 16 * wave, zero);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = wave * 16 + r4 + e, c = j * 16 + col;
-        a.dX[(at * C + r) * a.dvp + c0 + c] = dx[j][e];
-        Z[r * PV + c] = -eg[r] * dx[j][e];
-        Y[r * PV + c] *= a.scale * eg[r];
-      }
-    __syncthreads();
-    const float keep = expf((float)last);
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        acc[i][j] *= keep;
-        acc[i][j] = mm<true, false>(Q + (wave * RT + i) * 16, PK, Y + j * 16, PV, C, acc[i][j]);
-        acc[i][j] = mm<true, false>(K + (wave * RT + i) * 16, PK, Z + j * 16, PV, C, acc[i][j]);
-      }
-    __syncthreads();
-  }
-  if (a.d_state != nullptr) {
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = (wave * RT + i) * 16 + r4 + e, c = j * 16 + col;
-          if (r < a.d.dk && c < w) a.d_state[((long)head * a.d.dk + r) * a.d.dv + c0 + c] = acc[i][j][e];
-        }
-  }
-}
-
-// ---- grads: one chunk of one key head, its value heads one after the other ------------------------------------------
-// 8 waves.  Products with C rows and DK columns: wave w the 16 rows of block w & 3 and the columns of half w >> 2.
-template <typename T, int DK>
-__global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
-  constexpr int PK = DK + 4, CT = DK / 32;   // column tiles of 16 per wave
-  extern __shared__ __align__(16) char smem[];
-  float* K = reinterpret_cast<float*>(smem);
-  float* Q = K + C * PK;
-  float* S = Q + C * PK;         // slices of S and dS', later M1 and M2 (C x C)
-  float* dS = S + DK * PV;
-  float* E = dS + DK * PV;       // slices of E, dX, dO, U
-  float* dX = E + C * PV;
-  float* Y = dX + C * PV;
-  float* U = Y + C * PV;
-  double* G = reinterpret_cast<double*>(U + C * PV);
-  float* beta = reinterpret_cast<float*>(G + C);
-  float* dG = beta + C;          // 2 x C: the two column halves
-  float* colb = dG + 2 * C;      // dbeta's sums over the rows, one per wave row block (4 x C)
-  float* red = colb + 4 * C;     // 8 + 1
-  float* M1 = S;
-  float* M2 = M1 + C * PC;
-  static_assert(2 * C * PC <= 2 * DK * PV + 4 * C * PV, "M1 and M2 lie over the slices");
-  const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
-  int s, t0, len;
-  a.p.locate(slot, s, t0, len);
-  if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15;
-  const int rb = wave & 3, ch = wave >> 2;   // row block, column half
-  const long row = a.p.row(s);
-  load_rows<T, DK>(K, PK, a.d.k, a.d.k_st, row, t0, len, hk, 0, a.d.dk, 512);
-  load_rows<T, DK>(Q, PK, a.d.q, a.d.q_st, row, t0, len, hk, 0, a.d.dk, 512);
-  f4 dq[CT], dk[CT];   // over the value heads
-#pragma unroll
-  for (int j = 0; j < CT; ++j) dq[j] = dk[j] = f4{0, 0, 0, 0};
-  for (int m = 0; m < a.group; ++m) {
-    const int hv = hk * a.group + m;
-    const long at = (long)slot * a.d.value_heads + hv;
-    if (wave == 0) {
-      G[lane] = a.G[at * C + lane];
-      beta[lane] = lane < len ? a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs] : 0.f;
-    }
-    f4 q1[CT], kr[CT], kc[CT], dp[2], da[2];
-#pragma unroll
-    for (int j = 0; j < CT; ++j) q1[j] = kr[j] = kc[j] = f4{0, 0, 0, 0};
-    dp[0] = dp[1] = da[0] = da[1] = f4{0, 0, 0, 0};
-    float ss = 0.f;
-    for (int c0 = 0; c0 < a.dvp; c0 += DVT) {
-      const int w = min(DVT, a.d.dv - c0);
-      __syncthreads();
-      for (int i = t; i < DK * DVT; i += 512) {
-        const int r = i / DVT, c = i % DVT;
-        const long p = (at * a.d.dk + r) * a.dvp + c0 + c;
-        const float x = r < a.d.dk ? a.S[p] : 0.f, y = r < a.d.dk ? a.dS[p] : 0.f;
-        S[r * PV + c] = x;
-        dS[r * PV + c] = y;
-        ss = fmaf(x, y, ss);
-      }
-      for (int i = t; i < C * DVT; i += 512) {
-        const int r = i / DVT, c = i % DVT;
-        const long p = (at * C + r) * a.dvp + c0 + c;
-        const float e = a.E[p], x = a.dX[p];
-        E[r * PV + c] = e;
-        U[r * PV + c] = beta[r] * e;
-        dX[r * PV + c] = x;
-        if (r < len && c < w) st<T>(a.d_v, ((row * a.d.tokens + t0 + r) * a.d.value_heads + hv) * (long)a.d.dv + c0 + c, x);
-      }
-      load_rows<T, DVT>(Y, PV, a.d_o, a.do_st, row, t0, len, hv, c0, w, 512);
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int cb = ch * 2 + j;
-        if (cb <= rb) {
-          dp[j] = mm<false, true>(Y + rb * 16 * PV, PV, U + cb * 16 * PV, PV, DVT, dp[j]);
-          da[j] = mm<false, true>(dX + rb * 16 * PV, PV, E + cb * 16 * PV, PV, DVT, da[j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const int cb = (ch * CT + j) * 16;
-        q1[j] = mm<false, true>(Y + rb * 16 * PV, PV, S + cb * PV, PV, DVT, q1[j]);
-        kr[j] = mm<false, true>(dX + rb * 16 * PV, PV, S + cb * PV, PV, DVT, kr[j]);
-        kc[j] = mm<false, true>(U + rb * 16 * PV, PV, dS + cb * PV, PV, DVT, kc[j]);
-      }
-    }
-    __syncthreads();   // the slices are done with: M1 and M2 take their place
-    const double last = G[C - 1];
-    for (int o = 32; o > 0; o >>= 1) ss += __shfl_down(ss, o);
-    if (lane == 0) red[wave] = ss;
-    float cj[4] = {0, 0, 0, 0};   // k . state part of dKc
-#pragma unroll
-    for (int j = 0; j < CT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = rb * 16 + r4 + e, c = (ch * CT + j) * 16 + col;
-        const float eg = expf((float)G[r]);
-        q1[j][e] *= a.scale * eg;
-        kr[j][e] *= -eg;
-        kc[j][e] *= expf((float)(last - G[r]));
-        cj[e] = fmaf(K[r * PK + c], kc[j][e], cj[e]);
-      }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int cb = ch * 2 + j;
-      f4 kk = {0, 0, 0, 0};
-      if (cb <= rb) kk = mm<false, true>(K + rb * 16 * PK, PK, K + cb * 16 * PK, PK, DK, kk);
-      const int c = cb * 16 + col;
-      float db = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = rb * 16 + r4 + e;
-        const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
-        M1[r * PC + c] = r >= c ? a.scale * dp[j][e] * D : 0.f;
-        M2[r * PC + c] = r > c ? -da[j][e] * beta[c] * D : 0.f;
-        db -= r > c ? da[j][e] * kk[e] * D : 0.f;
-      }
-      db += __shfl_xor(db, 16);
-      db += __shfl_xor(db, 32);
-      if (lane < 16) colb[rb * C + c] = db;
-    }
-    __syncthreads();
-    float dg[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      const int cb = (ch * CT + j) * 16;
-      q1[j] = mm<false, false>(M1 + rb * 16 * PC, PC, K + cb, PK, 16 * rb + 16, q1[j]);
-      kr[j] = mm<false, false>(M2 + rb * 16 * PC, PC, K + cb, PK, 16 * rb + 16, kr[j]);
-      kc[j] = mm<true, false>(M2 + rb * 16 * PC + rb * 16, PC, K + rb * 16 * PK + cb, PK, C - 16 * rb, kc[j]);
-      kc[j] = mm<true, false>(M1 + rb * 16 * PC + rb * 16, PC, Q + rb * 16 * PK + cb, PK, C - 16 * rb, kc[j]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = rb * 16 + r4 + e, c = cb + col;
-        dg[e] = fmaf(Q[r * PK + c], q1[j][e], fmaf(K[r * PK + c], kr[j][e] - kc[j][e], dg[e]));
-      }
-      dq[j] += q1[j];
-      dk[j] += kr[j] + kc[j];
-    }
-    float csum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      csum += cj[e];
-      for (int o = 1; o < 16; o <<= 1) dg[e] += __shfl_xor(dg[e], o);
-      if (col == 0) dG[ch * C + rb * 16 + r4 + e] = dg[e];
-    }
-    for (int o = 32; o > 0; o >>= 1) csum += __shfl_down(csum, o);
-    __syncthreads();
-    if (lane == 0) red[wave] = fmaf(expf((float)last), red[wave], csum);
-    __syncthreads();
-    if (wave == 0) {
-      float end = 0.f;
-      for (int i = 0; i < 8; ++i) end += red[i];
-      float v = dG[lane] + dG[C + lane] + (lane == C - 1 ? end : 0.f);
-      for (int o = 1; o < 64; o <<= 1) {
-        const float u = __shfl_down(v, o);
-        if (lane + o < 64) v += u;
-      }
-      if (lane < len) {
-        const long p = (row * a.d.tokens + t0 + lane) * a.d.value_heads + hv;
-        a.d_g[p] = v;
-        float b = (colb[lane] + colb[C + lane]) + (colb[2 * C + lane] + colb[3 * C + lane]);
-        const float* part = a.part + at * (a.dvp / DVT) * C + lane;
-        for (int i = 0; i < a.dvp / DVT; ++i) b += part[i * C];
-        a.d_beta[p] = b;
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < CT; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = rb * 16 + r4 + e, c = (ch * CT + j) * 16 + col;
-      if (r < len && c < a.d.dk) {
-        const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + c;
-        st<T>(a.d_q, p, dq[j][e]);
-        st<T>(a.d_k, p, dk[j][e]);
-      }
-    }
 }
 
 // ---- planes -------------------------------------------------------------------------------------------------------------
@@ -706,6 +210,7 @@ __device__ __forceinline__ long frag(int block, int blocks, int ks, int lane) { 
 
 constexpr int KF = 4 * 4 * 64 * 8;   // elements of a plane of K or Q in state order, also of a C x C matrix twice over
 constexpr int TF = 4 * 2 * 64 * 8;   // of a C x C matrix
+constexpr int FACS = 6 * C;          // factors per head
 
 // C rows of one head as planes in LDS, pitch DK + 8
 template <typename T, int DK>
@@ -779,15 +284,15 @@ __device__ __forceinline__ void unit_lower_inverse(const float* A, float* Ti, fl
   }
 }
 
-// rows of a C x C matrix in LDS (pitch PC) as fragments in natural order
-template <int NPL>
+// rows, or with TR columns, of a C x C matrix in LDS (pitch PC) as fragments in natural order
+template <int NPL, bool TR>
 __device__ __forceinline__ void store_square(const float* M, __bf16* dst, int t) {
   for (int i = t; i < TF / 8; i += 256) {
     const int lane = i & 63, ks = i >> 6 & 1, rb = i >> 7;
-    const float* p = M + (rb * 16 + (lane & 15)) * PC + ks * 32 + (lane >> 4) * 8;
+    const int r = rb * 16 + (lane & 15), c = ks * 32 + (lane >> 4) * 8;
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = p[e];
+    for (int e = 0; e < 8; ++e) x[e] = TR ? M[(c + e) * PC + r] : M[r * PC + c + e];
     b8 v[NPL];
     split<8, NPL>(x, v);
 #pragma unroll
@@ -840,10 +345,14 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
     const int c = rb * 16 + (l & 15), r = ks * 32 + (l >> 4) * 8;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      b8 v;
+      b8 v, w;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = K[(k * C + r + e) * P + c];
+      for (int e = 0; e < 8; ++e) {
+        v[e] = K[(k * C + r + e) * P + c];
+        w[e] = Q[(k * C + r + e) * P + c];
+      }
       *reinterpret_cast<b8*>(a.KTf + (atk * N + k) * (DK * C) + i * 8) = v;
+      if (a.save) *reinterpret_cast<b8*>(a.QTf + (atk * N + k) * (DK * C) + i * 8) = w;
     }
   }
   // K K^T and Q K^T: wave w the rows 16 w ..
@@ -883,11 +392,14 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
       G[lane] = x;
       beta[lane] = b;
       a.G[at * C + lane] = x;
-      float* f = a.fac + at * 4 * C + lane;   // exp(G), beta, exp(G_C - G) beta, exp(G_C)
-      f[0] = expf((float)x);
+      float* f = a.fac + at * FACS + lane;
+      const float eg = expf((float)x), tail = expf((float)(last - x));
+      f[0] = eg;
       f[C] = b;
-      f[2 * C] = expf((float)(last - x)) * b;
+      f[2 * C] = tail * b;
       f[3 * C] = expf((float)last);
+      f[4 * C] = tail;
+      f[5 * C] = eg * b;
     }
     __syncthreads();
 #pragma unroll
@@ -902,18 +414,61 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
       }
     }
     __syncthreads();
-    store_square<OutPlanes<T>::N>(M, a.Pf + at * OutPlanes<T>::N * TF, t);
+    store_square<OutPlanes<T>::N, false>(M, a.Pf + at * OutPlanes<T>::N * TF, t);
+    if (a.save) store_square<3, true>(M, a.PTf + at * 3 * TF, t);
     __syncthreads();
     unit_lower_inverse(A, M, tmp, wave, lane);
-    store_square<3>(M, a.Tf + at * 3 * TF, t);
+    store_square<3, false>(M, a.Tf + at * 3 * TF, t);
     __syncthreads();
+    if (a.save) {   // the same with beta from the left
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = j * 16 + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = wave * 16 + r4 + e;
+          A[r * PC + c] = r > c ? nn[j][e] * expf((float)(G[r] - G[c])) * beta[r] : 0.f;
+        }
+      }
+      __syncthreads();
+      unit_lower_inverse(A, M, tmp, wave, lane);
+      store_square<3, true>(M, a.T2f + at * 3 * TF, t);
+      __syncthreads();
+    }
+    // V^T, 64 columns at a time through LDS
+    T* vt = reinterpret_cast<T*>(A);   // C x 66 of T
+    const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + t0 * a.d.v_st.rs + hv * a.d.v_st.cs;
+    for (int c0 = 0; c0 < a.dvp; c0 += 64) {
+      for (int i = t; i < C * 64; i += 256) {
+        const int r = i >> 6, c = i & 63;
+        vt[r * 66 + c] = r < len && c0 + c < a.d.dv ? V[r * a.d.v_st.rs + c0 + c] : T(0);
+      }
+      __syncthreads();
+      for (int i = t; i < min(64, a.dvp - c0) * 8; i += 256) {
+        const int c = i >> 3, r = (i & 7) * 8;
+        T x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = vt[(r + e) * 66 + c];
+        __builtin_memcpy(__builtin_assume_aligned(reinterpret_cast<T*>(a.V) + (at * a.dvp + c0 + c) * C + r, 16), x, sizeof(x));
+      }
+      __syncthreads();
+    }
   }
 }
 
-// ---- the scan: NT tiles of 16 columns of dv of one value head of one sequence ------------------------------------------------
-// Bound by the chain from chunk to chunk: K S (each wave with its own rows of S from its accumulators, partial sums through
-// LDS), X, E = T X, K^T U.  Fragments are loaded for the next chunk as soon as this chunk has used them.
-template <typename T, int DK, int NT>
+// ---- the scans: NT tiles of 16 columns of dv of one value head of one sequence ------------------------------------------------
+// Forward, chunk after chunk:    X = V - exp(G) K S;       E = T X;      S <- exp(G_C) S + K^T (exp(G_C - G) beta E)
+// Backward (BACK), from the last: X = Y + exp(G_C - G) K dS;  Z = T2^T X;   dS <- exp(G_C) dS - K^T (exp(G) beta Z) + Q^T Of
+// (Y = scale P^T dO, Of = scale exp(G) dO, from delta_back_prep_kernel).
+// Bound by the chain from chunk to chunk: the product with K (each wave with its own rows of S, which are in its accumulators;
+// partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.
+// Fragments are loaded for the next chunk as soon as this chunk has used them; every load is issued whatever comes, since loads behind
+// branches make the compiler wait for all that are under way.
+__device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes) {
+  return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
+}
+
+template <typename T, int DK, int NT, bool BACK>
 __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
   constexpr int N = Planes<T>::N, RT = DK / 64, PT = C + 8;
   __shared__ f4 part[4][4][NT][64];              // K S: wave, row block
@@ -925,10 +480,11 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
   const int c0 = slice * NT * 16;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15,
             g8 = (lane >> 4) * 8;
-  const long row = a.p.row(s);
   const int begin = a.p.begin(s), end = a.p.end(s), chunks = (end - begin + C - 1) / C;
-  const int slot0 = a.p.slot0(s);
+  const long slot0 = a.p.slot0(s);
+  const unsigned lb = lane * 16;
   f4 S[RT][NT];
+  const float* init = BACK ? a.d_state_out : a.state;
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -936,63 +492,76 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
-        S[i][j][e] = a.state != nullptr && r < a.d.dk && c < a.d.dv ? a.state[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
+        S[i][j][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
       }
-  b8 kf[4][N], tf[2][3], kt[RT][2][N];
-  T v[NT][4];   // converted where they are used: a conversion here would wait for the load
-  f4 eg, tb;
+  struct Four { T x[4]; };
+  b8 kf[4][N], tf[2][3], kt[RT][2][N], qt[RT][2][N], of[NT][2][3];
+  Four v[NT];
+  f4 y[NT], fx, fu;
   float keep = 1.f;
-  const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + hv * a.d.v_st.cs + c0;
-  auto load_k = [&](int n) {
-    const __bf16* p = a.Kf + ((long)(slot0 + n) * a.d.key_heads + hk) * N * KF + lane * 8;
+  auto load_k = [&](long slot) {
+    const __bf16* p = a.Kf + (slot * a.d.key_heads + hk) * N * KF + wave * 512;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int k = 0; k < N; ++k) kf[i][k] = *reinterpret_cast<const b8*>(p + k * KF + (i * 4 + wave) * 512);
+      for (int k = 0; k < N; ++k) kf[i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
   };
-  // Every load is issued whatever the chunk holds (behind the end it repeats the last token's, which is then not used): loads
-  // behind branches would make the compiler wait for all of them at once.
-  int vcol[NT];
+  auto load_x = [&](long at) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j) vcol[j] = min(j * 16 + col, a.d.dv - 1 - c0);   // may be negative: the slice's columns are padding
-  auto load_v = [&](int n) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[j][e] = V[(long)min(begin + n * C + wave * 16 + r4 + e, end - 1) * a.d.v_st.rs + vcol[j]];
-    eg = *reinterpret_cast<const f4*>(a.fac + ((long)(slot0 + n) * a.d.value_heads + hv) * 4 * C + wave * 16 + r4);
+    for (int j = 0; j < NT; ++j) {
+      const unsigned o = (unsigned)((j * 16 + col) * C + wave * 16 + r4);
+      if (BACK)
+        y[j] = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + o);
+      else
+        __builtin_memcpy(&v[j], __builtin_assume_aligned(reinterpret_cast<const T*>(a.V) + (at * a.dvp + c0) * C + o, 4 * sizeof(T)), sizeof(Four));
+    }
+    fx = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 4 * C : 0) + wave * 16 + r4);
   };
-  auto load_t = [&](int n) {
-    const long at = (long)(slot0 + n) * a.d.value_heads + hv;
-    const __bf16* p = a.Tf + at * 3 * TF + lane * 8;
+  auto load_t = [&](long at) {
+    const __bf16* p = (BACK ? a.T2f : a.Tf) + at * 3 * TF + wave * 2 * 512;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      tf[0][k] = *reinterpret_cast<const b8*>(p + k * TF + wave * 2 * 512);
-      tf[1][k] = *reinterpret_cast<const b8*>(p + k * TF + (wave * 2 + 1) * 512);
+      tf[0][k] = ld_frag(p + k * TF, lb);
+      tf[1][k] = ld_frag(p + k * TF + 512, lb);
     }
-    tb = *reinterpret_cast<const f4*>(a.fac + at * 4 * C + 2 * C + wave * 16 + r4);
+    fu = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 5 : 2) * C + wave * 16 + r4);
   };
-  auto load_kt = [&](int n) {
-    const __bf16* p = a.KTf + ((long)(slot0 + n) * a.d.key_heads + hk) * N * (DK * C) + lane * 8;
+  auto load_kt = [&](long slot, long at) {
+    const long o = (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-          kt[i][ks][k] = *reinterpret_cast<const b8*>(p + k * (DK * C) + ((wave * RT + i) * 2 + ks) * 512);
-    keep = a.fac[((long)(slot0 + n) * a.d.value_heads + hv) * 4 * C + 3 * C];
+        for (int k = 0; k < N; ++k) {
+          kt[i][ks][k] = ld_frag(a.KTf + o + k * (DK * C) + (i * 2 + ks) * 512, lb);
+          if (BACK) qt[i][ks][k] = ld_frag(a.QTf + o + k * (DK * C) + (i * 2 + ks) * 512, lb);
+        }
+    if (BACK) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            of[j][ks][k] = ld_frag(a.Of + (at * 3 + k) * (a.dvp * C) + (c0 / 16 + j) * 1024 + ks * 512, lb);
+    }
+    keep = a.fac[at * FACS + 3 * C];
   };
-  if (chunks > 0) {
-    load_k(0);
-    load_v(0);
-    load_t(0);
-    load_kt(0);
+  {
+    const long slot = slot0 + (BACK ? chunks - 1 : 0), at = slot * a.d.value_heads + hv;
+    if (chunks > 0) {
+      load_k(slot);
+      load_x(at);
+      load_t(at);
+      load_kt(slot, at);
+    }
   }
   for (int n = 0; n < chunks; ++n) {
-    const long at = (long)(slot0 + n) * a.d.value_heads + hv;
-    const int next = min(n + 1, chunks - 1), live = end - begin - n * C - wave * 16 - r4;   // rows e < live hold tokens
-    // S as planes and to memory
+    const long slot = slot0 + (BACK ? chunks - 1 - n : n), at = slot * a.d.value_heads + hv;
+    const int more = n + 1 < chunks ? (BACK ? -1 : 1) : 0;
+    const long nslot = slot + more, nat = at + more * a.d.value_heads;
+    // S as planes, and to memory
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float x[8];
@@ -1003,66 +572,113 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
       }
       b8 sb[3];
       split<8, 3>(x, sb);
-      f4* dst = reinterpret_cast<f4*>(a.S + ((at * (a.dvp / 16) + c0 / 16 + j) * 4 + wave) * 512 + lane * 8);
-      dst[0] = S[0][j];
-      if (RT == 2) dst[1] = S[RT - 1][j];
+      f4 p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][i][j][lane] = planes_mma<N, 3, 3>(kf[i], sb, f4{0, 0, 0, 0});
+      for (int i = 0; i < 4; ++i) p[i] = f4{0, 0, 0, 0};
+      // plane by plane over the four row blocks: four chains of matrix instructions side by side
+#pragma unroll
+      for (int m = 2; m >= 0; --m)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (m >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], sb[m - k], p[i], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[wave][i][j][lane] = p[i];
+      if (!BACK) {
+        f4* dst = reinterpret_cast<f4*>(a.S + ((at * (a.dvp / 16) + c0 / 16 + j) * 4 + wave) * 512 + lane * 8);
+        dst[0] = S[0][j];
+        if (RT == 2) dst[1] = S[RT - 1][j];
+      }
+      if (BACK || a.save) {
+        float* dst = (BACK ? a.dS : a.Srow) + (at * DK + wave * RT * 16) * a.dvp + c0 + j * 16;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[(unsigned)((i * 16 + r4 + e) * a.dvp + col)] = S[i][j][e];
+      }
     }
-    load_k(next);
+    load_k(nslot);
     lds_barrier();
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const f4 p = (part[0][wave][j][lane] + part[1][wave][j][lane]) + (part[2][wave][j][lane] + part[3][wave][j][lane]);
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = e < live && c0 + j * 16 + col < a.d.dv ? fmaf(-eg[e], p[e], (float)v[j][e]) : 0.f;
+      for (int e = 0; e < 4; ++e) x[e] = BACK ? fmaf(fx[e], p[e], y[j][e]) : fmaf(-fx[e], p[e], (float)v[j].x[e]);
       b4 xp[3];
       split<4, 3>(x, xp);
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&X[k][j * 16 + col][wave * 16 + r4]) = xp[k];
     }
-    load_v(next);
+    load_x(nat);
     lds_barrier();
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      f4 ev = {0, 0, 0, 0};
+      // T's upper, T2^T's lower half is zeros
+      f4 e0 = {0, 0, 0, 0}, e1 = {0, 0, 0, 0};
       b8 xb[3];
+      if (!BACK || wave < 2) {
 #pragma unroll
-      for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][g8]);
-      ev = planes_mma<3, 3, 3>(tf[0], xb, ev);
-      if (wave >= 2) {
+        for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][g8]);
+        e0 = planes_mma<3, 3, 3>(tf[0], xb, e0);
+      }
+      if (BACK || wave >= 2) {
 #pragma unroll
         for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][32 + g8]);
-        ev = planes_mma<3, 3, 3>(tf[1], xb, ev);
+        e1 = planes_mma<3, 3, 3>(tf[1], xb, e1);
       }
-      *reinterpret_cast<f4*>(a.E + (at * a.dvp + c0 + j * 16 + col) * C + wave * 16 + r4) = ev;
+      const f4 ev = e0 + e1;
       float u[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) u[e] = tb[e] * ev[e];
+      for (int e = 0; e < 4; ++e) u[e] = (BACK ? -fu[e] : fu[e]) * ev[e];
       b4 up[3];
       split<4, 3>(u, up);
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&U[k][j * 16 + col][wave * 16 + r4]) = up[k];
+      if (!BACK) *reinterpret_cast<f4*>(a.E + (at * a.dvp + c0 + j * 16) * C + (unsigned)(col * C + wave * 16 + r4)) = ev;
+      if (BACK || a.save) {
+        float* dst = (BACK ? a.Z : a.Erow) + (at * C + wave * 16) * a.dvp + c0 + j * 16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[(unsigned)((r4 + e) * a.dvp + col)] = ev[e];
+      }
     }
-    load_t(next);
+    load_t(nat);
     lds_barrier();
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+      f4 more_s[RT];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) S[i][j] *= keep;
+      for (int i = 0; i < RT; ++i) {
+        S[i][j] *= keep;
+        more_s[i] = f4{0, 0, 0, 0};
+      }
+      if (BACK) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) more_s[i] = planes_mma<N, 3, 3>(qt[i][ks], of[j][ks], more_s[i]);
+      }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         b8 ub[3];
 #pragma unroll
         for (int k = 0; k < 3; ++k) ub[k] = *reinterpret_cast<const b8*>(&U[k][j * 16 + col][ks * 32 + g8]);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) S[i][j] = planes_mma<N, 3, 3>(kt[i][ks], ub, S[i][j]);
+        for (int i = 0; i < RT; ++i) {
+          if (ks == 0)
+            S[i][j] = planes_mma<N, 3, 3>(kt[i][ks], ub, S[i][j]);
+          else
+            more_s[i] = planes_mma<N, 3, 3>(kt[i][ks], ub, more_s[i]);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) S[i][j] += more_s[i];
     }
-    load_kt(next);
+    load_kt(nslot, nat);
   }
-  if (a.state_out != nullptr) {
+  float* out = BACK ? a.d_state : a.state_out;
+  if (out != nullptr) {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -1070,7 +686,7 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
-          if (r < a.d.dk && c < a.d.dv) a.state_out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][j][e];
+          if (r < a.d.dk && c < a.d.dv) out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][j][e];
         }
   }
 }
@@ -1091,7 +707,7 @@ __global__ __launch_bounds__(256) void delta_out_kernel(const Args a) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
   const int ct = cg * 4 + wave;   // column tile
   if (ct * 16 < a.dvp) {
-    const float* fac = a.fac + at * 4 * C;
+    const float* fac = a.fac + at * FACS;
     b8 sb[4][NO], ub[2][NO];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -1150,6 +766,321 @@ __global__ __launch_bounds__(256) void delta_out_kernel(const Args a) {
       const int r = i >> 6, c = i & 63;
       if (r < len && c < w) out[r * rs + c] = st[r][c];
     }
+  }
+}
+
+// ---- backward, before the scan: Y and Of, a wave for each 16 columns of dv ----------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void delta_back_prep_kernel(const Args a) {
+  constexpr int N = Planes<T>::N;
+  const int groups = (a.dvp + 63) / 64;
+  const int cg = blockIdx.x % groups;
+  const long at = blockIdx.x / groups;
+  const int hv = (int)(at % a.d.value_heads), slot = (int)(at / a.d.value_heads);
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (len == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
+  const int ct = cg * 4 + wave;
+  if (ct * 16 >= a.dvp) return;
+  const int c = ct * 16 + col;
+  const T* dO = reinterpret_cast<const T*>(a.d_o) + a.p.row(s) * a.do_st.bs + t0 * a.do_st.rs + hv * a.do_st.cs + min(c, a.d.dv - 1);
+  const float* fac = a.fac + at * FACS;
+  b8 ob[2][N];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    T raw[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) raw[e] = dO[min(ks * 32 + g8 + e, len - 1) * a.do_st.rs];
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ks * 32 + g8 + e < len && c < a.d.dv ? (float)raw[e] : 0.f;
+    split<8, N>(x, ob[ks]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= a.scale * fac[ks * 32 + g8 + e];
+    b8 scaled[3];
+    split<8, 3>(x, scaled);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      *reinterpret_cast<b8*>(a.Of + (at * 3 + k) * (a.dvp * C) + ct * 1024 + ks * 512 + lane * 8) = scaled[k];
+  }
+  const __bf16* pt = a.PTf + at * 3 * TF + lane * 8;
+#pragma unroll
+  for (int rb = 0; rb < 4; ++rb) {
+    f4 y = {0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks * 2 + 1 < rb) continue;   // P^T is upper triangular
+      b8 p[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) p[k] = *reinterpret_cast<const b8*>(pt + k * TF + (rb * 2 + ks) * 512);
+      y = planes_mma<3, N, 3>(p, ob[ks], y);
+    }
+    *reinterpret_cast<f4*>(a.Y + (at * a.dvp + c) * C + rb * 16 + r4) = y * a.scale;
+  }
+}
+
+// ---- gradients: one chunk of one key head, its value heads one after the other ------------------------------------------------
+// 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
+// memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
+// the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
+template <typename T, int DK>
+__global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
+  constexpr int N = Planes<T>::N, W = DK / 16, P = 40, PM = C + 8;
+  constexpr int SL = C * P;                      // a plane of a slice
+  extern __shared__ __align__(16) char smem[];
+  __bf16* Y = reinterpret_cast<__bf16*>(smem);   // N planes
+  __bf16* X = Y + N * SL;                        // 3
+  __bf16* U = X + 3 * SL;                        // 3
+  __bf16* M = reinterpret_cast<__bf16*>(smem);   // later: a C x C matrix and its transpose, 3 planes each
+  __bf16* MT = M + 3 * C * PM;
+  constexpr size_t ROOM = (N + 6) * SL > 6 * C * PM ? (N + 6) * SL : 6 * C * PM;
+  double* G = reinterpret_cast<double*>(smem + ROOM * 2);
+  float* dG = reinterpret_cast<float*>(G + C);   // 8 x C: per wave
+  float* red = dG + 8 * C;      // 8
+  float* db = red + 8;          // C
+  const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (len == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15,
+            g8 = (lane >> 4) * 8;
+  const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
+  const bool own = wave < W;
+  const int kc0 = wave * 16 + col;   // this lane's column of dk
+  // a thread's place in a slice: four columns of one row
+  const int sr = t >> 3, sc = (t & 7) * 4;
+  f4 dq[4], dk[4];   // over the value heads
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dq[i] = dk[i] = f4{0, 0, 0, 0};
+  for (int m = 0; m < a.group; ++m) {
+    const int hv = hk * a.group + m;
+    const long at = (long)slot * a.d.value_heads + hv;
+    __syncthreads();
+    if (wave == 0) G[lane] = a.G[at * C + lane];
+    const float bt = a.fac[at * FACS + C + sr];
+    f4 q1[4], kr[4], kc[4], dp[2], da[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q1[i] = kr[i] = kc[i] = f4{0, 0, 0, 0};
+    dp[0] = dp[1] = da[0] = da[1] = f4{0, 0, 0, 0};
+    float ss = 0.f, dbeta = 0.f;
+    const T* dO = reinterpret_cast<const T*>(a.d_o) + row * a.do_st.bs + (t0 + min(sr, len - 1)) * a.do_st.rs + hv * a.do_st.cs;
+    T* dv = reinterpret_cast<T*>(a.d_v) + ((row * a.d.tokens + t0 + sr) * a.d.value_heads + hv) * (long)a.d.dv;
+    for (int c0 = 0; c0 < a.dvp; c0 += 32) {
+      const f4 ev = *reinterpret_cast<const f4*>(a.Erow + (at * C + sr) * a.dvp + c0 + sc);
+      const f4 zv = *reinterpret_cast<const f4*>(a.Z + (at * C + sr) * a.dvp + c0 + sc);
+      float x[4], u[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool live = sr < len && c0 + sc + e < a.d.dv;
+        y[e] = live ? (float)dO[min(c0 + sc + e, a.d.dv - 1)] : 0.f;
+        x[e] = bt * zv[e];
+        u[e] = bt * ev[e];
+        dbeta = fmaf(ev[e], zv[e], dbeta);
+        if (live) dv[c0 + sc + e] = (T)x[e];
+      }
+      b8 sb[3], db_[3];
+      if (own) {
+        float sx[8], dx[8];
+        const f4* p = reinterpret_cast<const f4*>(a.Srow + (at * DK + kc0) * a.dvp + c0 + g8);
+        const f4* q = reinterpret_cast<const f4*>(a.dS + (at * DK + kc0) * a.dvp + c0 + g8);
+        const f4 p0 = p[0], p1 = p[1], q0 = q[0], q1_ = q[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sx[e] = p0[e];
+          sx[4 + e] = p1[e];
+          dx[e] = q0[e];
+          dx[4 + e] = q1_[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(sx[e], dx[e], ss);
+        split<8, 3>(sx, sb);
+        split<8, 3>(dx, db_);
+      }
+      b4 yp[N], xp[3], up[3];
+      split<4, N>(y, yp);
+      split<4, 3>(x, xp);
+      split<4, 3>(u, up);
+      __syncthreads();   // the slice before this one, or M and MT, are done with
+#pragma unroll
+      for (int k = 0; k < N; ++k) *reinterpret_cast<b4*>(Y + k * SL + sr * P + sc) = yp[k];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        *reinterpret_cast<b4*>(X + k * SL + sr * P + sc) = xp[k];
+        *reinterpret_cast<b4*>(U + k * SL + sr * P + sc) = up[k];
+      }
+      __syncthreads();
+      auto rows = [&](const __bf16* base, int rb) { return *reinterpret_cast<const b8*>(base + (rb * 16 + col) * P + g8); };
+      if (own) {
+#pragma unroll
+        for (int rb = 0; rb < 4; ++rb) {
+          b8 yy[N], xx[3], uu[3];
+#pragma unroll
+          for (int k = 0; k < N; ++k) yy[k] = rows(Y + k * SL, rb);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            xx[k] = rows(X + k * SL, rb);
+            uu[k] = rows(U + k * SL, rb);
+          }
+          q1[rb] = planes_mma<N, 3, 3>(yy, sb, q1[rb]);
+          kr[rb] = planes_mma<3, 3, 3>(xx, sb, kr[rb]);
+          kc[rb] = planes_mma<3, 3, 3>(uu, db_, kc[rb]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tile = wave + 8 * h;   // of the ten
+        if (tile < 10) {
+          const int rb = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, cb = tile - rb * (rb + 1) / 2;
+          b8 yy[N], xx[3], uu[3];
+#pragma unroll
+          for (int k = 0; k < N; ++k) yy[k] = rows(Y + k * SL, rb);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            xx[k] = rows(X + k * SL, rb);
+            uu[k] = rows(U + k * SL, cb);
+          }
+          dp[h] = planes_mma<N, 3, 3>(yy, uu, dp[h]);
+          da[h] = planes_mma<3, 3, 3>(xx, uu, da[h]);
+        }
+      }
+    }
+    // row factors; k . state part of dKc
+    const double last = G[C - 1];
+    const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs + min(kc0, a.d.dk - 1);
+    const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs + min(kc0, a.d.dk - 1);
+    float csum = 0.f;
+    f4 kv[4], qv[4];
+    if (own) {
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = rb * 16 + r4 + e;
+          const bool live = r < len && kc0 < a.d.dk;
+          kv[rb][e] = live ? (float)Kg[min(r, len - 1) * a.d.k_st.rs] : 0.f;
+          qv[rb][e] = live ? (float)Qg[min(r, len - 1) * a.d.q_st.rs] : 0.f;
+          const float eg = expf((float)G[r]);
+          q1[rb][e] *= a.scale * eg;
+          kr[rb][e] *= -eg;
+          kc[rb][e] *= expf((float)(last - G[r]));
+          csum = fmaf(kv[rb][e], kc[rb][e], csum);
+        }
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+      csum += __shfl_xor(csum, o);
+      ss += __shfl_xor(ss, o);
+    }
+    if (lane == 0) red[wave] = fmaf(expf((float)last), ss, csum);
+    for (int o = 1; o < 8; o <<= 1) dbeta += __shfl_xor(dbeta, o);
+    if ((t & 7) == 0) db[sr] = dbeta;
+    // dP o D with K and Q, then dN o D with K
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      __syncthreads();
+      // the tiles above the diagonal
+      for (int i = t; i < 6 * 256; i += 512) {
+        const int tile = i >> 8, r = i >> 4 & 15, c = i & 15;
+        const int rb = tile < 3 ? 0 : tile < 5 ? 1 : 2, cb = tile < 3 ? tile + 1 : tile < 5 ? tile - 1 : 3;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          M[(k * C + rb * 16 + r) * PM + cb * 16 + c] = (__bf16)0.f;
+          MT[(k * C + cb * 16 + c) * PM + rb * 16 + r] = (__bf16)0.f;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tile = wave + 8 * h;
+        if (tile < 10) {
+          const int rb = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, cb = tile - rb * (rb + 1) / 2, c = cb * 16 + col;
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = rb * 16 + r4 + e;
+            const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
+            x[e] = w == 0 ? a.scale * dp[h][e] * D : r > c ? -da[h][e] * D : 0.f;
+          }
+          b4 xp[3];
+          split<4, 3>(x, xp);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            *reinterpret_cast<b4*>(MT + (k * C + c) * PM + rb * 16 + r4) = xp[k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) M[(k * C + rb * 16 + r4 + e) * PM + c] = xp[k][e];
+          }
+        }
+      }
+      __syncthreads();
+      if (own) {
+        b8 kt[2][N], qt[2][N];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            kt[ks][k] = ld_frag(a.KTf + (atk * N + k) * (DK * C) + (wave * 2 + ks) * 512, lane * 16);
+            if (w == 0) qt[ks][k] = ld_frag(a.QTf + (atk * N + k) * (DK * C) + (wave * 2 + ks) * 512, lane * 16);
+          }
+#pragma unroll
+        for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            b8 mm_[3];
+            if (ks * 2 <= rb) {
+#pragma unroll
+              for (int k = 0; k < 3; ++k) mm_[k] = *reinterpret_cast<const b8*>(M + (k * C + rb * 16 + col) * PM + ks * 32 + g8);
+              if (w == 0) q1[rb] = planes_mma<3, N, 3>(mm_, kt[ks], q1[rb]);
+              else kr[rb] = planes_mma<3, N, 3>(mm_, kt[ks], kr[rb]);
+            }
+            if (ks * 2 + 1 >= rb) {
+#pragma unroll
+              for (int k = 0; k < 3; ++k) mm_[k] = *reinterpret_cast<const b8*>(MT + (k * C + rb * 16 + col) * PM + ks * 32 + g8);
+              kc[rb] = planes_mma<3, N, 3>(mm_, w == 0 ? qt[ks] : kt[ks], kc[rb]);
+            }
+          }
+      }
+    }
+    // dG of this wave's columns
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      float g[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[e] = own ? fmaf(qv[rb][e], q1[rb][e], kv[rb][e] * (kr[rb][e] - kc[rb][e])) : 0.f;
+        for (int o = 1; o < 16; o <<= 1) g[e] += __shfl_xor(g[e], o);
+      }
+      if (col == 0)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dG[wave * C + rb * 16 + r4 + e] = g[e];
+      dq[rb] += q1[rb];
+      dk[rb] += kr[rb] + kc[rb];
+    }
+    __syncthreads();
+    if (wave == 0) {
+      float v = 0.f;
+      for (int i = 0; i < 8; ++i) v += dG[i * C + lane] + (lane == C - 1 ? red[i] : 0.f);
+      for (int o = 1; o < 64; o <<= 1) {
+        const float u = __shfl_down(v, o);
+        if (lane + o < 64) v += u;
+      }
+      if (lane < len) {
+        const long p = (row * a.d.tokens + t0 + lane) * a.d.value_heads + hv;
+        a.d_g[p] = v;
+        a.d_beta[p] = db[lane];
+      }
+    }
+  }
+  if (own && kc0 < a.d.dk) {
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 16 + r4 + e;
+        if (r < len) {
+          const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + kc0;
+          st<T>(a.d_q, p, dq[rb][e]);
+          st<T>(a.d_k, p, dk[rb][e]);
+        }
+      }
   }
 }
 
@@ -1312,48 +1243,53 @@ long slots_of(const gpx_delta* d) {
 }
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Parts of a workspace, in this order (use 0: forward, 1: forward that saves, 2: scratch of backward); nullptr base:
-// sizes only.
 bool recurrent(const gpx_delta* d, int save) { return !save && d->tokens <= RECURRENT_MAX; }
 
+// Parts of a workspace, in this order; nullptr base: sizes only.
+enum { WORK = 0, SAVED = 1, SCRATCH = 2, WORK_SAVING = 3 };
 size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
-  const size_t heads = (size_t)slots_of(d) * d->value_heads, dvp = (size_t)(d->dv + DVT - 1) / DVT * DVT;
+  const size_t dkp = d->dk <= 64 ? 64 : 128, dvp = (size_t)(d->dv + DVT - 1) / DVT * DVT;
+  const size_t heads = (size_t)slots_of(d) * d->value_heads, kheads = (size_t)slots_of(d) * d->key_heads;
+  const size_t n = d->dtype == GPX_F32 ? 3 : d->dtype == GPX_F16 ? 2 : 1, no = d->dtype == GPX_F32 ? 3 : 2;
   size_t at = 0;
-  auto part = [&](size_t bytes) {
-    char* p = base == nullptr ? nullptr : base + at;
-    at += up256(bytes);
-    return p;
-  };
   Args dummy;
   Args& x = a != nullptr ? *a : dummy;
-  if (use < 2) {
-    char* p = part(d->sequences > 0 ? (size_t)(d->sequences + 1) * 4 : 0);
-    if (off != nullptr) *off = reinterpret_cast<int*>(p);
+  auto part = [&](auto*& p, size_t bytes) {
+    p = base == nullptr ? nullptr : reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
+    at += up256(bytes);
+  };
+  if ((use == WORK || use == SAVED) && d->sequences > 0) {
+    int* p;
+    part(p, (size_t)(d->sequences + 1) * 4);
+    if (off != nullptr) *off = p;
   }
-  if (use == 0 && !recurrent(d, 0)) {
-    const size_t kheads = (size_t)slots_of(d) * d->key_heads, dkp = d->dk <= 64 ? 64 : 128;
-    const size_t n = d->dtype == GPX_F32 ? 3 : d->dtype == GPX_F16 ? 2 : 1, no = d->dtype == GPX_F32 ? 3 : 2;
-    x.G = reinterpret_cast<double*>(part(heads * C * 8));
-    x.fac = reinterpret_cast<float*>(part(heads * 4 * C * 4));
-    x.Kf = reinterpret_cast<__bf16*>(part(kheads * n * KF * 2));
-    x.Qf = reinterpret_cast<__bf16*>(part(kheads * n * KF * 2));
-    x.KTf = reinterpret_cast<__bf16*>(part(kheads * n * dkp * C * 2));
-    x.Tf = reinterpret_cast<__bf16*>(part(heads * 3 * TF * 2));
-    x.Pf = reinterpret_cast<__bf16*>(part(heads * no * TF * 2));
-    x.E = reinterpret_cast<float*>(part(heads * C * dvp * 4));
-    x.S = reinterpret_cast<float*>(part(heads * 128 * dvp * 4));
+  if (use == WORK && recurrent(d, 0)) return at;
+  if (use == WORK || use == SAVED) {
+    part(x.G, heads * C * 8);
+    part(x.fac, heads * FACS * 4);
+    part(x.Kf, kheads * n * KF * 2);
+    part(x.KTf, kheads * n * dkp * C * 2);
   }
-  if (use == 1) {
-    x.G = reinterpret_cast<double*>(part(heads * C * 8));
-    x.T = reinterpret_cast<float*>(part(heads * C * C * 4));
-    x.P = reinterpret_cast<float*>(part(heads * C * C * 4));
-    x.E = reinterpret_cast<float*>(part(heads * C * dvp * 4));
-    x.S = reinterpret_cast<float*>(part(heads * d->dk * dvp * 4));
+  if (use == SAVED) {
+    part(x.QTf, kheads * n * dkp * C * 2);
+    part(x.T2f, heads * 3 * TF * 2);
+    part(x.PTf, heads * 3 * TF * 2);
+    part(x.Erow, heads * C * dvp * 4);
+    part(x.Srow, heads * dkp * dvp * 4);
   }
-  if (use == 2) {
-    x.dX = reinterpret_cast<float*>(part(heads * C * dvp * 4));
-    x.dS = reinterpret_cast<float*>(part(heads * d->dk * dvp * 4));
-    x.part = reinterpret_cast<float*>(part(heads * (dvp / DVT) * C * 4));
+  if (use == WORK || use == WORK_SAVING) {
+    part(x.Qf, kheads * n * KF * 2);
+    part(x.Tf, heads * 3 * TF * 2);
+    part(x.Pf, heads * no * TF * 2);
+    part(x.V, heads * C * dvp * (d->dtype == GPX_F32 ? 4 : 2));
+    part(x.E, heads * C * dvp * 4);
+    part(x.S, heads * 128 * dvp * 4);
+  }
+  if (use == SCRATCH) {
+    part(x.Y, heads * C * dvp * 4);
+    part(x.Of, heads * 3 * C * dvp * 2);
+    part(x.Z, heads * C * dvp * 4);
+    part(x.dS, heads * dkp * dvp * 4);
   }
   return at;
 }
@@ -1405,30 +1341,9 @@ int allow_lds(F* kernel, size_t bytes) {
     if (rc_ != 0) return rc_; \
   } while (0)
 
-unsigned scan_grid(const Args& a) {
-  const unsigned heads = (unsigned)a.p.sequences * a.d.value_heads, slices = a.dvp / DVT;
-  return (heads + 7) / 8 * 8 * slices;
-}
-
-template <typename T, int DK>
-int run_chunks(hipStream_t s, const Args& a) {
-  constexpr int N = Planes<T>::N;
-  constexpr size_t lds = 2 * N * C * (DK + 8) * 2 + (2 * C * PC + 4 * 16 * 20) * 4 + C * 8 + C * 4;
-  static_assert(lds <= 160 * 1024, "LDS");
-  DELTA_TRY(allow_lds(&delta_chunk_kernel<T, DK>, lds));
-  const long slots = slots_of(&a.d);
-  if (slots > 0) {
-    hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(256), lds, s, a);
-    GPX_HIP(hipGetLastError());
-  }
+unsigned chain_grid(const Args& a, int nt) {
   const unsigned heads = (unsigned)a.p.sequences * a.d.value_heads;
-  hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1>), dim3((heads + 7) / 8 * 8 * (a.dvp / 16)), dim3(256), 0, s, a);
-  GPX_HIP(hipGetLastError());
-  if (slots > 0) {
-    hipLaunchKernelGGL((delta_out_kernel<T, DK>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
-    GPX_HIP(hipGetLastError());
-  }
-  return 0;
+  return (heads + 7) / 8 * 8 * (a.dvp / (16 * nt));
 }
 
 template <typename T, int DK>
@@ -1440,34 +1355,38 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
     GPX_HIP(hipGetLastError());
     return 0;
   }
-  if (!a.save) return run_chunks<T, DK>(s, a);
-  constexpr size_t prep = (2 * C * (DK + 4) + C * PC) * 4 + C * 8 + C * 4;
-  constexpr size_t scan = (2 * C * (DK + 4) + 2 * C * PC + DK * PV + 2 * C * PV + 3 * C) * 4;
-  static_assert(scan <= 160 * 1024, "LDS");
-  DELTA_TRY(allow_lds(&delta_prep_kernel<T, DK>, prep));
-  DELTA_TRY(allow_lds(&delta_scan_kernel<T, DK>, scan));
-  const unsigned n = (unsigned)(slots_of(&a.d) * a.d.value_heads);
-  if (n > 0) {
-    hipLaunchKernelGGL((delta_prep_kernel<T, DK>), dim3(n), dim3(256), prep, s, a);
+  constexpr size_t lds = 2 * Planes<T>::N * C * (DK + 8) * 2 + (2 * C * PC + 4 * 16 * 20) * 4 + C * 8 + C * 4;
+  static_assert(lds <= 160 * 1024, "LDS");
+  DELTA_TRY(allow_lds(&delta_chunk_kernel<T, DK>, lds));
+  const long slots = slots_of(&a.d);
+  if (slots > 0) {
+    hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(256), lds, s, a);
     GPX_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL((delta_scan_kernel<T, DK>), dim3(scan_grid(a)), dim3(256), scan, s, a);
+  hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1, false>), dim3(chain_grid(a, 1)), dim3(256), 0, s, a);
   GPX_HIP(hipGetLastError());
+  if (slots > 0) {
+    hipLaunchKernelGGL((delta_out_kernel<T, DK>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
+    GPX_HIP(hipGetLastError());
+  }
   return 0;
 }
 
 template <typename T, int DK>
 int run_backward(hipStream_t s, const Args& a) {
-  constexpr size_t back = (2 * C * (DK + 4) + 2 * C * PC + DK * PV + 2 * C * PV + 3 * C) * 4;
-  constexpr size_t grads = (2 * C * (DK + 4) + 2 * DK * PV + 4 * C * PV) * 4 + C * 8 + (C + 2 * C + 4 * C + 16) * 4;
-  static_assert(grads <= 160 * 1024, "LDS");
-  DELTA_TRY(allow_lds(&delta_back_kernel<T, DK>, back));
-  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK>, grads));
-  hipLaunchKernelGGL((delta_back_kernel<T, DK>), dim3(scan_grid(a)), dim3(256), back, s, a);
+  constexpr size_t room = (Planes<T>::N + 6) * C * 40 > 6 * C * (C + 8) ? (Planes<T>::N + 6) * C * 40 : 6 * C * (C + 8);
+  constexpr size_t lds = room * 2 + C * 8 + (8 * C + 8 + C) * 4;
+  static_assert(lds <= 160 * 1024, "LDS");
+  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK>, lds));
+  const long slots = slots_of(&a.d);
+  if (slots > 0) {
+    hipLaunchKernelGGL((delta_back_prep_kernel<T>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
+    GPX_HIP(hipGetLastError());
+  }
+  hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1, true>), dim3(chain_grid(a, 1)), dim3(256), 0, s, a);
   GPX_HIP(hipGetLastError());
-  const unsigned n = (unsigned)(slots_of(&a.d) * a.d.key_heads);
-  if (n > 0) {
-    hipLaunchKernelGGL((delta_grads_kernel<T, DK>), dim3(n), dim3(512), grads, s, a);
+  if (slots > 0) {
+    hipLaunchKernelGGL((delta_grads_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(512), lds, s, a);
     GPX_HIP(hipGetLastError());
   }
   return 0;
@@ -1510,24 +1429,26 @@ int check_work(const gpx_delta* d, int use, const void* work, size_t work_bytes,
 extern "C" {
 
 size_t gpx_delta_work_bytes(const gpx_delta* d, int use) {
-  if (use < 0 || use > 2 || check_delta(d, "delta_work_bytes") != 0) return 0;
+  if (use < 0 || use > 3 || check_delta(d, "delta_work_bytes") != 0) return 0;
   return lay_out(d, use, nullptr, nullptr, nullptr);
 }
 
-int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, void* o, float* state_out, int save,
-                      void* work, size_t work_bytes) {
+int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, void* o, float* state_out, void* work,
+                      size_t work_bytes, void* saved, size_t saved_bytes) {
   GPX_REQUIRE(h != nullptr, "null handle");
   DELTA_TRY(check_delta(d, "delta_forward"));
   if (sequences_of(d) == 0) return 0;
   GPX_REQUIRE(o != nullptr || d->tokens == 0, "delta_forward: null output");
   GPX_REQUIRE(state == nullptr || gpx_aligned16(state), "delta_forward: state must be 16-byte aligned");
   GPX_REQUIRE(state_out == nullptr || gpx_aligned16(state_out), "delta_forward: state_out must be 16-byte aligned");
-  save = save != 0;
-  DELTA_TRY(check_work(d, save, work, work_bytes, "delta_forward"));
+  const int save = saved != nullptr;
+  DELTA_TRY(check_work(d, save ? WORK_SAVING : WORK, work, work_bytes, "delta_forward"));
+  if (save) DELTA_TRY(check_work(d, SAVED, saved, saved_bytes, "delta_forward"));
   DeviceGuard dg(h->device);
   Args a = make_args(d);
   int* off = nullptr;
-  lay_out(d, save, static_cast<char*>(work), &a, &off);
+  lay_out(d, save ? WORK_SAVING : WORK, static_cast<char*>(work), &a, &off);
+  if (save) lay_out(d, SAVED, static_cast<char*>(saved), &a, &off);
   DELTA_TRY(plan(h->stream, d, a, off));
   a.state = state;
   a.o = o;
@@ -1548,13 +1469,13 @@ int gpx_delta_backward(gpx_handle* h, const gpx_delta* d, const void* d_o, const
     GPX_REQUIRE(d_o_st->bs >= 0 && d_o_st->rs >= 0 && d_o_st->cs >= 0, "delta_backward: negative stride");
     GPX_REQUIRE(d_q && d_k && d_v && d_g && d_beta, "delta_backward: null output");
   }
-  DELTA_TRY(check_work(d, 1, saved, saved_bytes, "delta_backward"));
-  DELTA_TRY(check_work(d, 2, scratch, scratch_bytes, "delta_backward"));
+  DELTA_TRY(check_work(d, SAVED, saved, saved_bytes, "delta_backward"));
+  DELTA_TRY(check_work(d, SCRATCH, scratch, scratch_bytes, "delta_backward"));
   DeviceGuard dg(h->device);
   Args a = make_args(d);
   int* off = nullptr;
-  lay_out(d, 1, static_cast<char*>(const_cast<void*>(saved)), &a, &off);
-  lay_out(d, 2, static_cast<char*>(scratch), &a, nullptr);
+  lay_out(d, SAVED, static_cast<char*>(const_cast<void*>(saved)), &a, &off);
+  lay_out(d, SCRATCH, static_cast<char*>(scratch), &a, nullptr);
   if (d->sequences > 0) a.p.off = off;   // the forward call's plan
   a.d_o = d_o;
   if (d_o_st != nullptr) a.do_st = *d_o_st;

@@ -86,6 +86,12 @@ def _desc(dtype, q, k, v, g, beta, scale, offsets, sequences):
                       _st(beta))
 
 
+def _bytes(rt, d, use):
+    """A workspace of the library, and its size."""
+    size = int(rt.lib.gpx_delta_work_bytes(C.byref(d), use))
+    return rt.torch.empty(max(size, 256), dtype=rt.torch.uint8, device=rt.dev), size
+
+
 def _version(t):
     return None if t.is_inference() else t._version   # inference tensors do not count their writes
 
@@ -131,15 +137,14 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
         d = _desc(dtype, q, k, v, g, beta, dk ** -0.5 if scale is None else scale, cu_seqlens, sequences)
         o = (torch.zeros if sequences else torch.empty)((B, T, Hv, dv), dtype=q.dtype, device=q.device)
         final = torch.empty(shape, dtype=torch.float32, device=q.device)
-        save = int(bool(save_for_backward))
-        size = int(rt.lib.gpx_delta_work_bytes(C.byref(d), save))
-        work = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
-        _lib.check(rt.lib.gpx_delta_forward(rt.h, C.byref(d), _opt(state), ptr(o), ptr(final), save, ptr(work), size),
+        work, size = _bytes(rt, d, 3 if save_for_backward else 0)
+        saved, kept = _bytes(rt, d, 1) if save_for_backward else (None, 0)
+        _lib.check(rt.lib.gpx_delta_forward(rt.h, C.byref(d), _opt(state), ptr(o), ptr(final), ptr(work), size, _opt(saved), kept),
                    "gpx_delta_forward")
     if not save_for_backward:
         return o, final
     inputs = [t for t in (q, k, v, g, beta, cu_seqlens) if t is not None]
-    return o, final, Saved(d, inputs, initial_state, work)
+    return o, final, Saved(d, inputs, initial_state, saved)
 
 
 def gated_delta_rule_backward(saved, d_o, d_final_state=None):
@@ -166,8 +171,7 @@ def gated_delta_rule_backward(saved, d_o, d_final_state=None):
         new = torch.zeros if d.sequences else torch.empty
         grads = [new(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]
         d_state = torch.empty(shape, dtype=torch.float32, device=q.device) if saved.has_state else None
-        size = int(rt.lib.gpx_delta_work_bytes(C.byref(d), 2))
-        scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
+        scratch, size = _bytes(rt, d, 2)
         st = _st(d_o)
         _lib.check(rt.lib.gpx_delta_backward(rt.h, C.byref(d), ptr(d_o), C.byref(st), _opt(d_final), *map(ptr, grads), _opt(d_state),
                                              ptr(saved.work), saved.work.numel(), ptr(scratch), size), "gpx_delta_backward")

@@ -327,17 +327,17 @@ typedef struct gpx_delta {
   const float *g, *beta;
   gpx_strided q_st, k_st, v_st, g_st, beta_st; /* {batch, token, head} */
 } gpx_delta;
-/* Device bytes of gpx_delta_forward's workspace (use 0), of the same when gpx_delta_backward will read it (use 1), and of
- * gpx_delta_backward's own scratch (use 2). */
+/* Device bytes of a workspace: use 0 gpx_delta_forward's when nothing is saved, 3 when something is; 1 what it saves for
+ * gpx_delta_backward; 2 gpx_delta_backward's scratch.  Each 256-byte aligned; work and scratch are not shared by calls that may
+ * overlap in time. */
 size_t gpx_delta_work_bytes(const gpx_delta* d, int use);
-/* o and the states after the last tokens.  state (before the first tokens) NULL: zeros; state_out may be NULL or state.
- * save == 0: work is scratch of gpx_delta_work_bytes(d, 0) bytes.  save != 0: of gpx_delta_work_bytes(d, 1) bytes, and
- * keeps what gpx_delta_backward reads.  256-byte aligned, not shared by calls that may overlap in time. */
-int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, void* o, float* state_out, int save,
-                      void* work, size_t work_bytes);
+/* o and the states after the last tokens.  state (before the first tokens) NULL: zeros; state_out may be NULL or state; both
+ * 16-byte aligned.  saved: NULL, or where to keep what gpx_delta_backward reads. */
+int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, void* o, float* state_out, void* work,
+                      size_t work_bytes, void* saved, size_t saved_bytes);
 /* Gradients of sum(d_o o) + sum(d_state_out state_out) with respect to q, k, v (their type), g, beta and state (fp32;
  * d_state may be NULL), all packed.  d_o: strides like v's; d_state_out NULL: zeros.  d and its inputs are those of the
- * forward call with save != 0, saved what that call left in its work (only read); scratch as above.  The gradient of a
+ * forward call, unchanged, saved what that call kept (only read).  The gradient of a
  * shared key head is summed over its value heads in a fixed order; no atomics are used. */
 int gpx_delta_backward(gpx_handle* h, const gpx_delta* d, const void* d_o, const gpx_strided* d_o_st,
                        const float* d_state_out, void* d_q, void* d_k, void* d_v, float* d_g, float* d_beta, float* d_state,

@@ -178,14 +178,16 @@ def test_work_bytes():
     lib = _lib.load()
     w = lambda use, **kw: lib.gpx_delta_work_bytes(C.byref(desc(**kw)), use)  # noqa: E731
     heads, kheads = 2 * 2 * 4, 2 * 2 * 2   # rows, chunks, heads; dv rounded up to 64, dk to 64
-    square = 64 * 64
-    assert w(0) == heads * (64 * 8 + 4 * 64 * 4 + 5 * square * 2 + 64 * 64 * 4 + 128 * 64 * 4) + kheads * (2 * 2 + 1) * square * 2
-    assert w(1) == heads * (64 * 8 + 2 * square * 4 + (64 + 64) * 64 * 4)
-    assert w(2) == heads * ((64 + 64) * 64 * 4 + 2 * 64 * 4)
+    square = 64 * 64                       # elements of a fragment-wise C x C or dk x C matrix; K and Q take two
+    both_ = heads * (64 * 8 + 6 * 64 * 4) + kheads * 3 * square * 2
+    work = kheads * 2 * square * 2 + heads * (5 * square * 2 + 64 * 64 * 2 + 64 * 64 * 4 + 128 * 64 * 4)
+    assert w(0) == both_ + work and w(3) == work
+    assert w(1) == both_ + kheads * square * 2 + heads * (6 * square * 2 + (64 + 64) * 64 * 4)
+    assert w(2) == heads * (64 * 64 * 4 + 3 * 64 * 64 * 2 + (64 + 64) * 64 * 4)
     assert w(0, tokens=16) == 0                                   # the recurrence needs none
     assert w(0, tokens=16, batch=1, sequences=5, offsets=256) == 256
-    assert w(3) == 0 and w(0, dk=129) == 0 and w(0, dtype=0) == 0 and w(0, value_heads=3) == 0
-    assert w(1, batch=1, sequences=5, offsets=256) == 256 + (1 + 5) * 4 * (64 * 8 + 2 * square * 4 + (64 + 64) * 64 * 4)
+    assert w(4) == 0 and w(0, dk=129) == 0 and w(0, dtype=0) == 0 and w(0, value_heads=3) == 0
+    assert w(1, batch=1, sequences=5, offsets=256) == 256 + w(1) * 6 // 4
     assert w(0, batch=1, sequences=5) == 0                       # no offsets
     assert w(1, batch=1 << 24, tokens=1 << 30) == 0              # beyond the grid
 
