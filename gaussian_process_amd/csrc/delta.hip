@@ -93,7 +93,6 @@ struct Args {
   float* fac;                   // per head: exp(G), beta, exp(G_C - G) beta, exp(G_C), exp(G_C - G), exp(G) beta; C each
   __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
-  void* V;                      // per head: V^T, dvp x C, of the inputs' type
   float *E, *Erow;              // per head: E^T, dvp x C; E, C x dvp
   float *S, *Srow;              // per head: S in state order, dvp / 16 x 4 x 64 x 8; S, DK x dvp
   float* Y;                     // per head: (scale P^T dO)^T, dvp x C
@@ -435,24 +434,6 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
       store_square<3, true>(M, a.T2f + at * 3 * TF, t);
       __syncthreads();
     }
-    // V^T, 64 columns at a time through LDS
-    T* vt = reinterpret_cast<T*>(A);   // C x 66 of T
-    const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + t0 * a.d.v_st.rs + hv * a.d.v_st.cs;
-    for (int c0 = 0; c0 < a.dvp; c0 += 64) {
-      for (int i = t; i < C * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        vt[r * 66 + c] = r < len && c0 + c < a.d.dv ? V[r * a.d.v_st.rs + c0 + c] : T(0);
-      }
-      __syncthreads();
-      for (int i = t; i < min(64, a.dvp - c0) * 8; i += 256) {
-        const int c = i >> 3, r = (i & 7) * 8;
-        T x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = vt[(r + e) * 66 + c];
-        __builtin_memcpy(__builtin_assume_aligned(reinterpret_cast<T*>(a.V) + (at * a.dvp + c0 + c) * C + r, 16), x, sizeof(x));
-      }
-      __syncthreads();
-    }
   }
 }
 
@@ -462,14 +443,17 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
 // (Y = scale P^T dO, Of = scale exp(G) dO, from delta_back_prep_kernel).
 // Bound by the chain from chunk to chunk: the product with K (each wave with its own rows of S, which are in its accumulators;
 // partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.
-// Fragments are loaded for the next chunk as soon as this chunk has used them; every load is issued whatever comes, since loads behind
-// branches make the compiler wait for all that are under way.
+// Fragments come straight from memory, for the next chunk as soon as this chunk has used its own (two chunks ahead gained
+// nothing); every load is issued whatever comes, since loads behind branches make the compiler wait for all that are under way.
 __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes) {
   return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
 }
 
+// two waves per SIMD where the fragments leave the registers for it
+constexpr int chain_waves(int planes, bool back) { return planes == 1 || (planes == 2 && !back) ? 2 : 1; }
+
 template <typename T, int DK, int NT, bool BACK>
-__global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
+__global__ __launch_bounds__(256, chain_waves(Planes<T>::N, BACK)) void delta_chain_kernel(const Args a) {
   constexpr int N = Planes<T>::N, RT = DK / 64, PT = C + 8;
   __shared__ f4 part[4][4][NT][64];              // K S: wave, row block
   __shared__ __align__(16) __bf16 X[3][NT * 16][PT], U[3][NT * 16][PT];
@@ -494,11 +478,12 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
         const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
         S[i][j][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
       }
-  struct Four { T x[4]; };
   b8 kf[4][N], tf[2][3], kt[RT][2][N], qt[RT][2][N], of[NT][2][3];
-  Four v[NT];
+  T v[NT][4];
   f4 y[NT], fx, fu;
-  float keep = 1.f;
+  float keep;
+  const T* V = reinterpret_cast<const T*>(a.d.v) + a.p.row(s) * a.d.v_st.bs + begin * a.d.v_st.rs + hv * a.d.v_st.cs;
+  const unsigned vrs = (unsigned)a.d.v_st.rs;
   auto load_k = [&](long slot) {
     const __bf16* p = a.Kf + (slot * a.d.key_heads + hk) * N * KF + wave * 512;
 #pragma unroll
@@ -506,14 +491,17 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
 #pragma unroll
       for (int k = 0; k < N; ++k) kf[i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
   };
-  auto load_x = [&](long at) {
+  auto load_x = [&](long at, int n) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const unsigned o = (unsigned)((j * 16 + col) * C + wave * 16 + r4);
-      if (BACK)
-        y[j] = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + o);
-      else
-        __builtin_memcpy(&v[j], __builtin_assume_aligned(reinterpret_cast<const T*>(a.V) + (at * a.dvp + c0) * C + o, 4 * sizeof(T)), sizeof(Four));
+      if (BACK) {
+        y[j] = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + (unsigned)((j * 16 + col) * C + wave * 16 + r4));
+      } else {   // rows and columns behind the end repeat the last; they are masked where they are used
+        const T* p = V + (long)n * C * a.d.v_st.rs;
+        const unsigned last = min(C, end - begin - n * C) - 1, c = min(c0 + j * 16 + col, a.d.dv - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = p[min((unsigned)(wave * 16 + r4 + e), last) * vrs + c];
+      }
     }
     fx = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 4 * C : 0) + wave * 16 + r4);
   };
@@ -546,21 +534,20 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
           for (int k = 0; k < 3; ++k)
             of[j][ks][k] = ld_frag(a.Of + (at * 3 + k) * (a.dvp * C) + (c0 / 16 + j) * 1024 + ks * 512, lb);
     }
-    keep = a.fac[at * FACS + 3 * C];
+    keep = a.fac[at * FACS + 3 * C + lane];   // by lane: a scalar load would be waited for with LDS
   };
-  {
-    const long slot = slot0 + (BACK ? chunks - 1 : 0), at = slot * a.d.value_heads + hv;
-    if (chunks > 0) {
-      load_k(slot);
-      load_x(at);
-      load_t(at);
-      load_kt(slot, at);
-    }
+  if (chunks > 0) {
+    const int m = BACK ? chunks - 1 : 0;
+    const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
+    load_k(slot);
+    load_x(at, m);
+    load_t(at);
+    load_kt(slot, at);
   }
   for (int n = 0; n < chunks; ++n) {
-    const long slot = slot0 + (BACK ? chunks - 1 - n : n), at = slot * a.d.value_heads + hv;
-    const int more = n + 1 < chunks ? (BACK ? -1 : 1) : 0;
-    const long nslot = slot + more, nat = at + more * a.d.value_heads;
+    const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - 1, 0) : min(m + 1, chunks - 1);
+    const long at = (slot0 + m) * a.d.value_heads + hv, nslot = slot0 + nm, nat = nslot * a.d.value_heads + hv;
+    const int live = BACK ? 0 : end - begin - n * C - wave * 16 - r4;   // rows e < live hold tokens
     // S as planes, and to memory
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -577,12 +564,12 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
       for (int i = 0; i < 4; ++i) p[i] = f4{0, 0, 0, 0};
       // plane by plane over the four row blocks: four chains of matrix instructions side by side
 #pragma unroll
-      for (int m = 2; m >= 0; --m)
+      for (int q = 2; q >= 0; --q)
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (m >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], sb[m - k], p[i], 0, 0, 0);
+            if (q >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], sb[q - k], p[i], 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) part[wave][i][j][lane] = p[i];
       if (!BACK) {
@@ -605,13 +592,14 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
       const f4 p = (part[0][wave][j][lane] + part[1][wave][j][lane]) + (part[2][wave][j][lane] + part[3][wave][j][lane]);
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = BACK ? fmaf(fx[e], p[e], y[j][e]) : fmaf(-fx[e], p[e], (float)v[j].x[e]);
+      for (int e = 0; e < 4; ++e) x[e] = BACK ? fmaf(fx[e], p[e], y[j][e])
+                    : e < live && c0 + j * 16 + col < a.d.dv ? fmaf(-fx[e], p[e], (float)v[j][e]) : 0.f;
       b4 xp[3];
       split<4, 3>(x, xp);
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&X[k][j * 16 + col][wave * 16 + r4]) = xp[k];
     }
-    load_x(nat);
+    load_x(nat, nm);
     lds_barrier();
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -629,11 +617,11 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(const Args a) {
         e1 = planes_mma<3, 3, 3>(tf[1], xb, e1);
       }
       const f4 ev = e0 + e1;
-      float u[4];
+      float w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) u[e] = (BACK ? -fu[e] : fu[e]) * ev[e];
+      for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fu[e] : fu[e]) * ev[e];
       b4 up[3];
-      split<4, 3>(u, up);
+      split<4, 3>(w, up);
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&U[k][j * 16 + col][wave * 16 + r4]) = up[k];
       if (!BACK) *reinterpret_cast<f4*>(a.E + (at * a.dvp + c0 + j * 16) * C + (unsigned)(col * C + wave * 16 + r4)) = ev;
@@ -824,7 +812,7 @@ __global__ __launch_bounds__(256) void delta_back_prep_kernel(const Args a) {
 // 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
 // memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
 // the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
-template <typename T, int DK>
+template <typename T, int DK, bool GROUPED>
 __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   constexpr int N = Planes<T>::N, W = DK / 16, P = 40, PM = C + 8;
   constexpr int SL = C * P;                      // a plane of a slice
@@ -839,6 +827,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   float* dG = reinterpret_cast<float*>(G + C);   // 8 x C: per wave
   float* red = dG + 8 * C;      // 8
   float* db = red + 8;          // C
+  f4* sums = reinterpret_cast<f4*>(db + C);   // GROUPED: dQ and dK over the value heads so far, 8 per thread
   const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
@@ -850,11 +839,11 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   const int kc0 = wave * 16 + col;   // this lane's column of dk
   // a thread's place in a slice: four columns of one row
   const int sr = t >> 3, sc = (t & 7) * 4;
-  f4 dq[4], dk[4];   // over the value heads
-#pragma unroll
-  for (int i = 0; i < 4; ++i) dq[i] = dk[i] = f4{0, 0, 0, 0};
-  for (int m = 0; m < a.group; ++m) {
-    const int hv = hk * a.group + m;
+  const int group = GROUPED ? a.group : 1;
+#pragma unroll 1
+  for (int m = 0; m < group; ++m) {
+    asm volatile("" ::: "memory");   // keeps the loads of K and Q inside: hoisted, they would not fit the registers
+    const int hv = hk * group + m;
     const long at = (long)slot * a.d.value_heads + hv;
     __syncthreads();
     if (wave == 0) G[lane] = a.G[at * C + lane];
@@ -866,34 +855,42 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     float ss = 0.f, dbeta = 0.f;
     const T* dO = reinterpret_cast<const T*>(a.d_o) + row * a.do_st.bs + (t0 + min(sr, len - 1)) * a.do_st.rs + hv * a.do_st.cs;
     T* dv = reinterpret_cast<T*>(a.d_v) + ((row * a.d.tokens + t0 + sr) * a.d.value_heads + hv) * (long)a.d.dv;
+    // a slice's values, loaded while the slice before it is multiplied
+    f4 ev, zv, sv[2], tv[2];
+    T yv[4];
+    auto load_slice = [&](int c0) {
+      ev = *reinterpret_cast<const f4*>(a.Erow + (at * C + sr) * a.dvp + c0 + sc);
+      zv = *reinterpret_cast<const f4*>(a.Z + (at * C + sr) * a.dvp + c0 + sc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) yv[e] = dO[min(c0 + sc + e, a.d.dv - 1)];
+      const f4* p = reinterpret_cast<const f4*>(a.Srow + (at * DK + min(kc0, DK - 1)) * a.dvp + c0 + g8);
+      const f4* q = reinterpret_cast<const f4*>(a.dS + (at * DK + min(kc0, DK - 1)) * a.dvp + c0 + g8);
+      sv[0] = p[0];
+      sv[1] = p[1];
+      tv[0] = q[0];
+      tv[1] = q[1];
+    };
+    load_slice(0);
     for (int c0 = 0; c0 < a.dvp; c0 += 32) {
-      const f4 ev = *reinterpret_cast<const f4*>(a.Erow + (at * C + sr) * a.dvp + c0 + sc);
-      const f4 zv = *reinterpret_cast<const f4*>(a.Z + (at * C + sr) * a.dvp + c0 + sc);
       float x[4], u[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool live = sr < len && c0 + sc + e < a.d.dv;
-        y[e] = live ? (float)dO[min(c0 + sc + e, a.d.dv - 1)] : 0.f;
+        y[e] = live ? (float)yv[e] : 0.f;
         x[e] = bt * zv[e];
         u[e] = bt * ev[e];
         dbeta = fmaf(ev[e], zv[e], dbeta);
         if (live) dv[c0 + sc + e] = (T)x[e];
       }
       b8 sb[3], db_[3];
-      if (own) {
+      {
         float sx[8], dx[8];
-        const f4* p = reinterpret_cast<const f4*>(a.Srow + (at * DK + kc0) * a.dvp + c0 + g8);
-        const f4* q = reinterpret_cast<const f4*>(a.dS + (at * DK + kc0) * a.dvp + c0 + g8);
-        const f4 p0 = p[0], p1 = p[1], q0 = q[0], q1_ = q[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sx[e] = p0[e];
-          sx[4 + e] = p1[e];
-          dx[e] = q0[e];
-          dx[4 + e] = q1_[e];
+        for (int e = 0; e < 8; ++e) {
+          sx[e] = sv[e >> 2][e & 3];
+          dx[e] = tv[e >> 2][e & 3];
+          ss = own ? fmaf(sx[e], dx[e], ss) : 0.f;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(sx[e], dx[e], ss);
         split<8, 3>(sx, sb);
         split<8, 3>(dx, db_);
       }
@@ -910,6 +907,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         *reinterpret_cast<b4*>(U + k * SL + sr * P + sc) = up[k];
       }
       __syncthreads();
+      load_slice(min(c0 + 32, a.dvp - 32));
       auto rows = [&](const __bf16* base, int rb) { return *reinterpret_cast<const b8*>(base + (rb * 16 + col) * P + g8); };
       if (own) {
 #pragma unroll
@@ -950,21 +948,20 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs + min(kc0, a.d.dk - 1);
     const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs + min(kc0, a.d.dk - 1);
     float csum = 0.f;
-    f4 kv[4], qv[4];
+    auto element = [&](const T* p, const gpx_strided& st_, int r) {
+      return r < len && kc0 < a.d.dk ? (float)p[min(r, len - 1) * st_.rs] : 0.f;
+    };
     if (own) {
 #pragma unroll
       for (int rb = 0; rb < 4; ++rb)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = rb * 16 + r4 + e;
-          const bool live = r < len && kc0 < a.d.dk;
-          kv[rb][e] = live ? (float)Kg[min(r, len - 1) * a.d.k_st.rs] : 0.f;
-          qv[rb][e] = live ? (float)Qg[min(r, len - 1) * a.d.q_st.rs] : 0.f;
           const float eg = expf((float)G[r]);
           q1[rb][e] *= a.scale * eg;
           kr[rb][e] *= -eg;
           kc[rb][e] *= expf((float)(last - G[r]));
-          csum = fmaf(kv[rb][e], kc[rb][e], csum);
+          csum = fmaf(element(Kg, a.d.k_st, r), kc[rb][e], csum);
         }
     }
     for (int o = 1; o < 64; o <<= 1) {
@@ -1045,14 +1042,33 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
       float g[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        g[e] = own ? fmaf(qv[rb][e], q1[rb][e], kv[rb][e] * (kr[rb][e] - kc[rb][e])) : 0.f;
+        const int r = rb * 16 + r4 + e;
+        g[e] = own ? fmaf(element(Qg, a.d.q_st, r), q1[rb][e], element(Kg, a.d.k_st, r) * (kr[rb][e] - kc[rb][e])) : 0.f;
         for (int o = 1; o < 16; o <<= 1) g[e] += __shfl_xor(g[e], o);
       }
       if (col == 0)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dG[wave * C + rb * 16 + r4 + e] = g[e];
-      dq[rb] += q1[rb];
-      dk[rb] += kr[rb] + kc[rb];
+      kr[rb] += kc[rb];
+      if (GROUPED) {
+        if (m > 0) {
+          q1[rb] += sums[rb * 512 + t];
+          kr[rb] += sums[(4 + rb) * 512 + t];
+        }
+        sums[rb * 512 + t] = q1[rb];
+        sums[(4 + rb) * 512 + t] = kr[rb];
+      }
+      if (m + 1 == group && own && kc0 < a.d.dk) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = rb * 16 + r4 + e;
+          if (r < len) {
+            const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + kc0;
+            st<T>(a.d_q, p, q1[rb][e]);
+            st<T>(a.d_k, p, kr[rb][e]);
+          }
+        }
+      }
     }
     __syncthreads();
     if (wave == 0) {
@@ -1068,19 +1084,6 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         a.d_beta[p] = db[lane];
       }
     }
-  }
-  if (own && kc0 < a.d.dk) {
-#pragma unroll
-    for (int rb = 0; rb < 4; ++rb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = rb * 16 + r4 + e;
-        if (r < len) {
-          const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + kc0;
-          st<T>(a.d_q, p, dq[rb][e]);
-          st<T>(a.d_k, p, dk[rb][e]);
-        }
-      }
   }
 }
 
@@ -1281,7 +1284,6 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
     part(x.Qf, kheads * n * KF * 2);
     part(x.Tf, heads * 3 * TF * 2);
     part(x.Pf, heads * no * TF * 2);
-    part(x.V, heads * C * dvp * (d->dtype == GPX_F32 ? 4 : 2));
     part(x.E, heads * C * dvp * 4);
     part(x.S, heads * 128 * dvp * 4);
   }
@@ -1310,6 +1312,7 @@ int check_delta(const gpx_delta* d, const char* what) {
   GPX_REQUIRE(heads * 40 < 2.0e9, "%s: too many heads and chunks for one call", what);
   for (const gpx_strided* s : {&d->q_st, &d->k_st, &d->v_st, &d->g_st, &d->beta_st})
     GPX_REQUIRE(s->bs >= 0 && s->rs >= 0 && s->cs >= 0, "%s: negative stride", what);
+  GPX_REQUIRE(d->v_st.rs <= (1 << 22), "%s: token stride of v beyond 2^22", what);   // 32-bit offsets inside a chunk
   if (d->batch > 0 && d->tokens > 0)
     GPX_REQUIRE(d->q && d->k && d->v && d->g && d->beta, "%s: null input", what);
   return 0;
@@ -1375,9 +1378,10 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
 template <typename T, int DK>
 int run_backward(hipStream_t s, const Args& a) {
   constexpr size_t room = (Planes<T>::N + 6) * C * 40 > 6 * C * (C + 8) ? (Planes<T>::N + 6) * C * 40 : 6 * C * (C + 8);
-  constexpr size_t lds = room * 2 + C * 8 + (8 * C + 8 + C) * 4;
-  static_assert(lds <= 160 * 1024, "LDS");
-  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK>, lds));
+  constexpr size_t lds = room * 2 + C * 8 + (8 * C + 8 + C) * 4, grouped = lds + 8 * 512 * 16;
+  static_assert(grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
+  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK, false>, lds));
+  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK, true>, grouped));
   const long slots = slots_of(&a.d);
   if (slots > 0) {
     hipLaunchKernelGGL((delta_back_prep_kernel<T>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
@@ -1386,7 +1390,11 @@ int run_backward(hipStream_t s, const Args& a) {
   hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1, true>), dim3(chain_grid(a, 1)), dim3(256), 0, s, a);
   GPX_HIP(hipGetLastError());
   if (slots > 0) {
-    hipLaunchKernelGGL((delta_grads_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(512), lds, s, a);
+    const dim3 grid((unsigned)(slots * a.d.key_heads));
+    if (a.group == 1)
+      hipLaunchKernelGGL((delta_grads_kernel<T, DK, false>), grid, dim3(512), lds, s, a);
+    else
+      hipLaunchKernelGGL((delta_grads_kernel<T, DK, true>), grid, dim3(512), grouped, s, a);
     GPX_HIP(hipGetLastError());
   }
   return 0;

@@ -23,7 +23,8 @@ _TYPES = ("float32", "float16", "bfloat16")
 
 
 def _dense(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t, or a packed copy where its last dimension is not dense or its tokens lie too far apart for the library."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-3) <= 1 << 22 else t.contiguous()
 
 
 def _st(t):

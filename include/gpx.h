@@ -318,7 +318,7 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m);
  * clamped, a decreasing value is read as the one before it).  Tokens behind the last sequence or before the first are
  * not read and their outputs not written.  Sequences may be empty: their state passes through.
  * g may be -infinity (the state is forgotten).  beta == 0 and g == 0 leave the state as it is.  1 <= dk <= 128,
- * 1 <= dv <= 1024.  States, decays and all sums are fp32 or wider. */
+ * 1 <= dv <= 1024; a token stride of v of at most 2^22.  States, decays and all sums are fp32 or wider. */
 typedef struct gpx_delta {
   int dtype, batch, tokens, sequences, key_heads, value_heads, dk, dv;
   double scale;
