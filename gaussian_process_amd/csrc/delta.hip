@@ -93,8 +93,7 @@ struct Args {
   float* fac;                   // per head: exp(G), beta, exp(G_C - G) beta, exp(G_C), exp(G_C - G), exp(G) beta; C each
   __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
-  float *E, *Erow;              // per head: E^T, dvp x C; E, C x dvp
-  float *S, *Srow;              // per head: S in state order, dvp / 16 x 4 x 64 x 8; S, DK x dvp
+  float *Erow, *Srow;           // per head: E, C x dvp; S, DK x dvp
   float* Y;                     // per head: (scale P^T dO)^T, dvp x C
   __bf16* Of;                   // per head: scale exp(G) dO as fragments, dvp / 16 x 2 x 64 x 8 by three planes
   float *Z, *dS;                // per head: Z (dX = beta Z), C x dvp; dS', DK x dvp
@@ -211,36 +210,49 @@ constexpr int KF = 4 * 4 * 64 * 8;   // elements of a plane of K or Q in state o
 constexpr int TF = 4 * 2 * 64 * 8;   // of a C x C matrix
 constexpr int FACS = 6 * C;          // factors per head
 
-// C rows of one head as planes in LDS, pitch DK + 8
+// C rows of one head as planes in LDS, pitch DK + 8: fetch() has all loads under way, put() splits and writes
 template <typename T, int DK>
-__device__ __forceinline__ void load_planes(__bf16* dst, const void* src, const gpx_strided& s, long row, int t0, int len, int head, int dk,
-                                            int t) {
-  constexpr int P = DK + 8, N = Planes<T>::N;
-  const T* base = reinterpret_cast<const T*>(src) + row * s.bs + t0 * s.rs + head * s.cs;
-  const bool vec = ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(s.rs * sizeof(T))) & 15) == 0;
-  for (int i = t; i < C * DK / 8; i += 256) {
-    const int r = i / (DK / 8), c = i % (DK / 8) * 8;
-    float x[8];
-    if (r < len && vec && c + 8 <= dk) {
-      T v[8];
-      constexpr int W = sizeof(T) * 8 / 16;
-      const uint4* q = reinterpret_cast<const uint4*>(base + r * s.rs + c);
-      uint4 u[W];
+struct Rows {
+  static constexpr int IT = C * DK / 8 / 256, W = sizeof(T) / 2;
+  uint4 raw[IT][W];
+  __device__ __forceinline__ void fetch(const void* src, const gpx_strided& s, long row, int t0, int len, int head, int dk, int t) {
+    const T* base = reinterpret_cast<const T*>(src) + row * s.bs + t0 * s.rs + head * s.cs;
+    if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(s.rs * sizeof(T))) & 15) == 0 && dk == DK) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) u[k] = q[k];
-      __builtin_memcpy(v, u, sizeof(v));
+      for (int i = 0; i < IT; ++i) {   // rows behind the end repeat the last
+        const int q = i * 256 + t, r = min(q / (DK / 8), len - 1), c = q % (DK / 8) * 8;
+        const uint4* p = reinterpret_cast<const uint4*>(base + r * s.rs + c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+        for (int w = 0; w < W; ++w) raw[i][w] = p[w];
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = r < len && c + e < dk ? (float)base[r * s.rs + c + e] : 0.f;
-    }
-    b8 p[N];
-    split<8, N>(x, p);
+      for (int i = 0; i < IT; ++i) {
+        const int q = i * 256 + t, r = min(q / (DK / 8), len - 1), c = q % (DK / 8) * 8;
+        T v[8];
 #pragma unroll
-    for (int k = 0; k < N; ++k) *reinterpret_cast<b8*>(dst + (k * C + r) * P + c) = p[k];
+        for (int e = 0; e < 8; ++e) v[e] = base[r * s.rs + min(c + e, dk - 1)];
+        __builtin_memcpy(raw[i], v, sizeof(v));
+      }
+    }
   }
-}
+  __device__ __forceinline__ void put(__bf16* dst, int len, int dk, int t) const {
+    constexpr int P = DK + 8, N = Planes<T>::N;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int q = i * 256 + t, r = q / (DK / 8), c = q % (DK / 8) * 8;
+      T v[8];
+      __builtin_memcpy(v, raw[i], sizeof(v));
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = r < len && c + e < dk ? (float)v[e] : 0.f;
+      b8 p[N];
+      split<8, N>(x, p);
+#pragma unroll
+      for (int k = 0; k < N; ++k) *reinterpret_cast<b8*>(dst + (k * C + r) * P + c) = p[k];
+    }
+  }
+};
 
 // T = (I + A)^-1 for the strictly lower A (LDS, pitch PC), 4 waves.  The 16 x 16 diagonal blocks by substitution, one column
 // per lane; then block T_ij = -T_ii sum_l A_il T_lj for i - j = 1, 2, 3, on the fp32 matrix cores.  tmp: 4 x 16 x 20 floats.
@@ -320,8 +332,13 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
   if (len == 0) return;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
   const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
-  load_planes<T, DK>(K, a.d.k, a.d.k_st, row, t0, len, hk, a.d.dk, t);
-  load_planes<T, DK>(Q, a.d.q, a.d.q_st, row, t0, len, hk, a.d.dk, t);
+  {
+    Rows<T, DK> k, q;
+    k.fetch(a.d.k, a.d.k_st, row, t0, len, hk, a.d.dk, t);
+    q.fetch(a.d.q, a.d.q_st, row, t0, len, hk, a.d.dk, t);
+    k.put(K, len, a.d.dk, t);
+    q.put(Q, len, a.d.dk, t);
+  }
   __syncthreads();
   // K and Q in state order, K^T in natural order
   for (int i = t; i < KF / 8; i += 256) {
@@ -437,322 +454,327 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
   }
 }
 
-// ---- the scans: NT tiles of 16 columns of dv of one value head of one sequence ------------------------------------------------
+// ---- the scans: 16 columns of dv of one value head of one sequence ----------------------------------------------------------------
 // Forward, chunk after chunk:    X = V - exp(G) K S;       E = T X;      S <- exp(G_C) S + K^T (exp(G_C - G) beta E)
 // Backward (BACK), from the last: X = Y + exp(G_C - G) K dS;  Z = T2^T X;   dS <- exp(G_C) dS - K^T (exp(G) beta Z) + Q^T Of
 // (Y = scale P^T dO, Of = scale exp(G) dO, from delta_back_prep_kernel).
 // Bound by the chain from chunk to chunk: the product with K (each wave with its own rows of S, which are in its accumulators;
-// partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.
-// Fragments come straight from memory, for the next chunk as soon as this chunk has used its own (two chunks ahead gained
-// nothing); every load is issued whatever comes, since loads behind branches make the compiler wait for all that are under way.
+// partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.  Four waves do that
+// and nothing else; four more take S and E from LDS and do what the chain does not wait for -- forward the outputs
+// O = scale (exp(G) Q S + P beta E), backward Q^T Of, and all stores.  (A wave waits for its memory accesses in order: with
+// the stores in the chain's waves its loads waited for them, 256 us for 8192 tokens x 16 heads against 186 without stores and 137 without
+// any access.)  Fragments come straight from memory, SETS chunks ahead; every load is issued whatever comes, since loads behind
+// branches make the compiler wait for all that are under way.
 __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes) {
   return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
 }
 
-// two waves per SIMD where the fragments leave the registers for it
-constexpr int chain_waves(int planes, bool back) { return planes == 1 || (planes == 2 && !back) ? 2 : 1; }
-
-template <typename T, int DK, int NT, bool BACK>
-__global__ __launch_bounds__(256, chain_waves(Planes<T>::N, BACK)) void delta_chain_kernel(const Args a) {
-  constexpr int N = Planes<T>::N, RT = DK / 64, PT = C + 8;
-  __shared__ f4 part[4][4][NT][64];              // K S: wave, row block
-  __shared__ __align__(16) __bf16 X[3][NT * 16][PT], U[3][NT * 16][PT];
-  const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / (NT * 16);
+template <typename T, int DK, bool BACK>
+__global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
+  constexpr int N = Planes<T>::N, NO = OutPlanes<T>::N, RT = DK / 64, PT = C + 8, PE = C + 4;
+  constexpr int SETS = N == 1 ? 2 : 1;           // as many as the registers hold
+  __shared__ f4 part[4][4][64];                  // K S: wave, row block
+  __shared__ f4 Sx[4][2][64];                    // S: wave, tile
+  __shared__ f4 Rx[4][2][64];                    // BACK: Q^T Of, likewise
+  __shared__ __align__(16) float Ex[16][PE];     // E^T or Z^T
+  __shared__ __align__(16) __bf16 X[3][16][PT], U[3][16][PT];
+  const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / 16;
   int slice, head;
   if (!scan_coords(blockIdx.x, slices, heads, slice, head)) return;
   const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
-  const int c0 = slice * NT * 16;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15,
-            g8 = (lane >> 4) * 8;
+  const int c0 = slice * 16;
+  const int t = threadIdx.x, lane = t & 63, wave8 = __builtin_amdgcn_readfirstlane(t >> 6), wave = wave8 & 3, r4 = (lane >> 4) * 4,
+            col = lane & 15, g8 = (lane >> 4) * 8;
   const int begin = a.p.begin(s), end = a.p.end(s), chunks = (end - begin + C - 1) / C;
-  const long slot0 = a.p.slot0(s);
+  const long slot0 = a.p.slot0(s), row = a.p.row(s);
   const unsigned lb = lane * 16;
-  f4 S[RT][NT];
-  const float* init = BACK ? a.d_state_out : a.state;
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
-        S[i][j][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
-      }
-  b8 kf[4][N], tf[2][3], kt[RT][2][N], qt[RT][2][N], of[NT][2][3];
-  T v[NT][4];
-  f4 y[NT], fx, fu;
-  float keep;
-  const T* V = reinterpret_cast<const T*>(a.d.v) + a.p.row(s) * a.d.v_st.bs + begin * a.d.v_st.rs + hv * a.d.v_st.cs;
-  const unsigned vrs = (unsigned)a.d.v_st.rs;
-  auto load_k = [&](long slot) {
-    const __bf16* p = a.Kf + (slot * a.d.key_heads + hk) * N * KF + wave * 512;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < N; ++k) kf[i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
-  };
-  auto load_x = [&](long at, int n) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (BACK) {
-        y[j] = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + (unsigned)((j * 16 + col) * C + wave * 16 + r4));
-      } else {   // rows and columns behind the end repeat the last; they are masked where they are used
-        const T* p = V + (long)n * C * a.d.v_st.rs;
-        const unsigned last = min(C, end - begin - n * C) - 1, c = min(c0 + j * 16 + col, a.d.dv - 1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = p[min((unsigned)(wave * 16 + r4 + e), last) * vrs + c];
-      }
-    }
-    fx = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 4 * C : 0) + wave * 16 + r4);
-  };
-  auto load_t = [&](long at) {
-    const __bf16* p = (BACK ? a.T2f : a.Tf) + at * 3 * TF + wave * 2 * 512;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      tf[0][k] = ld_frag(p + k * TF, lb);
-      tf[1][k] = ld_frag(p + k * TF + 512, lb);
-    }
-    fu = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 5 : 2) * C + wave * 16 + r4);
-  };
-  auto load_kt = [&](long slot, long at) {
-    const long o = (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
+
+  if (wave8 < 4) {   // ---- the chain
+    f4 S[RT];
+    const float* init = BACK ? a.d_state_out : a.state;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+      for (int e = 0; e < 4; ++e) {
+        const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + col;
+        S[i][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
+      }
+    b8 kf[SETS][4][N], tf[SETS][2][3], kt[SETS][RT][2][N];
+    T v[SETS][4];
+    f4 y[SETS], fx[SETS], fu[SETS];
+    float keep[SETS];
+    const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + begin * a.d.v_st.rs + hv * a.d.v_st.cs;
+    const unsigned vrs = (unsigned)a.d.v_st.rs, vcol = min(c0 + col, a.d.dv - 1);
+    auto load_k = [&](int u, long slot) {
+      const __bf16* p = a.Kf + (slot * a.d.key_heads + hk) * N * KF + wave * 512;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          kt[i][ks][k] = ld_frag(a.KTf + o + k * (DK * C) + (i * 2 + ks) * 512, lb);
-          if (BACK) qt[i][ks][k] = ld_frag(a.QTf + o + k * (DK * C) + (i * 2 + ks) * 512, lb);
-        }
-    if (BACK) {
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+        for (int k = 0; k < N; ++k) kf[u][i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
+    };
+    auto load_x = [&](int u, long at, int m) {
+      if (BACK) {
+        y[u] = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + (unsigned)(col * C + wave * 16 + r4));
+      } else {   // rows and columns behind the end repeat the last; they are masked where they are used
+        const T* p = V + (long)m * C * a.d.v_st.rs;
+        const unsigned last = min(C, end - begin - m * C) - 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[u][e] = p[min((unsigned)(wave * 16 + r4 + e), last) * vrs + vcol];
+      }
+      fx[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 4 * C : 0) + wave * 16 + r4);
+    };
+    auto load_t = [&](int u, long at) {
+      const __bf16* p = (BACK ? a.T2f : a.Tf) + at * 3 * TF + wave * 2 * 512;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        tf[u][0][k] = ld_frag(p + k * TF, lb);
+        tf[u][1][k] = ld_frag(p + k * TF + 512, lb);
+      }
+      fu[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 5 : 2) * C + wave * 16 + r4);
+    };
+    auto load_kt = [&](int u, long slot, long at) {
+      const __bf16* p = a.KTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int k = 0; k < 3; ++k)
-            of[j][ks][k] = ld_frag(a.Of + (at * 3 + k) * (a.dvp * C) + (c0 / 16 + j) * 1024 + ks * 512, lb);
-    }
-    keep = a.fac[at * FACS + 3 * C + lane];   // by lane: a scalar load would be waited for with LDS
-  };
-  if (chunks > 0) {
-    const int m = BACK ? chunks - 1 : 0;
-    const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
-    load_k(slot);
-    load_x(at, m);
-    load_t(at);
-    load_kt(slot, at);
-  }
-  for (int n = 0; n < chunks; ++n) {
-    const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - 1, 0) : min(m + 1, chunks - 1);
-    const long at = (slot0 + m) * a.d.value_heads + hv, nslot = slot0 + nm, nat = nslot * a.d.value_heads + hv;
-    const int live = BACK ? 0 : end - begin - n * C - wave * 16 - r4;   // rows e < live hold tokens
-    // S as planes, and to memory
+          for (int k = 0; k < N; ++k) kt[u][i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
+      keep[u] = a.fac[at * FACS + 3 * C + lane];   // by lane: a scalar load would be waited for with LDS
+    };
+    auto chunk = [&](int u, int n) {
+      const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - SETS, 0) : min(m + SETS, chunks - 1);
+      const long nslot = slot0 + nm, nat = nslot * a.d.value_heads + hv;
+      const int live = BACK ? 0 : end - begin - n * C - wave * 16 - r4;   // rows e < live hold tokens
+      {
+        float x[8];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float x[8];
+        for (int e = 0; e < 4; ++e) {
+          x[e] = S[0][e];
+          x[4 + e] = RT == 2 ? S[RT - 1][e] : 0.f;
+        }
+        Sx[wave][0][lane] = S[0];
+        if (RT == 2) Sx[wave][1][lane] = S[RT - 1];
+        b8 sb[3];
+        split<8, 3>(x, sb);
+        f4 p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = S[0][j][e];
-        x[4 + e] = RT == 2 ? S[RT - 1][j][e] : 0.f;
+        for (int i = 0; i < 4; ++i) p[i] = f4{0, 0, 0, 0};
+        // plane by plane over the four row blocks: four chains of matrix instructions side by side
+#pragma unroll
+        for (int q = 2; q >= 0; --q)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (q >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[u][i][k], sb[q - k], p[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][i][lane] = p[i];
       }
-      b8 sb[3];
-      split<8, 3>(x, sb);
-      f4 p[4];
+      load_k(u, nslot);
+      lds_barrier();
+      {
+        const f4 p = (part[0][wave][lane] + part[1][wave][lane]) + (part[2][wave][lane] + part[3][wave][lane]);
+        float x[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = f4{0, 0, 0, 0};
-      // plane by plane over the four row blocks: four chains of matrix instructions side by side
+        for (int e = 0; e < 4; ++e)
+          x[e] = BACK ? fmaf(fx[u][e], p[e], y[u][e]) : e < live && c0 + col < a.d.dv ? fmaf(-fx[u][e], p[e], (float)v[u][e]) : 0.f;
+        b4 xp[3];
+        split<4, 3>(x, xp);
 #pragma unroll
-      for (int q = 2; q >= 0; --q)
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&X[k][col][wave * 16 + r4]) = xp[k];
+      }
+      load_x(u, nat, nm);
+      lds_barrier();
+      {
+        // T's upper, T2^T's lower half is zeros
+        f4 e0 = {0, 0, 0, 0}, e1 = {0, 0, 0, 0};
+        b8 xb[3];
+        if (!BACK || wave < 2) {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
+          for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][col][g8]);
+          e0 = planes_mma<3, 3, 3>(tf[u][0], xb, e0);
+        }
+        if (BACK || wave >= 2) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (q >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], sb[q - k], p[i], 0, 0, 0);
+          for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][col][32 + g8]);
+          e1 = planes_mma<3, 3, 3>(tf[u][1], xb, e1);
+        }
+        const f4 ev = e0 + e1;
+        float w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][i][j][lane] = p[i];
-      if (!BACK) {
-        f4* dst = reinterpret_cast<f4*>(a.S + ((at * (a.dvp / 16) + c0 / 16 + j) * 4 + wave) * 512 + lane * 8);
-        dst[0] = S[0][j];
-        if (RT == 2) dst[1] = S[RT - 1][j];
+        for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fu[u][e] : fu[u][e]) * ev[e];
+        b4 up[3];
+        split<4, 3>(w, up);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&U[k][col][wave * 16 + r4]) = up[k];
+        *reinterpret_cast<f4*>(&Ex[col][wave * 16 + r4]) = ev;
+      }
+      load_t(u, nat);
+      lds_barrier();
+      {
+        f4 more[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          S[i] *= keep[u];
+          more[i] = BACK ? Rx[wave][i][lane] : f4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          b8 ub[3];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) ub[k] = *reinterpret_cast<const b8*>(&U[k][col][ks * 32 + g8]);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            if (ks == 0)
+              S[i] = planes_mma<N, 3, 3>(kt[u][i][ks], ub, S[i]);
+            else
+              more[i] = planes_mma<N, 3, 3>(kt[u][i][ks], ub, more[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) S[i] += more[i];
+      }
+      load_kt(u, nslot, nat);
+    };
+    if (chunks > 0) {
+#pragma unroll
+      for (int u = 0; u < SETS; ++u) {
+        const int m = BACK ? max(chunks - 1 - u, 0) : min(u, chunks - 1);
+        const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
+        load_k(u, slot);
+        load_x(u, at, m);
+        load_t(u, at);
+        load_kt(u, slot, at);
+      }
+    }
+    for (int n = 0; n < chunks; n += SETS) {
+      chunk(0, n);
+      if (SETS == 2 && n + 1 < chunks) chunk(SETS - 1, n + 1);
+    }
+    float* out = BACK ? a.d_state : a.state_out;
+    if (out != nullptr) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + col;
+          if (r < a.d.dk && c < a.d.dv) out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][e];
+        }
+    }
+  } else {   // ---- beside the chain; the same three barriers per chunk
+    b8 qf[4][N], pf[2][NO], qt[RT][2][N], of[2][3];
+    f4 eg, bt[4];
+    auto load = [&](long slot, long at) {
+      if (BACK) {
+        const __bf16* p = a.QTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int k = 0; k < N; ++k) qt[i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) of[ks][k] = ld_frag(a.Of + (at * 3 + k) * (a.dvp * C) + slice * 1024 + ks * 512, lb);
+        }
+      } else {
+        const __bf16* q = a.Qf + (slot * a.d.key_heads + hk) * N * KF + wave * 4 * 512;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < N; ++k) qf[i][k] = ld_frag(q + k * KF + i * 512, lb);
+        const __bf16* p = a.Pf + at * NO * TF + wave * 2 * 512;
+#pragma unroll
+        for (int k = 0; k < NO; ++k) {
+          pf[0][k] = ld_frag(p + k * TF, lb);
+          pf[1][k] = ld_frag(p + k * TF + 512, lb);
+        }
+        const float* f = a.fac + at * FACS;
+        eg = *reinterpret_cast<const f4*>(f + wave * 16 + r4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bt[i] = *reinterpret_cast<const f4*>(f + C + (i >> 1) * 32 + g8 + (i & 1) * 4);
+      }
+    };
+    if (chunks > 0) {
+      const long slot = slot0 + (BACK ? chunks - 1 : 0);
+      load(slot, slot * a.d.value_heads + hv);
+    }
+    for (int n = 0; n < chunks; ++n) {
+      const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - 1, 0) : min(m + 1, chunks - 1);
+      const long at = (slot0 + m) * a.d.value_heads + hv;
+      f4 o = {0, 0, 0, 0}, mine[2];
+      if (BACK) {
+        f4 r[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) r[i] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[i][ks], of[ks], r[i]);
+        lds_barrier();   // the chain has read the Rx of the chunk before
+#pragma unroll
+        for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) mine[i] = Sx[wave][i][lane];
+      } else {
+        lds_barrier();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const f4 s0 = Sx[w][0][lane], s1 = RT == 2 ? Sx[w][1][lane] : f4{0, 0, 0, 0};
+          if (w == wave) {
+            mine[0] = s0;
+            mine[1] = s1;
+          }
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = s0[e];
+            x[4 + e] = s1[e];
+          }
+          b8 sb[NO];
+          split<8, NO>(x, sb);
+          o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[w], sb, o);
+        }
+        o *= eg;
       }
       if (BACK || a.save) {
-        float* dst = (BACK ? a.dS : a.Srow) + (at * DK + wave * RT * 16) * a.dvp + c0 + j * 16;
+        float* dst = (BACK ? a.dS : a.Srow) + (at * DK + wave * RT * 16) * a.dvp + c0;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dst[(unsigned)((i * 16 + r4 + e) * a.dvp + col)] = S[i][j][e];
+          for (int e = 0; e < 4; ++e) dst[(unsigned)((i * 16 + r4 + e) * a.dvp + col)] = mine[i][e];
       }
-    }
-    load_k(nslot);
-    lds_barrier();
+      lds_barrier();
+      lds_barrier();
+      if (!BACK) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const f4 p = (part[0][wave][j][lane] + part[1][wave][j][lane]) + (part[2][wave][j][lane] + part[3][wave][j][lane]);
-      float x[4];
+        for (int ks = 0; ks < 2; ++ks) {
+          if (ks * 2 > wave) continue;   // P is lower triangular
+          const f4 e0 = *reinterpret_cast<const f4*>(&Ex[col][ks * 32 + g8]), e1 = *reinterpret_cast<const f4*>(&Ex[col][ks * 32 + g8 + 4]);
+          float x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = BACK ? fmaf(fx[e], p[e], y[j][e])
-                    : e < live && c0 + j * 16 + col < a.d.dv ? fmaf(-fx[e], p[e], (float)v[j][e]) : 0.f;
-      b4 xp[3];
-      split<4, 3>(x, xp);
+          for (int e = 0; e < 4; ++e) {
+            x[e] = e0[e] * bt[ks * 2][e];
+            x[4 + e] = e1[e] * bt[ks * 2 + 1][e];
+          }
+          b8 ub[NO];
+          split<8, NO>(x, ub);
+          o = planes_mma<NO, NO, NO>(pf[ks], ub, o);
+        }
+        const int t0 = begin + n * C + wave * 16 + r4;
+        T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + t0) * a.d.value_heads + hv) * (long)a.d.dv + c0 + col;
+        if (c0 + col < a.d.dv)
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&X[k][j * 16 + col][wave * 16 + r4]) = xp[k];
-    }
-    load_x(nat, nm);
-    lds_barrier();
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      // T's upper, T2^T's lower half is zeros
-      f4 e0 = {0, 0, 0, 0}, e1 = {0, 0, 0, 0};
-      b8 xb[3];
-      if (!BACK || wave < 2) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][g8]);
-        e0 = planes_mma<3, 3, 3>(tf[0], xb, e0);
+          for (int e = 0; e < 4; ++e)
+            if (t0 + e < end) out[(long)e * a.d.value_heads * a.d.dv] = (T)(a.scale * o[e]);
       }
-      if (BACK || wave >= 2) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][j * 16 + col][32 + g8]);
-        e1 = planes_mma<3, 3, 3>(tf[1], xb, e1);
-      }
-      const f4 ev = e0 + e1;
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fu[e] : fu[e]) * ev[e];
-      b4 up[3];
-      split<4, 3>(w, up);
-#pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&U[k][j * 16 + col][wave * 16 + r4]) = up[k];
-      if (!BACK) *reinterpret_cast<f4*>(a.E + (at * a.dvp + c0 + j * 16) * C + (unsigned)(col * C + wave * 16 + r4)) = ev;
       if (BACK || a.save) {
-        float* dst = (BACK ? a.Z : a.Erow) + (at * C + wave * 16) * a.dvp + c0 + j * 16;
+        const f4 ev = *reinterpret_cast<const f4*>(&Ex[col][wave * 16 + r4]);
+        float* dst = (BACK ? a.Z : a.Erow) + (at * C + wave * 16) * a.dvp + c0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) dst[(unsigned)((r4 + e) * a.dvp + col)] = ev[e];
       }
-    }
-    load_t(nat);
-    lds_barrier();
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      f4 more_s[RT];
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        S[i][j] *= keep;
-        more_s[i] = f4{0, 0, 0, 0};
-      }
-      if (BACK) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int i = 0; i < RT; ++i) more_s[i] = planes_mma<N, 3, 3>(qt[i][ks], of[j][ks], more_s[i]);
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        b8 ub[3];
-#pragma unroll
-        for (int k = 0; k < 3; ++k) ub[k] = *reinterpret_cast<const b8*>(&U[k][j * 16 + col][ks * 32 + g8]);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          if (ks == 0)
-            S[i][j] = planes_mma<N, 3, 3>(kt[i][ks], ub, S[i][j]);
-          else
-            more_s[i] = planes_mma<N, 3, 3>(kt[i][ks], ub, more_s[i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < RT; ++i) S[i][j] += more_s[i];
-    }
-    load_kt(nslot, nat);
-  }
-  float* out = BACK ? a.d_state : a.state_out;
-  if (out != nullptr) {
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + j * 16 + col;
-          if (r < a.d.dk && c < a.d.dv) out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][j][e];
-        }
-  }
-}
-
-// ---- outputs: one chunk, 64 columns of dv, a wave for each 16 ----------------------------------------------------------------
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_out_kernel(const Args a) {
-  constexpr int N = Planes<T>::N, NO = OutPlanes<T>::N, RT = DK / 64;
-  constexpr int LIM = NO;   // planes i + j kept
-  __shared__ __align__(16) T st[C][64 + 8];
-  const int groups = (a.dvp + 63) / 64;
-  const int cg = blockIdx.x % groups;
-  const long at = blockIdx.x / groups;   // slot * value_heads + hv
-  const int hv = (int)(at % a.d.value_heads), slot = (int)(at / a.d.value_heads), hk = hv / a.group;
-  int s, t0, len;
-  a.p.locate(slot, s, t0, len);
-  if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
-  const int ct = cg * 4 + wave;   // column tile
-  if (ct * 16 < a.dvp) {
-    const float* fac = a.fac + at * FACS;
-    b8 sb[4][NO], ub[2][NO];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float* p = a.S + ((at * (a.dvp / 16) + ct) * 4 + w) * 512 + lane * 8;
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = RT == 2 || e < 4 ? p[e] : 0.f;
-      split<8, NO>(x, sb[w]);
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const float* p = a.E + (at * a.dvp + ct * 16 + col) * C + ks * 32 + g8;
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = p[e] * fac[C + ks * 32 + g8 + e];
-      split<8, NO>(x, ub[ks]);
-    }
-    const __bf16* qf = a.Qf + ((long)slot * a.d.key_heads + hk) * N * KF + lane * 8;
-    const __bf16* pf = a.Pf + at * NO * TF + lane * 8;
-#pragma unroll
-    for (int rb = 0; rb < 4; ++rb) {
-      f4 o = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        b8 q[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) q[k] = *reinterpret_cast<const b8*>(qf + k * KF + (rb * 4 + w) * 512);
-        o = planes_mma<N, NO, N == 2 ? 3 : LIM>(q, sb[w], o);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= fac[rb * 16 + r4 + e];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if (ks * 2 > rb) continue;
-        b8 p[NO];
-#pragma unroll
-        for (int k = 0; k < NO; ++k) p[k] = *reinterpret_cast<const b8*>(pf + k * TF + (rb * 2 + ks) * 512);
-        o = planes_mma<NO, NO, LIM>(p, ub[ks], o);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) st[rb * 16 + r4 + e][wave * 16 + col] = (T)(a.scale * o[e]);
-    }
-  }
-  __syncthreads();
-  const int c0 = cg * 64, w = min(64, a.d.dv - c0);
-  T* out = reinterpret_cast<T*>(a.o) + ((a.p.row(s) * a.d.tokens + t0) * a.d.value_heads + hv) * (long)a.d.dv + c0;
-  const long rs = (long)a.d.value_heads * a.d.dv;
-  constexpr int V = 16 / sizeof(T);
-  if (w == 64 && (a.d.dv * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0) {
-    for (int i = t; i < C * 64 / V; i += 256) {
-      const int r = i / (64 / V), c = i % (64 / V) * V;
-      if (r < len) *reinterpret_cast<uint4*>(out + r * rs + c) = *reinterpret_cast<const uint4*>(&st[r][c]);
-    }
-  } else {
-    for (int i = t; i < C * 64; i += 256) {
-      const int r = i >> 6, c = i & 63;
-      if (r < len && c < w) out[r * rs + c] = st[r][c];
+      load(slot0 + nm, (slot0 + nm) * a.d.value_heads + hv);
     }
   }
 }
@@ -1284,8 +1306,6 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
     part(x.Qf, kheads * n * KF * 2);
     part(x.Tf, heads * 3 * TF * 2);
     part(x.Pf, heads * no * TF * 2);
-    part(x.E, heads * C * dvp * 4);
-    part(x.S, heads * 128 * dvp * 4);
   }
   if (use == SCRATCH) {
     part(x.Y, heads * C * dvp * 4);
@@ -1344,9 +1364,9 @@ int allow_lds(F* kernel, size_t bytes) {
     if (rc_ != 0) return rc_; \
   } while (0)
 
-unsigned chain_grid(const Args& a, int nt) {
+unsigned chain_grid(const Args& a) {
   const unsigned heads = (unsigned)a.p.sequences * a.d.value_heads;
-  return (heads + 7) / 8 * 8 * (a.dvp / (16 * nt));
+  return (heads + 7) / 8 * 8 * (a.dvp / 16);
 }
 
 template <typename T, int DK>
@@ -1366,12 +1386,8 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
     hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(256), lds, s, a);
     GPX_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1, false>), dim3(chain_grid(a, 1)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((delta_chain_kernel<T, DK, false>), dim3(chain_grid(a)), dim3(512), 0, s, a);
   GPX_HIP(hipGetLastError());
-  if (slots > 0) {
-    hipLaunchKernelGGL((delta_out_kernel<T, DK>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
-    GPX_HIP(hipGetLastError());
-  }
   return 0;
 }
 
@@ -1387,7 +1403,7 @@ int run_backward(hipStream_t s, const Args& a) {
     hipLaunchKernelGGL((delta_back_prep_kernel<T>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
     GPX_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL((delta_chain_kernel<T, DK, 1, true>), dim3(chain_grid(a, 1)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((delta_chain_kernel<T, DK, true>), dim3(chain_grid(a)), dim3(512), 0, s, a);
   GPX_HIP(hipGetLastError());
   if (slots > 0) {
     const dim3 grid((unsigned)(slots * a.d.key_heads));

@@ -180,7 +180,7 @@ def test_work_bytes():
     heads, kheads = 2 * 2 * 4, 2 * 2 * 2   # rows, chunks, heads; dv rounded up to 64, dk to 64
     square = 64 * 64                       # elements of a fragment-wise C x C or dk x C matrix; K and Q take two
     both_ = heads * (64 * 8 + 6 * 64 * 4) + kheads * 3 * square * 2
-    work = kheads * 2 * square * 2 + heads * (5 * square * 2 + 64 * 64 * 4 + 128 * 64 * 4)
+    work = kheads * 2 * square * 2 + heads * 5 * square * 2
     assert w(0) == both_ + work and w(3) == work
     assert w(1) == both_ + kheads * square * 2 + heads * (6 * square * 2 + (64 + 64) * 64 * 4)
     assert w(2) == heads * (64 * 64 * 4 + 3 * 64 * 64 * 2 + (64 + 64) * 64 * 4)
