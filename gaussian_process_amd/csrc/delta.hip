@@ -316,15 +316,21 @@ template <typename T> struct OutPlanes { static constexpr int N = sizeof(T) == 2
 
 // ---- prep: one chunk of one key head and its value heads -----------------------------------------------------------------
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
+constexpr size_t chunk_room() {
+  constexpr size_t first = 2 * Planes<T>::N * C * (DK + 8) * 2, second = (2 * C * PC + 4 * 16 * 20) * 4;
+  return first > second ? first : second;
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kernel(const Args a) {
   constexpr int N = Planes<T>::N, P = DK + 8, RT = DK / 64, KSN = DK / 32;
   extern __shared__ __align__(16) char smem[];
   __bf16* K = reinterpret_cast<__bf16*>(smem);
   __bf16* Q = K + N * C * P;
-  float* A = reinterpret_cast<float*>(Q + N * C * P);
+  float* A = reinterpret_cast<float*>(smem);   // over K and Q, once these are in registers and memory
   float* M = A + C * PC;
   float* tmp = M + C * PC;
-  double* G = reinterpret_cast<double*>(tmp + 4 * 16 * 20);
+  double* G = reinterpret_cast<double*>(smem + chunk_room<T, DK>());
   float* beta = reinterpret_cast<float*>(G + C);
   const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
   int s, t0, len;
@@ -332,6 +338,13 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
   if (len == 0) return;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
   const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
+  float gv = 0.f, bv = 0.f;   // wave 0: g and beta of the next value head
+  auto load_g = [&](int hv) {
+    const int tok = t0 + min(lane, len - 1);
+    gv = a.d.g[row * a.d.g_st.bs + tok * a.d.g_st.rs + hv * a.d.g_st.cs];
+    bv = a.d.beta[row * a.d.beta_st.bs + tok * a.d.beta_st.rs + hv * a.d.beta_st.cs];
+  };
+  if (wave == 0) load_g(hk * a.group);
   {
     Rows<T, DK> k, q;
     k.fetch(a.d.k, a.d.k_st, row, t0, len, hk, a.d.dk, t);
@@ -394,11 +407,8 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
     const int hv = hk * a.group + m;
     const long at = (long)slot * a.d.value_heads + hv;
     if (wave == 0) {
-      float g = 0.f, b = 0.f;
-      if (lane < len) {
-        g = a.d.g[row * a.d.g_st.bs + (t0 + lane) * a.d.g_st.rs + hv * a.d.g_st.cs];
-        b = a.d.beta[row * a.d.beta_st.bs + (t0 + lane) * a.d.beta_st.rs + hv * a.d.beta_st.cs];
-      }
+      const float g = lane < len ? gv : 0.f, b = lane < len ? bv : 0.f;
+      load_g(min(hv + 1, a.d.value_heads - 1));
       double x = g < G_MIN ? G_MIN : g;
       for (int o = 1; o < 64; o <<= 1) {
         const double y = __shfl_up(x, o);
@@ -462,9 +472,10 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const Args a) {
 // partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.  Four waves do that
 // and nothing else; four more take S and E from LDS and do what the chain does not wait for -- forward the outputs
 // O = scale (exp(G) Q S + P beta E), backward Q^T Of, and all stores.  (A wave waits for its memory accesses in order: with
-// the stores in the chain's waves its loads waited for them, 256 us for 8192 tokens x 16 heads against 186 without stores and 137 without
-// any access.)  Fragments come straight from memory, SETS chunks ahead; every load is issued whatever comes, since loads behind
-// branches make the compiler wait for all that are under way.
+// the stores in the chain's waves its loads waited for them.  8192 tokens x 16 heads, bf16, dk = dv = 128: 256 us and 68 for the
+// outputs, against 226 together; 137 for the chain without any access to memory.)  Fragments come straight from memory, up to
+// a chunk ahead (two gained nothing), issued under the latency of LDS reads or matrix instructions; every load is issued
+// whatever comes, since loads behind branches make the compiler wait for all that are under way.
 __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes) {
   return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
 }
@@ -472,11 +483,10 @@ __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes
 template <typename T, int DK, bool BACK>
 __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   constexpr int N = Planes<T>::N, NO = OutPlanes<T>::N, RT = DK / 64, PT = C + 8, PE = C + 4;
-  constexpr int SETS = N == 1 ? 2 : 1;           // as many as the registers hold
   __shared__ f4 part[4][4][64];                  // K S: wave, row block
-  __shared__ f4 Sx[4][2][64];                    // S: wave, tile
+  __shared__ f4 Sx[2][4][2][64];                 // S: parity of the chunk, wave, tile
   __shared__ f4 Rx[4][2][64];                    // BACK: Q^T Of, likewise
-  __shared__ __align__(16) float Ex[16][PE];     // E^T or Z^T
+  __shared__ __align__(16) float Ex[2][16][PE];  // E^T or Z^T, parity of the chunk
   __shared__ __align__(16) __bf16 X[3][16][PT], U[3][16][PT];
   const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / 16;
   int slice, head;
@@ -490,6 +500,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   const unsigned lb = lane * 16;
 
   if (wave8 < 4) {   // ---- the chain
+    __builtin_amdgcn_s_setprio(3);
     f4 S[RT];
     const float* init = BACK ? a.d_state_out : a.state;
 #pragma unroll
@@ -499,52 +510,53 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + col;
         S[i][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
       }
-    b8 kf[SETS][4][N], tf[SETS][2][3], kt[SETS][RT][2][N];
-    T v[SETS][4];
-    f4 y[SETS], fx[SETS], fu[SETS];
-    float keep[SETS];
+    b8 kf[4][N], tf[2][3], kt[RT][2][N];
+    T v[4];
+    f4 y, fx, fu;
+    float keep;
     const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + begin * a.d.v_st.rs + hv * a.d.v_st.cs;
     const unsigned vrs = (unsigned)a.d.v_st.rs, vcol = min(c0 + col, a.d.dv - 1);
-    auto load_k = [&](int u, long slot) {
+    auto load_k = [&](long slot) {
       const __bf16* p = a.Kf + (slot * a.d.key_heads + hk) * N * KF + wave * 512;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < N; ++k) kf[u][i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
+        for (int k = 0; k < N; ++k) kf[i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
     };
-    auto load_x = [&](int u, long at, int m) {
+    auto load_x = [&](long at, int m) {
       if (BACK) {
-        y[u] = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + (unsigned)(col * C + wave * 16 + r4));
+        y = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + (unsigned)(col * C + wave * 16 + r4));
       } else {   // rows and columns behind the end repeat the last; they are masked where they are used
         const T* p = V + (long)m * C * a.d.v_st.rs;
         const unsigned last = min(C, end - begin - m * C) - 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][e] = p[min((unsigned)(wave * 16 + r4 + e), last) * vrs + vcol];
+        for (int e = 0; e < 4; ++e) v[e] = p[min((unsigned)(wave * 16 + r4 + e), last) * vrs + vcol];
       }
-      fx[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 4 * C : 0) + wave * 16 + r4);
+      fx = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 4 * C : 0) + wave * 16 + r4);
     };
-    auto load_t = [&](int u, long at) {
+    auto load_t = [&](long at) {
       const __bf16* p = (BACK ? a.T2f : a.Tf) + at * 3 * TF + wave * 2 * 512;
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        tf[u][0][k] = ld_frag(p + k * TF, lb);
-        tf[u][1][k] = ld_frag(p + k * TF + 512, lb);
+        tf[0][k] = ld_frag(p + k * TF, lb);
+        tf[1][k] = ld_frag(p + k * TF + 512, lb);
       }
-      fu[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 5 : 2) * C + wave * 16 + r4);
+      fu = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 5 : 2) * C + wave * 16 + r4);
     };
-    auto load_kt = [&](int u, long slot, long at) {
+    auto load_kt = [&](long slot, long at) {
       const __bf16* p = a.KTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int k = 0; k < N; ++k) kt[u][i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
-      keep[u] = a.fac[at * FACS + 3 * C + lane];   // by lane: a scalar load would be waited for with LDS
+          for (int k = 0; k < N; ++k) kt[i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
+      keep = a.fac[at * FACS + 3 * C + lane];   // by lane: a scalar load would be waited for with LDS
     };
-    auto chunk = [&](int u, int n) {
-      const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - SETS, 0) : min(m + SETS, chunks - 1);
+    auto chunk = [&](int n) {
+      const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - 1, 0) : min(m + 1, chunks - 1);
       const long nslot = slot0 + nm, nat = nslot * a.d.value_heads + hv;
+      const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
       const int live = BACK ? 0 : end - begin - n * C - wave * 16 - r4;   // rows e < live hold tokens
       {
         float x[8];
@@ -553,8 +565,8 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
           x[e] = S[0][e];
           x[4 + e] = RT == 2 ? S[RT - 1][e] : 0.f;
         }
-        Sx[wave][0][lane] = S[0];
-        if (RT == 2) Sx[wave][1][lane] = S[RT - 1];
+        Sx[n & 1][wave][0][lane] = S[0];
+        if (RT == 2) Sx[n & 1][wave][1][lane] = S[RT - 1];
         b8 sb[3];
         split<8, 3>(x, sb);
         f4 p[4];
@@ -567,91 +579,86 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
           for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (q >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[u][i][k], sb[q - k], p[i], 0, 0, 0);
+              if (q >= k) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], sb[q - k], p[i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_kt(slot, at);   // this chunk's: used behind its third barrier
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[wave][i][lane] = p[i];
       }
-      load_k(u, nslot);
       lds_barrier();
       {
-        const f4 p = (part[0][wave][lane] + part[1][wave][lane]) + (part[2][wave][lane] + part[3][wave][lane]);
+        const f4 p0 = part[0][wave][lane], p1 = part[1][wave][lane], p2 = part[2][wave][lane], p3 = part[3][wave][lane];
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(nslot);
+        __builtin_amdgcn_sched_barrier(0);
+        const f4 p = (p0 + p1) + (p2 + p3);
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          x[e] = BACK ? fmaf(fx[u][e], p[e], y[u][e]) : e < live && c0 + col < a.d.dv ? fmaf(-fx[u][e], p[e], (float)v[u][e]) : 0.f;
+          x[e] = BACK ? fmaf(fx[e], p[e], y[e]) : e < live && c0 + col < a.d.dv ? fmaf(-fx[e], p[e], (float)v[e]) : 0.f;
         b4 xp[3];
         split<4, 3>(x, xp);
 #pragma unroll
         for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&X[k][col][wave * 16 + r4]) = xp[k];
       }
-      load_x(u, nat, nm);
       lds_barrier();
       {
         // T's upper, T2^T's lower half is zeros
         f4 e0 = {0, 0, 0, 0}, e1 = {0, 0, 0, 0};
-        b8 xb[3];
-        if (!BACK || wave < 2) {
+        b8 xb[2][3];
 #pragma unroll
-          for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][col][g8]);
-          e0 = planes_mma<3, 3, 3>(tf[u][0], xb, e0);
-        }
-        if (BACK || wave >= 2) {
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int k = 0; k < 3; ++k) xb[k] = *reinterpret_cast<const b8*>(&X[k][col][32 + g8]);
-          e1 = planes_mma<3, 3, 3>(tf[u][1], xb, e1);
-        }
+          for (int k = 0; k < 3; ++k) xb[ks][k] = *reinterpret_cast<const b8*>(&X[k][col][ks * 32 + g8]);
+        __builtin_amdgcn_sched_barrier(0);
+        load_x(nat, nm);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!BACK || wave < 2) e0 = planes_mma<3, 3, 3>(tf[0], xb[0], e0);
+        if (BACK || wave >= 2) e1 = planes_mma<3, 3, 3>(tf[1], xb[1], e1);
         const f4 ev = e0 + e1;
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fu[u][e] : fu[u][e]) * ev[e];
+        for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fu[e] : fu[e]) * ev[e];
         b4 up[3];
         split<4, 3>(w, up);
 #pragma unroll
         for (int k = 0; k < 3; ++k) *reinterpret_cast<b4*>(&U[k][col][wave * 16 + r4]) = up[k];
-        *reinterpret_cast<f4*>(&Ex[col][wave * 16 + r4]) = ev;
+        *reinterpret_cast<f4*>(&Ex[n & 1][col][wave * 16 + r4]) = ev;
       }
-      load_t(u, nat);
       lds_barrier();
       {
         f4 more[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-          S[i] *= keep[u];
+          S[i] *= keep;
           more[i] = BACK ? Rx[wave][i][lane] : f4{0, 0, 0, 0};
         }
+        b8 ub[2][3];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          b8 ub[3];
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int k = 0; k < 3; ++k) ub[k] = *reinterpret_cast<const b8*>(&U[k][col][ks * 32 + g8]);
+          for (int k = 0; k < 3; ++k) ub[ks][k] = *reinterpret_cast<const b8*>(&U[k][col][ks * 32 + g8]);
+        __builtin_amdgcn_sched_barrier(0);
+        load_t(nat);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            if (ks == 0)
-              S[i] = planes_mma<N, 3, 3>(kt[u][i][ks], ub, S[i]);
-            else
-              more[i] = planes_mma<N, 3, 3>(kt[u][i][ks], ub, more[i]);
-          }
+        for (int i = 0; i < RT; ++i) {
+          S[i] = planes_mma<N, 3, 3>(kt[i][0], ub[0], S[i]);
+          more[i] = planes_mma<N, 3, 3>(kt[i][1], ub[1], more[i]);
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) S[i] += more[i];
       }
-      load_kt(u, nslot, nat);
     };
     if (chunks > 0) {
-#pragma unroll
-      for (int u = 0; u < SETS; ++u) {
-        const int m = BACK ? max(chunks - 1 - u, 0) : min(u, chunks - 1);
-        const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
-        load_k(u, slot);
-        load_x(u, at, m);
-        load_t(u, at);
-        load_kt(u, slot, at);
-      }
+      const int m = BACK ? chunks - 1 : 0;
+      const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
+      load_k(slot);
+      load_x(at, m);
+      load_t(at);
     }
-    for (int n = 0; n < chunks; n += SETS) {
-      chunk(0, n);
-      if (SETS == 2 && n + 1 < chunks) chunk(SETS - 1, n + 1);
-    }
+    for (int n = 0; n < chunks; ++n) chunk(n);
     float* out = BACK ? a.d_state : a.state_out;
     if (out != nullptr) {
 #pragma unroll
@@ -662,10 +669,13 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
           if (r < a.d.dk && c < a.d.dv) out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][e];
         }
     }
-  } else {   // ---- beside the chain; the same three barriers per chunk
+  } else {
+    // ---- beside the chain, one chunk behind it: the work on chunk n - 1 is spread over the three stretches of chunk n, the longest
+    // first, so that no barrier waits for it.  Backward, Rx is that of chunk n itself.
     b8 qf[4][N], pf[2][NO], qt[RT][2][N], of[2][3];
-    f4 eg, bt[4];
-    auto load = [&](long slot, long at) {
+    f4 eg, bt[4], o, mine[2];
+    auto load_q = [&](int m) {
+      const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
       if (BACK) {
         const __bf16* p = a.QTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
 #pragma unroll
@@ -683,74 +693,66 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int k = 0; k < N; ++k) qf[i][k] = ld_frag(q + k * KF + i * 512, lb);
-        const __bf16* p = a.Pf + at * NO * TF + wave * 2 * 512;
-#pragma unroll
-        for (int k = 0; k < NO; ++k) {
-          pf[0][k] = ld_frag(p + k * TF, lb);
-          pf[1][k] = ld_frag(p + k * TF + 512, lb);
-        }
-        const float* f = a.fac + at * FACS;
-        eg = *reinterpret_cast<const f4*>(f + wave * 16 + r4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bt[i] = *reinterpret_cast<const f4*>(f + C + (i >> 1) * 32 + g8 + (i & 1) * 4);
+        eg = *reinterpret_cast<const f4*>(a.fac + at * FACS + wave * 16 + r4);
       }
     };
-    if (chunks > 0) {
-      const long slot = slot0 + (BACK ? chunks - 1 : 0);
-      load(slot, slot * a.d.value_heads + hv);
-    }
-    for (int n = 0; n < chunks; ++n) {
-      const int m = BACK ? chunks - 1 - n : n, nm = BACK ? max(m - 1, 0) : min(m + 1, chunks - 1);
+    auto load_p = [&](int m) {
       const long at = (slot0 + m) * a.d.value_heads + hv;
-      f4 o = {0, 0, 0, 0}, mine[2];
-      if (BACK) {
-        f4 r[RT];
+      const __bf16* p = a.Pf + at * NO * TF + wave * 2 * 512;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) r[i] = f4{0, 0, 0, 0};
+      for (int k = 0; k < NO; ++k) {
+        pf[0][k] = ld_frag(p + k * TF, lb);
+        pf[1][k] = ld_frag(p + k * TF + 512, lb);
+      }
+      const float* f = a.fac + at * FACS + C + g8;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+      for (int i = 0; i < 4; ++i) bt[i] = *reinterpret_cast<const f4*>(f + (i >> 1) * 32 + (i & 1) * 4);
+    };
+    auto order = [&](int n) { return BACK ? chunks - 1 - n : n; };
+    // Q S, the terms of chain wave w
+    auto q_part = [&](int n, int w) {
+      const f4 s0 = Sx[n & 1][w][0][lane], s1 = RT == 2 ? Sx[n & 1][w][1][lane] : f4{0, 0, 0, 0};
+      float x[8];
 #pragma unroll
-          for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[i][ks], of[ks], r[i]);
-        lds_barrier();   // the chain has read the Rx of the chunk before
-#pragma unroll
-        for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) mine[i] = Sx[wave][i][lane];
-      } else {
-        lds_barrier();
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const f4 s0 = Sx[w][0][lane], s1 = RT == 2 ? Sx[w][1][lane] : f4{0, 0, 0, 0};
-          if (w == wave) {
-            mine[0] = s0;
-            mine[1] = s1;
-          }
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = s0[e];
-            x[4 + e] = s1[e];
-          }
-          b8 sb[NO];
-          split<8, NO>(x, sb);
-          o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[w], sb, o);
-        }
-        o *= eg;
+      for (int e = 0; e < 4; ++e) {
+        x[e] = s0[e];
+        x[4 + e] = s1[e];
+      }
+      b8 sb[NO];
+      split<8, NO>(x, sb);
+      o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[w], sb, o);
+    };
+    auto first = [&](int n) {
+      if (!BACK) {
+        o = f4{0, 0, 0, 0};
+        q_part(n, 0);
+        q_part(n, 1);
+        q_part(n, 2);
       }
       if (BACK || a.save) {
-        float* dst = (BACK ? a.dS : a.Srow) + (at * DK + wave * RT * 16) * a.dvp + c0;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) mine[i] = Sx[n & 1][wave][i][lane];
+        float* dst = (BACK ? a.dS : a.Srow) + (((slot0 + order(n)) * a.d.value_heads + hv) * DK + wave * RT * 16) * a.dvp + c0;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) dst[(unsigned)((i * 16 + r4 + e) * a.dvp + col)] = mine[i][e];
       }
-      lds_barrier();
-      lds_barrier();
+    };
+    auto second = [&](int n, int next) {
+      if (!BACK) {
+        q_part(n, 3);
+        o *= eg;
+        load_q(next);
+      }
+    };
+    auto third = [&](int n, int next) {
       if (!BACK) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
           if (ks * 2 > wave) continue;   // P is lower triangular
-          const f4 e0 = *reinterpret_cast<const f4*>(&Ex[col][ks * 32 + g8]), e1 = *reinterpret_cast<const f4*>(&Ex[col][ks * 32 + g8 + 4]);
+          const f4 e0 = *reinterpret_cast<const f4*>(&Ex[n & 1][col][ks * 32 + g8]),
+                   e1 = *reinterpret_cast<const f4*>(&Ex[n & 1][col][ks * 32 + g8 + 4]);
           float x[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -761,6 +763,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
           split<8, NO>(x, ub);
           o = planes_mma<NO, NO, NO>(pf[ks], ub, o);
         }
+        load_p(next);
         const int t0 = begin + n * C + wave * 16 + r4;
         T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + t0) * a.d.value_heads + hv) * (long)a.d.dv + c0 + col;
         if (c0 + col < a.d.dv)
@@ -769,12 +772,42 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
             if (t0 + e < end) out[(long)e * a.d.value_heads * a.d.dv] = (T)(a.scale * o[e]);
       }
       if (BACK || a.save) {
-        const f4 ev = *reinterpret_cast<const f4*>(&Ex[col][wave * 16 + r4]);
-        float* dst = (BACK ? a.Z : a.Erow) + (at * C + wave * 16) * a.dvp + c0;
+        const f4 ev = *reinterpret_cast<const f4*>(&Ex[n & 1][col][wave * 16 + r4]);
+        float* dst = (BACK ? a.Z : a.Erow) + (((slot0 + order(n)) * a.d.value_heads + hv) * C + wave * 16) * a.dvp + c0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) dst[(unsigned)((r4 + e) * a.dvp + col)] = ev[e];
       }
-      load(slot0 + nm, (slot0 + nm) * a.d.value_heads + hv);
+    };
+    if (chunks > 0) {
+      load_q(order(0));
+      if (!BACK) load_p(0);
+    }
+    for (int n = 0; n < chunks; ++n) {
+      if (n > 0) first(n - 1);
+      f4 r[RT];
+      if (BACK) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) r[i] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[i][ks], of[ks], r[i]);
+      }
+      lds_barrier();
+      if (BACK) {   // the chain has read the Rx of the chunk before
+#pragma unroll
+        for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];
+        load_q(order(min(n + 1, chunks - 1)));
+      }
+      if (n > 0) second(n - 1, n);
+      lds_barrier();
+      if (n > 0) third(n - 1, n);
+      lds_barrier();
+    }
+    if (chunks > 0) {
+      first(chunks - 1);
+      second(chunks - 1, chunks - 1);
+      third(chunks - 1, chunks - 1);
     }
   }
 }
@@ -849,7 +882,11 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   float* dG = reinterpret_cast<float*>(G + C);   // 8 x C: per wave
   float* red = dG + 8 * C;      // 8
   float* db = red + 8;          // C
-  f4* sums = reinterpret_cast<f4*>(db + C);   // GROUPED: dQ and dK over the value heads so far, 8 per thread
+  constexpr bool TILES = !(GROUPED && sizeof(T) == 4);   // K and Q in LDS, where they fit
+  constexpr int PK = DK + 16 / sizeof(T);
+  T* Kt = reinterpret_cast<T*>(db + C);
+  T* Qt = Kt + (TILES ? C * PK : 0);
+  f4* sums = reinterpret_cast<f4*>(Qt + (TILES ? C * PK : 0));   // GROUPED: dQ and dK over the value heads so far, 8 per thread
   const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
@@ -862,6 +899,25 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   // a thread's place in a slice: four columns of one row
   const int sr = t >> 3, sc = (t & 7) * 4;
   const int group = GROUPED ? a.group : 1;
+  if (TILES) {
+    const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs;
+    const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs;
+    constexpr int IT = C * DK / 512;
+    T k[IT], q[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = min((i * 512 + t) / DK, len - 1), c = min((i * 512 + t) % DK, a.d.dk - 1);
+      k[i] = Kg[r * a.d.k_st.rs + c];
+      q[i] = Qg[r * a.d.q_st.rs + c];
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = (i * 512 + t) / DK, c = (i * 512 + t) % DK;
+      const bool live = r < len && c < a.d.dk;
+      Kt[r * PK + c] = live ? k[i] : T(0);
+      Qt[r * PK + c] = live ? q[i] : T(0);
+    }
+  }
 #pragma unroll 1
   for (int m = 0; m < group; ++m) {
     asm volatile("" ::: "memory");   // keeps the loads of K and Q inside: hoisted, they would not fit the registers
@@ -970,9 +1026,20 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs + min(kc0, a.d.dk - 1);
     const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs + min(kc0, a.d.dk - 1);
     float csum = 0.f;
-    auto element = [&](const T* p, const gpx_strided& st_, int r) {
+    auto element = [&](const T* tile, const T* p, const gpx_strided& st_, int r) {
+      if (TILES) return (float)tile[r * PK + kc0];
       return r < len && kc0 < a.d.dk ? (float)p[min(r, len - 1) * st_.rs] : 0.f;
     };
+    // K^T and Q^T, from here on under way
+    b8 kt[2][N], qt[2][N];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const long o = (atk * N + k) * (DK * C) + (min(wave, W - 1) * 2 + ks) * 512;
+        kt[ks][k] = ld_frag(a.KTf + o, lane * 16);
+        qt[ks][k] = ld_frag(a.QTf + o, lane * 16);
+      }
     if (own) {
 #pragma unroll
       for (int rb = 0; rb < 4; ++rb)
@@ -983,7 +1050,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
           q1[rb][e] *= a.scale * eg;
           kr[rb][e] *= -eg;
           kc[rb][e] *= expf((float)(last - G[r]));
-          csum = fmaf(element(Kg, a.d.k_st, r), kc[rb][e], csum);
+          csum = fmaf(element(Kt, Kg, a.d.k_st, r), kc[rb][e], csum);
         }
     }
     for (int o = 1; o < 64; o <<= 1) {
@@ -1031,14 +1098,6 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
       }
       __syncthreads();
       if (own) {
-        b8 kt[2][N], qt[2][N];
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int k = 0; k < N; ++k) {
-            kt[ks][k] = ld_frag(a.KTf + (atk * N + k) * (DK * C) + (wave * 2 + ks) * 512, lane * 16);
-            if (w == 0) qt[ks][k] = ld_frag(a.QTf + (atk * N + k) * (DK * C) + (wave * 2 + ks) * 512, lane * 16);
-          }
 #pragma unroll
         for (int rb = 0; rb < 4; ++rb)
 #pragma unroll
@@ -1065,7 +1124,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = rb * 16 + r4 + e;
-        g[e] = own ? fmaf(element(Qg, a.d.q_st, r), q1[rb][e], element(Kg, a.d.k_st, r) * (kr[rb][e] - kc[rb][e])) : 0.f;
+        g[e] = own ? fmaf(element(Qt, Qg, a.d.q_st, r), q1[rb][e], element(Kt, Kg, a.d.k_st, r) * (kr[rb][e] - kc[rb][e])) : 0.f;
         for (int o = 1; o < 16; o <<= 1) g[e] += __shfl_xor(g[e], o);
       }
       if (col == 0)
@@ -1378,7 +1437,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
     GPX_HIP(hipGetLastError());
     return 0;
   }
-  constexpr size_t lds = 2 * Planes<T>::N * C * (DK + 8) * 2 + (2 * C * PC + 4 * 16 * 20) * 4 + C * 8 + C * 4;
+  constexpr size_t lds = chunk_room<T, DK>() + C * 8 + C * 4;
   static_assert(lds <= 160 * 1024, "LDS");
   DELTA_TRY(allow_lds(&delta_chunk_kernel<T, DK>, lds));
   const long slots = slots_of(&a.d);
@@ -1394,8 +1453,9 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
 template <typename T, int DK>
 int run_backward(hipStream_t s, const Args& a) {
   constexpr size_t room = (Planes<T>::N + 6) * C * 40 > 6 * C * (C + 8) ? (Planes<T>::N + 6) * C * 40 : 6 * C * (C + 8);
-  constexpr size_t lds = room * 2 + C * 8 + (8 * C + 8 + C) * 4, grouped = lds + 8 * 512 * 16;
-  static_assert(grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
+  constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = room * 2 + C * 8 + (8 * C + 8 + C) * 4;
+  constexpr size_t lds = base + tiles, grouped = base + (sizeof(T) == 4 ? 0 : tiles) + 8 * 512 * 16;
+  static_assert(lds <= 160 * 1024 && grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
   DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK, false>, lds));
   DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK, true>, grouped));
   const long slots = slots_of(&a.d);
