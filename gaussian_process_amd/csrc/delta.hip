@@ -95,7 +95,7 @@ struct Args {
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
   float *Erow, *Srow;           // per head: E, C x dvp; S, DK x dvp
   float* Y;                     // per head: (scale P^T dO)^T, dvp x C
-  __bf16* Of;                   // per head: scale exp(G) dO as fragments, dvp / 16 x 2 x 64 x 8 by three planes
+  __bf16* Of;                   // per head: dO as fragments, dvp / 16 x 2 x 64 x 8
   float *Z, *dS;                // per head: Z (dX = beta Z), C x dvp; dS', DK x dvp
   const float *state, *d_state_out;
   float *state_out, *d_state, *d_g, *d_beta;
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kerne
 // ---- the scans: 16 columns of dv of one value head of one sequence ----------------------------------------------------------------
 // Forward, chunk after chunk:    X = V - exp(G) K S;       E = T X;      S <- exp(G_C) S + K^T (exp(G_C - G) beta E)
 // Backward (BACK), from the last: X = Y + exp(G_C - G) K dS;  Z = T2^T X;   dS <- exp(G_C) dS - K^T (exp(G) beta Z) + Q^T Of
-// (Y = scale P^T dO, Of = scale exp(G) dO, from delta_back_prep_kernel).
+// (Y = scale P^T dO from delta_back_prep_kernel, Of = scale exp(G) dO).
 // Bound by the chain from chunk to chunk: the product with K (each wave with its own rows of S, which are in its accumulators;
 // partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.  Four waves do that
 // and nothing else; four more take S and E from LDS and do what the chain does not wait for -- forward the outputs
@@ -488,6 +488,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   __shared__ f4 Rx[4][2][64];                    // BACK: Q^T Of, likewise
   __shared__ __align__(16) float Ex[2][16][PE];  // E^T or Z^T, parity of the chunk
   __shared__ __align__(16) __bf16 X[3][16][PT], U[3][16][PT];
+  __shared__ __align__(16) float Ox[4][16][20];  // a wave's outputs, transposed
   const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / 16;
   int slice, head;
   if (!scan_coords(blockIdx.x, slices, heads, slice, head)) return;
@@ -672,10 +673,15 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   } else {
     // ---- beside the chain, one chunk behind it: the work on chunk n - 1 is spread over the three stretches of chunk n, the longest
     // first, so that no barrier waits for it.  Backward, Rx is that of chunk n itself.
-    b8 qf[4][N], pf[2][NO], qt[RT][2][N], of[2][3];
-    f4 eg, bt[4], o, mine[2];
-    auto load_q = [&](int m) {
-      const long slot = slot0 + m, at = slot * a.d.value_heads + hv;
+    // Two sets of fragments, two chunks ahead: what a wave loads waits for what it stored before.
+    b8 qf[2][4][N], pf[2][2][NO], qt[2][RT][2][N], of[2][2][N];
+    f4 eg[2], bt[2][4], o;   // BACK: bt holds exp(G)
+    // Stores go through LDS, 4 columns of one row per lane: whole 64-byte pieces
+    const int srow = lane >> 2, sc = (lane & 3) * 4;
+    const bool wide = (a.d.dv & 3) == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
+    auto order = [&](int n) { return BACK ? chunks - 1 - n : n; };
+    auto load_q = [&](int u, int n) {
+      const long slot = slot0 + order(min(n, chunks - 1)), at = slot * a.d.value_heads + hv;
       if (BACK) {
         const __bf16* p = a.QTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
 #pragma unroll
@@ -683,34 +689,36 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
 #pragma unroll
           for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int k = 0; k < N; ++k) qt[i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
+            for (int k = 0; k < N; ++k) qt[u][i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
 #pragma unroll
-          for (int k = 0; k < 3; ++k) of[ks][k] = ld_frag(a.Of + (at * 3 + k) * (a.dvp * C) + slice * 1024 + ks * 512, lb);
+          for (int k = 0; k < N; ++k) of[u][ks][k] = ld_frag(a.Of + (at * N + k) * (a.dvp * C) + slice * 1024 + ks * 512, lb);
         }
+        const float* f = a.fac + at * FACS + g8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bt[u][i] = *reinterpret_cast<const f4*>(f + (i >> 1) * 32 + (i & 1) * 4);
       } else {
         const __bf16* q = a.Qf + (slot * a.d.key_heads + hk) * N * KF + wave * 4 * 512;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int k = 0; k < N; ++k) qf[i][k] = ld_frag(q + k * KF + i * 512, lb);
-        eg = *reinterpret_cast<const f4*>(a.fac + at * FACS + wave * 16 + r4);
+          for (int k = 0; k < N; ++k) qf[u][i][k] = ld_frag(q + k * KF + i * 512, lb);
+        eg[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + wave * 16 + r4);
       }
     };
-    auto load_p = [&](int m) {
-      const long at = (slot0 + m) * a.d.value_heads + hv;
+    auto load_p = [&](int u, int n) {
+      const long at = (slot0 + min(n, chunks - 1)) * a.d.value_heads + hv;
       const __bf16* p = a.Pf + at * NO * TF + wave * 2 * 512;
 #pragma unroll
       for (int k = 0; k < NO; ++k) {
-        pf[0][k] = ld_frag(p + k * TF, lb);
-        pf[1][k] = ld_frag(p + k * TF + 512, lb);
+        pf[u][0][k] = ld_frag(p + k * TF, lb);
+        pf[u][1][k] = ld_frag(p + k * TF + 512, lb);
       }
       const float* f = a.fac + at * FACS + C + g8;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bt[i] = *reinterpret_cast<const f4*>(f + (i >> 1) * 32 + (i & 1) * 4);
+      for (int i = 0; i < 4; ++i) bt[u][i] = *reinterpret_cast<const f4*>(f + (i >> 1) * 32 + (i & 1) * 4);
     };
-    auto order = [&](int n) { return BACK ? chunks - 1 - n : n; };
     // Q S, the terms of chain wave w
-    auto q_part = [&](int n, int w) {
+    auto q_part = [&](int u, int n, int w) {
       const f4 s0 = Sx[n & 1][w][0][lane], s1 = RT == 2 ? Sx[n & 1][w][1][lane] : f4{0, 0, 0, 0};
       float x[8];
 #pragma unroll
@@ -720,94 +728,135 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
       }
       b8 sb[NO];
       split<8, NO>(x, sb);
-      o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[w], sb, o);
+      o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[u][w], sb, o);
     };
-    auto first = [&](int n) {
+    // what is left of chunk n: O from Ox, E or Z
+    auto flush = [&](int n) {
+      if (!BACK) {
+        const int tok = begin + n * C + wave * 16 + srow;
+        T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + tok) * a.d.value_heads + hv) * (long)a.d.dv + c0 + sc;
+        struct __align__(sizeof(T) * 4) Four { T x[4]; } w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.x[e] = (T)Ox[wave][sc + e][srow];
+        __builtin_amdgcn_wave_barrier();
+        if (tok < end) {
+          if (wide) {
+            if (c0 + sc < a.d.dv) *reinterpret_cast<Four*>(out) = w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c0 + sc + e < a.d.dv) out[e] = w.x[e];
+          }
+        }
+      }
+      if (BACK || a.save) {
+        float* dst = (BACK ? a.Z : a.Erow) + (((slot0 + order(n)) * a.d.value_heads + hv) * C + wave * 16) * a.dvp + c0;
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
+        *reinterpret_cast<f4*>(dst + (unsigned)(srow * a.dvp + sc)) = v;
+      }
+    };
+    auto first = [&](int u, int n) {
+      if (n > 0) flush(n - 1);
       if (!BACK) {
         o = f4{0, 0, 0, 0};
-        q_part(n, 0);
-        q_part(n, 1);
-        q_part(n, 2);
+        q_part(u, n, 0);
+        q_part(u, n, 1);
+        q_part(u, n, 2);
       }
       if (BACK || a.save) {
-#pragma unroll
-        for (int i = 0; i < RT; ++i) mine[i] = Sx[n & 1][wave][i][lane];
         float* dst = (BACK ? a.dS : a.Srow) + (((slot0 + order(n)) * a.d.value_heads + hv) * DK + wave * RT * 16) * a.dvp + c0;
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dst[(unsigned)((i * 16 + r4 + e) * a.dvp + col)] = mine[i][e];
-      }
-    };
-    auto second = [&](int n, int next) {
-      if (!BACK) {
-        q_part(n, 3);
-        o *= eg;
-        load_q(next);
-      }
-    };
-    auto third = [&](int n, int next) {
-      if (!BACK) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          if (ks * 2 > wave) continue;   // P is lower triangular
-          const f4 e0 = *reinterpret_cast<const f4*>(&Ex[n & 1][col][ks * 32 + g8]),
-                   e1 = *reinterpret_cast<const f4*>(&Ex[n & 1][col][ks * 32 + g8 + 4]);
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = e0[e] * bt[ks * 2][e];
-            x[4 + e] = e1[e] * bt[ks * 2 + 1][e];
-          }
-          b8 ub[NO];
-          split<8, NO>(x, ub);
-          o = planes_mma<NO, NO, NO>(pf[ks], ub, o);
+        for (int i = 0; i < RT; ++i) {
+          const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
+          *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * a.dvp + sc)) = f4{p[0], p[4], p[8], p[12]};
         }
-        load_p(next);
-        const int t0 = begin + n * C + wave * 16 + r4;
-        T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + t0) * a.d.value_heads + hv) * (long)a.d.dv + c0 + col;
-        if (c0 + col < a.d.dv)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (t0 + e < end) out[(long)e * a.d.value_heads * a.d.dv] = (T)(a.scale * o[e]);
-      }
-      if (BACK || a.save) {
-        const f4 ev = *reinterpret_cast<const f4*>(&Ex[n & 1][col][wave * 16 + r4]);
-        float* dst = (BACK ? a.Z : a.Erow) + (((slot0 + order(n)) * a.d.value_heads + hv) * C + wave * 16) * a.dvp + c0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dst[(unsigned)((r4 + e) * a.dvp + col)] = ev[e];
       }
     };
-    if (chunks > 0) {
-      load_q(order(0));
-      if (!BACK) load_p(0);
-    }
-    for (int n = 0; n < chunks; ++n) {
-      if (n > 0) first(n - 1);
+    auto second = [&](int u, int n) {
+      if (!BACK) {
+        q_part(u, n, 3);
+        o *= eg[u];
+        load_q(u, n + 2);
+      }
+    };
+    auto third = [&](int u, int n) {
+      if (BACK) return;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks * 2 > wave) continue;   // P is lower triangular
+        const f4 e0 = *reinterpret_cast<const f4*>(&Ex[n & 1][col][ks * 32 + g8]),
+                 e1 = *reinterpret_cast<const f4*>(&Ex[n & 1][col][ks * 32 + g8 + 4]);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = e0[e] * bt[u][ks * 2][e];
+          x[4 + e] = e1[e] * bt[u][ks * 2 + 1][e];
+        }
+        b8 ub[NO];
+        split<8, NO>(x, ub);
+        o = planes_mma<NO, NO, NO>(pf[u][ks], ub, o);
+      }
+      load_p(u, n + 2);
+      *reinterpret_cast<f4*>(&Ox[wave][col][r4]) = o * a.scale;
+      __builtin_amdgcn_wave_barrier();
+    };
+    // u: the set of chunk n
+    auto chunk = [&](int u, int n) {
+      if (n > 0) first(1 - u, n - 1);
       f4 r[RT];
       if (BACK) {
 #pragma unroll
         for (int i = 0; i < RT; ++i) r[i] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks) {
+          float x[8];
 #pragma unroll
-          for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[i][ks], of[ks], r[i]);
+          for (int e = 0; e < 8; ++e) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < N; ++k) v += (float)of[u][ks][k][e];
+            x[e] = a.scale * bt[u][ks * 2 + (e >> 2)][e & 3] * v;
+          }
+          b8 ob[3];
+          split<8, 3>(x, ob);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[u][i][ks], ob, r[i]);
+        }
       }
       lds_barrier();
       if (BACK) {   // the chain has read the Rx of the chunk before
 #pragma unroll
         for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];
-        load_q(order(min(n + 1, chunks - 1)));
+        load_q(u, n + 2);
       }
-      if (n > 0) second(n - 1, n);
+      if (n > 0) second(1 - u, n - 1);
       lds_barrier();
-      if (n > 0) third(n - 1, n);
+      if (n > 0) third(1 - u, n - 1);
       lds_barrier();
-    }
+    };
     if (chunks > 0) {
-      first(chunks - 1);
-      second(chunks - 1, chunks - 1);
-      third(chunks - 1, chunks - 1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        load_q(u, u);
+        if (!BACK) load_p(u, u);
+      }
+      for (int n = 0; n < chunks; n += 2) {
+        chunk(0, n);
+        if (n + 1 < chunks) chunk(1, n + 1);
+      }
+      const int n = chunks - 1;
+      if (n & 1) {
+        first(1, n);
+        second(1, n);
+        third(1, n);
+      } else {
+        first(0, n);
+        second(0, n);
+        third(0, n);
+      }
+      flush(n);
     }
   }
 }
@@ -828,7 +877,6 @@ __global__ __launch_bounds__(256) void delta_back_prep_kernel(const Args a) {
   if (ct * 16 >= a.dvp) return;
   const int c = ct * 16 + col;
   const T* dO = reinterpret_cast<const T*>(a.d_o) + a.p.row(s) * a.do_st.bs + t0 * a.do_st.rs + hv * a.do_st.cs + min(c, a.d.dv - 1);
-  const float* fac = a.fac + at * FACS;
   b8 ob[2][N];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
@@ -840,12 +888,8 @@ __global__ __launch_bounds__(256) void delta_back_prep_kernel(const Args a) {
     for (int e = 0; e < 8; ++e) x[e] = ks * 32 + g8 + e < len && c < a.d.dv ? (float)raw[e] : 0.f;
     split<8, N>(x, ob[ks]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= a.scale * fac[ks * 32 + g8 + e];
-    b8 scaled[3];
-    split<8, 3>(x, scaled);
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-      *reinterpret_cast<b8*>(a.Of + (at * 3 + k) * (a.dvp * C) + ct * 1024 + ks * 512 + lane * 8) = scaled[k];
+    for (int k = 0; k < N; ++k)
+      *reinterpret_cast<b8*>(a.Of + (at * N + k) * (a.dvp * C) + ct * 1024 + ks * 512 + lane * 8) = ob[ks][k];
   }
   const __bf16* pt = a.PTf + at * 3 * TF + lane * 8;
 #pragma unroll
@@ -891,13 +935,9 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
   if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15,
-            g8 = (lane >> 4) * 8;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
   const bool own = wave < W;
-  const int kc0 = wave * 16 + col;   // this lane's column of dk
-  // a thread's place in a slice: four columns of one row
-  const int sr = t >> 3, sc = (t & 7) * 4;
   const int group = GROUPED ? a.group : 1;
   if (TILES) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs;
@@ -920,7 +960,12 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   }
 #pragma unroll 1
   for (int m = 0; m < group; ++m) {
-    asm volatile("" ::: "memory");   // keeps the loads of K and Q inside: hoisted, they would not fit the registers
+    // Opaque, so that neither loads nor addresses of one head's work are kept in registers for the next head
+    int tt = threadIdx.x;
+    asm volatile("" : "+v"(tt)::"memory");
+    const int t = tt, lane = t & 63, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
+    const int kc0 = wave * 16 + col;   // this lane's column of dk
+    const int sr = t >> 3, sc = (t & 7) * 4;   // a thread's place in a slice: four columns of one row
     const int hv = hk * group + m;
     const long at = (long)slot * a.d.value_heads + hv;
     __syncthreads();
@@ -1368,7 +1413,7 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
   }
   if (use == SCRATCH) {
     part(x.Y, heads * C * dvp * 4);
-    part(x.Of, heads * 3 * C * dvp * 2);
+    part(x.Of, heads * n * C * dvp * 2);
     part(x.Z, heads * C * dvp * 4);
     part(x.dS, heads * dkp * dvp * 4);
   }
