@@ -484,11 +484,12 @@ template <typename T, int DK, bool BACK>
 __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   constexpr int N = Planes<T>::N, NO = OutPlanes<T>::N, RT = DK / 64, PT = C + 8, PE = C + 4;
   __shared__ f4 part[4][4][64];                  // K S: wave, row block
-  __shared__ f4 Sx[2][4][2][64];                 // S: parity of the chunk, wave, tile
+  constexpr int NS = BACK ? 0 : NO;
+  __shared__ b8 Sp[2][4][NS + 1][64];            // planes of S for the outputs: parity of the chunk, wave
+  __shared__ f4 Sx[2][4][2][64];                 // S to be stored: parity, wave, tile
   __shared__ f4 Rx[4][2][64];                    // BACK: Q^T Of, likewise
   __shared__ __align__(16) float Ex[2][16][PE];  // E^T or Z^T, parity of the chunk
   __shared__ __align__(16) __bf16 X[3][16][PT], U[3][16][PT];
-  __shared__ __align__(16) float Ox[4][16][20];  // a wave's outputs, transposed
   const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / 16;
   int slice, head;
   if (!scan_coords(blockIdx.x, slices, heads, slice, head)) return;
@@ -566,10 +567,14 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
           x[e] = S[0][e];
           x[4 + e] = RT == 2 ? S[RT - 1][e] : 0.f;
         }
-        Sx[n & 1][wave][0][lane] = S[0];
-        if (RT == 2) Sx[n & 1][wave][1][lane] = S[RT - 1];
         b8 sb[3];
         split<8, 3>(x, sb);
+#pragma unroll
+        for (int k = 0; k < NS; ++k) Sp[n & 1][wave][k][lane] = sb[k];
+        if (BACK || a.save) {
+          Sx[n & 1][wave][0][lane] = S[0];
+          if (RT == 2) Sx[n & 1][wave][1][lane] = S[RT - 1];
+        }
         f4 p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = f4{0, 0, 0, 0};
@@ -617,10 +622,14 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         __builtin_amdgcn_sched_barrier(0);
         if (!BACK || wave < 2) e0 = planes_mma<3, 3, 3>(tf[0], xb[0], e0);
         if (BACK || wave >= 2) e1 = planes_mma<3, 3, 3>(tf[1], xb[1], e1);
+        const f4 fv = fu;
+        __builtin_amdgcn_sched_barrier(0);
+        load_t(nat);
+        __builtin_amdgcn_sched_barrier(0);
         const f4 ev = e0 + e1;
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fu[e] : fu[e]) * ev[e];
+        for (int e = 0; e < 4; ++e) w[e] = (BACK ? -fv[e] : fv[e]) * ev[e];
         b4 up[3];
         split<4, 3>(w, up);
 #pragma unroll
@@ -640,9 +649,6 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int k = 0; k < 3; ++k) ub[ks][k] = *reinterpret_cast<const b8*>(&U[k][col][ks * 32 + g8]);
-        __builtin_amdgcn_sched_barrier(0);
-        load_t(nat);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           S[i] = planes_mma<N, 3, 3>(kt[i][0], ub[0], S[i]);
@@ -676,9 +682,8 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
     // Two sets of fragments, two chunks ahead: what a wave loads waits for what it stored before.
     b8 qf[2][4][N], pf[2][2][NO], qt[2][RT][2][N], of[2][2][N];
     f4 eg[2], bt[2][4], o;   // BACK: bt holds exp(G)
-    // Stores go through LDS, 4 columns of one row per lane: whole 64-byte pieces
+    // S, E and Z go to memory 4 columns of one row per lane: whole 64-byte pieces
     const int srow = lane >> 2, sc = (lane & 3) * 4;
-    const bool wide = (a.d.dv & 3) == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
     auto order = [&](int n) { return BACK ? chunks - 1 - n : n; };
     auto load_q = [&](int u, int n) {
       const long slot = slot0 + order(min(n, chunks - 1)), at = slot * a.d.value_heads + hv;
@@ -719,36 +724,13 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
     };
     // Q S, the terms of chain wave w
     auto q_part = [&](int u, int n, int w) {
-      const f4 s0 = Sx[n & 1][w][0][lane], s1 = RT == 2 ? Sx[n & 1][w][1][lane] : f4{0, 0, 0, 0};
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = s0[e];
-        x[4 + e] = s1[e];
-      }
       b8 sb[NO];
-      split<8, NO>(x, sb);
+#pragma unroll
+      for (int k = 0; k < NS; ++k) sb[k] = Sp[n & 1][w][k][lane];
       o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[u][w], sb, o);
     };
-    // what is left of chunk n: O from Ox, E or Z
+    // E or Z of chunk n
     auto flush = [&](int n) {
-      if (!BACK) {
-        const int tok = begin + n * C + wave * 16 + srow;
-        T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + tok) * a.d.value_heads + hv) * (long)a.d.dv + c0 + sc;
-        struct __align__(sizeof(T) * 4) Four { T x[4]; } w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w.x[e] = (T)Ox[wave][sc + e][srow];
-        __builtin_amdgcn_wave_barrier();
-        if (tok < end) {
-          if (wide) {
-            if (c0 + sc < a.d.dv) *reinterpret_cast<Four*>(out) = w;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c0 + sc + e < a.d.dv) out[e] = w.x[e];
-          }
-        }
-      }
       if (BACK || a.save) {
         float* dst = (BACK ? a.Z : a.Erow) + (((slot0 + order(n)) * a.d.value_heads + hv) * C + wave * 16) * a.dvp + c0;
         f4 v;
@@ -799,8 +781,12 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         o = planes_mma<NO, NO, NO>(pf[u][ks], ub, o);
       }
       load_p(u, n + 2);
-      *reinterpret_cast<f4*>(&Ox[wave][col][r4]) = o * a.scale;
-      __builtin_amdgcn_wave_barrier();
+      const int tok = begin + n * C + wave * 16 + r4;
+      T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + tok) * a.d.value_heads + hv) * (long)a.d.dv + c0 + col;
+      if (c0 + col < a.d.dv)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tok + e < end) out[(long)e * a.d.value_heads * a.d.dv] = (T)(a.scale * o[e]);
     };
     // u: the set of chunk n
     auto chunk = [&](int u, int n) {
@@ -1456,15 +1442,21 @@ Args make_args(const gpx_delta* d) {
   return a;
 }
 
-template <typename F>
-int allow_lds(F* kernel, size_t bytes) {
-  GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// once per thread, kernel and device
+template <auto Kernel>
+int allow_lds(size_t bytes) {
+  static thread_local bool done[GPX_MAX_DEVICES] = {};
+  int dev = 0;
+  GPX_HIP(hipGetDevice(&dev));
+  if (dev < GPX_MAX_DEVICES && done[dev]) return 0;
+  GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (dev < GPX_MAX_DEVICES) done[dev] = true;
   return 0;
 }
 
-#define DELTA_TRY(expr)       \
+#define DELTA_TRY(...)        \
   do {                        \
-    int rc_ = (expr);         \
+    int rc_ = (__VA_ARGS__);  \
     if (rc_ != 0) return rc_; \
   } while (0)
 
@@ -1484,7 +1476,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
   }
   constexpr size_t lds = chunk_room<T, DK>() + C * 8 + C * 4;
   static_assert(lds <= 160 * 1024, "LDS");
-  DELTA_TRY(allow_lds(&delta_chunk_kernel<T, DK>, lds));
+  DELTA_TRY(allow_lds<&delta_chunk_kernel<T, DK>>(lds));
   const long slots = slots_of(&a.d);
   if (slots > 0) {
     hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(256), lds, s, a);
@@ -1501,8 +1493,8 @@ int run_backward(hipStream_t s, const Args& a) {
   constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = room * 2 + C * 8 + (8 * C + 8 + C) * 4;
   constexpr size_t lds = base + tiles, grouped = base + (sizeof(T) == 4 ? 0 : tiles) + 8 * 512 * 16;
   static_assert(lds <= 160 * 1024 && grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
-  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK, false>, lds));
-  DELTA_TRY(allow_lds(&delta_grads_kernel<T, DK, true>, grouped));
+  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, false>>(lds));
+  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, true>>(grouped));
   const long slots = slots_of(&a.d);
   if (slots > 0) {
     hipLaunchKernelGGL((delta_back_prep_kernel<T>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
@@ -1623,7 +1615,7 @@ int gpx_delta_step(gpx_handle* h, const gpx_delta* d, int slots, const int* slot
   DELTA_TRY(check_delta(d, "delta_step"));
   GPX_REQUIRE(d->tokens == 1 && d->sequences == 0, "delta_step: one token per row");
   GPX_REQUIRE(slots >= 0 && (slot != nullptr || slots == d->batch), "delta_step: %d states for %d rows", slots, d->batch);
-  if (d->batch == 0) return 0;
+  if (d->batch == 0 || slots == 0) return 0;   // no row has a state
   GPX_REQUIRE(o != nullptr && state_out != nullptr && state != nullptr, "delta_step: null state or output");
   GPX_REQUIRE(gpx_aligned16(state) && gpx_aligned16(state_out), "delta_step: states must be 16-byte aligned");
   DeviceGuard dg(h->device);

@@ -19,17 +19,27 @@ from . import _lib
 from .device import ptr, tensor_runtime
 from .orthogonal import check_tensor, type_id
 
-_TYPES = ("float32", "float16", "bfloat16")
-
-
 def _dense(t):
     """t, or a packed copy where its last dimension is not dense or its tokens lie too far apart for the library."""
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-3) <= 1 << 22 else t.contiguous()
 
 
+def _dense_row(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
 def _st(t):
     """{batch, token, head} strides; a dimension of one has none."""
-    return _lib.Strided(*(t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)))
+    a, b, c = t.shape[:3]
+    x, y, z = t.stride()[:3]
+    return (x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0)
+
+
+def _st_row(t):
+    """The same of a (batch, head) tensor of one token each."""
+    a, c = t.shape[:2]
+    x, z = t.stride()[:2]
+    return (x if a > 1 else 0, 0, z if c > 1 else 0)
 
 
 def _opt(t):
@@ -37,38 +47,44 @@ def _opt(t):
 
 
 def _check(q, k, v, g, beta, dims):
+    """(type number, key heads, dk, value heads, dv) of inputs that fit together."""
     import torch
-    for name, t, n in (("q", q, dims), ("k", k, dims), ("v", v, dims), ("g", g, dims - 1), ("beta", beta, dims - 1)):
-        check_tensor(t, name)
-        if t.dim() != n:
-            raise ValueError("%s must have %d dimensions" % (name, n))
-    dtype = type_id(q, _TYPES)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    Tensor = torch.Tensor
+    if not (isinstance(q, Tensor) and isinstance(k, Tensor) and isinstance(v, Tensor) and isinstance(g, Tensor)
+            and isinstance(beta, Tensor)):
+        for name, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
+            check_tensor(t, name)
+    kind = q.dtype
+    dtype = type_id(q)
+    if not dtype:   # float64 has number 0
+        raise TypeError("element type %s is not one of float32, float16, bfloat16" % kind)
+    if k.dtype != kind or v.dtype != kind:
         raise TypeError("q, k and v must have one type")
-    for name, t in (("g", g), ("beta", beta)):
-        if t.dtype != torch.float32:
-            raise TypeError("%s must be float32" % name)
-    if q.shape != k.shape:
+    if g.dtype != torch.float32 or beta.dtype != torch.float32:
+        raise TypeError("g and beta must be float32")
+    qs, vs = q.shape, v.shape
+    if len(qs) != dims or len(vs) != dims:
+        raise ValueError("q, k and v must have %d dimensions" % dims)
+    if k.shape != qs:
         raise ValueError("q and k must have the same shape")
-    if v.shape[:-2] != q.shape[:-2] or g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+    if vs[:-2] != qs[:-2] or g.shape != vs[:-1] or beta.shape != vs[:-1]:
         raise ValueError("q, k, v, g and beta do not agree in batch, tokens or value heads")
-    Hk, dk = q.shape[-2:]
-    Hv, dv = v.shape[-2:]
+    Hk, dk = qs[-2:]
+    Hv, dv = vs[-2:]
     if Hk < 1 or Hv < 1 or Hv % Hk:
         raise ValueError("the value heads (%d) must be a multiple of the key heads (%d)" % (Hv, Hk))
     if not 1 <= dk <= 128 or not 1 <= dv <= 1024:
         raise ValueError("dk = %d must be in [1, 128], dv = %d in [1, 1024]" % (dk, dv))
-    return dtype
+    return dtype, Hk, dk, Hv, dv
 
 
-def _check_state(t, shape, name, like):
+def _check_state(t, shape, name):
     import torch
     if t is None:
-        return None
+        return
     check_tensor(t, name)
-    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
+    if t.dtype != torch.float32 or t.shape != shape:
         raise ValueError("%s must be float32 of shape %s" % (name, tuple(shape)))
-    return t
 
 
 def _aligned(t):
@@ -77,14 +93,6 @@ def _aligned(t):
     if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def _desc(dtype, q, k, v, g, beta, scale, offsets, sequences):
-    B, T, Hk, dk = q.shape
-    Hv, dv = v.shape[2:]
-    return _lib.Delta(dtype, B, T, sequences, Hk, Hv, dk, dv, float(scale), offsets.data_ptr() if offsets is not None else None,
-                      q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _st(q), _st(k), _st(v), _st(g),
-                      _st(beta))
 
 
 def _bytes(rt, d, use):
@@ -116,9 +124,8 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
     Long inputs run in chunks of 64 tokens on the matrix cores, up to 16 tokens go through the recurrence.  Asynchronous
     on the current stream; may be captured into a graph after one call outside."""
     import torch
-    dtype = _check(q, k, v, g, beta, 4)
-    B, T, Hk, dk = q.shape
-    Hv, dv = v.shape[2:]
+    dtype, Hk, dk, Hv, dv = _check(q, k, v, g, beta, 4)
+    B, T = q.shape[:2]
     sequences = 0
     if cu_seqlens is not None:
         check_tensor(cu_seqlens, "cu_seqlens")
@@ -128,14 +135,16 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
             raise ValueError("packed sequences need a batch of one")
         sequences = cu_seqlens.numel() - 1
     shape = (sequences or B, Hv, dk, dv)
-    _check_state(initial_state, shape, "initial_state", q)
+    _check_state(initial_state, shape, "initial_state")
     rt = tensor_runtime(q, k, v, g, beta, initial_state, cu_seqlens)
     with rt.current_stream():
         q, k, v = _dense(q), _dense(k), _dense(v)
         if cu_seqlens is not None:
             cu_seqlens = cu_seqlens.contiguous()
         state = _aligned(initial_state)
-        d = _desc(dtype, q, k, v, g, beta, dk ** -0.5 if scale is None else scale, cu_seqlens, sequences)
+        d = _lib.Delta(dtype, B, T, sequences, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale),
+                       cu_seqlens.data_ptr() if sequences else None, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+                       beta.data_ptr(), _st(q), _st(k), _st(v), _st(g), _st(beta))
         o = (torch.zeros if sequences else torch.empty)((B, T, Hv, dv), dtype=q.dtype, device=q.device)
         final = torch.empty(shape, dtype=torch.float32, device=q.device)
         work, size = _bytes(rt, d, 3 if save_for_backward else 0)
@@ -165,7 +174,7 @@ def gated_delta_rule_backward(saved, d_o, d_final_state=None):
     if d_o.shape != v.shape or d_o.dtype != v.dtype:
         raise ValueError("d_o must have the shape and the type of o")
     shape = (d.sequences or d.batch, d.value_heads, d.dk, d.dv)
-    _check_state(d_final_state, shape, "d_final_state", q)
+    _check_state(d_final_state, shape, "d_final_state")
     rt = tensor_runtime(q, d_o, d_final_state)
     with rt.current_stream():
         d_o, d_final = _dense(d_o), _aligned(d_final_state)
@@ -173,7 +182,7 @@ def gated_delta_rule_backward(saved, d_o, d_final_state=None):
         grads = [new(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]
         d_state = torch.empty(shape, dtype=torch.float32, device=q.device) if saved.has_state else None
         scratch, size = _bytes(rt, d, 2)
-        st = _st(d_o)
+        st = _lib.Strided(*_st(d_o))
         _lib.check(rt.lib.gpx_delta_backward(rt.h, C.byref(d), ptr(d_o), C.byref(st), _opt(d_final), *map(ptr, grads), _opt(d_state),
                                              ptr(saved.work), saved.work.numel(), ptr(scratch), size), "gpx_delta_backward")
     return (*grads, d_state)
@@ -187,12 +196,11 @@ def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, s
     is outside [0, n) is padding: its o is zero and no state is written for it; states that no row names are not touched.  Rows with
     the same slot are taken in their order, as successive tokens of one sequence."""
     import torch
-    dtype = _check(q, k, v, g, beta, 3)
-    B, Hk, dk = q.shape
-    Hv, dv = v.shape[1:]
+    dtype, Hk, dk, Hv, dv = _check(q, k, v, g, beta, 3)
+    B = q.shape[0]
     check_tensor(state, "state")
     n = state.shape[0] if state.dim() else 0
-    _check_state(state, (n, Hv, dk, dv), "state", q)
+    _check_state(state, (n, Hv, dk, dv), "state")
     if slots is None:
         if n != B:
             raise ValueError("%d states for %d rows: name them with slots" % (n, B))
@@ -202,20 +210,23 @@ def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, s
             raise ValueError("slots must be an int32 tensor with one value per row")
     if state_out is None:
         state_out = state
-    _check_state(state_out, state.shape, "state_out", q)
-    for name, t in (("state", state), ("state_out", state_out)):
-        if not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError("%s must be packed and 16-byte aligned" % name)
-    if state_out.data_ptr() != state.data_ptr() and state.numel():
-        gap = abs(state_out.data_ptr() - state.data_ptr())
-        if gap < state.numel() * 4:
-            raise ValueError("state_out overlaps state")
+    else:
+        _check_state(state_out, state.shape, "state_out")
+    at, to = state.data_ptr(), state_out.data_ptr()
+    if not state.is_contiguous() or not state_out.is_contiguous() or (at | to) % 16:
+        raise ValueError("state and state_out must be packed and 16-byte aligned")
+    if 0 < abs(to - at) < state.numel() * 4:
+        raise ValueError("state_out overlaps state")
     rt = tensor_runtime(q, k, v, g, beta, state, slots, state_out)
     with rt.current_stream():
-        q, k, v = _dense(q), _dense(k), _dense(v)
+        q, k, v = _dense_row(q), _dense_row(k), _dense_row(v)
         if slots is not None:
             slots = slots.contiguous()
         o = (torch.empty if slots is None else torch.zeros)((B, Hv, dv), dtype=q.dtype, device=q.device)
-        d = _desc(dtype, *(t.unsqueeze(1) for t in (q, k, v, g, beta)), dk ** -0.5 if scale is None else scale, None, 0)
-        _lib.check(rt.lib.gpx_delta_step(rt.h, C.byref(d), n, _opt(slots), ptr(state), ptr(state_out), ptr(o)), "gpx_delta_step")
+        d = _lib.Delta(dtype, B, 1, 0, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), None, q.data_ptr(),
+                       k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _st_row(q), _st_row(k), _st_row(v), _st_row(g),
+                       _st_row(beta))
+        rc = rt.lib.gpx_delta_step(rt.h, C.byref(d), n, _opt(slots), at, to, o.data_ptr())
+        if rc:
+            _lib.check(rc, "gpx_delta_step")
     return o, state_out

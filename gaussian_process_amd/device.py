@@ -2,7 +2,6 @@
 
 PyTorch is used only for allocation, H2D/D2H copies and stream identity; all arithmetic is in
 libgpx.so."""
-import contextlib
 import ctypes as C
 import threading
 
@@ -16,6 +15,23 @@ _runtimes = {}
 
 def _round_up(x, m):
     return ((x + m - 1) // m) * m
+
+
+class _OnStream:
+    __slots__ = ("rt", "raw", "set")
+
+    def __init__(self, rt):
+        self.rt, self.raw, self.set = rt, rt.torch._C._cuda_getCurrentRawStream, rt.lib.gpx_set_stream
+
+    def __enter__(self):
+        rt = self.rt
+        rt.lock.acquire()
+        self.set(rt.h, self.raw(rt.index))
+
+    def __exit__(self, *_):
+        rt = self.rt
+        self.set(rt.h, rt._stream.cuda_stream if rt._stream is not None else 0)
+        rt.lock.release()
 
 
 class Runtime:
@@ -37,6 +53,7 @@ class Runtime:
         # last fetch (see on_device below).
         self.lock = threading.RLock()
         self._stream = None
+        self._on_stream = _OnStream(self)
 
     def bind_stream(self):
         """Bind the handle to torch's current stream.  When the stream changes, the new one first waits
@@ -51,19 +68,11 @@ class Runtime:
         self._stream = cur
         _lib.check(self.lib.gpx_set_stream(self.h, C.c_void_p(cur.cuda_stream)), "gpx_set_stream")
 
-    @contextlib.contextmanager
     def current_stream(self):
-        """The handle on torch's current stream for calls that use none of its scratch: such calls need not wait
-        for what other streams do with the handle, so no event is recorded (the calls may be captured into a graph)
-        and the binding of bind_stream() is put back."""
-        with self.lock, self.torch.cuda.device(self.index):
-            cur = self.torch.cuda.current_stream(self.dev)
-            _lib.check(self.lib.gpx_set_stream(self.h, C.c_void_p(cur.cuda_stream)), "gpx_set_stream")
-            try:
-                yield self
-            finally:
-                old = self._stream.cuda_stream if self._stream is not None else 0
-                _lib.check(self.lib.gpx_set_stream(self.h, C.c_void_p(old)), "gpx_set_stream")
+        """`with rt.current_stream():` -- the handle on torch's current stream of this device, for calls that use none of
+        the handle's scratch: such calls need not wait for what other streams do with the handle, so no event is recorded
+        (the calls may be captured into a graph) and the binding of bind_stream() is put back."""
+        return self._on_stream
 
     # ---- buffers -------------------------------------------------------------------
     def matrix(self, rows, cols):
@@ -127,11 +136,13 @@ def ptr(t):
     return C.c_void_p(t.data_ptr())
 
 
-def tensor_runtime(*tensors):
-    """The runtime of the one MI355X that all the given tensors (None allowed) live on."""
-    devices = {t.device for t in tensors if t is not None}
-    if any(d.type != "cuda" for d in devices):
+def tensor_runtime(first, *others):
+    """The runtime of the one MI355X that all the given tensors (None allowed after the first) live on."""
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError("the tensors are on different devices: %s and %s" % (device, t.device))
+    if device.type != "cuda":
         raise _lib.GpxError("the tensors must be on an MI355X (no CPU fallback)")
-    if len(devices) != 1:
-        raise ValueError("the tensors are on different devices: %s" % ", ".join(sorted(map(str, devices))))
-    return runtime(devices.pop().index)
+    rt = _runtimes.get(device.index)
+    return rt if rt is not None else runtime(device.index)

@@ -11,11 +11,15 @@ from .device import ptr, tensor_runtime
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
-def type_id(t, names=("float64", "float32", "float16", "bfloat16")):
-    name = str(t.dtype).replace("torch.", "")
-    if name not in names:
-        raise TypeError("element type %s is not one of %s" % (name, ", ".join(names)))
-    return _lib.GPX_TYPE[name]
+_ids = {}
+
+
+def type_id(t):
+    """gpx's number of a tensor's element type; None if it has none."""
+    try:
+        return _ids[t.dtype]
+    except KeyError:
+        return _ids.setdefault(t.dtype, _lib.GPX_TYPE.get(str(t.dtype).replace("torch.", "")))
 
 
 def check_tensor(t, name):
@@ -67,6 +71,8 @@ def orthogonalize(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, alpha=1.0, be
     import torch
     check_tensor(G, "G")
     dtype = type_id(G)
+    if dtype is None:
+        raise TypeError("element type %s is not one of %s" % (G.dtype, ", ".join(_lib.GPX_TYPE)))
     if G.dim() < 2:
         raise ValueError("G must have at least two dimensions")
     if beta != 0.0 and base is None:

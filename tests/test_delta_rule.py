@@ -254,6 +254,9 @@ def test_no_tokens_and_no_rows():
     assert o.shape == (0, 5, 2, 16) and f.shape == (0, 2, 16, 16)
     o, f = gated_delta_rule_step(*(t[:, 0] for t in args(x)), f)
     assert o.shape == (0, 2, 16)
+    x = inputs(2, 1, 1, 2, 16, 16)
+    o, f = gated_delta_rule_step(*(t[:, 0] for t in args(x)), x["state"][:0], slots=cu([0, -1]))
+    assert (o == 0).all()
 
 
 @pytest.mark.gpu
