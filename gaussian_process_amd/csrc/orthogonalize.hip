@@ -212,6 +212,91 @@ __device__ __forceinline__ void write_out(const NsGemm& g, const float* st, long
   }
 }
 
+// The end of a product for EM x EN of its elements at (row0, col0): stage() leaves the sums in st (pitch EN + 4); every load of E is
+// under way before.
+template <int NPL, int EM, int EN, typename F>
+__device__ __forceinline__ void finish(const NsGemm& g, float* st, long z, int row0, int col0, int lane, bool mirror, F stage) {
+  constexpr int P = EN + 4;
+  constexpr int RL = EN / 8, RR = 64 / RL, RQ = EM / RR;   // row pass: lanes per row, rows at a time, times
+  constexpr int CL = EM / 8, CR = 64 / CL, CQ = EN / CR;   // column pass
+  const long ldd = (long)g.dpl * g.N, ldt = (long)NPL * g.M;
+  const bool two = g.dpl == 2;
+  const _Float16* E = g.E == nullptr ? nullptr : g.E + z * g.sd;
+  _Float16* D = g.D == nullptr ? nullptr : g.D + z * g.sd;
+  _Float16* DT = g.DT == nullptr ? nullptr : g.DT + z * g.st;
+  h8 eh[RQ], el[RQ];
+#pragma unroll
+  for (int q = 0; q < RQ; ++q) {
+    eh[q] = el[q] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (E != nullptr) {
+      const _Float16* src = E + (row0 + q * RR + lane / RL) * ldd + col0 + (lane % RL) * 8;
+      eh[q] = *reinterpret_cast<const h8*>(src);
+      if (two) el[q] = *reinterpret_cast<const h8*>(src + g.N);
+    }
+  }
+  stage();
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int q = 0; q < RQ; ++q) {
+    const int r = q * RR + lane / RL, c = (lane % RL) * 8;
+    float* p = st + r * P + c;
+    float v[8];
+    h8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = fmaf(g.ca, (float)eh[q][e] + (float)el[q][e], g.cc * p[e]);
+      hi[e] = (_Float16)v[e];
+      lo[e] = (_Float16)(v[e] - (float)hi[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = v[e];
+    if (D != nullptr) {
+      _Float16* dst = D + (row0 + r) * ldd + col0 + c;
+      *reinterpret_cast<h8*>(dst) = hi;
+      if (two) *reinterpret_cast<h8*>(dst + g.N) = lo;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (DT != nullptr && mirror) {
+#pragma unroll
+    for (int q = 0; q < CQ; ++q) {
+      const int c = q * CR + lane / CL, r = (lane % CL) * 8;
+      h8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = st[(r + e) * P + c];
+        hi[e] = (_Float16)v;
+        lo[e] = (_Float16)(v - (float)hi[e]);
+      }
+      _Float16* dst = DT + (col0 + c) * ldt + row0 + r;
+      *reinterpret_cast<h8*>(dst) = hi;
+      if (NPL == 2) *reinterpret_cast<h8*>(dst + g.M) = lo;
+    }
+  }
+  if (g.out_type == GPX_F32) write_out<float, EM, EN, P>(g, st, z, row0, col0, lane);
+  else if (g.out_type == GPX_F16) write_out<_Float16, EM, EN, P>(g, st, z, row0, col0, lane);
+  else if (g.out_type == GPX_BF16) write_out<__bf16, EM, EN, P>(g, st, z, row0, col0, lane);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The tile of this workgroup.  Workgroups with equal id % 8 share an XCD and its L2: each XCD takes a run of consecutive
+// tiles, four tile rows high.
+__device__ __forceinline__ void tile_of(int lower, int tiles_m, int tiles_n, int& ti, int& tj) {
+  const unsigned per = gridDim.x >> 3, rest = gridDim.x & 7, x = blockIdx.x & 7;
+  const unsigned id = x * per + min(x, rest) + (blockIdx.x >> 3);
+  if (lower) {
+    unsigned r = (unsigned)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+    while ((r + 1) * (r + 2) / 2 <= id) ++r;
+    while (r * (r + 1) / 2 > id) --r;
+    ti = r;
+    tj = id - r * (r + 1) / 2;
+  } else {
+    const unsigned band = id / (4 * tiles_n), in = id % (4 * tiles_n), high = min(4u, (unsigned)tiles_m - band * 4);
+    ti = band * 4 + in % high;
+    tj = in / high;
+  }
+}
+
 // Tile BM x BN, WAVES_M x WAVES_N waves of (BM / WAVES_M) x (BN / WAVES_N) each in 32 x 32 x 16 matrix instructions.
 // A k-tile is 64 / NPL long: an LDS row is 128 bytes either way, 8 chunks of 16 bytes (NPL = 2: four of hi, four of
 // lo), chunk c of row r in slot c ^ (r >> 1 & 7): 16 rows cover the 64 banks once in a 16-byte fragment read.
@@ -223,23 +308,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const N
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
   extern __shared__ __align__(16) char smem[];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  // Workgroups with equal id % 8 share an XCD and its L2: each XCD takes a run of consecutive tiles, four tile rows high
   int ti, tj;
-  {
-    const unsigned per = gridDim.x >> 3, rest = gridDim.x & 7, x = blockIdx.x & 7;
-    const unsigned id = x * per + min(x, rest) + (blockIdx.x >> 3);
-    if (g.lower) {
-      unsigned r = (unsigned)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
-      while ((r + 1) * (r + 2) / 2 <= id) ++r;
-      while (r * (r + 1) / 2 > id) --r;
-      ti = r;
-      tj = id - r * (r + 1) / 2;
-    } else {
-      const unsigned band = id / (4 * tiles_n), in = id % (4 * tiles_n), high = min(4u, (unsigned)tiles_m - band * 4);
-      ti = band * 4 + in % high;
-      tj = in / high;
-    }
-  }
+  tile_of(g.lower, tiles_m, tiles_n, ti, tj);
   const int i0 = ti * BM, j0 = tj * BN;
   const long z = blockIdx.y;
   const long lda = g.lda * 2, ldb = g.ldb * 2;   // bytes
@@ -344,81 +414,132 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const N
   static_assert((STAGES - 1) * L < 64, "vmcnt has six bits");
   __syncthreads();   // the stages become the waves' own staging of 64 x 64 blocks
   constexpr int EM = WM % 64 ? 32 : 64, EN = WN % 64 ? 32 : 64, P = EN + 4;
-  constexpr int RL = EN / 8, RR = 64 / RL, RQ = EM / RR;   // row pass: lanes per row, rows at a time, times
-  constexpr int CL = EM / 8, CR = 64 / CL, CQ = EN / CR;   // column pass
   float* st = reinterpret_cast<float*>(smem) + wave * (EM * P);
-  const long ldd = (long)g.dpl * g.N, ldt = (long)NPL * g.M;
-  const bool two = g.dpl == 2;
-  const _Float16* E = g.E == nullptr ? nullptr : g.E + z * g.sd;
-  _Float16* D = g.D == nullptr ? nullptr : g.D + z * g.sd;
-  _Float16* DT = g.DT == nullptr ? nullptr : g.DT + z * g.st;
 #pragma unroll
   for (int bi = 0; bi < WM / EM; ++bi)
 #pragma unroll
     for (int bj = 0; bj < WN / EN; ++bj) {
       const int row0 = i0 + wm * WM + bi * EM, col0 = j0 + wn * WN + bj * EN;
       if (row0 >= g.M || col0 >= g.N) continue;   // uniform in the wave; sizes are multiples of 64
-      // every load of E is under way before the first is used
-      h8 eh[RQ], el[RQ];
+      finish<NPL, EM, EN>(g, st, z, row0, col0, lane, !(g.lower && ti == tj), [&] {
 #pragma unroll
-      for (int q = 0; q < RQ; ++q) {
-        eh[q] = el[q] = h8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (E != nullptr) {
-          const _Float16* src = E + (row0 + q * RR + lane / RL) * ldd + col0 + (lane % RL) * 8;
-          eh[q] = *reinterpret_cast<const h8*>(src);
-          if (two) el[q] = *reinterpret_cast<const h8*>(src + g.N);
-        }
-      }
+        for (int a = 0; a < EM / 32; ++a)
 #pragma unroll
-      for (int a = 0; a < EM / 32; ++a)
+          for (int b = 0; b < EN / 32; ++b)
 #pragma unroll
-        for (int b = 0; b < EN / 32; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            st[(a * 32 + (e >> 2) * 8 + kh * 4 + (e & 3)) * P + b * 32 + r32] = acc[bi * (EM / 32) + a][bj * (EN / 32) + b][e];
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int q = 0; q < RQ; ++q) {
-        const int r = q * RR + lane / RL, c = (lane % RL) * 8;
-        float* p = st + r * P + c;
-        float v[8];
-        h8 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = fmaf(g.ca, (float)eh[q][e] + (float)el[q][e], g.cc * p[e]);
-          hi[e] = (_Float16)v[e];
-          lo[e] = (_Float16)(v[e] - (float)hi[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = v[e];
-        if (D != nullptr) {
-          _Float16* dst = D + (row0 + r) * ldd + col0 + c;
-          *reinterpret_cast<h8*>(dst) = hi;
-          if (two) *reinterpret_cast<h8*>(dst + g.N) = lo;
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
-      if (DT != nullptr && !(g.lower && ti == tj)) {
-#pragma unroll
-        for (int q = 0; q < CQ; ++q) {
-          const int c = q * CR + lane / CL, r = (lane % CL) * 8;
-          h8 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = st[(r + e) * P + c];
-            hi[e] = (_Float16)v;
-            lo[e] = (_Float16)(v - (float)hi[e]);
-          }
-          _Float16* dst = DT + (col0 + c) * ldt + row0 + r;
-          *reinterpret_cast<h8*>(dst) = hi;
-          if (NPL == 2) *reinterpret_cast<h8*>(dst + g.M) = lo;
-        }
-      }
-      if (g.out_type == GPX_F32) write_out<float, EM, EN, P>(g, st, z, row0, col0, lane);
-      else if (g.out_type == GPX_F16) write_out<_Float16, EM, EN, P>(g, st, z, row0, col0, lane);
-      else if (g.out_type == GPX_BF16) write_out<__bf16, EM, EN, P>(g, st, z, row0, col0, lane);
-      __builtin_amdgcn_wave_barrier();
+            for (int e = 0; e < 16; ++e)
+              st[(a * 32 + (e >> 2) * 8 + kh * 4 + (e & 3)) * P + b * 32 + r32] = acc[bi * (EM / 32) + a][bj * (EN / 32) + b][e];
+      });
     }
+}
+
+// Small problems, where latency counts and not the rate: a 64 x 64 tile per workgroup, whose W waves take every
+// W-th k-tile each, with stages of their own and no barrier, and add their sums through LDS in the order of the waves.  n = 1024, one
+// plane: 8.4 us for A A, about 4 of which a launch takes that does nothing else; 16 TB/s from L2.
+template <int W, int NPL, int STAGES>
+__global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int tiles_m, int tiles_n) {
+  constexpr int BK = 64 / NPL, KS = BK / 16, STAGE = 128 * 128, P = 68, L = 16, ROWS = 64 / W;
+  static_assert(STAGES * L < 64, "vmcnt has six bits");
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int ti, tj;
+  tile_of(g.lower, tiles_m, tiles_n, ti, tj);
+  const int i0 = ti * 64, j0 = tj * 64;
+  const long z = blockIdx.y;
+  const long lda = g.lda * 2, ldb = g.ldb * 2;   // bytes
+  const __amdgpu_buffer_rsrc_t ra =
+      __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)(g.A + z * g.sa) + i0 * lda), 0, 0x7fffffff, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rb =
+      __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)(g.B + z * g.sb) + j0 * ldb), 0, 0x7fffffff, 0x00020000);
+  // piece p: rows 8 p .. 8 p + 7 of a tile, whose sizes are multiples of 64
+  unsigned va[8], vb[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int r = p * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+    const unsigned in = NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16;
+    va[p] = (unsigned)(r * lda) + in;
+    vb[p] = (unsigned)(r * ldb) + in;
+  }
+  char* mine = smem + wave * (STAGES * STAGE);
+  auto load = [&](int kt, int stage) {
+    char* d = mine + stage * STAGE;
+    const unsigned so = (unsigned)kt * (BK * 2);
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      dma16(ra, va[p], so, d + p * 1024);
+      dma16(rb, vb[p], so, d + 8192 + p * 1024);
+    }
+  };
+  f16acc acc[2][2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+  const int r32 = lane & 31, kh = lane >> 5;
+  const int nk = g.K / BK, own = nk > wave ? (nk - wave + W - 1) / W : 0;   // k-tiles wave, wave + W, ..
+#pragma unroll
+  for (int p = 0; p < STAGES; ++p)
+    if (p < own) load(wave + p * W, p);
+  int cur = 0;
+  for (int n = 0; n < own; ++n) {
+    if (n + STAGES <= own)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * L) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const char* sA = mine + cur * STAGE + r32 * 128;
+    h8 fa[KS][2][NPL], fb[KS][2][NPL];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int pl = 0; pl < NPL; ++pl) {
+        const int o = (((s * 2 + kh) ^ ((r32 >> 1) & 7)) * 16) ^ (pl * 64);
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          fa[s][a][pl] = *reinterpret_cast<const h8*>(sA + a * 4096 + o);
+          fb[s][a][pl] = *reinterpret_cast<const h8*>(sA + 8192 + a * 4096 + o);
+        }
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // in registers: the stage may be filled again
+    if (n + STAGES < own) load(wave + (n + STAGES) * W, cur);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (NPL == 2) {
+            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][a][0], fb[s][b][NPL - 1], acc[a][b], 0, 0, 0);
+            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][a][NPL - 1], fb[s][b][0], acc[a][b], 0, 0, 0);
+          }
+          acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][a][0], fb[s][b][0], acc[a][b], 0, 0, 0);
+        }
+    cur = cur + 1 == STAGES ? 0 : cur + 1;
+  }
+  __syncthreads();   // the stages become the waves' sums, 64 x 64 each
+  float* sum = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        sum[(wave * 64 + a * 32 + (e >> 2) * 8 + kh * 4 + (e & 3)) * P + b * 32 + r32] = acc[a][b][e];
+  __syncthreads();
+  // wave w: the rows ROWS w .. of all sums; they end in the first
+  float* st = sum + wave * ROWS * P;
+  finish<NPL, ROWS, 64>(g, st, z, i0 + wave * ROWS, j0, lane, !(g.lower && ti == tj), [&] {
+    constexpr int Q = ROWS * 64 / 4 / 64;   // four columns a lane
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = q * 64 + lane, r = i >> 4, c = (i & 15) * 4;
+      f4 v = *reinterpret_cast<const f4*>(st + r * P + c);
+#pragma unroll
+      for (int w = 1; w < W; ++w) v += *reinterpret_cast<const f4*>(st + w * 64 * P + r * P + c);
+      *reinterpret_cast<f4*>(st + r * P + c) = v;
+    }
+  });
 }
 
 template <int BM, int BN, int WAVES_M, int WAVES_N, int NPL, int STAGES>
@@ -443,10 +564,29 @@ int launch_cfg(hipStream_t s, const NsGemm& g, int batch) {
   return 0;
 }
 
+template <int W, int NPL, int STAGES>
+int launch_small(hipStream_t s, const NsGemm& g, int batch) {
+  constexpr size_t lds = std::max<size_t>((size_t)W * STAGES * 128 * 128, (size_t)W * 64 * 68 * 4);
+  static_assert(lds <= 160 * 1024, "LDS");
+  const int tm = g.M / 64, tn = g.N / 64;
+  static thread_local bool set[GPX_MAX_DEVICES] = {};
+  int dev = 0;
+  GPX_HIP(hipGetDevice(&dev));
+  if (dev < GPX_MAX_DEVICES && !set[dev]) {
+    GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_small_kernel<W, NPL, STAGES>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    set[dev] = true;
+  }
+  hipLaunchKernelGGL((ns_small_kernel<W, NPL, STAGES>), dim3(g.lower ? (unsigned)tm * (tm + 1) / 2 : (unsigned)tm * tn, batch),
+                     dim3(64 * W), lds, s, g, tm, tn);
+  GPX_HIP(hipGetLastError());
+  return 0;
+}
+
 // Tile by estimated time: rounds of the chip times what one round of a tile takes (measured at K = 4096, one plane, us;
-// two planes keep the ratios): 64 x 64 with 4 waves, two on a CU, 34; 128 x 128 with 8 waves 42; 192 x 192 with 6 waves
+// two planes keep the ratios): 64 x 64 with 4 waves (ns_small_kernel), two on a CU, 34; 128 x 128 with 8 waves 42; 192 x 192 with 6 waves
 // 84; 256 x 256 with 8 waves 110.  Larger tiles read LDS less per product, smaller ones fill the chip: A A at n = 4096
-// takes 162 / 117 / 84 / 97 us with them, B X 233 / 173 / 169 / 140, at n = 1024 8.8 / 14 / 26 / 35 and 10 / 14 / 27 / 36.
+// takes 162 / 117 / 84 / 97 us with them, B X 233 / 173 / 169 / 140, at n = 1024 8.4 / 14 / 26 / 35 and 9.3 / 14 / 27 / 36.
 template <int NPL>
 int ns_gemm(hipStream_t s, const NsGemm& g, int batch) {
   const int tile[4] = {64, 128, 192, 256}, slots[4] = {512, 256, 256, 256};
@@ -462,7 +602,7 @@ int ns_gemm(hipStream_t s, const NsGemm& g, int batch) {
     }
   }
   switch (best) {
-    case 0: return launch_cfg<64, 64, 2, 2, NPL, 4>(s, g, batch);
+    case 0: return launch_small<4, NPL, 1>(s, g, batch);
     case 1: return launch_cfg<128, 128, 2, 4, NPL, 4>(s, g, batch);
     case 2: return launch_cfg<192, 192, 2, 3, NPL, 3>(s, g, batch);
     default: return launch_cfg<256, 256, 2, 4, NPL, 2>(s, g, batch);
@@ -567,7 +707,9 @@ template <typename T>
 int norm_launch(hipStream_t s, const void* G, long bs, long rs, long cs, int n, int m, int batch, double* part, int& nparts) {
   const bool along_rows = rs == 1 && cs != 1;
   const int slow = along_rows ? m : n, fast = along_rows ? n : m;
-  nparts = slow < PARTS ? slow : PARTS;
+  // a block for every 8192 elements: more would only make the sums of the partials longer
+  const long blocks = std::max(1L, (long)n * m / 8192);
+  nparts = (int)std::min<long>(std::min(slow, PARTS), blocks);
   hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(nparts, batch), dim3(256), 0, s, (const T*)G, bs, along_rows ? cs : rs,
                      along_rows ? rs : cs, slow, fast, part);
   GPX_HIP(hipGetLastError());
