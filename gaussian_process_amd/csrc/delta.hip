@@ -93,10 +93,10 @@ struct Args {
   float* fac;                   // per head: exp(G), beta, exp(G_C - G) beta, exp(G_C), exp(G_C - G), exp(G) beta; C each
   __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
-  float *Erow, *Srow;           // per head: E, C x dvp; S, DK x dvp
+  float *Erow, *Srow;           // per head: E, dvp / 32 x C x 32; S, dvp / 32 x DK x 32
   float* Y;                     // per head: (scale P^T dO)^T, dvp x C
   __bf16* Of;                   // per head: dO as fragments, dvp / 16 x 2 x 64 x 8
-  float *Z, *dS;                // per head: Z (dX = beta Z), C x dvp; dS', DK x dvp
+  float *Z, *dS;                // per head: Z (dX = beta Z) like E; dS' like S
   const float *state, *d_state_out;
   float *state_out, *d_state, *d_g, *d_beta;
   void *o, *d_q, *d_k, *d_v;
@@ -189,6 +189,18 @@ __device__ __forceinline__ f4 planes_mma(const b8* a, const b8* b, f4 acc) {
       if (j >= 0 && j < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc, 0, 0, 0);
     }
   return acc;
+}
+
+// sum over the 16 lanes of a row, in every lane
+__device__ __forceinline__ float row_sum(float x) {
+  auto add = [&](auto ctrl) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  add(std::integral_constant<int, 0xB1>{});    // lane ^ 1
+  add(std::integral_constant<int, 0x4E>{});    // lane ^ 2
+  add(std::integral_constant<int, 0x141>{});   // mirrored in eight
+  add(std::integral_constant<int, 0x140>{});   // mirrored in sixteen
+  return x;
 }
 
 // a barrier that waits for this wave's LDS accesses, not for its global ones
@@ -732,11 +744,12 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
     // E or Z of chunk n
     auto flush = [&](int n) {
       if (BACK || a.save) {
-        float* dst = (BACK ? a.Z : a.Erow) + (((slot0 + order(n)) * a.d.value_heads + hv) * C + wave * 16) * a.dvp + c0;
+        float* dst = (BACK ? a.Z : a.Erow) + ((slot0 + order(n)) * a.d.value_heads + hv) * (long)(C * a.dvp) + (c0 / DVT) * (C * DVT) +
+                     wave * 16 * DVT + c0 % DVT;
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
-        *reinterpret_cast<f4*>(dst + (unsigned)(srow * a.dvp + sc)) = v;
+        *reinterpret_cast<f4*>(dst + (unsigned)(srow * DVT + sc)) = v;
       }
     };
     auto first = [&](int u, int n) {
@@ -748,11 +761,12 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         q_part(u, n, 2);
       }
       if (BACK || a.save) {
-        float* dst = (BACK ? a.dS : a.Srow) + (((slot0 + order(n)) * a.d.value_heads + hv) * DK + wave * RT * 16) * a.dvp + c0;
+        float* dst = (BACK ? a.dS : a.Srow) + ((slot0 + order(n)) * a.d.value_heads + hv) * (long)(DK * a.dvp) +
+                     (c0 / DVT) * (DK * DVT) + wave * RT * 16 * DVT + c0 % DVT;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
-          *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * a.dvp + sc)) = f4{p[0], p[4], p[8], p[12]};
+          *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * DVT + sc)) = f4{p[0], p[4], p[8], p[12]};
         }
       }
     };
@@ -897,6 +911,13 @@ __global__ __launch_bounds__(256) void delta_back_prep_kernel(const Args a) {
 // 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
 // memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
 // the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
+// LDS of the slices, which a C x C matrix of three planes takes over
+template <typename T>
+constexpr size_t grads_room() {
+  constexpr size_t slices = (Planes<T>::N + 6) * C * 40, square = 3 * C * (C + 8);
+  return 2 * (slices > square ? slices : square);
+}
+
 template <typename T, int DK, bool GROUPED>
 __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   constexpr int N = Planes<T>::N, W = DK / 16, P = 40, PM = C + 8;
@@ -905,12 +926,11 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   __bf16* Y = reinterpret_cast<__bf16*>(smem);   // N planes
   __bf16* X = Y + N * SL;                        // 3
   __bf16* U = X + 3 * SL;                        // 3
-  __bf16* M = reinterpret_cast<__bf16*>(smem);   // later: a C x C matrix and its transpose, 3 planes each
-  __bf16* MT = M + 3 * C * PM;
-  constexpr size_t ROOM = (N + 6) * SL > 6 * C * PM ? (N + 6) * SL : 6 * C * PM;
-  double* G = reinterpret_cast<double*>(smem + ROOM * 2);
+  __bf16* M = reinterpret_cast<__bf16*>(smem);   // later: a C x C matrix, 3 planes
+  double* G = reinterpret_cast<double*>(smem + grads_room<T>());
   float* dG = reinterpret_cast<float*>(G + C);   // 8 x C: per wave
-  float* red = dG + 8 * C;      // 8
+  float* ef = dG + 8 * C;       // exp(G), exp(G_C - G): C each
+  float* red = ef + 2 * C;      // 8
   float* db = red + 8;          // C
   constexpr bool TILES = !(GROUPED && sizeof(T) == 4);   // K and Q in LDS, where they fit
   constexpr int PK = DK + 16 / sizeof(T);
@@ -924,6 +944,9 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
   const bool own = wave < W;
+  // 4 values of dO and of d_v at a time
+  const long dmask = a.do_st.bs | a.do_st.rs | a.do_st.cs;
+  const bool wide = (a.d.dv & 3) == 0 && (dmask & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.d_o) | reinterpret_cast<uintptr_t>(a.d_v)) & 15) == 0;
   const int group = GROUPED ? a.group : 1;
   if (TILES) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs;
@@ -955,7 +978,12 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     const int hv = hk * group + m;
     const long at = (long)slot * a.d.value_heads + hv;
     __syncthreads();
-    if (wave == 0) G[lane] = a.G[at * C + lane];
+    if (wave == 0) {
+      G[lane] = a.G[at * C + lane];
+      ef[lane] = a.fac[at * FACS + lane];
+      ef[C + lane] = a.fac[at * FACS + 4 * C + lane];
+    }
+    const float keep = a.fac[at * FACS + 3 * C];
     const float bt = a.fac[at * FACS + C + sr];
     f4 q1[4], kr[4], kc[4], dp[2], da[2];
 #pragma unroll
@@ -964,16 +992,23 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     float ss = 0.f, dbeta = 0.f;
     const T* dO = reinterpret_cast<const T*>(a.d_o) + row * a.do_st.bs + (t0 + min(sr, len - 1)) * a.do_st.rs + hv * a.do_st.cs;
     T* dv = reinterpret_cast<T*>(a.d_v) + ((row * a.d.tokens + t0 + sr) * a.d.value_heads + hv) * (long)a.d.dv;
-    // a slice's values, loaded while the slice before it is multiplied
     f4 ev, zv, sv[2], tv[2];
     T yv[4];
+    // a slice's values, loaded while the slice before it is multiplied (two workgroups on a CU instead, with 128 registers
+    // and 56 of them spilled: 330 us for 270)
     auto load_slice = [&](int c0) {
-      ev = *reinterpret_cast<const f4*>(a.Erow + (at * C + sr) * a.dvp + c0 + sc);
-      zv = *reinterpret_cast<const f4*>(a.Z + (at * C + sr) * a.dvp + c0 + sc);
+      const long eo = at * (C * a.dvp) + (long)c0 * C + sr * DVT + sc;
+      ev = *reinterpret_cast<const f4*>(a.Erow + eo);
+      zv = *reinterpret_cast<const f4*>(a.Z + eo);
+      if (wide) {
+        __builtin_memcpy(yv, __builtin_assume_aligned(dO + min(c0 + sc, a.d.dv - 4), 4 * sizeof(T)), sizeof(yv));
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) yv[e] = dO[min(c0 + sc + e, a.d.dv - 1)];
-      const f4* p = reinterpret_cast<const f4*>(a.Srow + (at * DK + min(kc0, DK - 1)) * a.dvp + c0 + g8);
-      const f4* q = reinterpret_cast<const f4*>(a.dS + (at * DK + min(kc0, DK - 1)) * a.dvp + c0 + g8);
+        for (int e = 0; e < 4; ++e) yv[e] = dO[min(c0 + sc + e, a.d.dv - 1)];
+      }
+      const long so = at * (DK * a.dvp) + (long)c0 * DK + min(kc0, DK - 1) * DVT + g8;
+      const f4* p = reinterpret_cast<const f4*>(a.Srow + so);
+      const f4* q = reinterpret_cast<const f4*>(a.dS + so);
       sv[0] = p[0];
       sv[1] = p[1];
       tv[0] = q[0];
@@ -989,7 +1024,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         x[e] = bt * zv[e];
         u[e] = bt * ev[e];
         dbeta = fmaf(ev[e], zv[e], dbeta);
-        if (live) dv[c0 + sc + e] = (T)x[e];
+        if (live && !wide) dv[c0 + sc + e] = (T)x[e];
+      }
+      if (wide && sr < len && c0 + sc < a.d.dv) {
+        struct __align__(sizeof(T) * 4) Four { T x[4]; } w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.x[e] = (T)x[e];
+        *reinterpret_cast<Four*>(dv + c0 + sc) = w;
       }
       b8 sb[3], db_[3];
       {
@@ -1053,7 +1094,6 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
       }
     }
     // row factors; k . state part of dKc
-    const double last = G[C - 1];
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs + min(kc0, a.d.dk - 1);
     const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs + min(kc0, a.d.dk - 1);
     float csum = 0.f;
@@ -1077,53 +1117,64 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = rb * 16 + r4 + e;
-          const float eg = expf((float)G[r]);
+          const float eg = ef[r];
           q1[rb][e] *= a.scale * eg;
           kr[rb][e] *= -eg;
-          kc[rb][e] *= expf((float)(last - G[r]));
+          kc[rb][e] *= ef[C + r];
           csum = fmaf(element(Kt, Kg, a.d.k_st, r), kc[rb][e], csum);
         }
     }
-    for (int o = 1; o < 64; o <<= 1) {
+    csum = row_sum(csum);
+    ss = row_sum(ss);
+    for (int o = 16; o < 64; o <<= 1) {
       csum += __shfl_xor(csum, o);
       ss += __shfl_xor(ss, o);
     }
-    if (lane == 0) red[wave] = fmaf(expf((float)last), ss, csum);
+    if (lane == 0) red[wave] = fmaf(keep, ss, csum);
     for (int o = 1; o < 8; o <<= 1) dbeta += __shfl_xor(dbeta, o);
     if ((t & 7) == 0) db[sr] = dbeta;
-    // dP o D with K and Q, then dN o D with K
+    f4 D[2];
+    // dP o D with K, its transpose with Q; then dN o D and its transpose with K
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
+    for (int w = 0; w < 4; ++w) {
+      const bool tr = w & 1;
       __syncthreads();
-      // the tiles above the diagonal
-      for (int i = t; i < 6 * 256; i += 512) {
-        const int tile = i >> 8, r = i >> 4 & 15, c = i & 15;
-        const int rb = tile < 3 ? 0 : tile < 5 ? 1 : 2, cb = tile < 3 ? tile + 1 : tile < 5 ? tile - 1 : 3;
+      // of the tiles that hold zeros only two are read
+      {
+        const int z = t >> 8, r = t >> 4 & 15, c = t & 15, rb = z * 2 + (tr ? 1 : 0), cb = z * 2 + (tr ? 0 : 1);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          M[(k * C + rb * 16 + r) * PM + cb * 16 + c] = (__bf16)0.f;
-          MT[(k * C + cb * 16 + c) * PM + rb * 16 + r] = (__bf16)0.f;
-        }
+        for (int k = 0; k < 3; ++k) M[(k * C + rb * 16 + r) * PM + cb * 16 + c] = (__bf16)0.f;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int tile = wave + 8 * h;
         if (tile < 10) {
           const int rb = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, cb = tile - rb * (rb + 1) / 2, c = cb * 16 + col;
+          if (w % 2 == 0) {   // the values, in place of the sums
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = rb * 16 + r4 + e;
+              if (w == 0) {
+                D[h][e] = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
+                dp[h][e] *= a.scale * D[h][e];
+              } else {
+                da[h][e] = r > c ? -da[h][e] * D[h][e] : 0.f;
+              }
+            }
+          }
           float x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = rb * 16 + r4 + e;
-            const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
-            x[e] = w == 0 ? a.scale * dp[h][e] * D : r > c ? -da[h][e] * D : 0.f;
-          }
+          for (int e = 0; e < 4; ++e) x[e] = w < 2 ? dp[h][e] : da[h][e];
           b4 xp[3];
           split<4, 3>(x, xp);
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
-            *reinterpret_cast<b4*>(MT + (k * C + c) * PM + rb * 16 + r4) = xp[k];
+            if (tr) {
+              *reinterpret_cast<b4*>(M + (k * C + c) * PM + rb * 16 + r4) = xp[k];
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) M[(k * C + rb * 16 + r4 + e) * PM + c] = xp[k][e];
+              for (int e = 0; e < 4; ++e) M[(k * C + rb * 16 + r4 + e) * PM + c] = xp[k][e];
+            }
           }
         }
       }
@@ -1133,18 +1184,14 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         for (int rb = 0; rb < 4; ++rb)
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
+            if (tr ? ks * 2 + 1 < rb : ks * 2 > rb) continue;   // zeros
             b8 mm_[3];
-            if (ks * 2 <= rb) {
 #pragma unroll
-              for (int k = 0; k < 3; ++k) mm_[k] = *reinterpret_cast<const b8*>(M + (k * C + rb * 16 + col) * PM + ks * 32 + g8);
-              if (w == 0) q1[rb] = planes_mma<3, N, 3>(mm_, kt[ks], q1[rb]);
-              else kr[rb] = planes_mma<3, N, 3>(mm_, kt[ks], kr[rb]);
-            }
-            if (ks * 2 + 1 >= rb) {
-#pragma unroll
-              for (int k = 0; k < 3; ++k) mm_[k] = *reinterpret_cast<const b8*>(MT + (k * C + rb * 16 + col) * PM + ks * 32 + g8);
-              kc[rb] = planes_mma<3, N, 3>(mm_, w == 0 ? qt[ks] : kt[ks], kc[rb]);
-            }
+            for (int k = 0; k < 3; ++k) mm_[k] = *reinterpret_cast<const b8*>(M + (k * C + rb * 16 + col) * PM + ks * 32 + g8);
+            if (w == 0) q1[rb] = planes_mma<3, N, 3>(mm_, kt[ks], q1[rb]);
+            if (w == 1) kc[rb] = planes_mma<3, N, 3>(mm_, qt[ks], kc[rb]);
+            if (w == 2) kr[rb] = planes_mma<3, N, 3>(mm_, kt[ks], kr[rb]);
+            if (w == 3) kc[rb] = planes_mma<3, N, 3>(mm_, kt[ks], kc[rb]);
           }
       }
     }
@@ -1156,7 +1203,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
       for (int e = 0; e < 4; ++e) {
         const int r = rb * 16 + r4 + e;
         g[e] = own ? fmaf(element(Qt, Qg, a.d.q_st, r), q1[rb][e], element(Kt, Kg, a.d.k_st, r) * (kr[rb][e] - kc[rb][e])) : 0.f;
-        for (int o = 1; o < 16; o <<= 1) g[e] += __shfl_xor(g[e], o);
+        g[e] = row_sum(g[e]);
       }
       if (col == 0)
 #pragma unroll
@@ -1489,8 +1536,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
 
 template <typename T, int DK>
 int run_backward(hipStream_t s, const Args& a) {
-  constexpr size_t room = (Planes<T>::N + 6) * C * 40 > 6 * C * (C + 8) ? (Planes<T>::N + 6) * C * 40 : 6 * C * (C + 8);
-  constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = room * 2 + C * 8 + (8 * C + 8 + C) * 4;
+  constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = grads_room<T>() + C * 8 + (8 * C + 2 * C + 8 + C) * 4;
   constexpr size_t lds = base + tiles, grouped = base + (sizeof(T) == 4 ? 0 : tiles) + 8 * 512 * 16;
   static_assert(lds <= 160 * 1024 && grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
   DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, false>>(lds));
