@@ -1387,7 +1387,8 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const StepArgs x) 
     if (r >= a.d.dk) continue;
     float* p = a.state_out + base + (long)r * a.d.dv + c0;
     if (vec && c0 < a.d.dv) {
-      *reinterpret_cast<f4*>(p) = f4{S[i][0], S[i][1], S[i][2], S[i][3]};
+      // past the caches: 64 users' states of 32 x 128 x 128 are 268 MB there and back, 49.7 us with plain stores, 44.6 with these
+      __builtin_nontemporal_store(f4{S[i][0], S[i][1], S[i][2], S[i][3]}, reinterpret_cast<f4*>(p));
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
