@@ -108,15 +108,12 @@ struct Args {
 template <typename T> __device__ __forceinline__ float ld(const void* p, long i) { return (float)reinterpret_cast<const T*>(p)[i]; }
 template <typename T> __device__ __forceinline__ void st(void* p, long i, float v) { reinterpret_cast<T*>(p)[i] = (T)v; }
 
-// acc (16 x 16, rows (lane >> 4) * 4 + e, column lane & 15) += A B over k < K (a multiple of 4).  A is 16 x K, stored
-// [row][k] or with TA [k][row]; B is K x 16, stored [k][col] or with TB [col][k].
-template <bool TA, bool TB>
+// acc (16 x 16, rows (lane >> 4) * 4 + e, column lane & 15) += A B over k < K (a multiple of 4), A 16 x K, B K x 16
 __device__ __forceinline__ f4 mm(const float* A, int pa, const float* B, int pb, int K, f4 acc) {
   const int r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-  const float* a = TA ? A + g * pa + r : A + r * pa + g;
-  const float* b = TB ? B + r * pb + g : B + g * pb + r;
-  const int sa = TA ? 4 * pa : 4, sb = TB ? 4 : 4 * pb;
-  for (int k = 0; k < K; k += 4, a += sa, b += sb) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(*a, *b, acc, 0, 0, 0);
+  A += r * pa + g;
+  B += g * pb + r;
+  for (int k = 0; k < K; k += 4) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(A[k], B[k * pb], acc, 0, 0, 0);
   return acc;
 }
 
@@ -203,6 +200,9 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
+// exp(x) for x <= 0: the argument is rounded once, as by a cast to float, and what is below 2^-126 becomes 0
+__device__ __forceinline__ float decay(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
+
 // a barrier that waits for this wave's LDS accesses, not for its global ones
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -267,7 +267,7 @@ struct Rows {
 };
 
 // T = (I + A)^-1 for the strictly lower A (LDS, pitch PC), 4 waves.  The 16 x 16 diagonal blocks by substitution, one column
-// per lane; then block T_ij = -T_ii sum_l A_il T_lj for i - j = 1, 2, 3, on the fp32 matrix cores.  tmp: 4 x 16 x 20 floats.
+// per lane; then, twice, [T0 0; -T1 A10 T0 T1] of two blocks and what is under them, on the fp32 matrix cores.  tmp: 32 x 36.
 __device__ __forceinline__ void unit_lower_inverse(const float* A, float* Ti, float* tmp, int wave, int lane) {
   const int r4 = (lane >> 4) * 4, col = lane & 15;
   for (int j = wave + 1; j < 4; ++j)
@@ -286,33 +286,39 @@ __device__ __forceinline__ void unit_lower_inverse(const float* A, float* Ti, fl
     }
   }
   __syncthreads();
-  float* mine = tmp + wave * 16 * 20;
-  for (int d = 1; d < 4; ++d) {
-    const int i = wave, j = wave - d;   // waves without a block only meet the barriers
-    if (j >= 0) {
-      f4 acc = {0, 0, 0, 0};
-      for (int l = j; l < i; ++l)
-        acc = mm<false, false>(A + i * 16 * PC + l * 16, PC, Ti + l * 16 * PC + j * 16, PC, 16, acc);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine[(r4 + e) * 20 + col] = acc[e];
+  for (int n = 1; n < 3; ++n) {   // blocks of n times 16 rows
+    // this wave's 16 x 16 of the products: rows i, columns j of the n x n under the diagonal, in units of 16
+    const int lo = n == 1 ? wave * 2 : 0, hi = lo + n, i = n == 1 ? 0 : wave >> 1, j = n == 1 ? 0 : wave & 1;
+    const bool works = n == 2 || wave < 2;
+    float* mine = tmp + (n == 1 ? wave * 16 : i * 16) * 36 + j * 16;
+    if (works) {
+      f4 acc = {0, 0, 0, 0};
+      for (int l = j; l < n; ++l)
+        acc = mm(A + (hi + i) * 16 * PC + (lo + l) * 16, PC, Ti + (lo + l) * 16 * PC + (lo + j) * 16, PC, 16, acc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(r4 + e) * 36 + col] = acc[e];
     }
     __syncthreads();
-    if (j >= 0) {
+    if (works) {
       f4 acc = {0, 0, 0, 0};
-      acc = mm<false, false>(Ti + i * 16 * PC + i * 16, PC, mine, 20, 16, acc);
+      for (int l = 0; l <= i; ++l)
+        acc = mm(Ti + (hi + i) * 16 * PC + (hi + l) * 16, PC, mine + (l - i) * 16 * 36, 36, 16, acc);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) Ti[(i * 16 + r4 + e) * PC + j * 16 + col] = -acc[e];
+      for (int e = 0; e < 4; ++e) Ti[((hi + i) * 16 + r4 + e) * PC + (lo + j) * 16 + col] = -acc[e];
     }
     __syncthreads();
   }
 }
 
-// rows, or with TR columns, of a C x C matrix in LDS (pitch PC) as fragments in natural order
+// rows, or with TR columns, of a lower triangular C x C matrix in LDS (pitch PC) as fragments in natural order; those that
+// hold only zeros are neither written nor read
 template <int NPL, bool TR>
 __device__ __forceinline__ void store_square(const float* M, __bf16* dst, int t) {
   for (int i = t; i < TF / 8; i += 256) {
     const int lane = i & 63, ks = i >> 6 & 1, rb = i >> 7;
     const int r = rb * 16 + (lane & 15), c = ks * 32 + (lane >> 4) * 8;
+    if (TR ? ks * 2 + 1 < rb : ks * 2 > rb) continue;
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = TR ? M[(c + e) * PC + r] : M[r * PC + c + e];
@@ -329,12 +335,12 @@ template <typename T> struct OutPlanes { static constexpr int N = sizeof(T) == 2
 // ---- prep: one chunk of one key head and its value heads -----------------------------------------------------------------
 template <typename T, int DK>
 constexpr size_t chunk_room() {
-  constexpr size_t first = 2 * Planes<T>::N * C * (DK + 8) * 2, second = (2 * C * PC + 4 * 16 * 20) * 4;
+  constexpr size_t first = 2 * Planes<T>::N * C * (DK + 8) * 2, second = (2 * C * PC + 32 * 36) * 4;
   return first > second ? first : second;
 }
 
 template <typename T, int DK>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kernel(const Args a) {
+__global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_kernel(const Args a) {
   constexpr int N = Planes<T>::N, P = DK + 8, RT = DK / 64, KSN = DK / 32;
   extern __shared__ __align__(16) char smem[];
   __bf16* K = reinterpret_cast<__bf16*>(smem);
@@ -348,7 +354,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kerne
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
   if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
   const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
   float gv = 0.f, bv = 0.f;   // wave 0: g and beta of the next value head
   auto load_g = [&](int hv) {
@@ -357,10 +363,34 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kerne
     bv = a.d.beta[row * a.d.beta_st.bs + tok * a.d.beta_st.rs + hv * a.d.beta_st.cs];
   };
   if (wave == 0) load_g(hk * a.group);
+  // wave 0: G, beta and the factors of value head hv; the next head's values set off
+  auto factors = [&](int hv) {
+    const long at = (long)slot * a.d.value_heads + hv;
+    const float g = lane < len ? gv : 0.f, b = lane < len ? bv : 0.f;
+    load_g(min(hv + 1, a.d.value_heads - 1));
+    double x = g < G_MIN ? G_MIN : g;
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    const double last = __shfl(x, 63);
+    G[lane] = x;
+    beta[lane] = b;
+    a.G[at * C + lane] = x;
+    float* f = a.fac + at * FACS + lane;
+    const float eg = expf((float)x), tail = expf((float)(last - x));
+    f[0] = eg;
+    f[C] = b;
+    f[2 * C] = tail * b;
+    f[3 * C] = expf((float)last);
+    f[4 * C] = tail;
+    f[5 * C] = eg * b;
+  };
   {
     Rows<T, DK> k, q;
     k.fetch(a.d.k, a.d.k_st, row, t0, len, hk, a.d.dk, t);
     q.fetch(a.d.q, a.d.q_st, row, t0, len, hk, a.d.dk, t);
+    if (wave == 0) factors(hk * a.group);
     k.put(K, len, a.d.dk, t);
     q.put(Q, len, a.d.dk, t);
   }
@@ -417,38 +447,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kerne
   }
   for (int m = 0; m < a.group; ++m) {
     const int hv = hk * a.group + m;
+    int tt = threadIdx.x;
+    asm volatile("" : "+v"(tt));   // opaque: addresses of all matrices held over the loop are spilled
+    const int t = tt, lane = t & 63, r4 = (lane >> 4) * 4, col = lane & 15;
     const long at = (long)slot * a.d.value_heads + hv;
-    if (wave == 0) {
-      const float g = lane < len ? gv : 0.f, b = lane < len ? bv : 0.f;
-      load_g(min(hv + 1, a.d.value_heads - 1));
-      double x = g < G_MIN ? G_MIN : g;
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-      }
-      const double last = __shfl(x, 63);
-      G[lane] = x;
-      beta[lane] = b;
-      a.G[at * C + lane] = x;
-      float* f = a.fac + at * FACS + lane;
-      const float eg = expf((float)x), tail = expf((float)(last - x));
-      f[0] = eg;
-      f[C] = b;
-      f[2 * C] = tail * b;
-      f[3 * C] = expf((float)last);
-      f[4 * C] = tail;
-      f[5 * C] = eg * b;
-    }
+    if (m > 0 && wave == 0) factors(hv);
     __syncthreads();
+    f4 nd[4];   // N
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = j * 16 + col;
+      nd[j] = f4{0, 0, 0, 0};
+      if (j <= wave) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = wave * 16 + r4 + e;
-        const float D = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
-        A[r * PC + c] = r > c ? nn[j][e] * D * beta[c] : 0.f;
-        M[r * PC + c] = r >= c ? pp[j][e] * D : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          const int r = wave * 16 + r4 + e;
+          const float D = r >= c ? decay(G[r] - G[c]) : 0.f;
+          nd[j][e] = r > c ? nn[j][e] * D : 0.f;
+          A[r * PC + c] = nd[j][e] * beta[c];
+          M[r * PC + c] = r >= c ? pp[j][e] * D : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) A[(wave * 16 + r4 + e) * PC + c] = M[(wave * 16 + r4 + e) * PC + c] = 0.f;
       }
     }
     __syncthreads();
@@ -457,22 +478,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void delta_chunk_kerne
     __syncthreads();
     unit_lower_inverse(A, M, tmp, wave, lane);
     store_square<3, false>(M, a.Tf + at * 3 * TF, t);
-    __syncthreads();
-    if (a.save) {   // the same with beta from the left
+    if (a.save) {   // (I + diag(beta) N)^-1 = I - diag(beta) T N
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) A[(wave * 16 + r4 + e) * PC + j * 16 + col] = nd[j][e];
+      __syncthreads();
+      f4 t2[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        t2[j] = f4{0, 0, 0, 0};
+        if (j <= wave) t2[j] = mm(M + wave * 16 * PC + j * 16, PC, A + j * 16 * PC + j * 16, PC, (wave + 1 - j) * 16, t2[j]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j > wave) continue;   // zeros already
         const int c = j * 16 + col;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = wave * 16 + r4 + e;
-          A[r * PC + c] = r > c ? nn[j][e] * expf((float)(G[r] - G[c])) * beta[r] : 0.f;
+          A[r * PC + c] = (r == c ? 1.f : 0.f) - beta[r] * t2[j][e];
         }
       }
       __syncthreads();
-      unit_lower_inverse(A, M, tmp, wave, lane);
-      store_square<3, true>(M, a.T2f + at * 3 * TF, t);
-      __syncthreads();
+      store_square<3, true>(A, a.T2f + at * 3 * TF, t);
     }
+    __syncthreads();
   }
 }
 
@@ -550,10 +582,11 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
     };
     auto load_t = [&](long at) {
       const __bf16* p = (BACK ? a.T2f : a.Tf) + at * 3 * TF + wave * 2 * 512;
+      const int k0 = BACK && wave >= 2 ? 512 : 0, k1 = !BACK && wave < 2 ? 0 : 512;   // not the zeros: these are not there
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        tf[0][k] = ld_frag(p + k * TF, lb);
-        tf[1][k] = ld_frag(p + k * TF + 512, lb);
+        tf[0][k] = ld_frag(p + k * TF + k0, lb);
+        tf[1][k] = ld_frag(p + k * TF + k1, lb);
       }
       fu = *reinterpret_cast<const f4*>(a.fac + at * FACS + (BACK ? 5 : 2) * C + wave * 16 + r4);
     };
@@ -728,7 +761,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
 #pragma unroll
       for (int k = 0; k < NO; ++k) {
         pf[u][0][k] = ld_frag(p + k * TF, lb);
-        pf[u][1][k] = ld_frag(p + k * TF + 512, lb);
+        pf[u][1][k] = ld_frag(p + k * TF + (wave < 2 ? 0 : 512), lb);
       }
       const float* f = a.fac + at * FACS + C + g8;
 #pragma unroll
@@ -1155,7 +1188,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
             for (int e = 0; e < 4; ++e) {
               const int r = rb * 16 + r4 + e;
               if (w == 0) {
-                D[h][e] = r >= c ? expf((float)(G[r] - G[c])) : 0.f;
+                D[h][e] = r >= c ? decay(G[r] - G[c]) : 0.f;
                 dp[h][e] *= a.scale * D[h][e];
               } else {
                 da[h][e] = r > c ? -da[h][e] * D[h][e] : 0.f;
