@@ -82,14 +82,17 @@ __global__ void delta_plan_kernel(const int* in, int n, int tokens, int* out) {
   }
 }
 
+typedef float f2 __attribute__((ext_vector_type(2)));
+
 struct Args {
   gpx_delta d;
   Plan p;
   int group;                    // value heads per key head
+  int parts;                    // prep: workgroups among which a key head's value heads are dealt, 1 or group
   int dvp;                      // dv rounded up to DVT
   float scale;
   // Parts of the workspaces; "per key head", "per head": of a slot and a key or value head.  Fragments are explained below.
-  double* G;                    // per head: C
+  f2* G;                        // per head: C, the sums of g in two parts
   float* fac;                   // per head: exp(G), beta, exp(G_C - G) beta, exp(G_C), exp(G_C - G), exp(G) beta; C each
   __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
@@ -200,8 +203,14 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-// exp(x) for x <= 0: the argument is rounded once, as by a cast to float, and what is below 2^-126 becomes 0
-__device__ __forceinline__ float decay(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
+// Sums of g, in double: kept times log2(e) as a float and what that leaves out.  exp(x - y) has then the error of one rounding
+// of x - y and one of the power; powers below 2^-126 become 0.
+__device__ __forceinline__ f2 in_parts(double g) {
+  g *= 1.4426950408889634;
+  const float hi = (float)g;
+  return f2{hi, (float)(g - (double)hi)};
+}
+__device__ __forceinline__ float decay(f2 x, f2 y) { return __builtin_amdgcn_exp2f((x[0] - y[0]) + (x[1] - y[1])); }
 
 // a barrier that waits for this wave's LDS accesses, not for its global ones
 __device__ __forceinline__ void lds_barrier() {
@@ -279,8 +288,11 @@ __device__ __forceinline__ void unit_lower_inverse(const float* A, float* Ti, fl
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float v = i == lane ? 1.f : 0.f;
+      f4 al[4];
 #pragma unroll
-      for (int l = 0; l < i; ++l) v = fmaf(-a[i * PC + l], x[l], v);
+      for (int l = 0; l < (i + 3) / 4; ++l) al[l] = *reinterpret_cast<const f4*>(a + i * PC + l * 4);
+#pragma unroll
+      for (int l = 0; l < i; ++l) v = fmaf(-al[l / 4][l % 4], x[l], v);
       x[i] = v;
       Ti[(wave * 16 + i) * PC + wave * 16 + lane] = v;
     }
@@ -348,9 +360,10 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
   float* A = reinterpret_cast<float*>(smem);   // over K and Q, once these are in registers and memory
   float* M = A + C * PC;
   float* tmp = M + C * PC;
-  double* G = reinterpret_cast<double*>(smem + chunk_room<T, DK>());
+  f2* G = reinterpret_cast<f2*>(smem + chunk_room<T, DK>());
   float* beta = reinterpret_cast<float*>(G + C);
-  const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
+  const int part = blockIdx.x % a.parts, hk = blockIdx.x / a.parts % a.d.key_heads, slot = blockIdx.x / a.parts / a.d.key_heads;
+  const int first = a.group / a.parts * part, last = first + a.group / a.parts;   // value heads of the key head
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
   if (len == 0) return;
@@ -362,7 +375,7 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
     gv = a.d.g[row * a.d.g_st.bs + tok * a.d.g_st.rs + hv * a.d.g_st.cs];
     bv = a.d.beta[row * a.d.beta_st.bs + tok * a.d.beta_st.rs + hv * a.d.beta_st.cs];
   };
-  if (wave == 0) load_g(hk * a.group);
+  if (wave == 0) load_g(hk * a.group + first);
   // wave 0: G, beta and the factors of value head hv; the next head's values set off
   auto factors = [&](int hv) {
     const long at = (long)slot * a.d.value_heads + hv;
@@ -373,16 +386,15 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
       const double y = __shfl_up(x, o);
       if (lane >= o) x += y;
     }
-    const double last = __shfl(x, 63);
-    G[lane] = x;
+    const double sum = __shfl(x, 63);
+    G[lane] = a.G[at * C + lane] = in_parts(x);
     beta[lane] = b;
-    a.G[at * C + lane] = x;
     float* f = a.fac + at * FACS + lane;
-    const float eg = expf((float)x), tail = expf((float)(last - x));
+    const float eg = expf((float)x), tail = expf((float)(sum - x));
     f[0] = eg;
     f[C] = b;
     f[2 * C] = tail * b;
-    f[3 * C] = expf((float)last);
+    f[3 * C] = expf((float)sum);
     f[4 * C] = tail;
     f[5 * C] = eg * b;
   };
@@ -390,13 +402,14 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
     Rows<T, DK> k, q;
     k.fetch(a.d.k, a.d.k_st, row, t0, len, hk, a.d.dk, t);
     q.fetch(a.d.q, a.d.q_st, row, t0, len, hk, a.d.dk, t);
-    if (wave == 0) factors(hk * a.group);
+    if (wave == 0) factors(hk * a.group + first);
     k.put(K, len, a.d.dk, t);
     q.put(Q, len, a.d.dk, t);
   }
   __syncthreads();
   // K and Q in state order, K^T in natural order
-  for (int i = t; i < KF / 8; i += 256) {
+  const int mine = part == 0 ? t : KF;   // one workgroup writes them
+  for (int i = mine; i < KF / 8; i += 256) {
     const int l = i & 63, w = i >> 6 & 3, rb = i >> 8;
     const int r = rb * 16 + (l & 15), c = w * RT * 16 + (l >> 4) * 4;
 #pragma unroll
@@ -411,7 +424,7 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
       *reinterpret_cast<b8*>(a.Qf + (atk * N + k) * KF + i * 8) = __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  for (int i = t; i < DK * C / 8; i += 256) {
+  for (int i = mine; i < DK * C / 8; i += 256) {
     const int l = i & 63, ks = i >> 6 & 1, rb = i >> 7;
     const int c = rb * 16 + (l & 15), r = ks * 32 + (l >> 4) * 8;
 #pragma unroll
@@ -445,13 +458,13 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
       pp[j] = planes_mma<N, N, 3>(y, z, pp[j]);
     }
   }
-  for (int m = 0; m < a.group; ++m) {
+  for (int m = first; m < last; ++m) {
     const int hv = hk * a.group + m;
     int tt = threadIdx.x;
     asm volatile("" : "+v"(tt));   // opaque: addresses of all matrices held over the loop are spilled
     const int t = tt, lane = t & 63, r4 = (lane >> 4) * 4, col = lane & 15;
     const long at = (long)slot * a.d.value_heads + hv;
-    if (m > 0 && wave == 0) factors(hv);
+    if (m > first && wave == 0) factors(hv);
     __syncthreads();
     f4 nd[4];   // N
 #pragma unroll
@@ -462,7 +475,7 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = wave * 16 + r4 + e;
-          const float D = r >= c ? decay(G[r] - G[c]) : 0.f;
+          const float D = r >= c ? decay(G[r], G[c]) : 0.f;
           nd[j][e] = r > c ? nn[j][e] * D : 0.f;
           A[r * PC + c] = nd[j][e] * beta[c];
           M[r * PC + c] = r >= c ? pp[j][e] * D : 0.f;
@@ -486,10 +499,12 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
       __syncthreads();
       f4 t2[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        t2[j] = f4{0, 0, 0, 0};
-        if (j <= wave) t2[j] = mm(M + wave * 16 * PC + j * 16, PC, A + j * 16 * PC + j * 16, PC, (wave + 1 - j) * 16, t2[j]);
-      }
+      for (int j = 0; j < 4; ++j) t2[j] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int l = 0; l < 4; ++l)   // N's block rows, each for up to four sums side by side
+        if (l <= wave)
+#pragma unroll
+          for (int j = 0; j <= l; ++j) t2[j] = mm(M + wave * 16 * PC + l * 16, PC, A + l * 16 * PC + j * 16, PC, 16, t2[j]);
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -960,13 +975,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   __bf16* X = Y + N * SL;                        // 3
   __bf16* U = X + 3 * SL;                        // 3
   __bf16* M = reinterpret_cast<__bf16*>(smem);   // later: a C x C matrix, 3 planes
-  double* G = reinterpret_cast<double*>(smem + grads_room<T>());
+  f2* G = reinterpret_cast<f2*>(smem + grads_room<T>());
   float* dG = reinterpret_cast<float*>(G + C);   // 8 x C: per wave
   float* ef = dG + 8 * C;       // exp(G), exp(G_C - G): C each
   float* red = ef + 2 * C;      // 8
   float* db = red + 8;          // C
   constexpr bool TILES = !(GROUPED && sizeof(T) == 4);   // K and Q in LDS, where they fit
-  constexpr int PK = DK + 16 / sizeof(T);
+  constexpr int PV = 16 / sizeof(T), PK = DK + PV;
   T* Kt = reinterpret_cast<T*>(db + C);
   T* Qt = Kt + (TILES ? C * PK : 0);
   f4* sums = reinterpret_cast<f4*>(Qt + (TILES ? C * PK : 0));   // GROUPED: dQ and dK over the value heads so far, 8 per thread
@@ -980,6 +995,8 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   // 4 values of dO and of d_v at a time
   const long dmask = a.do_st.bs | a.do_st.rs | a.do_st.cs;
   const bool wide = (a.d.dv & 3) == 0 && (dmask & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.d_o) | reinterpret_cast<uintptr_t>(a.d_v)) & 15) == 0;
+  // rows of d_q and d_k 16 bytes at a time
+  const bool whole = TILES && a.d.dk == DK && ((reinterpret_cast<uintptr_t>(a.d_q) | reinterpret_cast<uintptr_t>(a.d_k)) & 15) == 0;
   const int group = GROUPED ? a.group : 1;
   if (TILES) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs;
@@ -1188,7 +1205,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
             for (int e = 0; e < 4; ++e) {
               const int r = rb * 16 + r4 + e;
               if (w == 0) {
-                D[h][e] = r >= c ? decay(G[r] - G[c]) : 0.f;
+                D[h][e] = r >= c ? decay(G[r], G[c]) : 0.f;
                 dp[h][e] *= a.scale * D[h][e];
               } else {
                 da[h][e] = r > c ? -da[h][e] * D[h][e] : 0.f;
@@ -1247,14 +1264,19 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
           q1[rb] += sums[rb * 512 + t];
           kr[rb] += sums[(4 + rb) * 512 + t];
         }
-        sums[rb * 512 + t] = q1[rb];
-        sums[(4 + rb) * 512 + t] = kr[rb];
+        if (m + 1 < group) {
+          sums[rb * 512 + t] = q1[rb];
+          sums[(4 + rb) * 512 + t] = kr[rb];
+        }
       }
       if (m + 1 == group && own && kc0 < a.d.dk) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = rb * 16 + r4 + e;
-          if (r < len) {
+          if (whole) {   // in place of Q and K, which this lane alone has read here
+            Qt[r * PK + kc0] = (T)q1[rb][e];
+            Kt[r * PK + kc0] = (T)kr[rb][e];
+          } else if (r < len) {
             const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + kc0;
             st<T>(a.d_q, p, q1[rb][e]);
             st<T>(a.d_k, p, kr[rb][e]);
@@ -1263,6 +1285,17 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
       }
     }
     __syncthreads();
+    if (whole && m + 1 == group) {
+      const long p = ((row * a.d.tokens + t0) * a.d.key_heads + hk) * (long)DK;
+      const unsigned pitch = (unsigned)a.d.key_heads * DK;
+#pragma unroll
+      for (int i = t; i < C * DK / PV; i += 512) {
+        const int r = i / (DK / PV), c = i % (DK / PV) * PV;
+        if (r >= len) continue;
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.d_q) + p + r * pitch + c) = *reinterpret_cast<const uint4*>(Qt + r * PK + c);
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.d_k) + p + r * pitch + c) = *reinterpret_cast<const uint4*>(Kt + r * PK + c);
+      }
+    }
     if (wave == 0) {
       float v = 0.f;
       for (int i = 0; i < 8; ++i) v += dG[i * C + lane] + (lane == C - 1 ? red[i] : 0.f);
@@ -1513,6 +1546,7 @@ Args make_args(const gpx_delta* d) {
   Args a = {};
   a.d = *d;
   a.group = d->value_heads / d->key_heads;
+  a.parts = slots_of(d) * d->value_heads <= 512 ? a.group : 1;
   a.dvp = (d->dv + DVT - 1) / DVT * DVT;
   a.scale = (float)d->scale;
   a.p.sequences = sequences_of(d);
@@ -1560,7 +1594,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
   DELTA_TRY(allow_lds<&delta_chunk_kernel<T, DK>>(lds));
   const long slots = slots_of(&a.d);
   if (slots > 0) {
-    hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads)), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads * a.parts)), dim3(256), lds, s, a);
     GPX_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL((delta_chain_kernel<T, DK, false>), dim3(chain_grid(a)), dim3(512), 0, s, a);
