@@ -63,11 +63,16 @@ struct Plan {
     if (len < 0 || slot < slot0(s)) len = 0;   // behind the sequence's last chunk, or before the first sequence
   }
   __device__ __forceinline__ long row(int s) const { return off ? 0 : s; }   // batch row
+  __device__ __forceinline__ int by_length(int i) const { return off ? off[sequences + 1 + i] : i; }   // the i-th sequence to start
 };
 
-// offsets made non-decreasing and inside [0, tokens]: every later kernel's accesses follow from these
+// One wave.  out: the offsets made non-decreasing and inside [0, tokens] (every later kernel's accesses follow from these), then
+// the sequences, the longest first, as the scans start them: their workgroups outnumber the compute units, and one long
+// sequence started last is waited for alone.  Lengths within a quarter of a power of two count as equal.
 __global__ void delta_plan_kernel(const int* in, int n, int tokens, int* out) {
-  const int lane = threadIdx.x;
+  __shared__ int start[128];
+  const int lane = threadIdx.x, sequences = n - 1;
+  start[lane] = start[lane + 64] = 0;
   int carry = 0;
   for (int base = 0; base < n; base += 64) {
     const int i = base + lane;
@@ -80,6 +85,26 @@ __global__ void delta_plan_kernel(const int* in, int n, int tokens, int* out) {
     carry = __shfl(v, 63);
     if (i < n) out[i] = v;
   }
+  __syncthreads();
+  auto rank = [&](int i) {   // 0: the longest; a length of 2^30 has 16 M chunks
+    const unsigned len = (unsigned)(out[i + 1] - out[i]), chunks = len / C + (len % C != 0), w = chunks * 4 + 3;
+    const int e = 31 - __clz(w);   // 1 (no chunk) to 26
+    return 127 - (e * 4 + (int)(w >> (e - 1) & 1) * 2 + (e > 1 ? (int)(w >> (e - 2) & 1) : 0));
+  };
+  for (int i = lane; i < sequences; i += 64) atomicAdd(&start[rank(i)], 1);
+  __syncthreads();
+  const int a = start[2 * lane], b = start[2 * lane + 1];
+  int before = a + b;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(before, o);
+    if (lane >= o) before += u;
+  }
+  before -= a + b;
+  __syncthreads();
+  start[2 * lane] = before;
+  start[2 * lane + 1] = before + a;
+  __syncthreads();
+  for (int i = lane; i < sequences; i += 64) out[n + atomicAdd(&start[rank(i)], 1)] = i;
 }
 
 typedef float f2 __attribute__((ext_vector_type(2)));
@@ -552,7 +577,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / 16;
   int slice, head;
   if (!scan_coords(blockIdx.x, slices, heads, slice, head)) return;
-  const int s = head / a.d.value_heads, hv = head % a.d.value_heads, hk = hv / a.group;
+  const int s = a.p.by_length(head / a.d.value_heads), hv = head % a.d.value_heads, hk = hv / a.group;
   const int c0 = slice * 16;
   const int t = threadIdx.x, lane = t & 63, wave8 = __builtin_amdgcn_readfirstlane(t >> 6), wave = wave8 & 3, r4 = (lane >> 4) * 4,
             col = lane & 15, g8 = (lane >> 4) * 8;
@@ -569,7 +594,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + col;
-        S[i][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[((long)head * a.d.dk + r) * a.d.dv + c] : 0.f;
+        S[i][e] = init != nullptr && r < a.d.dk && c < a.d.dv ? init[(((long)s * a.d.value_heads + hv) * a.d.dk + r) * a.d.dv + c] : 0.f;
       }
     b8 kf[4][N], tf[2][3], kt[RT][2][N];
     T v[4];
@@ -733,7 +758,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = (wave * RT + i) * 16 + r4 + e, c = c0 + col;
-          if (r < a.d.dk && c < a.d.dv) out[((long)head * a.d.dk + r) * a.d.dv + c] = S[i][e];
+          if (r < a.d.dk && c < a.d.dv) out[(((long)s * a.d.value_heads + hv) * a.d.dk + r) * a.d.dv + c] = S[i][e];
         }
     }
   } else {
@@ -1489,7 +1514,7 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
   };
   if ((use == WORK || use == SAVED) && d->sequences > 0) {
     int* p;
-    part(p, (size_t)(d->sequences + 1) * 4);
+    part(p, (size_t)(2 * d->sequences + 1) * 4);
     if (off != nullptr) *off = p;
   }
   if (use == WORK && recurrent(d, 0)) return at;

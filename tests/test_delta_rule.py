@@ -224,6 +224,17 @@ def test_short_ragged():
 
 
 @pytest.mark.gpu
+def test_many_sequences():
+    """More sequences than one wave's lanes, most of them short or empty, a few long ones last."""
+    rng = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 12, (150,), generator=rng).tolist() + [300, 65, 500]
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    both(inputs(1, offsets[-1], 1, 2, 32, 24, "f32", seqs=len(lens), seed=9), "f32", offsets)
+
+
+@pytest.mark.gpu
 def test_bad_offsets_stay_inside():
     """Values outside the tokens are clamped, decreasing ones read as the one before."""
     from gaussian_process_amd import gated_delta_rule, gated_delta_rule_backward
