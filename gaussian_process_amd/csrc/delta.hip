@@ -564,8 +564,8 @@ __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes
   return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
 }
 
-template <typename T, int DK, bool BACK>
-__global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
+template <typename T, int DK, bool BACK, bool TWO>
+__global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Args a) {
   constexpr int N = Planes<T>::N, NO = OutPlanes<T>::N, RT = DK / 64, PT = C + 8, PE = C + 4;
   __shared__ f4 part[4][4][64];                  // K S: wave, row block
   constexpr int NS = BACK ? 0 : NO;
@@ -764,9 +764,10 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
   } else {
     // ---- beside the chain, one chunk behind it: the work on chunk n - 1 is spread over the three stretches of chunk n, the longest
     // first, so that no barrier waits for it.  Backward, Rx is that of chunk n itself.
-    // Two sets of fragments, two chunks ahead: what a wave loads waits for what it stored before.
-    b8 qf[2][4][N], pf[2][2][NO], qt[2][RT][2][N], of[2][2][N];
-    f4 eg[2], bt[2][4], o;   // BACK: bt holds exp(G)
+    // Fragments a chunk ahead; forward, where registers allow it, two sets and two chunks (8192 tokens: 237 us for 248).
+    constexpr int SETS = BACK || TWO ? 1 : 2;
+    b8 qf[SETS][4][N], pf[SETS][2][NO], qt[SETS][RT][2][N], of[SETS][2][N];
+    f4 eg[SETS], bt[SETS][4], o;   // BACK: bt holds exp(G)
     // S, E and Z go to memory 4 columns of one row per lane: whole 64-byte pieces
     const int srow = lane >> 2, sc = (lane & 3) * 4;
     auto order = [&](int n) { return BACK ? chunks - 1 - n : n; };
@@ -847,7 +848,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
       if (!BACK) {
         q_part(u, n, 3);
         o *= eg[u];
-        load_q(u, n + 2);
+        load_q(u, n + SETS);
       }
     };
     auto third = [&](int u, int n) {
@@ -867,7 +868,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
         split<8, NO>(x, ub);
         o = planes_mma<NO, NO, NO>(pf[u][ks], ub, o);
       }
-      load_p(u, n + 2);
+      load_p(u, n + SETS);
       const int tok = begin + n * C + wave * 16 + r4;
       T* out = reinterpret_cast<T*>(a.o) + ((row * a.d.tokens + tok) * a.d.value_heads + hv) * (long)a.d.dv + c0 + col;
       if (c0 + col < a.d.dv)
@@ -877,7 +878,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
     };
     // u: the set of chunk n
     auto chunk = [&](int u, int n) {
-      if (n > 0) first(1 - u, n - 1);
+      if (n > 0) first(SETS - 1 - u, n - 1);
       f4 r[RT];
       if (BACK) {
 #pragma unroll
@@ -902,33 +903,33 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(const Args a) {
       if (BACK) {   // the chain has read the Rx of the chunk before
 #pragma unroll
         for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];
-        load_q(u, n + 2);
+        load_q(u, n + SETS);
       }
-      if (n > 0) second(1 - u, n - 1);
+      if (n > 0) second(SETS - 1 - u, n - 1);
       lds_barrier();
-      if (n > 0) third(1 - u, n - 1);
+      if (n > 0) third(SETS - 1 - u, n - 1);
       lds_barrier();
     };
     if (chunks > 0) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < SETS; ++u) {
         load_q(u, u);
         if (!BACK) load_p(u, u);
       }
-      for (int n = 0; n < chunks; n += 2) {
+      for (int n = 0; n < chunks; n += SETS) {
         chunk(0, n);
-        if (n + 1 < chunks) chunk(1, n + 1);
+        if (SETS == 2 && n + 1 < chunks) chunk(SETS - 1, n + 1);
       }
+      auto rest = [&](int u, int n) {
+        first(u, n);
+        second(u, n);
+        third(u, n);
+      };
       const int n = chunks - 1;
-      if (n & 1) {
-        first(1, n);
-        second(1, n);
-        third(1, n);
-      } else {
-        first(0, n);
-        second(0, n);
-        third(0, n);
-      }
+      if (SETS == 2 && (n & 1))
+        rest(SETS - 1, n);
+      else
+        rest(0, n);
       flush(n);
     }
   }
@@ -1605,6 +1606,23 @@ unsigned chain_grid(const Args& a) {
   return (heads + 7) / 8 * 8 * (a.dvp / 16);
 }
 
+// More workgroups than compute units: two at a time on each, in 128 registers a wave, which only bf16 has next to no spills in
+// (512 workgroups, training: 201 -> 176 us, 1024, forward: 143 -> 117; 256 of them: 200 -> 205)
+template <typename T, int DK, bool BACK>
+int run_chain(hipStream_t s, const Args& a) {
+  const unsigned grid = chain_grid(a);
+  if constexpr (Planes<T>::N == 1) {
+    if (grid > 256) {
+      hipLaunchKernelGGL((delta_chain_kernel<T, DK, BACK, true>), dim3(grid), dim3(512), 0, s, a);
+      GPX_HIP(hipGetLastError());
+      return 0;
+    }
+  }
+  hipLaunchKernelGGL((delta_chain_kernel<T, DK, BACK, false>), dim3(grid), dim3(512), 0, s, a);
+  GPX_HIP(hipGetLastError());
+  return 0;
+}
+
 template <typename T, int DK>
 int run_forward(hipStream_t s, const Args& a, int rec) {
   if (rec) {
@@ -1622,9 +1640,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
     hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads * a.parts)), dim3(256), lds, s, a);
     GPX_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL((delta_chain_kernel<T, DK, false>), dim3(chain_grid(a)), dim3(512), 0, s, a);
-  GPX_HIP(hipGetLastError());
-  return 0;
+  return run_chain<T, DK, false>(s, a);
 }
 
 template <typename T, int DK>
@@ -1639,8 +1655,7 @@ int run_backward(hipStream_t s, const Args& a) {
     hipLaunchKernelGGL((delta_back_prep_kernel<T>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
     GPX_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL((delta_chain_kernel<T, DK, true>), dim3(chain_grid(a)), dim3(512), 0, s, a);
-  GPX_HIP(hipGetLastError());
+  DELTA_TRY((run_chain<T, DK, true>(s, a)));
   if (slots > 0) {
     const dim3 grid((unsigned)(slots * a.d.key_heads));
     if (a.group == 1)

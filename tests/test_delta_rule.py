@@ -224,6 +224,12 @@ def test_short_ragged():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(128, 128), (40, 100)])
+def test_more_workgroups_than_compute_units(dk, dv):
+    both(inputs(3, 150, 7, 14, dk, dv, "bf16", seed=dk), "bf16")
+
+
+@pytest.mark.gpu
 def test_many_sequences():
     """More sequences than one wave's lanes, most of them short or empty, a few long ones last."""
     rng = torch.Generator().manual_seed(3)
