@@ -122,8 +122,6 @@ struct Args {
   __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
   float *Erow, *Srow;           // per head: E, dvp / 32 x C x 32; S, dvp / 32 x DK x 32
-  float* Y;                     // per head: (scale P^T dO)^T, dvp x C
-  __bf16* Of;                   // per head: dO as fragments, dvp / 16 x 2 x 64 x 8
   float *Z, *dS;                // per head: Z (dX = beta Z) like E; dS' like S
   const float *state, *d_state_out;
   float *state_out, *d_state, *d_g, *d_beta;
@@ -551,7 +549,7 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
 // ---- the scans: 16 columns of dv of one value head of one sequence ----------------------------------------------------------------
 // Forward, chunk after chunk:    X = V - exp(G) K S;       E = T X;      S <- exp(G_C) S + K^T (exp(G_C - G) beta E)
 // Backward (BACK), from the last: X = Y + exp(G_C - G) K dS;  Z = T2^T X;   dS <- exp(G_C) dS - K^T (exp(G) beta Z) + Q^T Of
-// (Y = scale P^T dO from delta_back_prep_kernel, Of = scale exp(G) dO).
+// (Y = scale P^T dO, Of = scale exp(G) dO).
 // Bound by the chain from chunk to chunk: the product with K (each wave with its own rows of S, which are in its accumulators;
 // partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.  Four waves do that
 // and nothing else; four more take S and E from LDS and do what the chain does not wait for -- forward the outputs
@@ -571,7 +569,10 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
   constexpr int NS = BACK ? 0 : NO;
   __shared__ b8 Sp[2][4][NS + 1][64];            // planes of S for the outputs: parity of the chunk, wave
   __shared__ f4 Sx[2][4][2][64];                 // S to be stored: parity, wave, tile
+  constexpr int NB = BACK ? 1 : 0;
   __shared__ f4 Rx[4][2][64];                    // BACK: Q^T Of, likewise
+  __shared__ __align__(16) float Yx[NB + 1][16][PE];       // BACK: Y^T, parity
+  __shared__ __align__(16) __bf16 Ox[N][16][PT];           // BACK: dO^T
   __shared__ __align__(16) float Ex[2][16][PE];  // E^T or Z^T, parity of the chunk
   __shared__ __align__(16) __bf16 X[3][16][PT], U[3][16][PT];
   const int heads = a.p.sequences * a.d.value_heads, slices = a.dvp / 16;
@@ -598,7 +599,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       }
     b8 kf[4][N], tf[2][3], kt[RT][2][N];
     T v[4];
-    f4 y, fx, fu;
+    f4 fx, fu;
     float keep;
     const T* V = reinterpret_cast<const T*>(a.d.v) + row * a.d.v_st.bs + begin * a.d.v_st.rs + hv * a.d.v_st.cs;
     const unsigned vrs = (unsigned)a.d.v_st.rs, vcol = min(c0 + col, a.d.dv - 1);
@@ -610,9 +611,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
         for (int k = 0; k < N; ++k) kf[i][k] = ld_frag(p + k * KF + i * 4 * 512, lb);
     };
     auto load_x = [&](long at, int m) {
-      if (BACK) {
-        y = *reinterpret_cast<const f4*>(a.Y + (at * a.dvp + c0) * C + (unsigned)(col * C + wave * 16 + r4));
-      } else {   // rows and columns behind the end repeat the last; they are masked where they are used
+      if (!BACK) {   // rows and columns behind the end repeat the last; they are masked where they are used
         const T* p = V + (long)m * C * a.d.v_st.rs;
         const unsigned last = min(C, end - begin - m * C) - 1;
 #pragma unroll
@@ -680,6 +679,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       lds_barrier();
       {
         const f4 p0 = part[0][wave][lane], p1 = part[1][wave][lane], p2 = part[2][wave][lane], p3 = part[3][wave][lane];
+        const f4 y = BACK ? *reinterpret_cast<const f4*>(&Yx[n & NB][col][wave * 16 + r4]) : f4{0, 0, 0, 0};
         __builtin_amdgcn_sched_barrier(0);
         load_k(nslot);
         __builtin_amdgcn_sched_barrier(0);
@@ -749,6 +749,10 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       load_k(slot);
       load_x(at, m);
       load_t(at);
+      if (BACK) {   // the other waves' start
+        lds_barrier();
+        lds_barrier();
+      }
     }
     for (int n = 0; n < chunks; ++n) chunk(n);
     float* out = BACK ? a.d_state : a.state_out;
@@ -761,40 +765,136 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
           if (r < a.d.dk && c < a.d.dv) out[(((long)s * a.d.value_heads + hv) * a.d.dk + r) * a.d.dv + c] = S[i][e];
         }
     }
+  } else if constexpr (BACK) {
+    // ---- beside the chain: Q^T Of of this chunk, Y of the next, all stores
+    b8 qt[RT][2][N], of[2][N], pt[2][3];
+    f4 eg[4];
+    T d[4];
+    const int srow = lane >> 2, sc = (lane & 3) * 4;   // S, Z: 4 columns of one row per lane, whole 64-byte pieces
+    auto slot_of = [&](int n) { return slot0 + chunks - 1 - min(n, chunks - 1); };
+    auto load_q = [&](int n) {
+      const long slot = slot_of(n), at = slot * a.d.value_heads + hv;
+      const __bf16* p = a.QTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int k = 0; k < N; ++k) qt[i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
+      const float* f = a.fac + at * FACS + g8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) eg[i] = *reinterpret_cast<const f4*>(f + (i >> 1) * 32 + (i & 1) * 4);
+    };
+    auto load_p = [&](int n) {   // P^T is upper triangular, its zeros are not there
+      const __bf16* p = a.PTf + (slot_of(n) * a.d.value_heads + hv) * 3 * TF + wave * 2 * 512;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        pt[0][k] = ld_frag(p + k * TF + (wave < 2 ? 0 : 512), lb);
+        pt[1][k] = ld_frag(p + k * TF + 512, lb);
+      }
+    };
+    const T* dO = reinterpret_cast<const T*>(a.d_o) + row * a.do_st.bs + hv * a.do_st.cs + min(c0 + col, a.d.dv - 1);
+    auto load_o = [&](int n) {
+      const int tok = begin + (chunks - 1 - min(n, chunks - 1)) * C + wave * 16 + r4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[e] = dO[min(tok + e, end - 1) * a.do_st.rs];
+    };
+    auto put_o = [&](int n) {   // what load_o(n) brought
+      const int live = end - begin - (chunks - 1 - min(n, chunks - 1)) * C - wave * 16 - r4;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = e < live && c0 + col < a.d.dv ? (float)d[e] : 0.f;
+      b4 xp[N];
+      split<4, N>(x, xp);
+#pragma unroll
+      for (int k = 0; k < N; ++k) *reinterpret_cast<b4*>(&Ox[k][col][wave * 16 + r4]) = xp[k];
+    };
+    auto product_y = [&](int n) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int k = 0; k < N; ++k) of[ks][k] = *reinterpret_cast<const b8*>(&Ox[k][col][ks * 32 + g8]);
+      f4 y = {0, 0, 0, 0};
+      if (wave < 2) y = planes_mma<3, N, 3>(pt[0], of[0], y);
+      y = planes_mma<3, N, 3>(pt[1], of[1], y);
+      *reinterpret_cast<f4*>(&Yx[n & NB][col][wave * 16 + r4]) = y * a.scale;
+    };
+    auto place = [&](float* base, int n, int rows) {
+      return base + (slot_of(n) * a.d.value_heads + hv) * (long)(rows * a.dvp) + (c0 / DVT) * (rows * DVT) + c0 % DVT;
+    };
+    auto store_z = [&](int n) {
+      f4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
+      *reinterpret_cast<f4*>(place(a.Z, n, C) + (unsigned)((wave * 16 + srow) * DVT + sc)) = v;
+    };
+    auto chunk = [&](int n) {
+      f4 r[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) r[i] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = 0.f;
+#pragma unroll
+          for (int k = 0; k < N; ++k) v += (float)of[ks][k][e];
+          x[e] = a.scale * eg[ks * 2 + (e >> 2)][e & 3] * v;
+        }
+        b8 ob[3];
+        split<8, 3>(x, ob);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[i][ks], ob, r[i]);
+      }
+      put_o(n + 1);
+      load_o(n + 2);
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];   // the chain has read those of the chunk before
+      load_q(n + 1);
+      product_y(n + 1);
+      load_p(n + 2);
+      lds_barrier();
+      if (n > 0) store_z(n - 1);
+      float* dst = place(a.dS, n, DK) + wave * RT * 16 * DVT;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
+        *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * DVT + sc)) = f4{p[0], p[4], p[8], p[12]};
+      }
+      lds_barrier();
+    };
+    if (chunks > 0) {
+      load_o(0);
+      load_q(0);
+      load_p(0);
+      put_o(0);
+      load_o(1);
+      lds_barrier();
+      product_y(0);
+      load_p(1);
+      lds_barrier();
+      for (int n = 0; n < chunks; ++n) chunk(n);
+      store_z(chunks - 1);
+    }
   } else {
     // ---- beside the chain, one chunk behind it: the work on chunk n - 1 is spread over the three stretches of chunk n, the longest
-    // first, so that no barrier waits for it.  Backward, Rx is that of chunk n itself.
-    // Fragments a chunk ahead; forward, where registers allow it, two sets and two chunks (8192 tokens: 237 us for 248).
-    constexpr int SETS = BACK || TWO ? 1 : 2;
-    b8 qf[SETS][4][N], pf[SETS][2][NO], qt[SETS][RT][2][N], of[SETS][2][N];
-    f4 eg[SETS], bt[SETS][4], o;   // BACK: bt holds exp(G)
-    // S, E and Z go to memory 4 columns of one row per lane: whole 64-byte pieces
+    // first, so that no barrier waits for it.
+    // Fragments a chunk ahead; where registers allow it, two sets and two chunks (8192 tokens: 237 us for 248).
+    constexpr int SETS = TWO ? 1 : 2;
+    b8 qf[SETS][4][N], pf[SETS][2][NO];
+    f4 eg[SETS], bt[SETS][4], o;
+    // S and E go to memory 4 columns of one row per lane: whole 64-byte pieces
     const int srow = lane >> 2, sc = (lane & 3) * 4;
-    auto order = [&](int n) { return BACK ? chunks - 1 - n : n; };
     auto load_q = [&](int u, int n) {
-      const long slot = slot0 + order(min(n, chunks - 1)), at = slot * a.d.value_heads + hv;
-      if (BACK) {
-        const __bf16* p = a.QTf + (slot * a.d.key_heads + hk) * N * (DK * C) + wave * RT * 2 * 512;
+      const long slot = slot0 + min(n, chunks - 1), at = slot * a.d.value_heads + hv;
+      const __bf16* q = a.Qf + (slot * a.d.key_heads + hk) * N * KF + wave * 4 * 512;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int k = 0; k < N; ++k) qt[u][i][ks][k] = ld_frag(p + k * (DK * C) + (i * 2 + ks) * 512, lb);
-#pragma unroll
-          for (int k = 0; k < N; ++k) of[u][ks][k] = ld_frag(a.Of + (at * N + k) * (a.dvp * C) + slice * 1024 + ks * 512, lb);
-        }
-        const float* f = a.fac + at * FACS + g8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bt[u][i] = *reinterpret_cast<const f4*>(f + (i >> 1) * 32 + (i & 1) * 4);
-      } else {
-        const __bf16* q = a.Qf + (slot * a.d.key_heads + hk) * N * KF + wave * 4 * 512;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int k = 0; k < N; ++k) qf[u][i][k] = ld_frag(q + k * KF + i * 512, lb);
-        eg[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + wave * 16 + r4);
-      }
+        for (int k = 0; k < N; ++k) qf[u][i][k] = ld_frag(q + k * KF + i * 512, lb);
+      eg[u] = *reinterpret_cast<const f4*>(a.fac + at * FACS + wave * 16 + r4);
     };
     auto load_p = [&](int u, int n) {
       const long at = (slot0 + min(n, chunks - 1)) * a.d.value_heads + hv;
@@ -815,10 +915,10 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       for (int k = 0; k < NS; ++k) sb[k] = Sp[n & 1][w][k][lane];
       o = planes_mma<N, NO, N == 2 ? 3 : NO>(qf[u][w], sb, o);
     };
-    // E or Z of chunk n
+    // E of chunk n
     auto flush = [&](int n) {
-      if (BACK || a.save) {
-        float* dst = (BACK ? a.Z : a.Erow) + ((slot0 + order(n)) * a.d.value_heads + hv) * (long)(C * a.dvp) + (c0 / DVT) * (C * DVT) +
+      if (a.save) {
+        float* dst = a.Erow + ((slot0 + n) * a.d.value_heads + hv) * (long)(C * a.dvp) + (c0 / DVT) * (C * DVT) +
                      wave * 16 * DVT + c0 % DVT;
         f4 v;
 #pragma unroll
@@ -828,14 +928,12 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
     };
     auto first = [&](int u, int n) {
       if (n > 0) flush(n - 1);
-      if (!BACK) {
-        o = f4{0, 0, 0, 0};
-        q_part(u, n, 0);
-        q_part(u, n, 1);
-        q_part(u, n, 2);
-      }
-      if (BACK || a.save) {
-        float* dst = (BACK ? a.dS : a.Srow) + ((slot0 + order(n)) * a.d.value_heads + hv) * (long)(DK * a.dvp) +
+      o = f4{0, 0, 0, 0};
+      q_part(u, n, 0);
+      q_part(u, n, 1);
+      q_part(u, n, 2);
+      if (a.save) {
+        float* dst = a.Srow + ((slot0 + n) * a.d.value_heads + hv) * (long)(DK * a.dvp) +
                      (c0 / DVT) * (DK * DVT) + wave * RT * 16 * DVT + c0 % DVT;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -845,14 +943,11 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       }
     };
     auto second = [&](int u, int n) {
-      if (!BACK) {
-        q_part(u, n, 3);
-        o *= eg[u];
-        load_q(u, n + SETS);
-      }
+      q_part(u, n, 3);
+      o *= eg[u];
+      load_q(u, n + SETS);
     };
     auto third = [&](int u, int n) {
-      if (BACK) return;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         if (ks * 2 > wave) continue;   // P is lower triangular
@@ -879,32 +974,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
     // u: the set of chunk n
     auto chunk = [&](int u, int n) {
       if (n > 0) first(SETS - 1 - u, n - 1);
-      f4 r[RT];
-      if (BACK) {
-#pragma unroll
-        for (int i = 0; i < RT; ++i) r[i] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float v = 0.f;
-#pragma unroll
-            for (int k = 0; k < N; ++k) v += (float)of[u][ks][k][e];
-            x[e] = a.scale * bt[u][ks * 2 + (e >> 2)][e & 3] * v;
-          }
-          b8 ob[3];
-          split<8, 3>(x, ob);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) r[i] = planes_mma<N, 3, 3>(qt[u][i][ks], ob, r[i]);
-        }
-      }
       lds_barrier();
-      if (BACK) {   // the chain has read the Rx of the chunk before
-#pragma unroll
-        for (int i = 0; i < RT; ++i) Rx[wave][i][lane] = r[i];
-        load_q(u, n + SETS);
-      }
       if (n > 0) second(SETS - 1 - u, n - 1);
       lds_barrier();
       if (n > 0) third(SETS - 1 - u, n - 1);
@@ -914,7 +984,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 #pragma unroll
       for (int u = 0; u < SETS; ++u) {
         load_q(u, u);
-        if (!BACK) load_p(u, u);
+        load_p(u, u);
       }
       for (int n = 0; n < chunks; n += SETS) {
         chunk(0, n);
@@ -932,52 +1002,6 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
         rest(0, n);
       flush(n);
     }
-  }
-}
-
-// ---- backward, before the scan: Y and Of, a wave for each 16 columns of dv ----------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void delta_back_prep_kernel(const Args a) {
-  constexpr int N = Planes<T>::N;
-  const int groups = (a.dvp + 63) / 64;
-  const int cg = blockIdx.x % groups;
-  const long at = blockIdx.x / groups;
-  const int hv = (int)(at % a.d.value_heads), slot = (int)(at / a.d.value_heads);
-  int s, t0, len;
-  a.p.locate(slot, s, t0, len);
-  if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
-  const int ct = cg * 4 + wave;
-  if (ct * 16 >= a.dvp) return;
-  const int c = ct * 16 + col;
-  const T* dO = reinterpret_cast<const T*>(a.d_o) + a.p.row(s) * a.do_st.bs + t0 * a.do_st.rs + hv * a.do_st.cs + min(c, a.d.dv - 1);
-  b8 ob[2][N];
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    T raw[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) raw[e] = dO[min(ks * 32 + g8 + e, len - 1) * a.do_st.rs];
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = ks * 32 + g8 + e < len && c < a.d.dv ? (float)raw[e] : 0.f;
-    split<8, N>(x, ob[ks]);
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      *reinterpret_cast<b8*>(a.Of + (at * N + k) * (a.dvp * C) + ct * 1024 + ks * 512 + lane * 8) = ob[ks][k];
-  }
-  const __bf16* pt = a.PTf + at * 3 * TF + lane * 8;
-#pragma unroll
-  for (int rb = 0; rb < 4; ++rb) {
-    f4 y = {0, 0, 0, 0};
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks * 2 + 1 < rb) continue;   // P^T is upper triangular
-      b8 p[3];
-#pragma unroll
-      for (int k = 0; k < 3; ++k) p[k] = *reinterpret_cast<const b8*>(pt + k * TF + (rb * 2 + ks) * 512);
-      y = planes_mma<3, N, 3>(p, ob[ks], y);
-    }
-    *reinterpret_cast<f4*>(a.Y + (at * a.dvp + c) * C + rb * 16 + r4) = y * a.scale;
   }
 }
 
@@ -1538,8 +1562,6 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
     part(x.Pf, heads * no * TF * 2);
   }
   if (use == SCRATCH) {
-    part(x.Y, heads * C * dvp * 4);
-    part(x.Of, heads * n * C * dvp * 2);
     part(x.Z, heads * C * dvp * 4);
     part(x.dS, heads * dkp * dvp * 4);
   }
@@ -1651,10 +1673,6 @@ int run_backward(hipStream_t s, const Args& a) {
   DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, false>>(lds));
   DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, true>>(grouped));
   const long slots = slots_of(&a.d);
-  if (slots > 0) {
-    hipLaunchKernelGGL((delta_back_prep_kernel<T>), dim3((unsigned)(slots * a.d.value_heads * ((a.dvp + 63) / 64))), dim3(256), 0, s, a);
-    GPX_HIP(hipGetLastError());
-  }
   DELTA_TRY((run_chain<T, DK, true>(s, a)));
   if (slots > 0) {
     const dim3 grid((unsigned)(slots * a.d.key_heads));
