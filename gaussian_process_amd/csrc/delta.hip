@@ -6,11 +6,11 @@
 //   X = V - diag(exp G) K S;   E = T X with T = (I + N diag(beta))^-1;   U = diag(beta) E
 //   O = scale (diag(exp G) Q S + P U);   S' = exp(G_C) S + K^T diag(exp(G_C - G)) U
 // (in terms of the errors E instead of beta E, so that beta = 0 divides nothing).  Backward, given dO and dS':
-//   dU = scale P^T dO + diag(exp(G_C - G)) K dS';   dX = T^T diag(beta) dU;   dV = dX;   dA = -dX E^T
+//   dU = scale P^T dO + diag(exp(G_C - G)) K dS';   Z = (I + diag(beta) N)^-T dU;   dV = dX = diag(beta) Z
 //   dS = exp(G_C) dS' + scale Q^T diag(exp G) dO - K^T diag(exp G) dX
-//   dP = scale dO U^T;   dQ = scale diag(exp G) dO S^T + (dP o D) K;   dbeta_j = E_j . dU_j + sum_i dA_ij N_ij
-//   dK = dKr + dKc:  dKr = (dA diag(beta) o D) K - diag(exp G) dX S^T        (the key that reads: row of N, of K S)
-//                    dKc = (dA diag(beta) o D)^T K + (dP o D)^T Q + diag(exp(G_C - G)) U dS'^T   (the key that writes)
+//   dP = scale dO U^T;   dN = -dX U^T;   dQ = scale diag(exp G) dO S^T + (dP o D) K;   dbeta_j = E_j . Z_j
+//   dK = dKr + dKc:  dKr = (dN o D) K - diag(exp G) dX S^T        (the key that reads: row of N, of K S)
+//                    dKc = (dN o D)^T K + (dP o D)^T Q + diag(exp(G_C - G)) U dS'^T   (the key that writes)
 //   dG = q . dQ + k . dKr - k . dKc, and at the last token + sum_j (k . [state part of dKc])_j + exp(G_C) <dS', S>
 // because G_i enters only as exp(G_i) with what token i reads and exp(-G_j) with what token j writes; dg is the sum
 // of dG from its token to the end of the chunk.
@@ -18,9 +18,10 @@
 // G is summed in 64 bits, since differences of it are taken, and g is read as max(g, -200): exp(-200) is 0 in fp32,
 // and a g of -infinity then gives no infinity minus infinity.
 //
-// Kernels: prep (parallel over chunks: T, P, G), scan (over the chunks of a sequence, parallel over heads and slices of
-// dv, which are independent), its reverse, and grads (parallel over chunks).  Short inputs and single tokens go through
-// the recurrence itself.
+// Kernels: plan (where packed sequences are), chunk (parallel over chunks: T, P, G, operands in the scans' order), the chain (over the
+// chunks of a sequence, parallel over heads and slices of dv, which are independent) and its reverse, and grads (parallel over
+// chunks).  Short inputs and single tokens go through the recurrence itself.  8192 tokens x 16 heads, bf16, dk = dv = 128: chunk 60 us,
+// chain 237; training on 2 x 4096 tokens: 84, 197 and 210, grads 235.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -39,7 +40,7 @@ constexpr float G_MIN = -200.f;
 // Where the chunks of a problem are.  Slot numbers need no table: sequence s starts at slot offsets[s] / C + s, which
 // leaves room for every sequence's last, partly filled chunk.
 struct Plan {
-  int sequences, tokens, batch;
+  int sequences, tokens;
   const int* off;        // sanitised offsets (device) or nullptr: sequence s is batch row s
   int chunks_per_row;    // plain batches
   __device__ __forceinline__ int begin(int s) const { return off ? off[s] : 0; }
@@ -250,7 +251,7 @@ __device__ __forceinline__ void lds_barrier() {
 // same of its second tile (none if DK = 64: zeros).
 __device__ __forceinline__ long frag(int block, int blocks, int ks, int lane) { return (((long)block * blocks + ks) * 64 + lane) * 8; }
 
-constexpr int KF = 4 * 4 * 64 * 8;   // elements of a plane of K or Q in state order, also of a C x C matrix twice over
+constexpr int KF = 4 * 4 * 64 * 8;   // elements of a plane of K or Q in state order
 constexpr int TF = 4 * 2 * 64 * 8;   // of a C x C matrix
 constexpr int FACS = 6 * C;          // factors per head
 
@@ -368,6 +369,9 @@ __device__ __forceinline__ void store_square(const float* M, __bf16* dst, int t)
 template <typename T> struct OutPlanes { static constexpr int N = sizeof(T) == 2 ? 2 : 3; };
 
 // ---- prep: one chunk of one key head and its value heads -----------------------------------------------------------------
+// Many chunks: bound by memory, mostly its own stores (2048 chunks of 128 x 128 in bf16: 231 MB in 60 us, 337 MB in 84 with what
+// training keeps).  Few: by the inverse and its barriers, 24 us for one chunk in fp32, so that value heads that share a key head get a
+// workgroup each while these fit the chip twice (fp32, 28 chunks of two heads: 33 -> 25 us; fp16, 348: 28 -> 38, so not there).
 template <typename T, int DK>
 constexpr size_t chunk_room() {
   constexpr size_t first = 2 * Planes<T>::N * C * (DK + 8) * 2, second = (2 * C * PC + 32 * 36) * 4;
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
   if (len == 0) return;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), col = lane & 15, g8 = (lane >> 4) * 8;
   const long row = a.p.row(s), atk = (long)slot * a.d.key_heads + hk;
   float gv = 0.f, bv = 0.f;   // wave 0: g and beta of the next value head
   auto load_g = [&](int hv) {
@@ -553,11 +557,14 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
 // Bound by the chain from chunk to chunk: the product with K (each wave with its own rows of S, which are in its accumulators;
 // partial sums through LDS), X through LDS, the product with T, U through LDS, the product with K^T: three barriers.  Four waves do that
 // and nothing else; four more take S and E from LDS and do what the chain does not wait for -- forward the outputs
-// O = scale (exp(G) Q S + P beta E), backward Q^T Of, and all stores.  (A wave waits for its memory accesses in order: with
-// the stores in the chain's waves its loads waited for them.  8192 tokens x 16 heads, bf16, dk = dv = 128: 256 us and 68 for the
-// outputs, against 226 together; 137 for the chain without any access to memory.)  Fragments come straight from memory, up to
-// a chunk ahead (two gained nothing), issued under the latency of LDS reads or matrix instructions; every load is issued
-// whatever comes, since loads behind branches make the compiler wait for all that are under way.
+// O = scale (exp(G) Q S + P beta E), backward Q^T Of and the next chunk's Y, and all stores.  (A wave waits for its memory accesses
+// in order: with the stores in the chain's waves its loads waited for them.)  Fragments come straight from memory, up to a chunk
+// ahead (two gained nothing), issued under the latency of LDS reads or matrix instructions; every load is issued whatever comes,
+// since loads behind branches make the compiler wait for all that are under way.
+// 8192 tokens x 16 heads, bf16, dk = dv = 128, 128 workgroups: 237 us, 1.85 a chunk, of which 78 KB of operands take 0.5 at L1's 64
+// bytes a clock; without any access to memory 137; with the outputs in a kernel of their own 256 and 68; with 32 columns to a
+// workgroup 349.  Training on 2 x 4096 tokens, 256 workgroups: 197 forward, 130 to 140 without the stores of S and E (200 MB),
+// 210 back, where Y from a kernel of its own took 54 more.
 __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes) {
   return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
 }
@@ -1009,6 +1016,9 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 // 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
 // memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
 // the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
+// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 235 us for 655 MB, 2.8 TB/s.  The slices wait for memory (a third of the time),
+// the steps after them for LDS, where all waves read the whole C x C matrix; neither overlaps the other, since the registers leave one
+// workgroup to a CU.  One that went on from chunk to chunk with the next one's first loads under way took as long.
 // LDS of the slices, which a C x C matrix of three planes takes over
 template <typename T>
 constexpr size_t grads_room() {
@@ -1364,7 +1374,8 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 
 // ---- the recurrence itself ---------------------------------------------------------------------------------------------
 // 64 columns of a state per workgroup: thread = 4 columns x RPT rows, in registers for all of its tokens.  One
-// reduction per token, since o = scale (q^T Sbar + (q . k) beta e).
+// reduction per token, since o = scale (q^T Sbar + (q . k) beta e).  A step of 64 users is bound by the states, 268 MB there and back
+// in 44.6 us (6.0 TB/s, a large copy's 5.2 to 5.8); one user's takes a launch (5.6 us, 8 states of 64 x 64).
 struct StepArgs {
   Args a;
   const int* slot;   // step: the state of each row
@@ -1579,14 +1590,20 @@ int check_delta(const gpx_delta* d, const char* what) {
   GPX_REQUIRE(d->tokens <= (1 << 30) && d->batch <= (1 << 24) && d->sequences <= (1 << 24), "%s: size out of range", what);
   GPX_REQUIRE(d->sequences == 0 || (d->batch == 1 && d->offsets != nullptr), "%s: packed sequences need batch == 1 and offsets", what);
   GPX_REQUIRE(std::isfinite(d->scale), "%s: scale is not finite", what);
-  // blocks of a launch: 32 bits, with room
-  const double heads = (double)std::max<long>(slots_of(d), sequences_of(d)) * d->value_heads;
-  GPX_REQUIRE(heads * 40 < 2.0e9, "%s: too many heads and chunks for one call", what);
   for (const gpx_strided* s : {&d->q_st, &d->k_st, &d->v_st, &d->g_st, &d->beta_st})
     GPX_REQUIRE(s->bs >= 0 && s->rs >= 0 && s->cs >= 0, "%s: negative stride", what);
   GPX_REQUIRE(d->v_st.rs <= (1 << 22), "%s: token stride of v beyond 2^22", what);   // 32-bit offsets inside a chunk
   if (d->batch > 0 && d->tokens > 0)
     GPX_REQUIRE(d->q && d->k && d->v && d->g && d->beta, "%s: null input", what);
+  return 0;
+}
+
+// threads of a launch have 32 bits
+int check_grid(const gpx_delta* d, bool rec, const char* what) {
+  const double scan = (sequences_of(d) * (double)d->value_heads + 7) * ((d->dv + DVT - 1) / DVT * DVT / 16) * 512;
+  const double steps = (double)sequences_of(d) * d->value_heads * ((d->dv + 63) / 64) * 256;
+  const double chunks = (double)slots_of(d) * d->key_heads * 512;
+  GPX_REQUIRE((rec ? steps : std::max(scan, chunks)) < 4.2e9, "%s: too many sequences, heads and chunks for one call", what);
   return 0;
 }
 
@@ -1599,7 +1616,6 @@ Args make_args(const gpx_delta* d) {
   a.scale = (float)d->scale;
   a.p.sequences = sequences_of(d);
   a.p.tokens = d->tokens;
-  a.p.batch = d->batch;
   a.p.chunks_per_row = (d->tokens + C - 1) / C;
   a.p.off = nullptr;
   return a;
@@ -1723,6 +1739,7 @@ extern "C" {
 
 size_t gpx_delta_work_bytes(const gpx_delta* d, int use) {
   if (use < 0 || use > 3 || check_delta(d, "delta_work_bytes") != 0) return 0;
+  if (check_grid(d, use == WORK && recurrent(d, 0), "delta_work_bytes") != 0) return 0;
   return lay_out(d, use, nullptr, nullptr, nullptr);
 }
 
@@ -1735,6 +1752,7 @@ int gpx_delta_forward(gpx_handle* h, const gpx_delta* d, const float* state, voi
   GPX_REQUIRE(state == nullptr || gpx_aligned16(state), "delta_forward: state must be 16-byte aligned");
   GPX_REQUIRE(state_out == nullptr || gpx_aligned16(state_out), "delta_forward: state_out must be 16-byte aligned");
   const int save = saved != nullptr;
+  DELTA_TRY(check_grid(d, recurrent(d, save), "delta_forward"));
   DELTA_TRY(check_work(d, save ? WORK_SAVING : WORK, work, work_bytes, "delta_forward"));
   if (save) DELTA_TRY(check_work(d, SAVED, saved, saved_bytes, "delta_forward"));
   DeviceGuard dg(h->device);
@@ -1762,6 +1780,7 @@ int gpx_delta_backward(gpx_handle* h, const gpx_delta* d, const void* d_o, const
     GPX_REQUIRE(d_o_st->bs >= 0 && d_o_st->rs >= 0 && d_o_st->cs >= 0, "delta_backward: negative stride");
     GPX_REQUIRE(d_q && d_k && d_v && d_g && d_beta, "delta_backward: null output");
   }
+  DELTA_TRY(check_grid(d, false, "delta_backward"));
   DELTA_TRY(check_work(d, SAVED, saved, saved_bytes, "delta_backward"));
   DELTA_TRY(check_work(d, SCRATCH, scratch, scratch_bytes, "delta_backward"));
   DeviceGuard dg(h->device);
@@ -1786,6 +1805,7 @@ int gpx_delta_step(gpx_handle* h, const gpx_delta* d, int slots, const int* slot
   GPX_REQUIRE(h != nullptr, "null handle");
   DELTA_TRY(check_delta(d, "delta_step"));
   GPX_REQUIRE(d->tokens == 1 && d->sequences == 0, "delta_step: one token per row");
+  DELTA_TRY(check_grid(d, true, "delta_step"));
   GPX_REQUIRE(slots >= 0 && (slot != nullptr || slots == d->batch), "delta_step: %d states for %d rows", slots, d->batch);
   if (d->batch == 0 || slots == 0) return 0;   // no row has a state
   GPX_REQUIRE(o != nullptr && state_out != nullptr && state != nullptr, "delta_step: null state or output");

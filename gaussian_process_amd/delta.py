@@ -19,6 +19,7 @@ from . import _lib
 from .device import ptr, tensor_runtime
 from .orthogonal import check_tensor, type_id
 
+
 def _dense(t):
     """t, or a packed copy where its last dimension is not dense or its tokens lie too far apart for the library."""
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-3) <= 1 << 22 else t.contiguous()
@@ -108,8 +109,8 @@ def _version(t):
 class Saved:
     """What a forward call keeps for its backward call."""
 
-    def __init__(self, desc, inputs, state, work):
-        self.desc, self.inputs, self.has_state, self.work = desc, inputs, state is not None, work
+    def __init__(self, desc, inputs, state, work, stream):
+        self.desc, self.inputs, self.has_state, self.work, self.stream = desc, inputs, state is not None, work, stream
         self.versions = [_version(t) for t in inputs]
 
 
@@ -121,7 +122,9 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
     outside [0, T] are clamped and a decreasing one is read as the one before it; outputs of tokens that belong
     to no sequence are zeros.  initial_state: (sequences, Hv, dk, dv) float32, None for zeros.  scale: dk ** -0.5 by default.
 
-    Long inputs run in chunks of 64 tokens on the matrix cores, up to 16 tokens go through the recurrence.  Asynchronous
+    Long inputs run in chunks of 64 tokens on the matrix cores, up to 16 tokens go through the recurrence.  There a NaN or an
+    infinity in a token's inputs may reach the tokens before it in its chunk, besides the later ones of its sequence and head that
+    it reaches in any case; never earlier chunks, other sequences or heads.  Asynchronous
     on the current stream; may be captured into a graph after one call outside."""
     import torch
     dtype, Hk, dk, Hv, dv = _check(q, k, v, g, beta, 4)
@@ -154,7 +157,7 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
     if not save_for_backward:
         return o, final
     inputs = [t for t in (q, k, v, g, beta, cu_seqlens) if t is not None]
-    return o, final, Saved(d, inputs, initial_state, saved)
+    return o, final, Saved(d, inputs, initial_state, saved, torch.cuda.current_stream(q.device))
 
 
 def gated_delta_rule_backward(saved, d_o, d_final_state=None):
@@ -176,6 +179,10 @@ def gated_delta_rule_backward(saved, d_o, d_final_state=None):
     shape = (d.sequences or d.batch, d.value_heads, d.dk, d.dv)
     _check_state(d_final_state, shape, "d_final_state")
     rt = tensor_runtime(q, d_o, d_final_state)
+    stream = torch.cuda.current_stream(q.device)
+    if stream != saved.stream:   # what the forward call allocated may be dropped while this stream still reads it
+        for t in (*saved.inputs, saved.work):
+            t.record_stream(stream)
     with rt.current_stream():
         d_o, d_final = _dense(d_o), _aligned(d_final_state)
         new = torch.zeros if d.sequences else torch.empty
@@ -229,4 +236,5 @@ def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, s
         rc = rt.lib.gpx_delta_step(rt.h, C.byref(d), n, _opt(slots), at, to, o.data_ptr())
         if rc:
             _lib.check(rc, "gpx_delta_step")
+        torch.autograd.graph.increment_version(state_out)   # written behind torch's back: what was saved of it is stale
     return o, state_out

@@ -117,4 +117,5 @@ def orthogonalize(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, alpha=1.0, be
             rt.h, dtype, batch, n, m, ptr(g3), C.byref(gs), int(steps), coef, float(eps), float(alpha), float(beta),
             ptr(b3) if b3 is not None else None, C.byref(bs) if bs is not None else None, ptr(o3), C.byref(os_),
             ptr(work), size), "gpx_orthogonalize")
+        torch.autograd.graph.increment_version(out)   # written behind torch's back: what was saved of it is stale
     return out

@@ -15,6 +15,8 @@
  *     every pointer is a DEVICE pointer unless the name ends in _host;
  *   - base pointers must be 16-byte aligned and leading dimensions even (the kernels use
  *     16-byte vector accesses); violations return GPX_EINVAL, they never fault;
+ *   - not so the two sections at the end, of learned maps: theirs are tensors of four element
+ *     types with any strides and any alignment the type has, unless they say otherwise;
  *   - "lower" matrices are referenced in their lower triangle only (row >= col);
  *   - the caller owns every buffer; the library allocates nothing in these calls except
  *     inside gpx_create;
@@ -317,7 +319,9 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m);
  * offsets[s] .. offsets[s + 1] (sequences + 1 values in DEVICE memory, not decreasing; values outside [0, tokens] are
  * clamped, a decreasing value is read as the one before it).  Tokens behind the last sequence or before the first are
  * not read and their outputs not written.  Sequences may be empty: their state passes through.
- * g may be -infinity (the state is forgotten).  beta == 0 and g == 0 leave the state as it is.  1 <= dk <= 128,
+ * g may be -infinity (the state is forgotten); it is read as max(g, -200).  beta == 0 and g == 0 leave the state as it is.
+ * A NaN or an infinity in a token's inputs reaches the later tokens of its sequence and heads, and may reach the earlier ones of
+ * the same 64 tokens (counted from the sequence's first); no others.  1 <= dk <= 128,
  * 1 <= dv <= 1024; a token stride of v of at most 2^22.  States, decays and all sums are fp32 or wider. */
 typedef struct gpx_delta {
   int dtype, batch, tokens, sequences, key_heads, value_heads, dk, dv;

@@ -190,6 +190,8 @@ def test_work_bytes():
     assert w(1, batch=1, sequences=5, offsets=256) == 256 + w(1) * 6 // 4
     assert w(0, batch=1, sequences=5) == 0                       # no offsets
     assert w(1, batch=1 << 24, tokens=1 << 30) == 0              # beyond the grid
+    big = dict(batch=1 << 20, key_heads=16, value_heads=16, dv=128)
+    assert w(0, tokens=64, **big) == 0 and w(1, tokens=1, **big) == 0 and w(0, tokens=64, **{**big, "batch": 1 << 15}) > 0
 
 
 # ---- GPU ----------------------------------------------------------------------------------------------------------
@@ -455,6 +457,36 @@ def test_saved_is_only_read_and_guarded():
     x["k"].mul_(2)
     with pytest.raises(RuntimeError):
         gated_delta_rule_backward(saved, d1)
+
+
+@pytest.mark.gpu
+def test_saved_notices_writes_of_this_package():
+    from gaussian_process_amd import gated_delta_rule, gated_delta_rule_backward, gated_delta_rule_step, orthogonalize
+    x = inputs(1, 70, 1, 1, 16, 16, "f32")
+    o, f, saved = gated_delta_rule(*args(x), save_for_backward=True)
+    orthogonalize(x["v"], out=x["v"])
+    with pytest.raises(RuntimeError):
+        gated_delta_rule_backward(saved, torch.ones_like(o))
+    before = f._version
+    gated_delta_rule_step(*(t[:, 0] for t in args(x)), f)
+    assert f._version > before
+
+
+@pytest.mark.gpu
+def test_backward_on_another_stream():
+    from gaussian_process_amd import gated_delta_rule, gated_delta_rule_backward
+    x = inputs(2, 200, 2, 4, 64, 64, "bf16")
+    d_o = torch.randn_like(x["v"])
+    want = gated_delta_rule_backward(gated_delta_rule(*args(x), save_for_backward=True)[2], d_o)
+    side = torch.cuda.Stream()
+    saved = gated_delta_rule(*args(x), save_for_backward=True)[2]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = gated_delta_rule_backward(saved, d_o)
+    del saved
+    torch.full((1 << 24,), float("nan"), device="cuda")   # where the saved values were, if they were given back too early
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got) if a is not None)
 
 
 @pytest.mark.gpu
