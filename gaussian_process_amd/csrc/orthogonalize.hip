@@ -160,6 +160,12 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const T* G, long bs, long 
   }
 }
 
+#define NS_TRY(expr)          \
+  do {                        \
+    int rc_ = (expr);         \
+    if (rc_ != 0) return rc_; \
+  } while (0)
+
 // ---- the product -------------------------------------------------------------------------------------------------
 // v = ca * E + cc * (A B^T); v goes to D [row][col], to DT [col][row], or as alpha * v + beta * base to the caller's
 // matrix.
@@ -179,7 +185,29 @@ struct NsGemm {
   long obs, ors, ocs, bbs, brs, bcs;
   int n, m;
   float alpha, beta;
+  // K split over `parts` workgroups per tile: their sums, [part][matrix][M][N], for ns_join_kernel
+  float* sums;
+  int parts;
 };
+
+// the k-tiles of this workgroup, from blockIdx.z
+__device__ __forceinline__ void k_range(const NsGemm& g, int nk, int& first, int& count) {
+  first = (int)((long)nk * blockIdx.z / g.parts);
+  count = (int)((long)nk * (blockIdx.z + 1) / g.parts) - first;
+}
+
+// the sums of one part, EM x EN of them at (row0, col0): stage() leaves them in st (pitch EN + 4)
+template <int EM, int EN, typename F>
+__device__ __forceinline__ void keep_sums(const NsGemm& g, const float* st, long z, int row0, int col0, int lane, F stage) {
+  constexpr int RL = EN / 4, RR = 64 / RL;   // lanes per row, rows at a time
+  float* dst = g.sums + (((long)blockIdx.z * gridDim.y + z) * g.M + row0) * g.N + col0 + (lane % RL) * 4;
+  stage();
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int r = lane / RL; r < EM; r += RR)
+    *reinterpret_cast<f4*>(dst + (long)r * g.N) = *reinterpret_cast<const f4*>(st + r * (EN + 4) + (lane % RL) * 4);
+  __builtin_amdgcn_wave_barrier();
+}
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, char* dst_wave) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst_wave, 16, voff, soff, 0, 0);
@@ -436,7 +464,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const N
 // Small problems, where latency counts and not the rate: a 64 x 64 tile per workgroup, whose W waves take every
 // W-th k-tile each, with stages of their own and no barrier, and add their sums through LDS in the order of the waves.  n = 1024, one
 // plane: 8.4 us for A A, about 4 of which a launch takes that does nothing else; 16 TB/s from L2.
-template <int W, int NPL, int STAGES>
+template <int W, int NPL, int STAGES, bool SPLIT>
 __global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int tiles_m, int tiles_n) {
   constexpr int BK = 64 / NPL, KS = BK / 16, STAGE = 128 * 128, P = 68, L = 16, ROWS = 64 / W;
   static_assert(STAGES * L < 64, "vmcnt has six bits");
@@ -478,10 +506,12 @@ __global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int ti
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
   const int r32 = lane & 31, kh = lane >> 5;
-  const int nk = g.K / BK, own = nk > wave ? (nk - wave + W - 1) / W : 0;   // k-tiles wave, wave + W, ..
+  int k0 = 0, nk = g.K / BK;
+  if (SPLIT) k_range(g, g.K / BK, k0, nk);
+  const int own = nk > wave ? (nk - wave + W - 1) / W : 0;   // k-tiles wave, wave + W, ..
 #pragma unroll
   for (int p = 0; p < STAGES; ++p)
-    if (p < own) load(wave + p * W, p);
+    if (p < own) load(k0 + wave + p * W, p);
   int cur = 0;
   for (int n = 0; n < own; ++n) {
     if (n + STAGES <= own)
@@ -502,7 +532,7 @@ __global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int ti
         }
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // in registers: the stage may be filled again
-    if (n + STAGES < own) load(wave + (n + STAGES) * W, cur);
+    if (n + STAGES < own) load(k0 + wave + (n + STAGES) * W, cur);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -529,7 +559,7 @@ __global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int ti
   __syncthreads();
   // wave w: the rows ROWS w .. of all sums; they end in the first
   float* st = sum + wave * ROWS * P;
-  finish<NPL, ROWS, 64>(g, st, z, i0 + wave * ROWS, j0, lane, !(g.lower && ti == tj), [&] {
+  auto stage = [&] {
     constexpr int Q = ROWS * 64 / 4 / 64;   // four columns a lane
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -539,6 +569,34 @@ __global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int ti
       for (int w = 1; w < W; ++w) v += *reinterpret_cast<const f4*>(st + w * 64 * P + r * P + c);
       *reinterpret_cast<f4*>(st + r * P + c) = v;
     }
+  };
+  if (SPLIT)
+    keep_sums<ROWS, 64>(g, st, z, i0 + wave * ROWS, j0, lane, stage);
+  else
+    finish<NPL, ROWS, 64>(g, st, z, i0 + wave * ROWS, j0, lane, !(g.lower && ti == tj), stage);
+}
+
+// The end of a product whose K was split: 64 x 64 a workgroup, the parts added in their order.
+__global__ __launch_bounds__(256) void ns_join_kernel(const NsGemm g, int tiles_m, int tiles_n) {
+  constexpr int P = 68, ROWS = 16, Q = ROWS * 64 / 4 / 64;
+  __shared__ __align__(16) float smem[4 * ROWS * P];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int ti, tj;
+  tile_of(g.lower, tiles_m, tiles_n, ti, tj);
+  const long z = blockIdx.y;
+  const int row0 = ti * 64 + wave * ROWS, col0 = tj * 64;
+  float* st = smem + wave * ROWS * P;
+  finish<2, ROWS, 64>(g, st, z, row0, col0, lane, !(g.lower && ti == tj), [&] {
+    const long part = (long)gridDim.y * g.M * g.N;
+    const float* src = g.sums + (z * g.M + row0) * g.N + col0;
+    f4 v[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) v[q] = f4{0, 0, 0, 0};
+    for (int p = 0; p < g.parts; ++p, src += part)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) v[q] += *reinterpret_cast<const f4*>(src + (long)(q * 4 + (lane >> 4)) * g.N + (lane & 15) * 4);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) *reinterpret_cast<f4*>(st + (q * 4 + (lane >> 4)) * P + (lane & 15) * 4) = v[q];
   });
 }
 
@@ -564,7 +622,7 @@ int launch_cfg(hipStream_t s, const NsGemm& g, int batch) {
   return 0;
 }
 
-template <int W, int NPL, int STAGES>
+template <int W, int NPL, int STAGES, bool SPLIT>
 int launch_small(hipStream_t s, const NsGemm& g, int batch) {
   constexpr size_t lds = std::max<size_t>((size_t)W * STAGES * 128 * 128, (size_t)W * 64 * 68 * 4);
   static_assert(lds <= 160 * 1024, "LDS");
@@ -573,11 +631,11 @@ int launch_small(hipStream_t s, const NsGemm& g, int batch) {
   int dev = 0;
   GPX_HIP(hipGetDevice(&dev));
   if (dev < GPX_MAX_DEVICES && !set[dev]) {
-    GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_small_kernel<W, NPL, STAGES>),
+    GPX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_small_kernel<W, NPL, STAGES, SPLIT>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     set[dev] = true;
   }
-  hipLaunchKernelGGL((ns_small_kernel<W, NPL, STAGES>), dim3(g.lower ? (unsigned)tm * (tm + 1) / 2 : (unsigned)tm * tn, batch),
+  hipLaunchKernelGGL((ns_small_kernel<W, NPL, STAGES, SPLIT>), dim3(g.lower ? (unsigned)tm * (tm + 1) / 2 : (unsigned)tm * tn, batch, SPLIT ? g.parts : 1),
                      dim3(64 * W), lds, s, g, tm, tn);
   GPX_HIP(hipGetLastError());
   return 0;
@@ -587,26 +645,68 @@ int launch_small(hipStream_t s, const NsGemm& g, int batch) {
 // two planes keep the ratios): 64 x 64 with 4 waves (ns_small_kernel), two on a CU, 34; 128 x 128 with 8 waves 42; 192 x 192 with 6 waves
 // 84; 256 x 256 with 8 waves 110.  Larger tiles read LDS less per product, smaller ones fill the chip: A A at n = 4096
 // takes 162 / 117 / 84 / 97 us with them, B X 233 / 173 / 169 / 140, at n = 1024 8.4 / 14 / 26 / 35 and 9.3 / 14 / 27 / 36.
+//
+// A product A A^T of two planes with few tiles and a long K leaves most of the chip idle while a tile's time goes with the bytes
+// that its CU loads, 9 ns per k.  K is then split over workgroups, at the price of a launch and of the sums to memory and
+// back, as far as all run at once: 10 tiles with K = 4096 36 -> 20 us, 66 with 2560 30 -> 22; not 136 of K = 3008 (33 -> 34), not of one
+// plane, whose rows come in whole lines (10 tiles with K = 4096 15 -> 14), and not larger tiles, which keep more of the chip busy
+// (136 of 128 x 128 with K = 8192 174 -> 148, nothing of it left in the whole call).
+struct Choice {
+  int tile, parts;
+};
 template <int NPL>
-int ns_gemm(hipStream_t s, const NsGemm& g, int batch) {
+Choice choose(int M, int N, int K, int lower, int batch) {
   const int tile[4] = {64, 128, 192, 256}, slots[4] = {512, 256, 256, 256};
   const double unit[4] = {34, 42, 84, 110};
-  int best = 0;
-  double least = 0;
+  Choice best = {0, 1};
+  double least = 0, tiles = 0;
   for (int i = 0; i < 4; ++i) {
-    const double tm = (g.M + tile[i] - 1) / tile[i], tn = (g.N + tile[i] - 1) / tile[i];
-    const double cost = std::ceil((g.lower ? tm * (tm + 1) / 2 : tm * tn) * batch / slots[i]) * unit[i];
+    const double tm = (M + tile[i] - 1) / tile[i], tn = (N + tile[i] - 1) / tile[i], t = (lower ? tm * (tm + 1) / 2 : tm * tn) * batch;
+    const double cost = std::ceil(t / slots[i]) * unit[i];
     if (i == 0 || cost < least) {
-      best = i;
+      best.tile = i;
       least = cost;
+      tiles = t;
     }
   }
-  switch (best) {
-    case 0: return launch_small<4, NPL, 1>(s, g, batch);
+  if (NPL == 2 && lower && best.tile == 0) {
+    double gain = 2;   // us
+    for (int p = 2; p <= 8 && tiles * p <= 256; ++p) {
+      const double g = K * 0.009 * (1 - 1.0 / p) - 8 - p * (1 + tiles * 0.008);
+      if (g > gain) {
+        gain = g;
+        best.parts = p;
+      }
+    }
+  }
+  return best;
+}
+
+template <int NPL>
+int ns_gemm(hipStream_t s, NsGemm g, int batch) {
+  const Choice c = choose<NPL>(g.M, g.N, g.K, g.lower, batch);
+  g.parts = c.parts;
+  if constexpr (NPL == 2) {
+    if (c.parts > 1) {
+      NS_TRY((launch_small<4, NPL, 1, true>(s, g, batch)));
+      const int tm = g.M / 64;
+      hipLaunchKernelGGL(ns_join_kernel, dim3((unsigned)tm * (tm + 1) / 2, batch), dim3(256), 0, s, g, tm, tm);
+      GPX_HIP(hipGetLastError());
+      return 0;
+    }
+  }
+  switch (c.tile) {
+    case 0: return launch_small<4, NPL, 1, false>(s, g, batch);
     case 1: return launch_cfg<128, 128, 2, 4, NPL, 4>(s, g, batch);
     case 2: return launch_cfg<192, 192, 2, 3, NPL, 3>(s, g, batch);
     default: return launch_cfg<256, 256, 2, 4, NPL, 2>(s, g, batch);
   }
+}
+
+// bytes of the sums that the products of a call keep, two planes
+size_t sums_bytes(int np, int mp, int batch) {
+  const int parts = std::max(choose<2>(np, np, mp, 1, batch).parts, choose<2>(np, np, np, 1, batch).parts);
+  return parts == 1 ? 0 : (size_t)parts * batch * np * np * 4;
 }
 
 // ---- fp64: the framework's own products ----------------------------------------------------------------------------
@@ -662,12 +762,6 @@ GemmDesc product(const double* A, long lda, const double* B, long ldb, int b_lay
   g.c_lower = lower; g.diag_add = 0.0; g.inplace = 0;
   return g;
 }
-
-#define NS_TRY(expr)          \
-  do {                        \
-    int rc_ = (expr);         \
-    if (rc_ != 0) return rc_; \
-  } while (0)
 
 // the largest |s (a + b s^2 + c s^4)| for 0 <= s <= r
 double step_bound(const double* k, double r) {
@@ -731,7 +825,8 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
   XT[0] = p; p += batch * ts;
   XT[1] = p; p += batch * ts;
   _Float16* A = p; p += batch * as;
-  _Float16* B = p;
+  _Float16* B = p; p += batch * as;
+  float* sums = reinterpret_cast<float*>(p);
   int nparts = 0;
   NS_TRY(norm_launch<T>(s, G, bs, rs, cs, n, m, batch, part, nparts));
   double r = 1.0;
@@ -746,6 +841,7 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
     const int sn = scale_exp(rn);
     NsGemm g = {};
     g.out_type = -1;
+    g.sums = sums;
     // A = X X^T
     g.A = g.B = X[cur]; g.lda = g.ldb = 2L * mp; g.sa = g.sb = xs;
     g.D = g.DT = A; g.dpl = NPL; g.sd = g.st = as;
@@ -822,7 +918,8 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m) {
     return parts + 8 * (2 * (size_t)small * pad32(large) + 2 * (size_t)small * pad32(small));
   const size_t np = pad64(small), mp = pad64(large);
   const size_t pl = planes_of(dtype);   // X twice with two planes, X^T twice, A and B
-  return parts + (size_t)batch * 2 * ((4 + 2 * pl) * np * mp + 2 * pl * np * np);
+  const size_t sums = pl == 1 ? 0 : sums_bytes((int)np, (int)mp, batch);
+  return parts + (size_t)batch * 2 * ((4 + 2 * pl) * np * mp + 2 * pl * np * np) + sums;
 }
 
 int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const void* G, const gpx_strided* g_st, int steps,
