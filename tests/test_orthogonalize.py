@@ -63,6 +63,10 @@ def test_work_bytes():
     assert lib.gpx_orthogonalize_work_bytes(0, 1, 5, 40) == 8192 + 8 * (2 * 5 * 64 + 2 * 5 * 32)
     assert lib.gpx_orthogonalize_work_bytes(9, 1, 5, 40) == 0
     assert lib.gpx_orthogonalize_work_bytes(1, 1, 0, 40) == 0
+    # a long K split over workgroups: room for the parts' sums
+    whole = 8192 + 2 * (8 * 256 * 4096 + 4 * 256 * 256)
+    assert (lib.gpx_orthogonalize_work_bytes(1, 1, 256, 4096) - whole) % (256 * 256 * 4) == 0
+    assert lib.gpx_orthogonalize_work_bytes(1, 1, 256, 4096) > whole
     # 64-bit sizes
     assert lib.gpx_orthogonalize_work_bytes(1, 1, 65536, 65536) == 8192 + 2 * 12 * 65536 ** 2
 
@@ -84,6 +88,18 @@ def test_matches_the_definition(shape, kind):
     assert O.shape == G.shape and O.dtype == G.dtype
     ref = plain(G)
     assert rel(O, ref) < TOL[kind], rel(O, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(100, 3000), (2, 260, 4100), (2600, 640), (3, 64, 8000)])
+def test_long_rows(shape, kind):
+    """Few tiles of a long K, which two planes split over workgroups."""
+    from gaussian_process_amd import orthogonalize
+    G = make(shape, kind, seed=shape[-1])
+    O = orthogonalize(G)
+    assert rel(O, plain(G)) < TOL[kind]
+    assert torch.equal(O, orthogonalize(G))
 
 
 @pytest.mark.gpu
