@@ -711,7 +711,7 @@ size_t sums_bytes(int np, int mp, int batch) {
 
 // ---- fp64: the framework's own products ----------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void ns_pack_f64_kernel(const double* G, long bs, long rs, long cs, int n, int m,
-                                                          const double* part, int nparts, double eps, double* X, long ldx) {
+                                                          const double* part, int nparts, double eps, double* X, double* Y, long ldx) {
   __shared__ double tile[64][65];
   __shared__ double sm[4];
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, t = threadIdx.x;
@@ -725,7 +725,44 @@ __global__ __launch_bounds__(256) void ns_pack_f64_kernel(const double* G, long 
   __syncthreads();
   for (int q = 0; q < 16; ++q) {
     const int i = q * 4 + (t >> 6), j = t & 63;
-    if (i0 + i < n && j0 + j < m) X[(i0 + i) * ldx + j0 + j] = tile[i][j];
+    if (i0 + i >= n || j0 + j >= ldx) continue;
+    X[(i0 + i) * ldx + j0 + j] = j0 + j < m ? tile[i][j] : 0.0;
+    if (j0 + j >= m) Y[(i0 + i) * ldx + j0 + j] = 0.0;   // the other buffer's padding too
+  }
+}
+
+// S = alpha sum of the parts + beta base for symmetric n x n matrices of which the parts hold the lower triangle; S whole, with zeros
+// in its padding.  32 x 32 a workgroup, every load under way at once.
+template <int PARTS_>
+__global__ __launch_bounds__(256) void ns_join_f64_kernel(int n, const double* sums, double alpha, double beta, const double* base,
+                                                          double* S, long ld) {
+  __shared__ double tile[32][33];
+  const int bi = blockIdx.y, bj = blockIdx.x, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  if (bj > bi) return;
+  const long part = n * ld;
+  double v[4][PARTS_], b[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int i = min(bi * 32 + q * 8 + ty, n - 1), j = min(bj * 32 + tx, i);
+    b[q] = base != nullptr ? base[i * ld + j] : 0.0;
+#pragma unroll
+    for (int p = 0; p < PARTS_; ++p) v[q][p] = sums[p * part + i * ld + j];
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = q * 8 + ty, i = bi * 32 + r, j = bj * 32 + tx;
+    double x = v[q][0];
+#pragma unroll
+    for (int p = 1; p < PARTS_; ++p) x += v[q][p];
+    x = base != nullptr ? alpha * x + beta * b[q] : alpha * x;
+    tile[r][tx] = x;
+    if (i < n && j <= i) S[i * ld + j] = x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = q * 8 + ty, i = bj * 32 + r, j = bi * 32 + tx;   // the mirror image
+    if (i < n && j > i && j < ld) S[i * ld + j] = j < n ? tile[tx][r] : 0.0;
   }
 }
 
@@ -876,6 +913,36 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
   return 0;
 }
 
+// Parts into which K (padded to 32) of a symmetric n x n product is split, as a batch of slices of K, until its tiles of 64 x 64 fill
+// most of the chip's 512 places.  Whole calls: 1024 x 2048 1131 -> 872 us (988 if half of the places will do), 300 x 700 669 -> 371.
+int parts_f64(int n, long k) {
+  const long nt = (n + 63) / 64, tiles = nt * (nt + 1) / 2;
+  int parts = 1;
+  while (parts < 8 && tiles * parts < 400 && k / (parts * 2) >= 128) parts *= 2;
+  return parts;
+}
+
+// S = alpha R R^T + beta base
+int symmetric_f64(hipStream_t s, const double* R, long ldr, int n, int k, double* S, long ld, double* sums, double alpha, double beta,
+                  const double* base) {
+  const int parts = parts_f64(n, ldr);
+  if (parts == 1) {
+    NS_TRY(gpx_gemm_launch(s, product(R, ldr, R, ldr, GPX_LAY_KC, base, S, ld, n, n, k, alpha, beta, 1)));
+    return gpx_symmetrize_launch(s, n, S, ld);
+  }
+  GemmDesc g = product(R, ldr, R, ldr, GPX_LAY_KC, nullptr, sums, ld, n, n, (int)(ldr / parts), 1.0, 0.0, 1);
+  g.batch = parts;
+  g.stride_a = g.stride_b = ldr / parts;
+  g.stride_d = n * ld;
+  NS_TRY(gpx_gemm_launch(s, g));
+  const dim3 grid((n + 31) / 32, (n + 31) / 32);
+  if (parts == 2) hipLaunchKernelGGL(ns_join_f64_kernel<2>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
+  else if (parts == 4) hipLaunchKernelGGL(ns_join_f64_kernel<4>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
+  else hipLaunchKernelGGL(ns_join_f64_kernel<8>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
+  GPX_HIP(hipGetLastError());
+  return 0;
+}
+
 int run_f64(hipStream_t s, int batch, int n, int m, const double* G, long bs, long rs, long cs, int steps, const double* k,
             double eps, double alpha, double beta, const double* base, const long* bst, double* out, const long* ost, char* work) {
   const long ldx = pad32(m), lda = pad32(n);
@@ -884,19 +951,18 @@ int run_f64(hipStream_t s, int batch, int n, int m, const double* G, long bs, lo
   X[1] = X[0] + n * ldx;
   double* A = X[1] + n * ldx;
   double* B = A + n * lda;
+  double* sums = B + n * lda;
   int nparts = 0;
   NS_TRY(norm_launch<double>(s, G, bs, rs, cs, n, m, batch, part, nparts));
   const dim3 grid((m + 63) / 64, (n + 63) / 64);
   for (int z = 0; z < batch; ++z) {
     hipLaunchKernelGGL(ns_pack_f64_kernel, grid, dim3(256), 0, s, G + z * bs, bs, rs, cs, n, m, part + (long)z * PARTS, nparts, eps,
-                       X[0], ldx);
+                       X[0], X[1], ldx);
     GPX_HIP(hipGetLastError());
     int cur = 0;
     for (int it = 0; it < steps; ++it, cur ^= 1) {
-      NS_TRY(gpx_gemm_launch(s, product(X[cur], ldx, X[cur], ldx, GPX_LAY_KC, nullptr, A, lda, n, n, m, 1.0, 0.0, 1)));
-      NS_TRY(gpx_symmetrize_launch(s, n, A, lda));
-      NS_TRY(gpx_gemm_launch(s, product(A, lda, A, lda, GPX_LAY_KC, A, B, lda, n, n, n, k[2], k[1], 1)));
-      NS_TRY(gpx_symmetrize_launch(s, n, B, lda));
+      NS_TRY(symmetric_f64(s, X[cur], ldx, n, m, A, lda, sums, 1.0, 0.0, nullptr));
+      NS_TRY(symmetric_f64(s, A, lda, n, n, B, lda, sums, k[2], k[1], A));
       NS_TRY(gpx_gemm_launch(s, product(B, lda, X[cur], ldx, GPX_LAY_RC, X[cur], X[cur ^ 1], ldx, n, m, n, 1.0, k[0], 0)));
     }
     hipLaunchKernelGGL(ns_out_f64_kernel, grid, dim3(256), 0, s, X[cur], ldx, n, m, out + z * ost[0], ost[1], ost[2],
@@ -914,8 +980,10 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m) {
   if (!dtype_ok(dtype) || batch <= 0 || n <= 0 || m <= 0) return 0;
   const int small = n < m ? n : m, large = n < m ? m : n;
   const size_t parts = (size_t)batch * PARTS * 8;
-  if (dtype == GPX_F64)   // the matrices of a stack take their turns in one set of buffers
-    return parts + 8 * (2 * (size_t)small * pad32(large) + 2 * (size_t)small * pad32(small));
+  if (dtype == GPX_F64) {   // the matrices of a stack take their turns in one set of buffers
+    const size_t most = std::max(parts_f64(small, pad32(large)), parts_f64(small, pad32(small))), sums = most == 1 ? 0 : most;
+    return parts + 8 * (2 * (size_t)small * pad32(large) + (2 + sums) * (size_t)small * pad32(small));
+  }
   const size_t np = pad64(small), mp = pad64(large);
   const size_t pl = planes_of(dtype);   // X twice with two planes, X^T twice, A and B
   const size_t sums = pl == 1 ? 0 : sums_bytes((int)np, (int)mp, batch);

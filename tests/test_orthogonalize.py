@@ -91,10 +91,10 @@ def test_matches_the_definition(shape, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("shape", [(100, 3000), (2, 260, 4100), (2600, 640), (3, 64, 8000)])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", [(100, 3000), (2, 260, 4100), (2600, 640), (3, 64, 8000), (333, 1001)])
 def test_long_rows(shape, kind):
-    """Few tiles of a long K, which two planes split over workgroups."""
+    """Few tiles of a long K, which fp64 and two planes split over workgroups."""
     from gaussian_process_amd import orthogonalize
     G = make(shape, kind, seed=shape[-1])
     O = orthogonalize(G)
