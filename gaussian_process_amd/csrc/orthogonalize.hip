@@ -14,7 +14,7 @@
 //
 // Layout.  Every product has both operands k-contiguous: A needs rows of X; A is symmetric, so A A does too; and
 // B X needs rows of X^T, so the step's epilogue writes X in both orientations.  Buffers are padded to multiples of 64
-// with zeros, which the iteration preserves; the planes of a row follow each other: [row][plane][ld].
+// with zeros, which the iteration preserves.
 // The symmetric products compute tiles on and below the diagonal and write them twice.
 #include <algorithm>
 #include <cmath>
@@ -103,6 +103,11 @@ __device__ __forceinline__ double inv_norm(const double* part, int nparts, doubl
   return 1.0 / (sqrt((sm[0] + sm[1]) + (sm[2] + sm[3])) + eps);
 }
 
+// Where column c of a row is, and from there its low plane, in a row of ld columns: two planes that products read both alternate
+// every 32 columns, so that a k-tile of 32 is one line of 128 bytes; otherwise the low plane follows the high one.
+template <int NPL> __host__ __device__ __forceinline__ int in_row(int c) { return NPL == 2 ? (c >> 5) * 64 + (c & 31) : c; }
+template <int NPL> __host__ __device__ __forceinline__ int to_lo(int ld) { return NPL == 2 ? 32 : ld; }
+
 // ---- X and X^T from G --------------------------------------------------------------------------------------------
 // One 64 x 64 tile through LDS, read along G's unit stride, written along rows of X and of X^T.
 template <typename T, int NPL>
@@ -152,11 +157,11 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const T* G, long bs, long 
       th[e] = (_Float16)y;
       if (NPL == 2) tl[e] = (_Float16)(y - (float)th[e]);
     }
-    const long px = (long)(i0 + r) * 2 * mp + j0 + c0 + half * 8, pt = (long)(j0 + r) * NPL * np + i0 + c0 + half * 8;
+    const long px = (long)(i0 + r) * 2 * mp + in_row<NPL>(j0 + c0 + half * 8), pt = (long)(j0 + r) * NPL * np + in_row<NPL>(i0 + c0 + half * 8);
     *reinterpret_cast<h8*>(X + px) = xh;
-    *reinterpret_cast<h8*>(X + px + mp) = xl;
+    *reinterpret_cast<h8*>(X + px + to_lo<NPL>(mp)) = xl;
     *reinterpret_cast<h8*>(XT + pt) = th;
-    if (NPL == 2) *reinterpret_cast<h8*>(XT + pt + np) = tl;
+    if (NPL == 2) *reinterpret_cast<h8*>(XT + pt + to_lo<NPL>(np)) = tl;
   }
 }
 
@@ -257,9 +262,9 @@ __device__ __forceinline__ void finish(const NsGemm& g, float* st, long z, int r
   for (int q = 0; q < RQ; ++q) {
     eh[q] = el[q] = h8{0, 0, 0, 0, 0, 0, 0, 0};
     if (E != nullptr) {
-      const _Float16* src = E + (row0 + q * RR + lane / RL) * ldd + col0 + (lane % RL) * 8;
+      const _Float16* src = E + (row0 + q * RR + lane / RL) * ldd + in_row<NPL>(col0 + (lane % RL) * 8);
       eh[q] = *reinterpret_cast<const h8*>(src);
-      if (two) el[q] = *reinterpret_cast<const h8*>(src + g.N);
+      if (two) el[q] = *reinterpret_cast<const h8*>(src + to_lo<NPL>(g.N));
     }
   }
   stage();
@@ -279,9 +284,9 @@ __device__ __forceinline__ void finish(const NsGemm& g, float* st, long z, int r
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = v[e];
     if (D != nullptr) {
-      _Float16* dst = D + (row0 + r) * ldd + col0 + c;
+      _Float16* dst = D + (row0 + r) * ldd + in_row<NPL>(col0 + c);
       *reinterpret_cast<h8*>(dst) = hi;
-      if (two) *reinterpret_cast<h8*>(dst + g.N) = lo;
+      if (two) *reinterpret_cast<h8*>(dst + to_lo<NPL>(g.N)) = lo;
     }
   }
   __builtin_amdgcn_wave_barrier();
@@ -296,9 +301,9 @@ __device__ __forceinline__ void finish(const NsGemm& g, float* st, long z, int r
         hi[e] = (_Float16)v;
         lo[e] = (_Float16)(v - (float)hi[e]);
       }
-      _Float16* dst = DT + (col0 + c) * ldt + row0 + r;
+      _Float16* dst = DT + (col0 + c) * ldt + in_row<NPL>(row0 + r);
       *reinterpret_cast<h8*>(dst) = hi;
-      if (NPL == 2) *reinterpret_cast<h8*>(dst + g.M) = lo;
+      if (NPL == 2) *reinterpret_cast<h8*>(dst + to_lo<NPL>(g.M)) = lo;
     }
   }
   if (g.out_type == GPX_F32) write_out<float, EM, EN, P>(g, st, z, row0, col0, lane);
@@ -352,18 +357,18 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void ns_gemm_kernel(const N
   for (int p = 0; p < PA; ++p) {
     const int s = p * NT + t, r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
     const int rr = min(r, g.M - 1 - i0);
-    va[p] = (unsigned)(rr * lda + (NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16));
+    va[p] = (unsigned)(rr * lda + c * 16);
   }
 #pragma unroll
   for (int p = 0; p < PB; ++p) {
     const int s = p * NT + t, r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
     const int rr = min(r, g.N - 1 - j0);
-    vb[p] = (unsigned)(rr * ldb + (NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16));
+    vb[p] = (unsigned)(rr * ldb + c * 16);
   }
   auto load = [&](int kt, char* stage) {
     char* sA = stage + wave * 1024;
     char* sB = sA + ABYTES;
-    const unsigned so = (unsigned)kt * (BK * 2);
+    const unsigned so = (unsigned)kt * 128;
 #pragma unroll
     for (int p = 0; p < PA; ++p) dma16(ra, va[p], so, sA + p * (NT * 16));
 #pragma unroll
@@ -484,14 +489,13 @@ __global__ __launch_bounds__(64 * W) void ns_small_kernel(const NsGemm g, int ti
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const int r = p * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-    const unsigned in = NPL == 1 ? c * 16 : (c >> 2) * g.K * 2 + (c & 3) * 16;
-    va[p] = (unsigned)(r * lda) + in;
-    vb[p] = (unsigned)(r * ldb) + in;
+    va[p] = (unsigned)(r * lda + c * 16);
+    vb[p] = (unsigned)(r * ldb + c * 16);
   }
   char* mine = smem + wave * (STAGES * STAGE);
   auto load = [&](int kt, int stage) {
     char* d = mine + stage * STAGE;
-    const unsigned so = (unsigned)kt * (BK * 2);
+    const unsigned so = (unsigned)kt * 128;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       dma16(ra, va[p], so, d + p * 1024);
