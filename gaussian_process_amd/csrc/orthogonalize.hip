@@ -596,6 +596,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const NsGemm g, int tiles_
     f4 v[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) v[q] = f4{0, 0, 0, 0};
+#pragma unroll 4
     for (int p = 0; p < g.parts; ++p, src += part)
 #pragma unroll
       for (int q = 0; q < Q; ++q) v[q] += *reinterpret_cast<const f4*>(src + (long)(q * 4 + (lane >> 4)) * g.N + (lane & 15) * 4);
@@ -651,10 +652,10 @@ int launch_small(hipStream_t s, const NsGemm& g, int batch) {
 // takes 162 / 117 / 84 / 97 us with them, B X 233 / 173 / 169 / 140, at n = 1024 8.4 / 14 / 26 / 35 and 9.3 / 14 / 27 / 36.
 //
 // A product A A^T of two planes with few tiles and a long K leaves most of the chip idle while a tile's time goes with the bytes
-// that its CU loads, 9 ns per k.  K is then split over workgroups, at the price of a launch and of the sums to memory and
-// back, as far as all run at once: 10 tiles with K = 4096 36 -> 20 us, 66 with 2560 30 -> 22; not 136 of K = 3008 (33 -> 34), not of one
-// plane, whose rows come in whole lines (10 tiles with K = 4096 15 -> 14), and not larger tiles, which keep more of the chip busy
-// (136 of 128 x 128 with K = 8192 174 -> 148, nothing of it left in the whole call).
+// that its CU loads, 5 to 7 ns per k.  K is then split over workgroups, at the price of a launch and of the sums to memory and back,
+// as far as all run at once: 10 tiles with K = 4096 24 -> 14 us, 55 with 4032 26 -> 17, 66 with 2560 21 -> 16; not 136 of K = 3008
+// (which would be a second round: 23 -> 25), not of one plane (10 tiles with K = 4096 15 -> 14), and not larger tiles, which keep more
+// of the chip busy (136 of 128 x 128 with K = 8192 174 -> 148, nothing of it left in the whole call).
 struct Choice {
   int tile, parts;
 };
@@ -676,7 +677,7 @@ Choice choose(int M, int N, int K, int lower, int batch) {
   if (NPL == 2 && lower && best.tile == 0) {
     double gain = 2;   // us
     for (int p = 2; p <= 8 && tiles * p <= 256; ++p) {
-      const double g = K * 0.009 * (1 - 1.0 / p) - 8 - p * (1 + tiles * 0.008);
+      const double g = K * (0.0048 + tiles * 0.00003) * (1 - 1.0 / p) - 3 - p * (0.8 + tiles * 0.008);
       if (g > gain) {
         gain = g;
         best.parts = p;
