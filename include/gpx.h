@@ -290,7 +290,8 @@ size_t gpx_ep_sweep_work_elems(int n);
  * momentum of matrix-shaped parameters.  It has no counterpart in the reference.
  * Matrix z, element (i, j) of G is G[z * bs + i * rs + j * cs] (strides in ELEMENTS, not negative: a
  * transposed view is rs = 1); likewise out and base (base may be NULL when beta == 0).  dtype: GPX_F64, GPX_F32,
- * GPX_F16, GPX_BF16, one type for G, base and out.  out may overlap G in any way (G is read before out is written) and
+ * GPX_F16, GPX_BF16, one type for G, base and out.  out may overlap G in any way (G is read before out is written; a
+ * stack in GPX_F64, whose matrices are taken one after the other, only as G itself with the same strides) and
  * may be base with the same strides, but must not overlap base otherwise; no two elements of out may share memory.
  * Arithmetic: GPX_F64 in fp64.  The other types on the fp16 matrix cores with fp32 accumulation and intermediates
  * scaled by powers of two: GPX_BF16 with one fp16 value per element (its 11 bits lie under the 8 of the result),
@@ -322,7 +323,8 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m);
  * g may be -infinity (the state is forgotten); it is read as max(g, -200).  beta == 0 and g == 0 leave the state as it is.
  * A NaN or an infinity in a token's inputs reaches the later tokens of its sequence and heads, and may reach the earlier ones of
  * the same 64 tokens (counted from the sequence's first); no others.  1 <= dk <= 128,
- * 1 <= dv <= 1024; a token stride of v of at most 2^22.  States, decays and all sums are fp32 or wider. */
+ * 1 <= dv <= 1024; a token stride of v of at most 2^22.  Outputs overlap neither inputs nor each other, except where it is
+ * said.  States, decays and all sums are fp32 or wider. */
 typedef struct gpx_delta {
   int dtype, batch, tokens, sequences, key_heads, value_heads, dk, dv;
   double scale;

@@ -192,6 +192,19 @@ def test_update_in_place(shape, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_out_over_a_shifted_stack(kind):
+    """out one matrix behind G in the same memory, and G's matrices in the opposite order."""
+    from gaussian_process_amd import orthogonalize
+    buf = make((4, 20, 33), kind, seed=8)
+    want = orthogonalize(buf[:3].clone())
+    assert torch.equal(orthogonalize(buf[:3], out=buf[1:]), want) and torch.equal(buf[1:], want)
+    G = make((33, 33), kind, seed=9)
+    want = orthogonalize(G.clone().mT)
+    assert torch.equal(orthogonalize(G.mT, out=G), want)
+
+
+@pytest.mark.gpu
 def test_empty():
     from gaussian_process_amd import orthogonalize
     for shape in ((0, 5), (5, 0), (0, 4, 4)):
