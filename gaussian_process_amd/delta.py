@@ -195,13 +195,13 @@ def gated_delta_rule_backward(saved, d_o, d_final_state=None):
     return (*grads, d_state)
 
 
-def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, scale=None):
-    """One token for each of B rows: q, k (B, Hk, dk); v (B, Hv, dv); g, beta (B, Hv).  Returns (o, state_out).
+# What a step of these types, shapes and strides has been found to be.  A decoder makes the same call for every token, and the
+# checks and the description take as long as the rest of the call (13.5 us with them).
+_known_steps = {}
 
-    state: (n, Hv, dk, dv) float32, packed, n = B unless ``slots`` names the state of each row (int32 tensor on the device).
-    It is updated in place unless ``state_out`` (its shape, no other view of its memory) is given.  A row whose slot
-    is outside [0, n) is padding: its o is zero and no state is written for it; states that no row names are not touched.  Rows with
-    the same slot are taken in their order, as successive tokens of one sequence."""
+
+def _step_description(q, k, v, g, beta, state, slots, state_out, scale):
+    """(the bytes of a gpx_delta without its pointers, whether q, k, v are used as they are, o's shape) of a valid step."""
     import torch
     dtype, Hk, dk, Hv, dv = _check(q, k, v, g, beta, 3)
     B = q.shape[0]
@@ -215,25 +215,57 @@ def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, s
         check_tensor(slots, "slots")
         if slots.dtype != torch.int32 or tuple(slots.shape) != (B,):
             raise ValueError("slots must be an int32 tensor with one value per row")
+    _check_state(state_out, state.shape, "state_out")
+    if not state.is_contiguous() or not state_out.is_contiguous():
+        raise ValueError("state and state_out must be packed and 16-byte aligned")
+    as_used = [_dense_row(t) for t in (q, k, v)]
+    dense = all(a is b for a, b in zip(as_used, (q, k, v)))
+    d = _lib.Delta(dtype, B, 1, 0, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else scale, None, None, None, None, None, None,
+                   *map(_st_row, as_used), _st_row(g), _st_row(beta))
+    return bytes(d), dense, (B, Hv, dv)
+
+
+def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, scale=None):
+    """One token for each of B rows: q, k (B, Hk, dk); v (B, Hv, dv); g, beta (B, Hv).  Returns (o, state_out).
+
+    state: (n, Hv, dk, dv) float32, packed, n = B unless ``slots`` names the state of each row (int32 tensor on the device).
+    It is updated in place unless ``state_out`` (its shape, no other view of its memory) is given.  A row whose slot
+    is outside [0, n) is padding: its o is zero and no state is written for it; states that no row names are not touched.  Rows with
+    the same slot are taken in their order, as successive tokens of one sequence."""
+    import torch
     if state_out is None:
         state_out = state
-    else:
-        _check_state(state_out, state.shape, "state_out")
+    if scale is not None:
+        scale = float(scale)
+    try:
+        key = (scale, q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), g.dtype, g.shape,
+               g.stride(), beta.dtype, beta.shape, beta.stride(), state.dtype, state.shape, state.stride(), state_out.dtype,
+               state_out.shape, state_out.stride(), slots if slots is None else (slots.dtype, slots.shape))
+        known = _known_steps.get(key)
+    except (AttributeError, TypeError):   # not tensors: _step_description says which
+        key = known = None
+    if known is None:
+        known = _step_description(q, k, v, g, beta, state, slots, state_out, scale)
+        if len(_known_steps) >= 256:
+            _known_steps.clear()
+        if key is not None:
+            _known_steps[key] = known
     at, to = state.data_ptr(), state_out.data_ptr()
-    if not state.is_contiguous() or not state_out.is_contiguous() or (at | to) % 16:
+    if (at | to) % 16:
         raise ValueError("state and state_out must be packed and 16-byte aligned")
     if 0 < abs(to - at) < state.numel() * 4:
         raise ValueError("state_out overlaps state")
     rt = tensor_runtime(q, k, v, g, beta, state, slots, state_out)
     with rt.current_stream():
-        q, k, v = _dense_row(q), _dense_row(k), _dense_row(v)
+        description, dense, shape = known
+        if not dense:
+            q, k, v = _dense_row(q), _dense_row(k), _dense_row(v)
         if slots is not None:
             slots = slots.contiguous()
-        o = (torch.empty if slots is None else torch.zeros)((B, Hv, dv), dtype=q.dtype, device=q.device)
-        d = _lib.Delta(dtype, B, 1, 0, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), None, q.data_ptr(),
-                       k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _st_row(q), _st_row(k), _st_row(v), _st_row(g),
-                       _st_row(beta))
-        rc = rt.lib.gpx_delta_step(rt.h, C.byref(d), n, _opt(slots), at, to, o.data_ptr())
+        o = (torch.empty if slots is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
+        d = _lib.Delta.from_buffer_copy(description)
+        d.q, d.k, d.v, d.g, d.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
+        rc = rt.lib.gpx_delta_step(rt.h, C.byref(d), state.shape[0], _opt(slots), at, to, o.data_ptr())
         if rc:
             _lib.check(rc, "gpx_delta_step")
         torch.autograd.graph.increment_version(state_out)   # written behind torch's back: what was saved of it is stale
