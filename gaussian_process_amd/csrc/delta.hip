@@ -124,6 +124,7 @@ struct Args {
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
   float *Erow, *Srow;           // per head: E, dvp / 32 x C x 32; S, dvp / 32 x DK x 32
   float *Z, *dS;                // per head: Z (dX = beta Z) like E; dS' like S
+  float *d_q_part, *d_k_part;   // per head: its part of dQ and dK, C x DK
   const float *state, *d_state_out;
   float *state_out, *d_state, *d_g, *d_beta;
   void *o, *d_q, *d_k, *d_v;
@@ -1026,7 +1027,11 @@ constexpr size_t grads_room() {
   return 2 * (slices > square ? slices : square);
 }
 
-template <typename T, int DK, bool GROUPED>
+// HEADS: what a workgroup takes of a key head -- its one value head; all, one after the other; one of several, leaving its dQ and dK in
+// fp32 to delta_join_heads_kernel (where workgroups are few: 700 ragged tokens, 2 key heads, fp32: 47 -> 27 us with the joining)
+enum { ALONE, GROUPED, APART };
+
+template <typename T, int DK, int HEADS>
 __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   constexpr int N = Planes<T>::N, W = DK / 16, P = 40, PM = C + 8;
   constexpr int SL = C * P;                      // a plane of a slice
@@ -1040,12 +1045,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   float* ef = dG + 8 * C;       // exp(G), exp(G_C - G): C each
   float* red = ef + 2 * C;      // 8
   float* db = red + 8;          // C
-  constexpr bool TILES = !(GROUPED && sizeof(T) == 4);   // K and Q in LDS, where they fit
+  constexpr bool TILES = !(HEADS == GROUPED && sizeof(T) == 4);   // K and Q in LDS, where they fit
   constexpr int PV = 16 / sizeof(T), PK = DK + PV;
   T* Kt = reinterpret_cast<T*>(db + C);
   T* Qt = Kt + (TILES ? C * PK : 0);
   f4* sums = reinterpret_cast<f4*>(Qt + (TILES ? C * PK : 0));   // GROUPED: dQ and dK over the value heads so far, 8 per thread
-  const int hk = blockIdx.x % a.d.key_heads, slot = blockIdx.x / a.d.key_heads;
+  const int heads = HEADS == APART ? a.d.value_heads : a.d.key_heads, head = blockIdx.x % heads, slot = blockIdx.x / heads;
+  const int hk = HEADS == APART ? head / a.group : head;
   int s, t0, len;
   a.p.locate(slot, s, t0, len);
   if (len == 0) return;
@@ -1056,8 +1062,8 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   const long dmask = a.do_st.bs | a.do_st.rs | a.do_st.cs;
   const bool wide = (a.d.dv & 3) == 0 && (dmask & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.d_o) | reinterpret_cast<uintptr_t>(a.d_v)) & 15) == 0;
   // rows of d_q and d_k 16 bytes at a time
-  const bool whole = TILES && a.d.dk == DK && ((reinterpret_cast<uintptr_t>(a.d_q) | reinterpret_cast<uintptr_t>(a.d_k)) & 15) == 0;
-  const int group = GROUPED ? a.group : 1;
+  const bool whole = TILES && HEADS != APART && a.d.dk == DK && ((reinterpret_cast<uintptr_t>(a.d_q) | reinterpret_cast<uintptr_t>(a.d_k)) & 15) == 0;
+  const int group = HEADS == GROUPED ? a.group : 1;
   if (TILES) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs;
     const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs;
@@ -1085,7 +1091,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     const int t = tt, lane = t & 63, r4 = (lane >> 4) * 4, col = lane & 15, g8 = (lane >> 4) * 8;
     const int kc0 = wave * 16 + col;   // this lane's column of dk
     const int sr = t >> 3, sc = (t & 7) * 4;   // a thread's place in a slice: four columns of one row
-    const int hv = hk * group + m;
+    const int hv = HEADS == APART ? head : hk * group + m;
     const long at = (long)slot * a.d.value_heads + hv;
     __syncthreads();
     if (wave == 0) {
@@ -1319,7 +1325,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) dG[wave * C + rb * 16 + r4 + e] = g[e];
       kr[rb] += kc[rb];
-      if (GROUPED) {
+      if (HEADS == GROUPED) {
         if (m > 0) {
           q1[rb] += sums[rb * 512 + t];
           kr[rb] += sums[(4 + rb) * 512 + t];
@@ -1333,7 +1339,10 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = rb * 16 + r4 + e;
-          if (whole) {   // in place of Q and K, which this lane alone has read here
+          if (HEADS == APART) {
+            a.d_q_part[(at * C + r) * DK + kc0] = q1[rb][e];
+            a.d_k_part[(at * C + r) * DK + kc0] = kr[rb][e];
+          } else if (whole) {   // in place of Q and K, which this lane alone has read here
             Qt[r * PK + kc0] = (T)q1[rb][e];
             Kt[r * PK + kc0] = (T)kr[rb][e];
           } else if (r < len) {
@@ -1369,6 +1378,36 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         a.d_beta[p] = db[lane];
       }
     }
+  }
+}
+
+// dQ and dK of a chunk and key head: the sums over its value heads, in their order; 8 rows a workgroup
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_join_heads_kernel(const Args a) {
+  const int r0 = blockIdx.x % 8 * 8, hk = blockIdx.x / 8 % a.d.key_heads, slot = blockIdx.x / 8 / a.d.key_heads;
+  int s, t0, len;
+  a.p.locate(slot, s, t0, len);
+  if (r0 >= len) return;
+  const long row = a.p.row(s), at = (long)slot * a.d.value_heads + hk * a.group;
+  constexpr int IT = 8 * DK / 256;
+  float q[IT], k[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) q[i] = k[i] = 0.f;
+#pragma unroll 2
+  for (int m = 0; m < a.group; ++m)
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const long p = ((at + m) * C + r0) * DK + i * 256 + threadIdx.x;
+      q[i] += a.d_q_part[p];
+      k[i] += a.d_k_part[p];
+    }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int r = r0 + (i * 256 + threadIdx.x) / DK, c = (i * 256 + threadIdx.x) % DK;
+    if (r >= len || c >= a.d.dk) continue;
+    const long p = ((row * a.d.tokens + t0 + r) * a.d.key_heads + hk) * (long)a.d.dk + c;
+    st<T>(a.d_q, p, q[i]);
+    st<T>(a.d_k, p, k[i]);
   }
 }
 
@@ -1535,6 +1574,9 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 bool recurrent(const gpx_delta* d, int save) { return !save && d->tokens <= RECURRENT_MAX; }
 
+// gradients: value heads that share a key head on workgroups of their own
+bool apart(const gpx_delta* d) { return d->value_heads > d->key_heads && slots_of(d) * d->value_heads <= 256; }
+
 // Parts of a workspace, in this order; nullptr base: sizes only.
 enum { WORK = 0, SAVED = 1, SCRATCH = 2, WORK_SAVING = 3 };
 size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
@@ -1575,6 +1617,10 @@ size_t lay_out(const gpx_delta* d, int use, char* base, Args* a, int** off) {
   if (use == SCRATCH) {
     part(x.Z, heads * C * dvp * 4);
     part(x.dS, heads * dkp * dvp * 4);
+    if (apart(d)) {
+      part(x.d_q_part, heads * C * dkp * 4);
+      part(x.d_k_part, heads * C * dkp * 4);
+    }
   }
   return at;
 }
@@ -1686,16 +1732,22 @@ int run_backward(hipStream_t s, const Args& a) {
   constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = grads_room<T>() + C * 8 + (8 * C + 2 * C + 8 + C) * 4;
   constexpr size_t lds = base + tiles, grouped = base + (sizeof(T) == 4 ? 0 : tiles) + 8 * 512 * 16;
   static_assert(lds <= 160 * 1024 && grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
-  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, false>>(lds));
-  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, true>>(grouped));
+  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, ALONE>>(lds));
+  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, GROUPED>>(grouped));
+  DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, APART>>(lds));
   const long slots = slots_of(&a.d);
   DELTA_TRY((run_chain<T, DK, true>(s, a)));
   if (slots > 0) {
     const dim3 grid((unsigned)(slots * a.d.key_heads));
-    if (a.group == 1)
-      hipLaunchKernelGGL((delta_grads_kernel<T, DK, false>), grid, dim3(512), lds, s, a);
-    else
-      hipLaunchKernelGGL((delta_grads_kernel<T, DK, true>), grid, dim3(512), grouped, s, a);
+    if (a.group == 1) {
+      hipLaunchKernelGGL((delta_grads_kernel<T, DK, ALONE>), grid, dim3(512), lds, s, a);
+    } else if (apart(&a.d)) {
+      hipLaunchKernelGGL((delta_grads_kernel<T, DK, APART>), dim3((unsigned)(slots * a.d.value_heads)), dim3(512), lds, s, a);
+      GPX_HIP(hipGetLastError());
+      hipLaunchKernelGGL((delta_join_heads_kernel<T, DK>), dim3(grid.x * 8), dim3(256), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((delta_grads_kernel<T, DK, GROUPED>), grid, dim3(512), grouped, s, a);
+    }
     GPX_HIP(hipGetLastError());
   }
   return 0;

@@ -183,7 +183,8 @@ def test_work_bytes():
     work = kheads * 2 * square * 2 + heads * 5 * square * 2
     assert w(0) == both_ + work and w(3) == work
     assert w(1) == both_ + kheads * square * 2 + heads * (6 * square * 2 + (64 + 64) * 64 * 4)
-    assert w(2) == heads * (64 + 64) * 64 * 4
+    assert w(2) == heads * (64 + 64) * 64 * 4 + 2 * heads * square * 4   # value heads apart: their parts of d_q and d_k
+    assert w(2, batch=40) == 20 * heads * (64 + 64) * 64 * 4 and w(2, key_heads=4) == heads * (64 + 64) * 64 * 4
     assert w(0, tokens=16) == 0                                   # the recurrence needs none
     assert w(0, tokens=16, batch=1, sequences=5, offsets=256) == 256
     assert w(4) == 0 and w(0, dk=129) == 0 and w(0, dtype=0) == 0 and w(0, value_heads=3) == 0
