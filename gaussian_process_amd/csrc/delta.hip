@@ -263,10 +263,10 @@ struct Rows {
   uint4 raw[IT][W];
   __device__ __forceinline__ void fetch(const void* src, const gpx_strided& s, long row, int t0, int len, int head, int dk, int t) {
     const T* base = reinterpret_cast<const T*>(src) + row * s.bs + t0 * s.rs + head * s.cs;
-    if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(s.rs * sizeof(T))) & 15) == 0 && dk == DK) {
+    if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(s.rs * sizeof(T))) & 15) == 0 && (dk & 7) == 0) {
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {   // rows behind the end repeat the last
-        const int q = i * 256 + t, r = min(q / (DK / 8), len - 1), c = q % (DK / 8) * 8;
+      for (int i = 0; i < IT; ++i) {   // rows and columns behind the end repeat the last
+        const int q = i * 256 + t, r = min(q / (DK / 8), len - 1), c = min(q % (DK / 8) * 8, dk - 8);
         const uint4* p = reinterpret_cast<const uint4*>(base + r * s.rs + c);
 #pragma unroll
         for (int w = 0; w < W; ++w) raw[i][w] = p[w];
@@ -1062,7 +1062,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   const long dmask = a.do_st.bs | a.do_st.rs | a.do_st.cs;
   const bool wide = (a.d.dv & 3) == 0 && (dmask & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.d_o) | reinterpret_cast<uintptr_t>(a.d_v)) & 15) == 0;
   // rows of d_q and d_k 16 bytes at a time
-  const bool whole = TILES && HEADS != APART && a.d.dk == DK && ((reinterpret_cast<uintptr_t>(a.d_q) | reinterpret_cast<uintptr_t>(a.d_k)) & 15) == 0;
+  const bool whole = TILES && HEADS != APART && a.d.dk % PV == 0 && ((reinterpret_cast<uintptr_t>(a.d_q) | reinterpret_cast<uintptr_t>(a.d_k)) & 15) == 0;
   const int group = HEADS == GROUPED ? a.group : 1;
   if (TILES) {
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs;
@@ -1355,12 +1355,11 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     }
     __syncthreads();
     if (whole && m + 1 == group) {
-      const long p = ((row * a.d.tokens + t0) * a.d.key_heads + hk) * (long)DK;
-      const unsigned pitch = (unsigned)a.d.key_heads * DK;
+      const long p = ((row * a.d.tokens + t0) * a.d.key_heads + hk) * (long)a.d.dk, pitch = (long)a.d.key_heads * a.d.dk;
 #pragma unroll
       for (int i = t; i < C * DK / PV; i += 512) {
         const int r = i / (DK / PV), c = i % (DK / PV) * PV;
-        if (r >= len) continue;
+        if (r >= len || c >= a.d.dk) continue;
         *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.d_q) + p + r * pitch + c) = *reinterpret_cast<const uint4*>(Qt + r * PK + c);
         *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.d_k) + p + r * pitch + c) = *reinterpret_cast<const uint4*>(Kt + r * PK + c);
       }
