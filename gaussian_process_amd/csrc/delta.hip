@@ -33,7 +33,7 @@ namespace {
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int C = 64;          // tokens per chunk
-constexpr int DVT = 32;        // columns of a slice of dv
+constexpr int DVT = 32;        // dv is rounded up to this: columns that the gradients take at a time
 constexpr int PC = 68;         // LDS pitch of [..][64] tiles
 constexpr float G_MIN = -200.f;
 
@@ -122,7 +122,7 @@ struct Args {
   float* fac;                   // per head: exp(G), beta, exp(G_C - G) beta, exp(G_C), exp(G_C - G), exp(G) beta; C each
   __bf16 *Kf, *Qf, *KTf, *QTf;  // per key head: K and Q in state order, K^T and Q^T
   __bf16 *Tf, *Pf, *T2f, *PTf;  // per head: T, P, (I + diag(beta) N)^-T, P^T
-  float *Erow, *Srow;           // per head: E, dvp / 32 x C x 32; S, dvp / 32 x DK x 32
+  float *Erow, *Srow;           // per head: E, dvp / 16 x C x 16; S, dvp / 16 x DK x 16
   float *Z, *dS;                // per head: Z (dX = beta Z) like E; dS' like S
   float *d_q_part, *d_k_part;   // per head: its part of dQ and dK, C x DK
   const float *state, *d_state_out;
@@ -782,7 +782,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
     b8 qt[RT][2][N], of[2][N], pt[2][3];
     f4 eg[4];
     T d[4];
-    const int srow = lane >> 2, sc = (lane & 3) * 4;   // S, Z: 4 columns of one row per lane, whole 64-byte pieces
+    const int srow = lane >> 2, sc = (lane & 3) * 4;   // S, Z: 4 columns of one row per lane, a kilobyte in a row
     auto slot_of = [&](int n) { return slot0 + chunks - 1 - min(n, chunks - 1); };
     auto load_q = [&](int n) {
       const long slot = slot_of(n), at = slot * a.d.value_heads + hv;
@@ -832,13 +832,13 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       *reinterpret_cast<f4*>(&Yx[n & NB][col][wave * 16 + r4]) = y * a.scale;
     };
     auto place = [&](float* base, int n, int rows) {
-      return base + (slot_of(n) * a.d.value_heads + hv) * (long)(rows * a.dvp) + (c0 / DVT) * (rows * DVT) + c0 % DVT;
+      return base + (slot_of(n) * a.d.value_heads + hv) * (long)(rows * a.dvp) + c0 * rows;
     };
     auto store_z = [&](int n) {
       f4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
-      *reinterpret_cast<f4*>(place(a.Z, n, C) + (unsigned)((wave * 16 + srow) * DVT + sc)) = v;
+      *reinterpret_cast<f4*>(place(a.Z, n, C) + (unsigned)((wave * 16 + srow) * 16 + sc)) = v;
     };
     auto chunk = [&](int n) {
       f4 r[RT];
@@ -869,11 +869,11 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       load_p(n + 2);
       lds_barrier();
       if (n > 0) store_z(n - 1);
-      float* dst = place(a.dS, n, DK) + wave * RT * 16 * DVT;
+      float* dst = place(a.dS, n, DK) + wave * RT * 256;
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
         const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
-        *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * DVT + sc)) = f4{p[0], p[4], p[8], p[12]};
+        *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * 16 + sc)) = f4{p[0], p[4], p[8], p[12]};
       }
       lds_barrier();
     };
@@ -897,7 +897,8 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
     constexpr int SETS = TWO ? 1 : 2;
     b8 qf[SETS][4][N], pf[SETS][2][NO];
     f4 eg[SETS], bt[SETS][4], o;
-    // S and E go to memory 4 columns of one row per lane: whole 64-byte pieces
+    // S and E go to memory 4 columns of one row per lane, a kilobyte in a row (in rows of 32 columns, which two workgroups share,
+    // 186 us for 176 on 512 workgroups)
     const int srow = lane >> 2, sc = (lane & 3) * 4;
     auto load_q = [&](int u, int n) {
       const long slot = slot0 + min(n, chunks - 1), at = slot * a.d.value_heads + hv;
@@ -930,12 +931,11 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
     // E of chunk n
     auto flush = [&](int n) {
       if (a.save) {
-        float* dst = a.Erow + ((slot0 + n) * a.d.value_heads + hv) * (long)(C * a.dvp) + (c0 / DVT) * (C * DVT) +
-                     wave * 16 * DVT + c0 % DVT;
+        float* dst = a.Erow + ((slot0 + n) * a.d.value_heads + hv) * (long)(C * a.dvp) + c0 * C + wave * 256;
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
-        *reinterpret_cast<f4*>(dst + (unsigned)(srow * DVT + sc)) = v;
+        *reinterpret_cast<f4*>(dst + (unsigned)(srow * 16 + sc)) = v;
       }
     };
     auto first = [&](int u, int n) {
@@ -945,12 +945,11 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       q_part(u, n, 1);
       q_part(u, n, 2);
       if (a.save) {
-        float* dst = a.Srow + ((slot0 + n) * a.d.value_heads + hv) * (long)(DK * a.dvp) +
-                     (c0 / DVT) * (DK * DVT) + wave * RT * 16 * DVT + c0 % DVT;
+        float* dst = a.Srow + ((slot0 + n) * a.d.value_heads + hv) * (long)(DK * a.dvp) + c0 * DK + wave * RT * 256;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
-          *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * DVT + sc)) = f4{p[0], p[4], p[8], p[12]};
+          *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * 16 + sc)) = f4{p[0], p[4], p[8], p[12]};
         }
       }
     };
@@ -1117,7 +1116,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
     // a slice's values, loaded while the slice before it is multiplied (two workgroups on a CU instead, with 128 registers
     // and 56 of them spilled: 330 us for 270)
     auto load_slice = [&](int c0) {
-      const long eo = at * (C * a.dvp) + (long)c0 * C + sr * DVT + sc;
+      const long eo = at * (C * a.dvp) + (long)(c0 + (sc & 16)) * C + sr * 16 + (sc & 15);
       ev = *reinterpret_cast<const f4*>(a.Erow + eo);
       zv = *reinterpret_cast<const f4*>(a.Z + eo);
       if (wide) {
@@ -1126,7 +1125,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) yv[e] = dO[min(c0 + sc + e, a.d.dv - 1)];
       }
-      const long so = at * (DK * a.dvp) + (long)c0 * DK + min(kc0, DK - 1) * DVT + g8;
+      const long so = at * (DK * a.dvp) + (long)(c0 + (g8 & 16)) * DK + min(kc0, DK - 1) * 16 + (g8 & 15);
       const f4* p = reinterpret_cast<const f4*>(a.Srow + so);
       const f4* q = reinterpret_cast<const f4*>(a.dS + so);
       sv[0] = p[0];
