@@ -838,7 +838,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
       f4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
-      *reinterpret_cast<f4*>(place(a.Z, n, C) + (unsigned)((wave * 16 + srow) * 16 + sc)) = v;
+      __builtin_nontemporal_store(v, reinterpret_cast<f4*>(place(a.Z, n, C) + (unsigned)((wave * 16 + srow) * 16 + sc)));
     };
     auto chunk = [&](int n) {
       f4 r[RT];
@@ -873,7 +873,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
         const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
-        *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * 16 + sc)) = f4{p[0], p[4], p[8], p[12]};
+        __builtin_nontemporal_store(f4{p[0], p[4], p[8], p[12]}, reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * 16 + sc)));
       }
       lds_barrier();
     };
@@ -897,8 +897,8 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
     constexpr int SETS = TWO ? 1 : 2;
     b8 qf[SETS][4][N], pf[SETS][2][NO];
     f4 eg[SETS], bt[SETS][4], o;
-    // S and E go to memory 4 columns of one row per lane, a kilobyte in a row (in rows of 32 columns, which two workgroups share,
-    // 186 us for 176 on 512 workgroups)
+    // S and E go to memory 4 columns of one row per lane, a kilobyte in a row, past the caches that the operands need (2 x 4096 tokens:
+    // 207 us in rows of 32 columns, which two workgroups share, 205 in a row, 201 past the caches; backward 200, 194, 185)
     const int srow = lane >> 2, sc = (lane & 3) * 4;
     auto load_q = [&](int u, int n) {
       const long slot = slot0 + min(n, chunks - 1), at = slot * a.d.value_heads + hv;
@@ -935,7 +935,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = Ex[n & 1][sc + e][wave * 16 + srow];
-        *reinterpret_cast<f4*>(dst + (unsigned)(srow * 16 + sc)) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<f4*>(dst + (unsigned)(srow * 16 + sc)));
       }
     };
     auto first = [&](int u, int n) {
@@ -949,7 +949,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           const float* p = reinterpret_cast<const float*>(&Sx[n & 1][wave][i][(srow >> 2) * 16 + sc]) + (srow & 3);
-          *reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * 16 + sc)) = f4{p[0], p[4], p[8], p[12]};
+          __builtin_nontemporal_store(f4{p[0], p[4], p[8], p[12]}, reinterpret_cast<f4*>(dst + (unsigned)((i * 16 + srow) * 16 + sc)));
         }
       }
     };
