@@ -348,9 +348,16 @@ __device__ __forceinline__ void unit_lower_inverse(const float* A, float* Ti, fl
   }
 }
 
+// PAST: past the caches
+template <bool PAST>
+__device__ __forceinline__ void store_frag(__bf16* p, b8 v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<b8*>(p));
+  else *reinterpret_cast<b8*>(p) = v;
+}
+
 // rows, or with TR columns, of a lower triangular C x C matrix in LDS (pitch PC) as fragments in natural order; those that
 // hold only zeros are neither written nor read
-template <int NPL, bool TR>
+template <int NPL, bool TR, bool PAST>
 __device__ __forceinline__ void store_square(const float* M, __bf16* dst, int t) {
   for (int i = t; i < TF / 8; i += 256) {
     const int lane = i & 63, ks = i >> 6 & 1, rb = i >> 7;
@@ -362,7 +369,7 @@ __device__ __forceinline__ void store_square(const float* M, __bf16* dst, int t)
     b8 v[NPL];
     split<8, NPL>(x, v);
 #pragma unroll
-    for (int k = 0; k < NPL; ++k) *reinterpret_cast<b8*>(dst + k * TF + i * 8) = v[k];
+    for (int k = 0; k < NPL; ++k) store_frag<PAST>(dst + k * TF + i * 8, v[k]);
   }
 }
 
@@ -373,13 +380,15 @@ template <typename T> struct OutPlanes { static constexpr int N = sizeof(T) == 2
 // Many chunks: bound by memory, mostly its own stores (2048 chunks of 128 x 128 in bf16: 231 MB in 60 us, 337 MB in 84 with what
 // training keeps).  Few: by the inverse and its barriers, 24 us for one chunk in fp32, so that value heads that share a key head get a
 // workgroup each while these fit the chip twice (fp32, 28 chunks of two heads: 33 -> 25 us; fp16, 348: 28 -> 38, so not there).
+// PAST: what it writes goes past the caches, for large training steps, in whose scans it would not last in them (2048 chunks: 83 -> 81 us,
+// the scans 193 -> 185; forward alone 59 -> 50, but the scan 239 -> 249; small steps 24 -> 23 and 22 -> 23).
 template <typename T, int DK>
 constexpr size_t chunk_room() {
   constexpr size_t first = 2 * Planes<T>::N * C * (DK + 8) * 2, second = (2 * C * PC + 32 * 36) * 4;
   return first > second ? first : second;
 }
 
-template <typename T, int DK>
+template <typename T, int DK, bool PAST>
 __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_kernel(const Args a) {
   constexpr int N = Planes<T>::N, P = DK + 8, RT = DK / 64, KSN = DK / 32;
   extern __shared__ __align__(16) char smem[];
@@ -448,8 +457,8 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
       const b4 x0 = *reinterpret_cast<const b4*>(x), y0 = *reinterpret_cast<const b4*>(y);
       const b4 x1 = RT == 2 ? *reinterpret_cast<const b4*>(x + 16 * (RT - 1)) : z;
       const b4 y1 = RT == 2 ? *reinterpret_cast<const b4*>(y + 16 * (RT - 1)) : z;
-      *reinterpret_cast<b8*>(a.Kf + (atk * N + k) * KF + i * 8) = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-      *reinterpret_cast<b8*>(a.Qf + (atk * N + k) * KF + i * 8) = __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7);
+      store_frag<PAST>(a.Kf + (atk * N + k) * KF + i * 8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+      store_frag<PAST>(a.Qf + (atk * N + k) * KF + i * 8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
   for (int i = mine; i < DK * C / 8; i += 256) {
@@ -463,8 +472,8 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
         v[e] = K[(k * C + r + e) * P + c];
         w[e] = Q[(k * C + r + e) * P + c];
       }
-      *reinterpret_cast<b8*>(a.KTf + (atk * N + k) * (DK * C) + i * 8) = v;
-      if (a.save) *reinterpret_cast<b8*>(a.QTf + (atk * N + k) * (DK * C) + i * 8) = w;
+      store_frag<PAST>(a.KTf + (atk * N + k) * (DK * C) + i * 8, v);
+      if (a.save) store_frag<PAST>(a.QTf + (atk * N + k) * (DK * C) + i * 8, w);
     }
   }
   // K K^T and Q K^T: wave w the rows 16 w ..
@@ -514,11 +523,11 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
       }
     }
     __syncthreads();
-    store_square<OutPlanes<T>::N, false>(M, a.Pf + at * OutPlanes<T>::N * TF, t);
-    if (a.save) store_square<3, true>(M, a.PTf + at * 3 * TF, t);
+    store_square<OutPlanes<T>::N, false, PAST>(M, a.Pf + at * OutPlanes<T>::N * TF, t);
+    if (a.save) store_square<3, true, PAST>(M, a.PTf + at * 3 * TF, t);
     __syncthreads();
     unit_lower_inverse(A, M, tmp, wave, lane);
-    store_square<3, false>(M, a.Tf + at * 3 * TF, t);
+    store_square<3, false, PAST>(M, a.Tf + at * 3 * TF, t);
     if (a.save) {   // (I + diag(beta) N)^-1 = I - diag(beta) T N
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -545,7 +554,7 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
         }
       }
       __syncthreads();
-      store_square<3, true>(A, a.T2f + at * 3 * TF, t);
+      store_square<3, true, PAST>(A, a.T2f + at * 3 * TF, t);
     }
     __syncthreads();
   }
@@ -1720,10 +1729,13 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
   }
   constexpr size_t lds = chunk_room<T, DK>() + C * 8 + C * 4;
   static_assert(lds <= 160 * 1024, "LDS");
-  DELTA_TRY(allow_lds<&delta_chunk_kernel<T, DK>>(lds));
+  DELTA_TRY(allow_lds<&delta_chunk_kernel<T, DK, false>>(lds));
+  DELTA_TRY(allow_lds<&delta_chunk_kernel<T, DK, true>>(lds));
   const long slots = slots_of(&a.d);
   if (slots > 0) {
-    hipLaunchKernelGGL((delta_chunk_kernel<T, DK>), dim3((unsigned)(slots * a.d.key_heads * a.parts)), dim3(256), lds, s, a);
+    const dim3 grid((unsigned)(slots * a.d.key_heads * a.parts));
+    if (a.save && slots * a.d.value_heads > 512) hipLaunchKernelGGL((delta_chunk_kernel<T, DK, true>), grid, dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((delta_chunk_kernel<T, DK, false>), grid, dim3(256), lds, s, a);
     GPX_HIP(hipGetLastError());
   }
   return run_chain<T, DK, false>(s, a);
