@@ -720,8 +720,11 @@ __global__ __launch_bounds__(256) void ns_pack_f64_kernel(const double* G, long 
   __shared__ double tile[64][65];
   __shared__ double sm[4];
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, t = threadIdx.x;
-  const double f = inv_norm(part, nparts, eps, sm);
+  const double f = inv_norm(part + (long)blockIdx.z * PARTS, nparts, eps, sm);
   const bool along_rows = rs == 1 && cs != 1;
+  G += blockIdx.z * bs;
+  X += blockIdx.z * (n * ldx);
+  Y += blockIdx.z * (n * ldx);
   for (int q = 0; q < 16; ++q) {
     const int a = q * 4 + (t >> 6), b = t & 63;
     const int i = along_rows ? b : a, j = along_rows ? a : b;
@@ -745,6 +748,9 @@ __global__ __launch_bounds__(256) void ns_join_f64_kernel(int n, const double* s
   const int bi = blockIdx.y, bj = blockIdx.x, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   if (bj > bi) return;
   const long part = n * ld;
+  sums += blockIdx.z * (PARTS_ * part);
+  S += blockIdx.z * part;
+  if (base != nullptr) base += blockIdx.z * part;
   double v[4][PARTS_], b[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -771,9 +777,13 @@ __global__ __launch_bounds__(256) void ns_join_f64_kernel(int n, const double* s
   }
 }
 
-__global__ __launch_bounds__(256) void ns_out_f64_kernel(const double* X, long ldx, int n, int m, double* out, long rs, long cs,
-                                                         const double* base, long brs, long bcs, double alpha, double beta) {
+__global__ __launch_bounds__(256) void ns_out_f64_kernel(const double* X, long ldx, int n, int m, double* out, long bs, long rs,
+                                                         long cs, const double* base, long bbs, long brs, long bcs, double alpha,
+                                                         double beta) {
   __shared__ double tile[64][65];
+  X += blockIdx.z * (n * ldx);
+  out += blockIdx.z * bs;
+  if (base != nullptr) base += blockIdx.z * bbs;
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, t = threadIdx.x;
   for (int q = 0; q < 16; ++q) {
     const int i = q * 4 + (t >> 6), j = t & 63;
@@ -920,28 +930,38 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
 
 // Parts into which K (padded to 32) of a symmetric n x n product is split, as a batch of slices of K, until its tiles of 64 x 64 fill
 // most of the chip's 512 places.  Whole calls: 1024 x 2048 1131 -> 872 us (988 if half of the places will do), 300 x 700 669 -> 371.
-int parts_f64(int n, long k) {
-  const long nt = (n + 63) / 64, tiles = nt * (nt + 1) / 2;
+int parts_f64(int n, long k, int batch) {
+  const long nt = (n + 63) / 64, tiles = nt * (nt + 1) / 2 * batch;
   int parts = 1;
   while (parts < 8 && tiles * parts < 400 && k / (parts * 2) >= 128) parts *= 2;
   return parts;
 }
+// the matrices of sums that the symmetric products of a call keep, per matrix of the stack
+int sums_f64(int n, long ldx, long lda, int batch) {
+  const int most = std::max(parts_f64(n, ldx, batch), parts_f64(n, lda, batch));
+  return batch == 1 && most == 1 ? 0 : most;
+}
 
-// S = alpha R R^T + beta base
-int symmetric_f64(hipStream_t s, const double* R, long ldr, int n, int k, double* S, long ld, double* sums, double alpha, double beta,
-                  const double* base) {
-  const int parts = parts_f64(n, ldr);
-  if (parts == 1) {
+// S = alpha R R^T + beta base, whole; matrices of a stack follow each other
+int symmetric_f64(hipStream_t s, const double* R, long ldr, int batch, int n, int k, double* S, long ld, double* sums, double alpha,
+                  double beta, const double* base) {
+  const int parts = parts_f64(n, ldr, batch);
+  if (batch == 1 && parts == 1) {
     NS_TRY(gpx_gemm_launch(s, product(R, ldr, R, ldr, GPX_LAY_KC, base, S, ld, n, n, k, alpha, beta, 1)));
     return gpx_symmetrize_launch(s, n, S, ld);
   }
-  GemmDesc g = product(R, ldr, R, ldr, GPX_LAY_KC, nullptr, sums, ld, n, n, (int)(ldr / parts), 1.0, 0.0, 1);
-  g.batch = parts;
-  g.stride_a = g.stride_b = ldr / parts;
+  const int slice = parts == 1 ? k : (int)(ldr / parts);   // the padding is zeros
+  GemmDesc g = product(R, ldr, R, ldr, GPX_LAY_KC, nullptr, sums, ld, n, n, slice, 1.0, 0.0, 1);
+  g.batch = batch * parts;
+  g.batch_inner = parts;
+  g.stride_a = g.stride_b = slice;
   g.stride_d = n * ld;
+  g.stride2_a = g.stride2_b = n * ldr;
+  g.stride2_d = parts * g.stride_d;
   NS_TRY(gpx_gemm_launch(s, g));
-  const dim3 grid((n + 31) / 32, (n + 31) / 32);
-  if (parts == 2) hipLaunchKernelGGL(ns_join_f64_kernel<2>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
+  const dim3 grid((n + 31) / 32, (n + 31) / 32, batch);
+  if (parts == 1) hipLaunchKernelGGL(ns_join_f64_kernel<1>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
+  else if (parts == 2) hipLaunchKernelGGL(ns_join_f64_kernel<2>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
   else if (parts == 4) hipLaunchKernelGGL(ns_join_f64_kernel<4>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
   else hipLaunchKernelGGL(ns_join_f64_kernel<8>, grid, dim3(256), 0, s, n, sums, alpha, beta, base, S, ld);
   GPX_HIP(hipGetLastError());
@@ -950,30 +970,31 @@ int symmetric_f64(hipStream_t s, const double* R, long ldr, int n, int k, double
 
 int run_f64(hipStream_t s, int batch, int n, int m, const double* G, long bs, long rs, long cs, int steps, const double* k,
             double eps, double alpha, double beta, const double* base, const long* bst, double* out, const long* ost, char* work) {
-  const long ldx = pad32(m), lda = pad32(n);
+  const long ldx = pad32(m), lda = pad32(n), xs = batch * (n * ldx), as = batch * (n * lda);
   double* part = reinterpret_cast<double*>(work);
   double* X[2] = {part + (size_t)batch * PARTS, nullptr};
-  X[1] = X[0] + n * ldx;
-  double* A = X[1] + n * ldx;
-  double* B = A + n * lda;
-  double* sums = B + n * lda;
+  X[1] = X[0] + xs;
+  double* A = X[1] + xs;
+  double* B = A + as;
+  double* sums = B + as;
   int nparts = 0;
   NS_TRY(norm_launch<double>(s, G, bs, rs, cs, n, m, batch, part, nparts));
-  const dim3 grid((m + 63) / 64, (n + 63) / 64);
-  for (int z = 0; z < batch; ++z) {
-    hipLaunchKernelGGL(ns_pack_f64_kernel, grid, dim3(256), 0, s, G + z * bs, bs, rs, cs, n, m, part + (long)z * PARTS, nparts, eps,
-                       X[0], X[1], ldx);
-    GPX_HIP(hipGetLastError());
-    int cur = 0;
-    for (int it = 0; it < steps; ++it, cur ^= 1) {
-      NS_TRY(symmetric_f64(s, X[cur], ldx, n, m, A, lda, sums, 1.0, 0.0, nullptr));
-      NS_TRY(symmetric_f64(s, A, lda, n, n, B, lda, sums, k[2], k[1], A));
-      NS_TRY(gpx_gemm_launch(s, product(B, lda, X[cur], ldx, GPX_LAY_RC, X[cur], X[cur ^ 1], ldx, n, m, n, 1.0, k[0], 0)));
-    }
-    hipLaunchKernelGGL(ns_out_f64_kernel, grid, dim3(256), 0, s, X[cur], ldx, n, m, out + z * ost[0], ost[1], ost[2],
-                       base == nullptr ? nullptr : base + z * bst[0], bst[1], bst[2], alpha, beta);
-    GPX_HIP(hipGetLastError());
+  const dim3 grid((m + 63) / 64, (n + 63) / 64, batch);
+  hipLaunchKernelGGL(ns_pack_f64_kernel, grid, dim3(256), 0, s, G, bs, rs, cs, n, m, part, nparts, eps, X[0], X[1], ldx);
+  GPX_HIP(hipGetLastError());
+  int cur = 0;
+  for (int it = 0; it < steps; ++it, cur ^= 1) {
+    NS_TRY(symmetric_f64(s, X[cur], ldx, batch, n, m, A, lda, sums, 1.0, 0.0, nullptr));
+    NS_TRY(symmetric_f64(s, A, lda, batch, n, n, B, lda, sums, k[2], k[1], A));
+    GemmDesc g = product(B, lda, X[cur], ldx, GPX_LAY_RC, X[cur], X[cur ^ 1], ldx, n, m, n, 1.0, k[0], 0);
+    g.batch = batch;
+    g.stride_a = n * lda;
+    g.stride_b = g.stride_d = n * ldx;
+    NS_TRY(gpx_gemm_launch(s, g));
   }
+  hipLaunchKernelGGL(ns_out_f64_kernel, grid, dim3(256), 0, s, X[cur], ldx, n, m, out, ost[0], ost[1], ost[2], base, bst[0], bst[1],
+                     bst[2], alpha, beta);
+  GPX_HIP(hipGetLastError());
   return 0;
 }
 
@@ -985,9 +1006,9 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m) {
   if (!dtype_ok(dtype) || batch <= 0 || n <= 0 || m <= 0) return 0;
   const int small = n < m ? n : m, large = n < m ? m : n;
   const size_t parts = (size_t)batch * PARTS * 8;
-  if (dtype == GPX_F64) {   // the matrices of a stack take their turns in one set of buffers
-    const size_t most = std::max(parts_f64(small, pad32(large)), parts_f64(small, pad32(small))), sums = most == 1 ? 0 : most;
-    return parts + 8 * (2 * (size_t)small * pad32(large) + (2 + sums) * (size_t)small * pad32(small));
+  if (dtype == GPX_F64) {
+    const size_t lx = pad32(large), la = pad32(small);
+    return parts + 8 * (size_t)batch * small * (2 * lx + (2 + sums_f64(small, lx, la, batch)) * la);
   }
   const size_t np = pad64(small), mp = pad64(large);
   const size_t pl = planes_of(dtype);   // X twice with two planes, X^T twice, A and B

@@ -95,9 +95,6 @@ def orthogonalize(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, alpha=1.0, be
     o3 = _stack(out)
     if o3 is None:
         raise ValueError("the leading dimensions of out have no common stride")
-    if (G.dtype == torch.float64 and G.untyped_storage().data_ptr() == out.untyped_storage().data_ptr()
-            and (G.data_ptr() != out.data_ptr() or G.stride() != out.stride())):
-        G = G.clone()   # another view of out's memory, whose matrices are read after others have been written
     g3 = _stack(G)
     if g3 is None:
         g3 = _stack(G.contiguous())

@@ -290,8 +290,7 @@ size_t gpx_ep_sweep_work_elems(int n);
  * momentum of matrix-shaped parameters.  It has no counterpart in the reference.
  * Matrix z, element (i, j) of G is G[z * bs + i * rs + j * cs] (strides in ELEMENTS, not negative: a
  * transposed view is rs = 1); likewise out and base (base may be NULL when beta == 0).  dtype: GPX_F64, GPX_F32,
- * GPX_F16, GPX_BF16, one type for G, base and out.  out may overlap G in any way (G is read before out is written; a
- * stack in GPX_F64, whose matrices are taken one after the other, only as G itself with the same strides) and
+ * GPX_F16, GPX_BF16, one type for G, base and out.  out may overlap G in any way (G is read before out is written) and
  * may be base with the same strides, but must not overlap base otherwise; no two elements of out may share memory.
  * Arithmetic: GPX_F64 in fp64.  The other types on the fp16 matrix cores with fp32 accumulation and intermediates
  * scaled by powers of two: GPX_BF16 with one fp16 value per element (its 11 bits lie under the 8 of the result),
