@@ -21,7 +21,7 @@
 // Kernels: plan (where packed sequences are), chunk (parallel over chunks: T, P, G, operands in the scans' order), the chain (over the
 // chunks of a sequence, parallel over heads and slices of dv, which are independent) and its reverse, and grads (parallel over
 // chunks).  Short inputs and single tokens go through the recurrence itself.  8192 tokens x 16 heads, bf16, dk = dv = 128: chunk 60 us,
-// chain 237; training on 2 x 4096 tokens: 84, 197 and 210, grads 235.
+// chain 237; training on 2 x 4096 tokens: 81, 191 and 182, grads 230.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -573,8 +573,8 @@ __global__ __launch_bounds__(256, Planes<T>::N == 1 ? 4 : 1) void delta_chunk_ke
 // since loads behind branches make the compiler wait for all that are under way.
 // 8192 tokens x 16 heads, bf16, dk = dv = 128, 128 workgroups: 237 us, 1.85 a chunk, of which 78 KB of operands take 0.5 at L1's 64
 // bytes a clock; without any access to memory 137; with the outputs in a kernel of their own 256 and 68; with 32 columns to a
-// workgroup 349.  Training on 2 x 4096 tokens, 256 workgroups: 197 forward, 130 to 140 without the stores of S and E (200 MB),
-// 210 back, where Y from a kernel of its own took 54 more.
+// workgroup 349.  Training on 2 x 4096 tokens, 256 workgroups: 191 forward, 130 to 140 without the stores of S and E (200 MB),
+// 182 back, where Y from a kernel of its own took 54 more.
 __device__ __forceinline__ b8 ld_frag(const __bf16* uniform, unsigned lane_bytes) {
   return *reinterpret_cast<const b8*>(reinterpret_cast<const char*>(uniform) + lane_bytes);
 }
@@ -1029,7 +1029,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 // 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
 // memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
 // the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
-// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 235 us for 655 MB, 2.8 TB/s.  The slices wait for memory (a third of the time),
+// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 230 us for 655 MB, 2.8 TB/s.  The slices wait for memory (a third of the time),
 // the steps after them for LDS, where all waves read the whole C x C matrix; neither overlaps the other, since the registers leave one
 // workgroup to a CU.  One that went on from chunk to chunk with the next one's first loads under way took as long.
 // LDS of the slices, which a C x C matrix of three planes takes over

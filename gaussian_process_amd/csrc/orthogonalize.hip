@@ -716,15 +716,15 @@ size_t sums_bytes(int np, int mp, int batch) {
 
 // ---- fp64: the framework's own products ----------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void ns_pack_f64_kernel(const double* G, long bs, long rs, long cs, int n, int m,
-                                                          const double* part, int nparts, double eps, double* X, double* Y, long ldx) {
+                                                          const double* part, int nparts, double eps, double* X, double* Y, int rows, long ldx) {
   __shared__ double tile[64][65];
   __shared__ double sm[4];
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, t = threadIdx.x;
   const double f = inv_norm(part + (long)blockIdx.z * PARTS, nparts, eps, sm);
   const bool along_rows = rs == 1 && cs != 1;
   G += blockIdx.z * bs;
-  X += blockIdx.z * (n * ldx);
-  Y += blockIdx.z * (n * ldx);
+  X += blockIdx.z * (rows * ldx);
+  Y += blockIdx.z * (rows * ldx);
   for (int q = 0; q < 16; ++q) {
     const int a = q * 4 + (t >> 6), b = t & 63;
     const int i = along_rows ? b : a, j = along_rows ? a : b;
@@ -733,9 +733,10 @@ __global__ __launch_bounds__(256) void ns_pack_f64_kernel(const double* G, long 
   __syncthreads();
   for (int q = 0; q < 16; ++q) {
     const int i = q * 4 + (t >> 6), j = t & 63;
-    if (i0 + i >= n || j0 + j >= ldx) continue;
-    X[(i0 + i) * ldx + j0 + j] = j0 + j < m ? tile[i][j] : 0.0;
-    if (j0 + j >= m) Y[(i0 + i) * ldx + j0 + j] = 0.0;   // the other buffer's padding too
+    if (i0 + i >= rows || j0 + j >= ldx) continue;
+    const bool in = i0 + i < n && j0 + j < m;
+    X[(i0 + i) * ldx + j0 + j] = in ? tile[i][j] : 0.0;
+    if (!in) Y[(i0 + i) * ldx + j0 + j] = 0.0;   // the other buffer's padding too
   }
 }
 
@@ -777,11 +778,27 @@ __global__ __launch_bounds__(256) void ns_join_f64_kernel(int n, const double* s
   }
 }
 
+// Y = alpha X + the sum of the parts, n x m; a row of a matrix a workgroup
+template <int PARTS_>
+__global__ __launch_bounds__(256) void ns_sum_f64_kernel(int n, int m, const double* sums, double alpha, const double* X, double* Y,
+                                                         int rows, long ld) {
+  const long at = blockIdx.z * (rows * ld) + blockIdx.y * ld, part = n * ld;
+  sums += blockIdx.z * (PARTS_ * part) + blockIdx.y * ld;
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= m) return;
+  double v[PARTS_], x = alpha * X[at + j];
+#pragma unroll
+  for (int p = 0; p < PARTS_; ++p) v[p] = sums[p * part + j];
+#pragma unroll
+  for (int p = 0; p < PARTS_; ++p) x += v[p];
+  Y[at + j] = x;
+}
+
 __global__ __launch_bounds__(256) void ns_out_f64_kernel(const double* X, long ldx, int n, int m, double* out, long bs, long rs,
                                                          long cs, const double* base, long bbs, long brs, long bcs, double alpha,
-                                                         double beta) {
+                                                         double beta, int rows) {
   __shared__ double tile[64][65];
-  X += blockIdx.z * (n * ldx);
+  X += blockIdx.z * (rows * ldx);
   out += blockIdx.z * bs;
   if (base != nullptr) base += blockIdx.z * bbs;
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, t = threadIdx.x;
@@ -928,24 +945,31 @@ int run_half(hipStream_t s, int dtype, int batch, int n, int m, const void* G, l
   return 0;
 }
 
-// Parts into which K (padded to 32) of a symmetric n x n product is split, as a batch of slices of K, until its tiles of 64 x 64 fill
-// most of the chip's 512 places.  Whole calls: 1024 x 2048 1131 -> 872 us (988 if half of the places will do), 300 x 700 669 -> 371.
-int parts_f64(int n, long k, int batch) {
-  const long nt = (n + 63) / 64, tiles = nt * (nt + 1) / 2 * batch;
+// Parts into which K (padded to 32 with zeros) of a product is split, as a batch of slices of K, until its tiles of 64 x 64 fill most of
+// the chip's 512 places.  Whole calls, half products alone: 1024 x 2048 1131 -> 872 us (988 if half of the places will do), 300 x 700
+// 669 -> 321 (371 with slices of 128 and more); with X's product 300 x 700 257, 1000 x 1000 845 -> 784.
+int parts_f64(long tiles, long k) {
   int parts = 1;
-  while (parts < 8 && tiles * parts < 400 && k / (parts * 2) >= 128) parts *= 2;
+  while (parts < 8 && tiles * parts < 400 && k / (parts * 2) >= 64) parts *= 2;
   return parts;
 }
-// the matrices of sums that the symmetric products of a call keep, per matrix of the stack
-int sums_f64(int n, long ldx, long lda, int batch) {
-  const int most = std::max(parts_f64(n, ldx, batch), parts_f64(n, lda, batch));
-  return batch == 1 && most == 1 ? 0 : most;
+int half_parts_f64(int n, long k, int batch) {
+  const long nt = (n + 63) / 64;
+  return parts_f64(nt * (nt + 1) / 2 * batch, k);
+}
+// of the product with X.  Where it is split the half products are, so that B's padding is zeros: they have fewer tiles.
+int step_parts_f64(int n, int m, int batch) { return parts_f64((long)((n + 63) / 64) * ((m + 63) / 64) * batch, pad32(n)); }
+// elements of the sums that a call keeps, per matrix of the stack
+size_t sums_f64(int n, int m, int batch) {
+  const long ldx = pad32(m), lda = pad32(n);
+  const int half = std::max(half_parts_f64(n, ldx, batch), half_parts_f64(n, lda, batch)), step = step_parts_f64(n, m, batch);
+  return std::max(batch == 1 && half == 1 ? 0 : half * (n * lda), step == 1 ? 0 : step * (n * ldx));
 }
 
 // S = alpha R R^T + beta base, whole; matrices of a stack follow each other
-int symmetric_f64(hipStream_t s, const double* R, long ldr, int batch, int n, int k, double* S, long ld, double* sums, double alpha,
-                  double beta, const double* base) {
-  const int parts = parts_f64(n, ldr, batch);
+int symmetric_f64(hipStream_t s, const double* R, long ldr, long rs, int batch, int n, int k, double* S, long ld, double* sums,
+                  double alpha, double beta, const double* base) {
+  const int parts = half_parts_f64(n, ldr, batch);
   if (batch == 1 && parts == 1) {
     NS_TRY(gpx_gemm_launch(s, product(R, ldr, R, ldr, GPX_LAY_KC, base, S, ld, n, n, k, alpha, beta, 1)));
     return gpx_symmetrize_launch(s, n, S, ld);
@@ -956,7 +980,7 @@ int symmetric_f64(hipStream_t s, const double* R, long ldr, int batch, int n, in
   g.batch_inner = parts;
   g.stride_a = g.stride_b = slice;
   g.stride_d = n * ld;
-  g.stride2_a = g.stride2_b = n * ldr;
+  g.stride2_a = g.stride2_b = rs;
   g.stride2_d = parts * g.stride_d;
   NS_TRY(gpx_gemm_launch(s, g));
   const dim3 grid((n + 31) / 32, (n + 31) / 32, batch);
@@ -970,30 +994,51 @@ int symmetric_f64(hipStream_t s, const double* R, long ldr, int batch, int n, in
 
 int run_f64(hipStream_t s, int batch, int n, int m, const double* G, long bs, long rs, long cs, int steps, const double* k,
             double eps, double alpha, double beta, const double* base, const long* bst, double* out, const long* ost, char* work) {
-  const long ldx = pad32(m), lda = pad32(n), xs = batch * (n * ldx), as = batch * (n * lda);
+  const long ldx = pad32(m), lda = pad32(n), xs = lda * ldx, as = n * lda;   // of a matrix: X has zeros for rows up to lda
   double* part = reinterpret_cast<double*>(work);
   double* X[2] = {part + (size_t)batch * PARTS, nullptr};
-  X[1] = X[0] + xs;
-  double* A = X[1] + xs;
-  double* B = A + as;
-  double* sums = B + as;
+  X[1] = X[0] + batch * xs;
+  double* A = X[1] + batch * xs;
+  double* B = A + batch * as;
+  double* sums = B + batch * as;
   int nparts = 0;
   NS_TRY(norm_launch<double>(s, G, bs, rs, cs, n, m, batch, part, nparts));
   const dim3 grid((m + 63) / 64, (n + 63) / 64, batch);
-  hipLaunchKernelGGL(ns_pack_f64_kernel, grid, dim3(256), 0, s, G, bs, rs, cs, n, m, part, nparts, eps, X[0], X[1], ldx);
+  hipLaunchKernelGGL(ns_pack_f64_kernel, grid, dim3(256), 0, s, G, bs, rs, cs, n, m, part, nparts, eps, X[0], X[1],
+                     (int)lda, ldx);
   GPX_HIP(hipGetLastError());
   int cur = 0;
   for (int it = 0; it < steps; ++it, cur ^= 1) {
-    NS_TRY(symmetric_f64(s, X[cur], ldx, batch, n, m, A, lda, sums, 1.0, 0.0, nullptr));
-    NS_TRY(symmetric_f64(s, A, lda, batch, n, n, B, lda, sums, k[2], k[1], A));
-    GemmDesc g = product(B, lda, X[cur], ldx, GPX_LAY_RC, X[cur], X[cur ^ 1], ldx, n, m, n, 1.0, k[0], 0);
-    g.batch = batch;
-    g.stride_a = n * lda;
-    g.stride_b = g.stride_d = n * ldx;
+    NS_TRY(symmetric_f64(s, X[cur], ldx, xs, batch, n, m, A, lda, sums, 1.0, 0.0, nullptr));
+    NS_TRY(symmetric_f64(s, A, lda, as, batch, n, n, B, lda, sums, k[2], k[1], A));
+    const int parts = step_parts_f64(n, m, batch);
+    if (parts == 1) {
+      GemmDesc g = product(B, lda, X[cur], ldx, GPX_LAY_RC, X[cur], X[cur ^ 1], ldx, n, m, n, 1.0, k[0], 0);
+      g.batch = batch;
+      g.stride_a = as;
+      g.stride_b = g.stride_d = xs;
+      NS_TRY(gpx_gemm_launch(s, g));
+      continue;
+    }
+    const int slice = (int)(lda / parts);
+    GemmDesc g = product(B, lda, X[cur], ldx, GPX_LAY_RC, nullptr, sums, ldx, n, m, slice, 1.0, 0.0, 0);
+    g.batch = batch * parts;
+    g.batch_inner = parts;
+    g.stride_a = slice;
+    g.stride_b = slice * ldx;
+    g.stride_d = n * ldx;
+    g.stride2_a = as;
+    g.stride2_b = xs;
+    g.stride2_d = parts * g.stride_d;
     NS_TRY(gpx_gemm_launch(s, g));
+    const dim3 rows((m + 255) / 256, n, batch);
+    if (parts == 2) hipLaunchKernelGGL(ns_sum_f64_kernel<2>, rows, dim3(256), 0, s, n, m, sums, k[0], X[cur], X[cur ^ 1], (int)lda, ldx);
+    else if (parts == 4) hipLaunchKernelGGL(ns_sum_f64_kernel<4>, rows, dim3(256), 0, s, n, m, sums, k[0], X[cur], X[cur ^ 1], (int)lda, ldx);
+    else hipLaunchKernelGGL(ns_sum_f64_kernel<8>, rows, dim3(256), 0, s, n, m, sums, k[0], X[cur], X[cur ^ 1], (int)lda, ldx);
+    GPX_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL(ns_out_f64_kernel, grid, dim3(256), 0, s, X[cur], ldx, n, m, out, ost[0], ost[1], ost[2], base, bst[0], bst[1],
-                     bst[2], alpha, beta);
+                     bst[2], alpha, beta, (int)lda);
   GPX_HIP(hipGetLastError());
   return 0;
 }
@@ -1008,7 +1053,7 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m) {
   const size_t parts = (size_t)batch * PARTS * 8;
   if (dtype == GPX_F64) {
     const size_t lx = pad32(large), la = pad32(small);
-    return parts + 8 * (size_t)batch * small * (2 * lx + (2 + sums_f64(small, lx, la, batch)) * la);
+    return parts + 8 * (size_t)batch * (2 * la * lx + 2 * small * la + sums_f64(small, large, batch));
   }
   const size_t np = pad64(small), mp = pad64(large);
   const size_t pl = planes_of(dtype);   // X twice with two planes, X^T twice, A and B

@@ -60,7 +60,7 @@ def test_work_bytes():
     for dtype, planes in ((1, 2), (2, 2), (3, 1)):
         assert lib.gpx_orthogonalize_work_bytes(dtype, 3, 65, 130) == 3 * (8192 + 2 * ((4 + 2 * planes) * 128 * 192 + 2 * planes * 128 * 128))
         assert lib.gpx_orthogonalize_work_bytes(dtype, 1, 130, 65) == lib.gpx_orthogonalize_work_bytes(dtype, 1, 65, 130)
-    assert lib.gpx_orthogonalize_work_bytes(0, 1, 5, 40) == 8192 + 8 * (2 * 5 * 64 + 2 * 5 * 32)
+    assert lib.gpx_orthogonalize_work_bytes(0, 1, 5, 40) == 8192 + 8 * (2 * 32 * 64 + 2 * 5 * 32)
     assert lib.gpx_orthogonalize_work_bytes(9, 1, 5, 40) == 0
     assert lib.gpx_orthogonalize_work_bytes(1, 1, 0, 40) == 0
     # a long K split over workgroups: room for the parts' sums
@@ -92,7 +92,7 @@ def test_matches_the_definition(shape, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("shape", [(100, 3000), (2, 260, 4100), (2600, 640), (3, 64, 8000), (333, 1001)])
+@pytest.mark.parametrize("shape", [(100, 3000), (2, 260, 4100), (2600, 640), (3, 64, 8000), (333, 1001), (3, 200, 520), (700, 300)])
 def test_long_rows(shape, kind):
     """Few tiles of a long K, which fp64 and two planes split over workgroups."""
     from gaussian_process_amd import orthogonalize
