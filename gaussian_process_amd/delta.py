@@ -106,12 +106,23 @@ def _version(t):
     return None if t.is_inference() else t._version   # inference tensors do not count their writes
 
 
+def _place(t):
+    """What changes when t is written, moved or given up."""
+    return _version(t), t.data_ptr(), t.untyped_storage().nbytes()
+
+
 class Saved:
     """What a forward call keeps for its backward call."""
 
     def __init__(self, desc, inputs, state, work, stream):
-        self.desc, self.inputs, self.has_state, self.work, self.stream = desc, inputs, state is not None, work, stream
-        self.versions = [_version(t) for t in inputs]
+        self.desc, self.has_state, self.work, self.stream = desc, state is not None, work, stream
+        # aliases, which hold the memory that desc points to: a caller's tensor may be given other memory (t.data = ...)
+        self.inputs = [t.detach() for t in inputs]
+        self.places = [_place(t) for t in self.inputs]
+
+    def check(self):
+        if [_place(t) for t in self.inputs] != self.places:
+            raise RuntimeError("an input of the forward call has been modified in place, or its memory resized, since")
 
 
 def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scale=None, save_for_backward=False):
@@ -163,14 +174,14 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
 def gated_delta_rule_backward(saved, d_o, d_final_state=None):
     """(d_q, d_k, d_v, d_g, d_beta, d_initial_state) of sum(d_o * o) + sum(d_final_state * final_state).
 
-    ``saved`` comes from the forward call; it is only read, so the call may be repeated with other d_o.  d_q, d_k, d_v have the type of
+    ``saved`` comes from the forward call; it is only read, so the call may be repeated with other d_o.  It holds the memory of the
+    forward call's inputs; RuntimeError if they have been written or their storage resized in between.  d_q, d_k, d_v have the type of
     q, k, v, the others float32; d_initial_state is None if the forward call had no initial_state.  Tokens that belong
     to no sequence get zeros."""
     import torch
     if not isinstance(saved, Saved):
         raise TypeError("saved must come from gated_delta_rule(..., save_for_backward=True)")
-    if [_version(t) for t in saved.inputs] != saved.versions:
-        raise RuntimeError("an input of the forward call has been modified in place since")
+    saved.check()
     q, k, v, g, beta = saved.inputs[:5]
     d = saved.desc
     check_tensor(d_o, "d_o")
