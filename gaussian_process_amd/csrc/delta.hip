@@ -11,9 +11,11 @@
 //   dP = scale dO U^T;   dN = -dX U^T;   dQ = scale diag(exp G) dO S^T + (dP o D) K;   dbeta_j = E_j . Z_j
 //   dK = dKr + dKc:  dKr = (dN o D) K - diag(exp G) dX S^T        (the key that reads: row of N, of K S)
 //                    dKc = (dN o D)^T K + (dP o D)^T Q + diag(exp(G_C - G)) U dS'^T   (the key that writes)
-//   dG = q . dQ + k . dKr - k . dKc, and at the last token + sum_j (k . [state part of dKc])_j + exp(G_C) <dS', S>
-// because G_i enters only as exp(G_i) with what token i reads and exp(-G_j) with what token j writes; dg is the sum
-// of dG from its token to the end of the chunk.
+//   dg_t = sum over i >= t > j of (dP o P + dN o N)_ij + sum over i >= t of r_i + sum over j < t of c_j + exp(G_C) <dS', S>
+//          r_i = scale exp(G_i) q_i . S dO_i - exp(G_i) k_i . S dX_i,  c_j = exp(G_C - G_j) k_j . dS' U_j
+// dg_t is formed from the pairs of tokens on both sides of it, all of which carry the factor exp(g_t): as a sum over the tokens behind
+// t of dG_i = q_i . dQ_i + k_i . (dKr - dKc)_i, the pairs on one side cancel only up to their rounding, which hid the whole
+// result of fast heads (relative error 7e-4 at g = -8, 0.02 to 0.1 at -12, 0.4 to 1.7 at -16; 3e-7 now, whatever g).
 //
 // G is summed in 64 bits, since differences of it are taken, and g is read as max(g, -200): exp(-200) is 0 in fp32,
 // and a g of -infinity then gives no infinity minus infinity.
@@ -21,7 +23,7 @@
 // Kernels: plan (where packed sequences are), chunk (parallel over chunks: T, P, G, operands in the scans' order), the chain (over the
 // chunks of a sequence, parallel over heads and slices of dv, which are independent) and its reverse, and grads (parallel over
 // chunks).  Short inputs and single tokens go through the recurrence itself.  8192 tokens x 16 heads, bf16, dk = dv = 128: chunk 60 us,
-// chain 237; training on 2 x 4096 tokens: 81, 191 and 182, grads 230.
+// chain 237; training on 2 x 4096 tokens: 81, 191 and 182, grads 240.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1029,7 +1031,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 // 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
 // memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
 // the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
-// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 230 us for 655 MB, 2.8 TB/s.  The slices wait for memory (a third of the time),
+// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 240 us for 655 MB, 2.7 TB/s, 10 of them for d_g.  The slices wait for memory (a third of the time),
 // the steps after them for LDS, where all waves read the whole C x C matrix; neither overlaps the other, since the registers leave one
 // workgroup to a CU.  One that went on from chunk to chunk with the next one's first loads under way took as long.
 // LDS of the slices, which a C x C matrix of three planes takes over
@@ -1053,10 +1055,14 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
   __bf16* U = X + 3 * SL;                        // 3
   __bf16* M = reinterpret_cast<__bf16*>(smem);   // later: a C x C matrix, 3 planes
   f2* G = reinterpret_cast<f2*>(smem + grads_room<T>());
-  float* dG = reinterpret_cast<float*>(G + C);   // 8 x C: per wave
-  float* ef = dG + 8 * C;       // exp(G), exp(G_C - G): C each
+  float* read = reinterpret_cast<float*>(G + C);   // r and c of the header, 8 x C each: per wave
+  float* written = read + 8 * C;
+  float* ef = written + 8 * C;  // exp(G), exp(G_C - G): C each
   float* red = ef + 2 * C;      // 8
-  float* db = red + 8;          // C
+  float* rows_ = red + 8;       // sums over dP o P + dN o N, 16 each of its ten tiles: of rows (on the diagonal, of i >= t > j),
+  float* cols_ = rows_ + 160;   // of columns,
+  float* tiles_ = cols_ + 160;  // of all, 16
+  float* db = tiles_ + 16;      // C
   constexpr bool TILES = !(HEADS == GROUPED && sizeof(T) == 4);   // K and Q in LDS, where they fit
   constexpr int PV = 16 / sizeof(T), PK = DK + PV;
   T* Kt = reinterpret_cast<T*>(db + C);
@@ -1221,10 +1227,9 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         }
       }
     }
-    // row factors; k . state part of dKc
+    // row factors; what tokens read of S and leave in S'
     const T* Kg = reinterpret_cast<const T*>(a.d.k) + row * a.d.k_st.bs + t0 * a.d.k_st.rs + hk * a.d.k_st.cs + min(kc0, a.d.dk - 1);
     const T* Qg = reinterpret_cast<const T*>(a.d.q) + row * a.d.q_st.bs + t0 * a.d.q_st.rs + hk * a.d.q_st.cs + min(kc0, a.d.dk - 1);
-    float csum = 0.f;
     auto element = [&](const T* tile, const T* p, const gpx_strided& st_, int r) {
       if (TILES) return (float)tile[r * PK + kc0];
       return r < len && kc0 < a.d.dk ? (float)p[min(r, len - 1) * st_.rs] : 0.f;
@@ -1245,23 +1250,107 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = rb * 16 + r4 + e;
-          const float eg = ef[r];
+          const float eg = ef[r], kv = element(Kt, Kg, a.d.k_st, r), qv = element(Qt, Qg, a.d.q_st, r);
           q1[rb][e] *= a.scale * eg;
           kr[rb][e] *= -eg;
           kc[rb][e] *= ef[C + r];
-          csum = fmaf(element(Kt, Kg, a.d.k_st, r), kc[rb][e], csum);
+          const float x = row_sum(fmaf(qv, q1[rb][e], kv * kr[rb][e])), y = row_sum(kv * kc[rb][e]);
+          if (col == 0) {
+            read[wave * C + r] = x;
+            written[wave * C + r] = y;
+          }
         }
     }
-    csum = row_sum(csum);
     ss = row_sum(ss);
-    for (int o = 16; o < 64; o <<= 1) {
-      csum += __shfl_xor(csum, o);
-      ss += __shfl_xor(ss, o);
-    }
-    if (lane == 0) red[wave] = fmaf(keep, ss, csum);
+    for (int o = 16; o < 64; o <<= 1) ss += __shfl_xor(ss, o);
+    if (lane == 0) red[wave] = keep * ss;
     for (int o = 1; o < 8; o <<= 1) dbeta += __shfl_xor(dbeta, o);
     if ((t & 7) == 0) db[sr] = dbeta;
-    f4 D[2];
+    // dP o D, dN o D, and the sums of dP o P + dN o N.  K K^T and Q K^T again, as in the chunk kernel; where K and Q are not in LDS, K's
+    // fragments and P^T's
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int tile = wave + 8 * h;
+      if (tile < 10) {
+        const int rb = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, cb = tile - rb * (rb + 1) / 2, c = cb * 16 + col;
+        f4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+        if constexpr (TILES) {
+          auto planes_of = [&](const T* m, int r, int c, b8* p) {
+            T v[8];
+            __builtin_memcpy(v, __builtin_assume_aligned(m + r * PK + c, 16), sizeof(v));
+            if constexpr (N == 1) {
+              __builtin_memcpy(p, v, sizeof(v));
+            } else {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+              split<8, N>(x, p);
+            }
+          };
+#pragma unroll
+          for (int ks = 0; ks < DK / 32; ++ks) {
+            b8 x[N], y[N], z[N];
+            planes_of(Kt, rb * 16 + col, ks * 32 + g8, x);
+            planes_of(Qt, rb * 16 + col, ks * 32 + g8, y);
+            planes_of(Kt, cb * 16 + col, ks * 32 + g8, z);
+            kk = planes_mma<N, N, 3>(x, z, kk);
+            qk = planes_mma<N, N, 3>(y, z, qk);
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            b8 x[N], z[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+              const __bf16* f = a.Kf + (atk * N + k) * KF + w * 512;
+              x[k] = ld_frag(f + rb * 4 * 512, lane * 16);
+              z[k] = ld_frag(f + cb * 4 * 512, lane * 16);
+            }
+            kk = planes_mma<N, N, 3>(x, z, kk);
+          }
+          const __bf16* f = a.PTf + at * 3 * TF + ((cb * 2 + (rb >> 1)) * 64 + ((rb & 1) * 2 + (lane >> 5)) * 16 + col) * 8 + (lane >> 4 & 1) * 4;
+#pragma unroll
+          for (int k = 2; k >= 0; --k) {
+            const b4 v = *reinterpret_cast<const b4*>(f + k * TF);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qk[e] += (float)v[e];
+          }
+        }
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = rb * 16 + r4 + e;
+          const float D = r >= c ? decay(G[r], G[c]) : 0.f, y = a.scale * dp[h][e], P = TILES ? qk[e] * D : qk[e];
+          dp[h][e] = y * D;
+          da[h][e] = r > c ? -da[h][e] * D : 0.f;
+          w[e] = r > c ? fmaf(da[h][e], kk[e], y * P) : 0.f;
+        }
+        if (rb == cb) {
+          // w[e]: the sum of its column from its row on
+#pragma unroll
+          for (int e = 2; e >= 0; --e) w[e] += w[e + 1];
+          const float a1 = __shfl_down(w[0], 16), a2 = __shfl_down(w[0], 32), a3 = __shfl_down(w[0], 48);
+          const float below = (lane < 48 ? a1 : 0.f) + (lane < 32 ? a2 : 0.f) + (lane < 16 ? a3 : 0.f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = row_sum(col < r4 + e ? w[e] + below : 0.f);
+            if (col == 0) rows_[tile * 16 + r4 + e] = x;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = row_sum(w[e]);
+            if (col == 0) rows_[tile * 16 + r4 + e] = x;
+          }
+          float x = (w[0] + w[1]) + (w[2] + w[3]);
+          x += __shfl_xor(x, 16);
+          x += __shfl_xor(x, 32);
+          if (lane < 16) cols_[tile * 16 + col] = x;
+          x = row_sum(x);
+          if (lane == 0) tiles_[tile] = x;
+        }
+      }
+    }
     // dP o D with K, its transpose with Q; then dN o D and its transpose with K
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -1278,18 +1367,6 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
         const int tile = wave + 8 * h;
         if (tile < 10) {
           const int rb = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, cb = tile - rb * (rb + 1) / 2, c = cb * 16 + col;
-          if (w % 2 == 0) {   // the values, in place of the sums
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = rb * 16 + r4 + e;
-              if (w == 0) {
-                D[h][e] = r >= c ? decay(G[r], G[c]) : 0.f;
-                dp[h][e] *= a.scale * D[h][e];
-              } else {
-                da[h][e] = r > c ? -da[h][e] * D[h][e] : 0.f;
-              }
-            }
-          }
           float x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = w < 2 ? dp[h][e] : da[h][e];
@@ -1323,19 +1400,8 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
           }
       }
     }
-    // dG of this wave's columns
 #pragma unroll
     for (int rb = 0; rb < 4; ++rb) {
-      float g[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = rb * 16 + r4 + e;
-        g[e] = own ? fmaf(element(Qt, Qg, a.d.q_st, r), q1[rb][e], element(Kt, Kg, a.d.k_st, r) * (kr[rb][e] - kc[rb][e])) : 0.f;
-        g[e] = row_sum(g[e]);
-      }
-      if (col == 0)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dG[wave * C + rb * 16 + r4 + e] = g[e];
       kr[rb] += kc[rb];
       if (HEADS == GROUPED) {
         if (m > 0) {
@@ -1377,12 +1443,36 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(const Args a) {
       }
     }
     if (wave == 0) {
-      float v = 0.f;
-      for (int i = 0; i < 8; ++i) v += dG[i * C + lane] + (lane == C - 1 ? red[i] : 0.f);
-      for (int o = 1; o < 64; o <<= 1) {
-        const float u = __shfl_down(v, o);
-        if (lane + o < 64) v += u;
+      const int tb = lane >> 4, n = lane & 15;
+      float behind = 0.f, before = 0.f, all = 0.f;   // of all tokens
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        behind += read[i * C + lane];
+        before += written[i * C + lane];
+        all += red[i];
       }
+      float x = 0.f, y = 0.f;   // rows of this token's block left of the diagonal, columns under it
+#pragma unroll
+      for (int rb = 1; rb < 4; ++rb)
+#pragma unroll
+        for (int cb = 0; cb < rb; ++cb) {
+          const int tile = rb * (rb + 1) / 2 + cb;
+          if (rb == tb) x += rows_[tile * 16 + n];
+          if (cb == tb) y += cols_[tile * 16 + n];
+          if (rb > tb && cb < tb) all += tiles_[tile];
+        }
+      before = __shfl_up(before, 1);   // sums before this token: none of them over it
+      y = __shfl_up(y, 1);
+      if (lane == 0) before = 0.f;
+      if (n == 0) y = 0.f;
+      for (int o = 1; o < 64; o <<= 1) {
+        const float u = __shfl_down(behind, o), w = __shfl_up(before, o), x1 = __shfl_down(x, o), y1 = __shfl_up(y, o);
+        if (lane + o < 64) behind += u;
+        if (lane >= o) before += w;
+        if (n + o < 16) x += x1;
+        if (n >= o) y += y1;
+      }
+      const float v = (behind + before) + (x + y) + (all + rows_[tb * (tb + 3) / 2 * 16 + n]);
       if (lane < len) {
         const long p = (row * a.d.tokens + t0 + lane) * a.d.value_heads + hv;
         a.d_g[p] = v;
@@ -1743,7 +1833,7 @@ int run_forward(hipStream_t s, const Args& a, int rec) {
 
 template <typename T, int DK>
 int run_backward(hipStream_t s, const Args& a) {
-  constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = grads_room<T>() + C * 8 + (8 * C + 2 * C + 8 + C) * 4;
+  constexpr size_t tiles = 2 * C * (DK + 16 / sizeof(T)) * sizeof(T), base = grads_room<T>() + C * 8 + (16 * C + 2 * C + 8 + 336 + C) * 4;
   constexpr size_t lds = base + tiles, grouped = base + (sizeof(T) == 4 ? 0 : tiles) + 8 * 512 * 16;
   static_assert(lds <= 160 * 1024 && grouped <= 160 * 1024 && lds % 16 == 0, "LDS");
   DELTA_TRY(allow_lds<&delta_grads_kernel<T, DK, ALONE>>(lds));
