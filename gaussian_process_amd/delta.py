@@ -12,7 +12,8 @@ i // (Hv // Hk)); g (the LOG of the decay, -inf forgets everything) and beta (B,
 1 <= dk <= 128, 1 <= dv <= 1024, any T.  Any strides; q, k, v with a last dimension that is not dense are copied first.
 
 Gradients are functions of their own, as everywhere in this package: nothing is recorded behind the
-caller's back, so a forward and a backward call may be captured into a graph together."""
+caller's back, so a forward and a backward call may be captured into a graph together.  Tensors that require a gradient are
+therefore refused where torch records (RuntimeError); pass them detached, or call under torch.no_grad()."""
 import ctypes as C
 
 from . import _lib

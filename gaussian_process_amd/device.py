@@ -137,11 +137,23 @@ def ptr(t):
 
 
 def tensor_runtime(first, *others):
-    """The runtime of the one MI355X that all the given tensors (None allowed after the first) live on."""
+    """The runtime of the one MI355X that all the given tensors (None allowed after the first) live on, for calls that record
+    no gradient: RuntimeError if one would be lost."""
+    import torch
     device = first.device
+    recording = torch.is_grad_enabled()
+    needed = recording and first.requires_grad
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError("the tensors are on different devices: %s and %s" % (device, t.device))
+        if t is not None:
+            if t.device != device:
+                raise ValueError("the tensors are on different devices: %s and %s" % (device, t.device))
+            if recording and t.requires_grad:
+                needed = True
+    if torch.autograd.forward_ad._current_level >= 0:
+        needed = needed or any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in (first, *others))
+    if needed:
+        raise RuntimeError("a tensor requires a gradient (or carries a tangent), which this call does not record: make it under "
+                           "torch.no_grad() or with detached tensors")
     if device.type != "cuda":
         raise _lib.GpxError("the tensors must be on an MI355X (no CPU fallback)")
     rt = _runtimes.get(device.index)

@@ -63,7 +63,8 @@ def orthogonalize(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, alpha=1.0, be
     G: (..., n, m) tensor on the MI355X, float64, float32, float16 or bfloat16, any strides (a transposed view costs
     nothing); leading dimensions are a stack of matrices, each with a norm of its own.  ``base`` (needed when beta != 0) and ``out``
     have G's shape and type; ``out`` may be ``base`` or ``G`` itself: ``orthogonalize(G, alpha=-lr, beta=1 - lr * decay,
-    base=W, out=W)`` is an optimiser's update.  Returns out.
+    base=W, out=W)`` is an optimiser's update.  Returns out.  No gradient is recorded: tensors that require one are refused
+    (RuntimeError) outside torch.no_grad(), as torch does with writes to a leaf.
 
     float64 is computed in float64; the other types on the fp16 matrix cores with float32 sums, with as many bits
     per intermediate value as the result has (bfloat16: 11, float16 and float32: 22).  A matrix of zeros gives zeros, one with a NaN
