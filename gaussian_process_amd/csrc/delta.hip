@@ -1533,7 +1533,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const StepArgs x) 
   const int slice = blockIdx.x % slices, hv = blockIdx.x / slices % heads, s = blockIdx.x / slices / heads;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, hk = hv / a.group;
   const int cc = (lane & 15) * 4, c0 = slice * 64 + cc, r0 = (wave * 4 + (lane >> 4)) * RPT;
-  const bool vec = (a.d.dv & 3) == 0;   // rows of states are 16-byte aligned
+  const bool vec = (a.d.dv & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.state_out)) & 15) == 0;
   int own = s, tok, end;
   long row = 0;
   if (x.step) {
@@ -1965,7 +1965,7 @@ int gpx_delta_step(gpx_handle* h, const gpx_delta* d, int slots, const int* slot
   GPX_REQUIRE(slots >= 0 && (slot != nullptr || slots == d->batch), "delta_step: %d states for %d rows", slots, d->batch);
   if (d->batch == 0 || slots == 0) return 0;   // no row has a state
   GPX_REQUIRE(o != nullptr && state_out != nullptr && state != nullptr, "delta_step: null state or output");
-  GPX_REQUIRE(gpx_aligned16(state) && gpx_aligned16(state_out), "delta_step: states must be 16-byte aligned");
+  GPX_REQUIRE(((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(state_out)) & 3) == 0, "delta_step: misaligned state");
   DeviceGuard dg(h->device);
   Args a = make_args(d);
   a.state = state;

@@ -229,7 +229,7 @@ def _step_description(q, k, v, g, beta, state, slots, state_out, scale):
             raise ValueError("slots must be an int32 tensor with one value per row")
     _check_state(state_out, state.shape, "state_out")
     if not state.is_contiguous() or not state_out.is_contiguous():
-        raise ValueError("state and state_out must be packed and 16-byte aligned")
+        raise ValueError("state and state_out must be packed")
     as_used = [_dense_row(t) for t in (q, k, v)]
     dense = all(a is b for a, b in zip(as_used, (q, k, v)))
     d = _lib.Delta(dtype, B, 1, 0, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else scale, None, None, None, None, None, None,
@@ -263,8 +263,6 @@ def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, s
         if key is not None:
             _known_steps[key] = known
     at, to = state.data_ptr(), state_out.data_ptr()
-    if (at | to) % 16:
-        raise ValueError("state and state_out must be packed and 16-byte aligned")
     if 0 < abs(to - at) < state.numel() * 4:
         raise ValueError("state_out overlaps state")
     rt = tensor_runtime(q, k, v, g, beta, state, slots, state_out)
