@@ -252,7 +252,6 @@ __device__ __forceinline__ void lds_barrier() {
 // accumulators of the wave that updates it, lane l holding column l & 15 and rows 4 g + e of each of its DK / 64 tiles, and
 // serves from there as the other operand; the terms of wave w are therefore dk = 16 (w DK / 64) + 4 g + e, e < 4, and the
 // same of its second tile (none if DK = 64: zeros).
-__device__ __forceinline__ long frag(int block, int blocks, int ks, int lane) { return (((long)block * blocks + ks) * 64 + lane) * 8; }
 
 constexpr int KF = 4 * 4 * 64 * 8;   // elements of a plane of K or Q in state order
 constexpr int TF = 4 * 2 * 64 * 8;   // of a C x C matrix
