@@ -64,3 +64,51 @@ def test_gradients_after_a_tensor_is_given_another():
     with pytest.raises(RuntimeError):
         saved.inputs[1].untyped_storage().resize_(0)
         gated_delta_rule_backward(saved, d_o)
+
+
+def _ranges(tensors):
+    return [(t.data_ptr(), t.data_ptr() + t.untyped_storage().nbytes()) for t in tensors]
+
+
+@pytest.mark.gpu
+def test_memory_is_kept_for_another_stream():
+    """The saved values are dropped while a backward call on another stream has yet to read them: their memory is not handed out before
+    that stream is done.  The control shows that the allocator does hand it out where nothing waits."""
+    from gaussian_process_amd import gated_delta_rule, gated_delta_rule_backward
+    torch.manual_seed(1)
+    B, T, H, d = 1, 4096, 8, 64
+    x = [0.1 * torch.randn(B, T, d, H, device="cuda").transpose(2, 3) for _ in range(2)]   # not dense: saved holds copies
+    x += [torch.randn(B, T, H, d, device="cuda"), -torch.rand(B, T, H, device="cuda"), torch.rand(B, T, H, device="cuda")]
+    d_o = torch.randn(B, T, H, d, device="cuda")
+    big = torch.randn(8192, 8192, device="cuda")
+    product = torch.empty_like(big)
+
+    def forward():
+        saved = gated_delta_rule(*x, save_for_backward=True)[2]
+        own = [saved.work, *saved.inputs[:2]]
+        assert saved.inputs[0].data_ptr() != x[0].data_ptr()
+        return saved, _ranges(own), [t.untyped_storage().nbytes() for t in own]
+
+    def handed_out(old, sizes):
+        new = _ranges([torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(3)])
+        return any(a < d and c < b for a, b in old for c, d in new)
+
+    want = gated_delta_rule_backward(forward()[0], d_o)
+    _, old, sizes = forward()
+    torch.cuda.synchronize()
+    del _
+    assert handed_out(old, sizes)
+    saved, old, sizes = forward()
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            torch.mm(big, big, out=product)   # some 10 ms each
+        got = gated_delta_rule_backward(saved, d_o)
+        done.record()
+    del saved
+    early = handed_out(old, sizes)
+    assert not done.query(), "the other stream was done before the test looked"
+    assert not early
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got) if a is not None)
