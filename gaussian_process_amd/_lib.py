@@ -12,6 +12,7 @@ GPX_KIND = {"rbf": 0, "ard": 1}
 GPX_FULL, GPX_LOWER = 0, 1
 GPX_NB = 128
 
+GPX_TWO_PLANES = 16
 GPX_TYPE = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
 
 

@@ -4,13 +4,14 @@
 // Numbers.  The polynomial keeps every singular value of X below a bound r that the host computes from the
 // coefficients (1.21 for the usual ones), so |X_ij| <= r, |A_ij| <= r^2 and |B_ij| <= max |b t + c t^2|: the
 // intermediates are stored in fp16, each scaled by the power of two that puts its bound just under fp16's largest
-// value, which leaves values down to 2^-28 of the bound as normal numbers.  fp16's 11 bits run at bf16's matrix
-// rate and lie 8 times nearer.  X itself is kept as two fp16 planes, v = hi + lo with 22 bits, because the term a X hands
-// its rounding on from step to step (a = 3.4 at small singular values); the products read hi alone.  On 512 x 512 with a
-// few strong directions, relative, 2-norm: 0.0006 off, against 0.0027 with one plane of X and 0.0017 for rounding the
-// exact result to bf16.  Results of more than 8 bits (fp32, fp16) use two planes everywhere and three products (hi hi + hi lo
-// + lo hi): 1.5e-6 off at worst here, as an fp32 product, at a third of the fp16 rate -- five times that of the fp32
-// matrix instructions.
+// value, which leaves values down to 2^-28 of the bound as normal numbers.  Values are two fp16 planes, v = hi + lo with 22 bits,
+// and a product three (hi hi + hi lo + lo hi): 1.5e-6 off at worst here, as an fp32 product, at a third of the fp16 rate -- five times
+// that of the fp32 matrix instructions.  A bf16 result's error is then that of its rounding alone.
+// For bf16 results the caller may choose one plane (GPX_BF16 without GPX_TWO_PLANES) for A, B, X^T and what products read of X, a third of
+// the products: 4096 x 4096 3744 -> 1543 us, 1024 x 1024 193 -> 142.  fp16's 11 bits run at bf16's matrix rate and lie 8 times
+// nearer.  X itself stays in two planes there, because the term a X hands its rounding on from step to step (a = 3.4 at small singular
+// values).  The result's error grows to 1.03 (1024 x 1024) .. 1.07 (512 x 512) .. 1.23 (130 x 260) times that of rounding the exact
+// result; with one plane of X to 1.6 times at 512 x 512.
 //
 // Layout.  Every product has both operands k-contiguous: A needs rows of X; A is symmetric, so A A does too; and
 // B X needs rows of X^T, so the step's epilogue writes X in both orientations.  Buffers are padded to multiples of 64
@@ -864,7 +865,7 @@ int scale_exp(double bound) { return 14 - (int)std::ceil(std::log2(std::fmax(bou
 
 int planes_of(int dtype) { return dtype == GPX_BF16 ? 1 : 2; }
 
-bool dtype_ok(int dtype) { return dtype == GPX_F64 || dtype == GPX_F32 || dtype == GPX_F16 || dtype == GPX_BF16; }
+bool dtype_ok(int dtype) { return dtype == GPX_F64 || dtype == GPX_F32 || dtype == GPX_F16 || dtype == GPX_BF16 || dtype == (GPX_BF16 | GPX_TWO_PLANES); }
 
 template <typename T>
 int norm_launch(hipStream_t s, const void* G, long bs, long rs, long cs, int n, int m, int batch, double* part, int& nparts) {
@@ -1111,6 +1112,9 @@ int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const v
     case GPX_F16:
       return run_half<_Float16, 2>(h->stream, dtype, batch, a, b, G, gst[0], gst[1], gst[2], steps, coef_host, eps, alpha, beta, base,
                                    bst, out, ost, w);
+    case GPX_BF16 | GPX_TWO_PLANES:
+      return run_half<__bf16, 2>(h->stream, GPX_BF16, batch, a, b, G, gst[0], gst[1], gst[2], steps, coef_host, eps, alpha, beta, base,
+                                 bst, out, ost, w);
     default:
       return run_half<__bf16, 1>(h->stream, dtype, batch, a, b, G, gst[0], gst[1], gst[2], steps, coef_host, eps, alpha, beta, base, bst,
                                  out, ost, w);

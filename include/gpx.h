@@ -293,12 +293,13 @@ size_t gpx_ep_sweep_work_elems(int n);
  * GPX_F16, GPX_BF16, one type for G, base and out.  out may overlap G in any way (G is read before out is written) and
  * may be base with the same strides, but must not overlap base otherwise; no two elements of out may share memory.
  * Arithmetic: GPX_F64 in fp64.  The other types on the fp16 matrix cores with fp32 accumulation and intermediates
- * scaled by powers of two: GPX_BF16 with one fp16 value per element (its 11 bits lie under the 8 of the result),
- * GPX_F32 and GPX_F16 with two (22 bits).  The norm is summed in fp64.
+ * scaled by powers of two: GPX_F32, GPX_F16 and GPX_BF16 | GPX_TWO_PLANES with two fp16 values per element (22 bits), GPX_BF16 alone
+ * with one, at a third of the products (11 bits under the 8 of the result, whose error grows by 3 to 23 %).  The norm is summed in fp64.
  * coef_host: (a, b, c), host memory.  GPX_EINVAL if the polynomial lets a singular value grow beyond 1000
  * (the iteration diverges).  1 <= steps <= 64; n, m <= 65536; batch <= 65535.
  * work: gpx_orthogonalize_work_bytes(dtype, batch, n, m) device bytes, 16-byte aligned, not shared by calls that may
  * overlap in time.  No other scratch is used and nothing is allocated: the call may be captured into a graph. */
+#define GPX_TWO_PLANES 16 /* with GPX_BF16, as dtype of the two calls below */
 typedef struct gpx_strided { long long bs, rs, cs; } gpx_strided;
 int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const void* G, const gpx_strided* g_st,
                       int steps, const double* coef_host, double eps, double alpha, double beta, const void* base,
