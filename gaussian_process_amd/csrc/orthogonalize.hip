@@ -860,8 +860,9 @@ double poly_bound(const double* k, double r) {
   }
   return best;
 }
-// exponent that puts values of at most `bound` (and 5 % for rounding) under 2^14, a quarter of fp16's largest
-int scale_exp(double bound) { return 14 - (int)std::ceil(std::log2(std::fmax(bound, 1e-3) * 1.05)); }
+// exponent that puts values of at most `bound` (and 5 % for rounding) under 2^14, a quarter of fp16's largest; under 1e-30, where a
+// polynomial that shrinks X may lead, the factors between the scales would leave fp32's range
+int scale_exp(double bound) { return 14 - (int)std::ceil(std::log2(std::fmax(bound, 1e-30) * 1.05)); }
 
 int planes_of(int dtype) { return dtype == GPX_BF16 ? 1 : 2; }
 

@@ -295,6 +295,8 @@ size_t gpx_ep_sweep_work_elems(int n);
  * Arithmetic: GPX_F64 in fp64.  The other types on the fp16 matrix cores with fp32 accumulation and intermediates
  * scaled by powers of two: GPX_F32, GPX_F16 and GPX_BF16 | GPX_TWO_PLANES with two fp16 values per element (22 bits), GPX_BF16 alone
  * with one, at a third of the products (11 bits under the 8 of the result, whose error grows by 3 to 23 %).  The norm is summed in fp64.
+ * A matrix of zeros gives zeros (NaNs with eps == 0).  Values below 2^-28 of the bound on the spectrum lose bits outside GPX_F64, where the
+ * squares of G must be normal numbers.
  * coef_host: (a, b, c), host memory.  GPX_EINVAL if the polynomial lets a singular value grow beyond 1000
  * (the iteration diverges).  1 <= steps <= 64; n, m <= 65536; batch <= 65535.
  * work: gpx_orthogonalize_work_bytes(dtype, batch, n, m) device bytes, 16-byte aligned, not shared by calls that may

@@ -90,3 +90,20 @@ def test_library_refuses_the_flag_for_other_types():
                                           buf.data_ptr(), C.byref(st), buf.data_ptr(), buf.numel() * 4)
         assert rc == -1
     assert (buf == 0).all() and np.isfinite(buf.cpu().numpy()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "f64"])
+@pytest.mark.parametrize("coef,steps", [((0.5, 0.0, 0.0), 13), ((0.25, -0.1, 0.02), 8), ((0.1, 0.3, 0.0), 5)])
+def test_coefficients_that_shrink(kind, coef, steps):
+    """The spectrum's bound falls by the polynomial's factor at every step, and the intermediates' scale goes with it: the tolerance of
+    test_orthogonalize.py.  Results down to 1e-4 are normal numbers of every type once alpha has brought them back."""
+    from gaussian_process_amd import orthogonalize
+    from test_orthogonalize import TOL
+    G = make((72, 200), kind, seed=steps)
+    want = plain(G, steps, coef) / coef[0] ** steps
+    got = orthogonalize(G, steps=steps, coefficients=coef, alpha=coef[0] ** -steps)
+    assert rel(got, want) < TOL[kind], rel(got, want)
+    if kind == "f32":   # far down; alpha is not needed there
+        want = plain(G, 4 * steps, coef)
+        assert rel(orthogonalize(G, steps=4 * steps, coefficients=coef), want) < TOL[kind]
