@@ -80,6 +80,7 @@ SIGNATURES = {
     "gpx_orthogonalize": (_i, [C.c_void_p, _i, _i, _i, _i, _dp, C.POINTER(Strided), _i, _hp, _d, _d, _d, _dp,
                                C.POINTER(Strided), _dp, C.POINTER(Strided), _dp, _sz]),
     "gpx_orthogonalize_work_bytes": (_sz, [_i, _i, _i, _i]),
+    "gpx_orthogonalize_tile": (_i, [_i, _i, _i, _i, _i]),
     "gpx_delta_work_bytes": (_sz, [C.POINTER(Delta), _i]),
     "gpx_delta_forward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, _dp, _dp, _dp, _sz, _dp, _sz]),
     "gpx_delta_backward": (_i, [C.c_void_p, C.POINTER(Delta), _dp, C.POINTER(Strided), _dp, _dp, _dp, _dp, _dp, _dp, _dp,

@@ -658,16 +658,17 @@ int launch_small(hipStream_t s, const NsGemm& g, int batch) {
 // (which would be a second round: 23 -> 25), not of one plane (10 tiles with K = 4096 15 -> 14), and not larger tiles, which keep more
 // of the chip busy (136 of 128 x 128 with K = 8192 174 -> 148, nothing of it left in the whole call).
 struct Choice {
-  int tile, parts;
+  int tile, parts;   // tile: of TILE
 };
+constexpr int TILE[4] = {64, 128, 192, 256};
 template <int NPL>
 Choice choose(int M, int N, int K, int lower, int batch) {
-  const int tile[4] = {64, 128, 192, 256}, slots[4] = {512, 256, 256, 256};
+  const int slots[4] = {512, 256, 256, 256};
   const double unit[4] = {34, 42, 84, 110};
   Choice best = {0, 1};
   double least = 0, tiles = 0;
   for (int i = 0; i < 4; ++i) {
-    const double tm = (M + tile[i] - 1) / tile[i], tn = (N + tile[i] - 1) / tile[i], t = (lower ? tm * (tm + 1) / 2 : tm * tn) * batch;
+    const double tm = (M + TILE[i] - 1) / TILE[i], tn = (N + TILE[i] - 1) / TILE[i], t = (lower ? tm * (tm + 1) / 2 : tm * tn) * batch;
     const double cost = std::ceil(t / slots[i]) * unit[i];
     if (i == 0 || cost < least) {
       best.tile = i;
@@ -1061,6 +1062,13 @@ size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m) {
   const size_t pl = planes_of(dtype);   // X twice with two planes, X^T twice, A and B
   const size_t sums = pl == 1 ? 0 : sums_bytes((int)np, (int)mp, batch);
   return parts + (size_t)batch * 2 * ((4 + 2 * pl) * np * mp + 2 * pl * np * np) + sums;
+}
+
+int gpx_orthogonalize_tile(int dtype, int batch, int n, int m, int product) {
+  if (!dtype_ok(dtype) || dtype == GPX_F64 || batch <= 0 || n <= 0 || m <= 0 || product < 0 || product > 2) return 0;
+  const int np = pad64(std::min(n, m)), mp = pad64(std::max(n, m)), lower = product < 2;
+  const int N = lower ? np : mp, K = product == 0 ? mp : np;
+  return TILE[(planes_of(dtype) == 1 ? choose<1>(np, N, K, lower, batch) : choose<2>(np, N, K, lower, batch)).tile];
 }
 
 int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const void* G, const gpx_strided* g_st, int steps,

@@ -307,6 +307,9 @@ int gpx_orthogonalize(gpx_handle* h, int dtype, int batch, int n, int m, const v
                       int steps, const double* coef_host, double eps, double alpha, double beta, const void* base,
                       const gpx_strided* base_st, void* out, const gpx_strided* out_st, void* work, size_t work_bytes);
 size_t gpx_orthogonalize_work_bytes(int dtype, int batch, int n, int m);
+/* The side of the square tiles in which such a call forms product 0 (X X^T), 1 (A A) or 2 (B X): for tests and measurements.  0 for GPX_F64,
+ * empty matrices and unknown types. */
+int gpx_orthogonalize_tile(int dtype, int batch, int n, int m, int product);
 
 /* ---- the gated delta rule: regression over a stream ---------------------------------------- */
 /* A state S (dk x dv) per sequence and value head maps keys to values; every token fades it and makes one gradient
