@@ -21,6 +21,9 @@ from .device import ptr, tensor_runtime
 from .orthogonal import check_tensor, type_id
 
 
+SIZE_MAX = 1 << 30   # the library's sizes are 32-bit
+
+
 def _dense(t):
     """t, or a packed copy where its last dimension is not dense or its tokens lie too far apart for the library."""
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-3) <= 1 << 22 else t.contiguous()
@@ -75,6 +78,8 @@ def _check(q, k, v, g, beta, dims):
     Hv, dv = vs[-2:]
     if Hk < 1 or Hv < 1 or Hv % Hk:
         raise ValueError("the value heads (%d) must be a multiple of the key heads (%d)" % (Hv, Hk))
+    if max(qs) > SIZE_MAX or max(vs) > SIZE_MAX:
+        raise ValueError("a size of q, k or v is beyond 2^30")
     if not 1 <= dk <= 128 or not 1 <= dv <= 1024:
         raise ValueError("dk = %d must be in [1, 128], dv = %d in [1, 1024]" % (dk, dv))
     return dtype, Hk, dk, Hv, dv
@@ -149,6 +154,8 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, cu_seqlens=None, scal
         if B != 1:
             raise ValueError("packed sequences need a batch of one")
         sequences = cu_seqlens.numel() - 1
+        if sequences > SIZE_MAX:
+            raise ValueError("%d sequences are too many" % sequences)
     shape = (sequences or B, Hv, dk, dv)
     _check_state(initial_state, shape, "initial_state")
     rt = tensor_runtime(q, k, v, g, beta, initial_state, cu_seqlens)
@@ -219,6 +226,8 @@ def _step_description(q, k, v, g, beta, state, slots, state_out, scale):
     B = q.shape[0]
     check_tensor(state, "state")
     n = state.shape[0] if state.dim() else 0
+    if n > SIZE_MAX:
+        raise ValueError("%d states are too many" % n)
     _check_state(state, (n, Hv, dk, dv), "state")
     if slots is None:
         if n != B:

@@ -78,6 +78,8 @@ def orthogonalize(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, alpha=1.0, be
         raise TypeError("element type %s is not one of %s" % (G.dtype, ", ".join(_lib.GPX_TYPE)))
     if G.dim() < 2:
         raise ValueError("G must have at least two dimensions")
+    if max(math.prod(G.shape[:-2]), *G.shape[-2:]) > 65536:   # before the library's 32-bit sizes cut it off
+        raise ValueError("G has more than 65535 matrices or 65536 rows or columns")
     if reduced and G.dtype != torch.bfloat16:
         raise ValueError("reduced is for bfloat16")
     if beta != 0.0 and base is None:
