@@ -23,7 +23,7 @@
 // Kernels: plan (where packed sequences are), chunk (parallel over chunks: T, P, G, operands in the scans' order), the chain (over the
 // chunks of a sequence, parallel over heads and slices of dv, which are independent) and its reverse, and grads (parallel over
 // chunks).  Short inputs and single tokens go through the recurrence itself.  8192 tokens x 16 heads, bf16, dk = dv = 128: chunk 60 us,
-// chain 237; training on 2 x 4096 tokens: 81, 191 and 182, grads 240.
+// chain 237; training on 2 x 4096 tokens: 81, 191 and 182, grads 235.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1031,7 +1031,7 @@ __global__ __launch_bounds__(512, TWO ? 4 : 2) void delta_chain_kernel(const Arg
 // 8 waves.  DK / 16 of them own 16 columns of dk each and all 64 rows of dQ, dKr and dKc; their operands over dv are S and dS' from
 // memory (a wave's own rows) and Y = dO, X = beta Z, U = beta E of 32 columns of dv at a time from LDS.  dP = dO U^T and dX U^T:
 // the ten 16 x 16 tiles on and below the diagonal, spread over the waves.
-// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 240 us for 655 MB, 2.7 TB/s, 10 of them for d_g.  The slices wait for memory (a third of the time),
+// 2 x 4096 tokens x 16 heads, bf16, 128 x 128: 235 us for 655 MB, 2.8 TB/s, 9 of them for d_g.  The slices wait for memory (a third of the time),
 // the steps after them for LDS, where all waves read the whole C x C matrix; neither overlaps the other, since the registers leave one
 // workgroup to a CU.  One that went on from chunk to chunk with the next one's first loads under way took as long.
 // LDS of the slices, which a C x C matrix of three planes takes over
@@ -1042,7 +1042,7 @@ constexpr size_t grads_room() {
 }
 
 // HEADS: what a workgroup takes of a key head -- its one value head; all, one after the other; one of several, leaving its dQ and dK in
-// fp32 to delta_join_heads_kernel (where workgroups are few: 700 ragged tokens, 2 key heads, fp32: 47 -> 27 us with the joining)
+// fp32 to delta_join_heads_kernel (where workgroups are few: 700 ragged tokens, 2 key heads, fp32: 53 -> 31 us with the joining)
 enum { ALONE, GROUPED, APART };
 
 template <typename T, int DK, int HEADS>

@@ -1,14 +1,15 @@
 """The gated delta rule on the MI355X (``gpx_delta_*``): regression over a stream.
 
-No counterpart in the reference.  It stands beside the exact GP as its streaming relative: the GP solves
-for all targets at once in O(n^3), this keeps one dk x dv map from keys to values and corrects it by the
-error of every token, in order, while it forgets -- for each sequence and head
+No counterpart in the reference, and no estimator of this package calls it: it is for programs that keep such a state of
+their own.  By its method it is the exact GP's streaming relative: the GP solves for all targets at once in O(n^3), this
+keeps one dk x dv map from keys to values and corrects it by the error of every token, in order, while it forgets --
+for each sequence and head
 
     Sbar = exp(g) S;   e = v - Sbar^T k;   S <- Sbar + beta k e^T;   o = scale S^T q
 
 Shapes: q, k (B, T, Hk, dk); v, o (B, T, Hv, dv), Hv a multiple of Hk (value head i reads key head
-i // (Hv // Hk)); g (the LOG of the decay, -inf forgets everything) and beta (B, T, Hv) in float32; states
-(sequences, Hv, dk, dv) in float32.  q, k, v, o: float32, float16 or bfloat16, one type, sums in float32.
+i // (Hv // Hk)); g (the LOG of the decay, at most 0, -inf forgets everything; growth, g > 0, costs as many bits as it
+multiplies in 64 tokens) and beta (B, T, Hv) in float32; states (sequences, Hv, dk, dv) in float32.  q, k, v, o: float32, float16 or bfloat16, one type, sums in float32.
 1 <= dk <= 128, 1 <= dv <= 1024, any T.  Any strides; q, k, v with a last dimension that is not dense are copied first.
 
 Gradients are functions of their own, as everywhere in this package: nothing is recorded behind the

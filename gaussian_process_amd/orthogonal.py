@@ -1,7 +1,7 @@
 """Orthogonalisation of matrix-shaped updates on the MI355X (``gpx_orthogonalize``).
 
-No counterpart in the reference: its parameters are scalars and length scales, which L-BFGS-B moves
-(base.py:21-58).  A learned feature map has matrices, and this is the step that moves those."""
+No counterpart in the reference, whose parameters are scalars and length scales that L-BFGS-B moves (base.py:21-58), as
+are those of the estimators here: none of them calls it.  It is for programs that train matrices of their own."""
 import ctypes as C
 import math
 
@@ -70,7 +70,8 @@ def orthogonalize(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, alpha=1.0, be
     value.  ``reduced`` (bfloat16 only) makes do with 11 bits, which takes a third of the products; the result's error is then 1.03 to
     1.23 times that of rounding the exact result (1024 x 1024 to 130 x 260), and 1.00 times without.  A matrix of zeros gives zeros
     (NaNs with eps = 0), one with a NaN or an infinity NaNs.  Of values below 2^-28 of the spectrum's bound, such as all of a matrix whose
-    norm is below 1e-4 eps, bits are lost outside float64; in float64 the squares of G must be normal numbers.  Asynchronous on the current stream; may be captured into a graph after one call outside."""
+    norm is below 1e-4 eps, bits are lost outside float64; in float64 the squares of G must be normal numbers.  Asynchronous on
+    the current stream; may be captured into a graph after one call outside."""
     import torch
     check_tensor(G, "G")
     dtype = type_id(G)

@@ -317,7 +317,7 @@ int gpx_orthogonalize_tile(int dtype, int batch, int n, int m, int product);
  *   Sbar = exp(g) S;   e = v - Sbar^T k;   S <- Sbar + beta k e^T;   o = scale S^T q
  * -- the rank-one updates in strict order of gpx_ep_sweep, with a matrix that forgets.  No counterpart in the reference.
  *   q, k: batch x tokens x key_heads x dk;   v, o: batch x tokens x value_heads x dv   (dtype: GPX_F32, GPX_F16, GPX_BF16)
- *   g (log decay), beta: batch x tokens x value_heads in fp32;   states: sequences x value_heads x dk x dv in fp32
+ *   g (log decay, <= 0), beta: batch x tokens x value_heads in fp32;   states: sequences x value_heads x dk x dv in fp32
  * value_heads is a multiple of key_heads; value head i reads key head i / (value_heads / key_heads).  Element
  * (b, t, h, c) of an input lies at b * bs + t * rs + h * cs + c (strides in elements, not negative).  Outputs and
  * states are packed in the order written above.
@@ -325,7 +325,8 @@ int gpx_orthogonalize_tile(int dtype, int batch, int n, int m, int product);
  * offsets[s] .. offsets[s + 1] (sequences + 1 values in DEVICE memory, not decreasing; values outside [0, tokens] are
  * clamped, a decreasing value is read as the one before it).  Tokens behind the last sequence or before the first are
  * not read and their outputs not written.  Sequences may be empty: their state passes through.
- * g may be -infinity (the state is forgotten); it is read as max(g, -200).  beta == 0 and g == 0 leave the state as it is.
+ * g may be -infinity (the state is forgotten); it is read as max(g, -200).  g > 0 is no decay: chunks of 64 tokens, which take
+ * differences of what has grown, lose as many bits as exp of its sum over a chunk has, and give NaNs where that overflows.  beta == 0 and g == 0 leave the state as it is.
  * A NaN or an infinity in a token's inputs reaches the later tokens of its sequence and heads, and may reach the earlier ones of
  * the same 64 tokens (counted from the sequence's first); no others.  1 <= dk <= 128,
  * 1 <= dv <= 1024; a token stride of v of at most 2^22.  Outputs overlap neither inputs nor each other, except where it is
