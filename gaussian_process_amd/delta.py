@@ -93,6 +93,8 @@ def _check_state(t, shape, name):
     check_tensor(t, name)
     if t.dtype != torch.float32 or t.shape != shape:
         raise ValueError("%s must be float32 of shape %s" % (name, tuple(shape)))
+    if not t.data_ptr() and t.numel():   # the library takes no address for no state
+        raise ValueError("%s has no memory" % name)
 
 
 def _aligned(t):
@@ -273,6 +275,8 @@ def gated_delta_rule_step(q, k, v, g, beta, state, slots=None, state_out=None, s
         if key is not None:
             _known_steps[key] = known
     at, to = state.data_ptr(), state_out.data_ptr()
+    if not (at and to) and state.numel():
+        raise ValueError("state or state_out has no memory")
     if 0 < abs(to - at) < state.numel() * 4:
         raise ValueError("state_out overlaps state")
     rt = tensor_runtime(q, k, v, g, beta, state, slots, state_out)

@@ -136,24 +136,31 @@ def ptr(t):
     return C.c_void_p(t.data_ptr())
 
 
+_torch = None
+
+
 def tensor_runtime(first, *others):
-    """The runtime of the one MI355X that all the given tensors (None allowed after the first) live on, for calls that record
-    no gradient: RuntimeError if one would be lost."""
-    import torch
+    """The runtime of the one MI355X that all the given tensors (None allowed after the first) live on, for calls that read and write
+    their memory as it is and record no gradient: refused where that would give other values or lose one."""
+    global _torch
+    if _torch is None:   # not by an import statement: a decoder comes here for every token
+        import torch as _torch
     device = first.device
-    recording = torch.is_grad_enabled()
-    needed = recording and first.requires_grad
+    lazy = first.is_neg()
     for t in others:
         if t is not None:
             if t.device != device:
                 raise ValueError("the tensors are on different devices: %s and %s" % (device, t.device))
-            if recording and t.requires_grad:
-                needed = True
-    if torch.autograd.forward_ad._current_level >= 0:
-        needed = needed or any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in (first, *others))
+            if t.is_neg():
+                lazy = True
+    needed = _torch.is_grad_enabled() and _torch._C._any_requires_grad(first, *others)
+    if _torch.autograd.forward_ad._current_level >= 0:
+        needed = needed or any(t is not None and _torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in (first, *others))
     if needed:
         raise RuntimeError("a tensor requires a gradient (or carries a tangent), which this call does not record: make it under "
                            "torch.no_grad() or with detached tensors")
+    if lazy:   # its memory holds the negated values
+        raise ValueError("a tensor has a pending negation: pass t.resolve_neg()")
     if device.type != "cuda":
         raise _lib.GpxError("the tensors must be on an MI355X (no CPU fallback)")
     rt = _runtimes.get(device.index)
